@@ -1,0 +1,788 @@
+// Attention of decoding sequences over a paged cache held in 4 bits, and such a cache expanded to bf16 tiles for prompts.
+//
+// The cache (ops/kv4.py): per page and kv head blocks of 16 tokens, 16 rows of D / 2 bytes and 16 x D / 64 pairs (scale, low); a
+// code c of a group stands for c scale + low. With the groups g of a head's dims, key j and query row r
+//   score  = sum_g scale_jg (q_rg . c_jg) + low_jg sum(q_rg)
+//   output = sum_j p_j (c'_jg scale'_jg + low'_jg) = sum_j (p_j scale'_jg) c'_jg + sum_j p_j low'_jg
+// so the codes go into the matrix instructions as they are and scales and low ends stay outside: four fused operations a score, two a
+// probability, instead of one or two for each of the D values of a key.
+//
+// Codes as 16-bit operands: a nibble at bits 0 (or 4) of an fp16 is the subnormal c 2^-24 (or 16 c 2^-24), exact, and the matrix
+// instructions take subnormals: one AND for two codes. Queries are scaled by a power of two to the upper end of fp16 (by a
+// further 1/16 where a nibble stands four bits up); eleven bits hold their eight. The values' codes meet probabilities of any
+// size, so there they are bf16: 0x4300 | c is 128 + c, and 128 times the sum of the (rounded) probabilities, which one more product with
+// ones gives, comes off again at the end: fp32 sums lose 2^-19 of the result to it, rounding the probabilities to bf16 2^-9.
+//
+// Keys are the rows of the products (m16n8k16: 16 keys x 8 query heads, then 16 dims x 8 heads), so eight query heads of
+// one kv head fill an instruction. A lane (g, t) = (lane / 4, lane % 4) holds
+//   codes of keys g, g + 8: 16 bytes (D = 128), the t-th quarter of the row: eight dims at a time of each group
+//   codes of values: tokens 2t, 2t + 1, 2t + 8, 2t + 9, eight bytes each: eight dims of each group, chunk g
+//   scores: keys g, g + 8 of heads 2t, 2t + 1; movmatrix turns the probabilities into the second product's operand
+//
+// A warp walks tiles of 32 keys by itself: it copies them (cp.async.bulk, one contiguous block of 9 D bytes for 16 tokens' keys or
+// values) into its own ring, two tiles deep. The tiles of all sequences and heads lie in one row, which is cut into equal
+// shares, one per CTA, on the device: ragged batches and few long sequences fill the machine alike. The eight warps of a CTA take
+// its tiles in turn and sum up in shared memory where a sequence's head ends; what a share has of a head that goes on in another
+// CTA goes to scratch, and a second kernel joins it.
+//
+// The reference of a head's exponentials follows its maximum only when a score passes it by 2^8 (one vote instead of three
+// shuffles a tile).
+#include "../common/bounded.cuh"
+#include "attn_common.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kV4Warps = 8, kV4Threads = kV4Warps * 32, kV4Keys = 32, kV4Stages = 2;
+constexpr int kV4Lens = 256;                             // lengths that a CTA keeps in shared memory, from its first sequence on
+constexpr float kV4Lazy = 8.f;
+
+struct Kv4Params {
+  const __nv_bfloat16* q;
+  int64_t q_ts;
+  __nv_bfloat16* out;                                    // [B, Hq, D]
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  int64_t pages;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  int B, max_blocks, Hq, Hkv, G, GP, page_size;          // GP query heads (at most 8 NT) of the G of a kv head at a time
+  float scale_log2;
+  float* part_o;                                         // [2 CTAs, 8 NT, D]
+  float* part_ml;                                        // [2 CTAs, 8 NT, 2]
+  int4* meta;                                            // [CTAs] (sequence, head group, last CTA, slot) of what starts here and goes on; sequence -1: nothing
+  WaitConfig waits;
+};
+
+template <int D, int NT>
+struct Kv4Smem {
+  static constexpr int kBlock = 9 * D;                   // 16 tokens' keys or values
+  static constexpr int kStage = 4 * kBlock;
+  static constexpr int kRing = kV4Warps * kV4Stages * kStage;
+  static constexpr int kSums = 4 * 32 * (D / 16 * 4 * NT) * 4;    // four warps' sums
+  static constexpr int kMl = kV4Warps * 8 * NT * 2 * 4;
+  static constexpr int kBytes = kRing + kSums + kMl + kV4Lens * 4 + kV4Warps * kV4Stages * 8 + 64;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void lds64(uint32_t addr, uint32_t& a, uint32_t& b) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t a;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a) : "r"(addr));
+  return a;
+}
+// d += a b, 16 x 8 x 16
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// tiles of a sequence; one at least, so that a sequence of no keys gets its zeros
+__device__ __forceinline__ int kv4_tiles(int len) { return max(1, (len + kV4Keys - 1) / kV4Keys); }
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel(const Kv4Params p) {
+  using SM = Kv4Smem<D, NT>;
+  constexpr int GR = D / 64;                             // groups of a head
+  constexpr int KS = D / 16;                             // 16-dim steps of the first product, and dim tiles of the second
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* sums = reinterpret_cast<float*>(smem + SM::kRing);
+  float* ml = reinterpret_cast<float*>(smem + SM::kRing + SM::kSums);              // [warp][head][m, l]
+  int* lens = reinterpret_cast<int*>(smem + SM::kRing + SM::kSums + SM::kMl);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(lens + kV4Lens);
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + kV4Warps * kV4Stages);      // gave up, first sequence, its first tile
+  const WaitGuard guard{words, p.waits};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+
+  if (tid == 0) *guard.dead = 0;
+  if (tid < kV4Warps * kV4Stages) mbar_init(&bars[tid], 1);
+  fence_mbar_init();
+  griddep_launch();
+  griddep_wait();
+
+  // ---- this CTA's share [begin, end) of all tiles: sequence by sequence, head group by head group
+  const int H = p.Hkv * (p.G / p.GP);
+  __shared__ int scan[kV4Warps + 1];
+  auto block_scan = [&](int v, int& total) {             // inclusive
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kV4Warps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    return x + before;
+  };
+  int all = 0;
+  for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
+    int total;
+    block_scan(s0 + tid < p.B ? kv4_tiles(p.seq_lens[s0 + tid]) : 0, total);
+    all += total;
+  }
+  const int64_t work = static_cast<int64_t>(all) * H;
+  const int64_t share = max((work + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kV4Warps));
+  const int64_t begin = share * blockIdx.x, end = min(begin + share, work);
+  if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (begin >= work) return;
+  {
+    int base = 0;                                        // tiles of one head group before this round
+    for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
+      int total;
+      const int n = s0 + tid < p.B ? kv4_tiles(p.seq_lens[s0 + tid]) : 0;
+      const int upto = block_scan(n, total) + base;
+      if (begin >= static_cast<int64_t>(upto - n) * H && begin < static_cast<int64_t>(upto) * H) {
+        words[1] = s0 + tid;
+        words[2] = upto - n;
+      }
+      base += total;
+    }
+    __syncthreads();
+  }
+  const int seq0 = words[1];
+  for (int i = tid; i < kV4Lens; i += kV4Threads) lens[i] = seq0 + i < p.B ? p.seq_lens[seq0 + i] : 0;
+  __syncthreads();
+  auto len_of = [&](int s) { return s - seq0 < kV4Lens ? lens[s - seq0] : p.seq_lens[s]; };
+
+  struct Place {                                         // of a tile in the row
+    int seq, head, tile, n;
+  };
+  const int first_in = static_cast<int>(begin - static_cast<int64_t>(words[2]) * H);
+  Place at;
+  at.seq = seq0;
+  at.n = kv4_tiles(len_of(seq0));
+  at.head = first_in / at.n;
+  at.tile = first_in - at.head * at.n;
+  auto advance = [&](Place& x, int by) {
+    x.tile += by;
+    while (x.tile >= x.n) {
+      x.tile -= x.n;
+      if (++x.head == H) {
+        x.head = 0;
+        if (++x.seq >= p.B) {                            // behind the last tile: never used
+          x.seq = p.B - 1;
+          x.tile = 0;
+          return;
+        }
+        x.n = kv4_tiles(len_of(x.seq));
+      }
+    }
+  };
+
+  // ---- copies: lanes 0-3 have a block each, (keys, values) x 16 tokens
+  const uint32_t ring = smem_u32(smem) + warp * (kV4Stages * SM::kStage);
+  uint64_t* bar = bars + warp * kV4Stages;
+  const int64_t head_bytes = static_cast<int64_t>(p.page_size / 16) * SM::kBlock;
+  const int hg = p.G / p.GP;
+  auto page_of = [&](const Place& x) {                   // lane's page of this tile; a table entry that is no page reads another one
+    const int tok = x.tile * kV4Keys + (lane & 1) * 16;
+    if (lane >= 4 || tok >= len_of(x.seq)) return 0;
+    return p.block_table[static_cast<size_t>(x.seq) * p.max_blocks + min(tok / p.page_size, p.max_blocks - 1)];
+  };
+  auto issue = [&](const Place& x, int page, int stage) {
+    const int len = len_of(x.seq), blocks = min(2, (len - x.tile * kV4Keys + 15) / 16);
+    if (blocks <= 0) {                                   // an empty sequence
+      if (lane == 0) mbar_arrive(&bar[stage]);
+      return;
+    }
+    if (lane == 0) mbar_expect_tx(&bar[stage], blocks * 2 * SM::kBlock);
+    __syncwarp();
+    const int sub = lane & 1;
+    if (lane < 4 && sub < blocks) {
+      const int64_t in_range = min(static_cast<int64_t>(static_cast<uint32_t>(page)), p.pages - 1);
+      const int in_page = (x.tile * kV4Keys + sub * 16) % p.page_size / 16;
+      const uint8_t* src = (lane & 2 ? p.v_cache : p.k_cache) + (in_range * p.Hkv + x.head / hg) * head_bytes + in_page * SM::kBlock;
+      bulk_load(ring + stage * SM::kStage + lane * SM::kBlock, src, SM::kBlock, &bar[stage]);
+    }
+  };
+
+  Place fetch = at;                                      // the next tile to copy
+  int64_t fetch_x = begin + warp;
+  advance(fetch, warp);
+  uint32_t issued = 0, used = 0;
+#pragma unroll
+  for (int s = 0; s < kV4Stages; ++s) {
+    if (fetch_x < end) {
+      issue(fetch, page_of(fetch), s);
+      ++issued;
+      fetch_x += kV4Warps;
+      advance(fetch, kV4Warps);
+    }
+  }
+
+  // ---- segment by segment (the tiles of one head group of one sequence)
+  int64_t mine = begin + warp;                           // this warp's next tile
+  bool ok = true;
+  if (guard.cfg.limit_ns == 0) ok = __all_sync(0xffffffffu, mine >= end || guard.first(&bar[0]));
+  int64_t seg = begin;
+  while (seg < end) {
+    const int64_t seg_end = min(end, seg + (at.n - at.tile));
+    const bool whole = at.tile == 0 && seg_end - seg == at.n;
+    const int len = len_of(at.seq);
+    const int head0 = at.head / hg * p.G + at.head % hg * p.GP;
+    const __nv_bfloat16* q = p.q + at.seq * p.q_ts + static_cast<int64_t>(head0) * D;
+
+    // queries of heads 8 nt + g as operands; sums and factors of heads 8 nt + 2t, + 2t + 1
+    uint32_t qf[NT][KS][2];
+    float unscale[NT][2], qsum[NT][2][GR];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = 8 * nt + g;
+      uint32_t raw[GR][2][4];                            // chunk 2t, 2t + 1 of each group, eight dims each
+      float most = 0.f, sum[GR];
+#pragma unroll
+      for (int gr = 0; gr < GR; ++gr) {
+        sum[gr] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (h < p.GP) v = *reinterpret_cast<const uint4*>(q + h * D + gr * 64 + (2 * t + c) * 8);
+          raw[gr][c][0] = v.x; raw[gr][c][1] = v.y; raw[gr][c][2] = v.z; raw[gr][c][3] = v.w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16(raw[gr][c][e]);
+            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+            sum[gr] += f.x + f.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], o);
+      }
+      // 2^k with the largest |q| in [2^14, 2^15); rows below 2^-112 (zeros, say) are taken as that, rows beyond 2^117 become
+      // infinities
+      const int ex = max(static_cast<int>(__float_as_uint(most) >> 23), 15);
+      const float up = ex > 244 ? 1.f : __uint_as_float(static_cast<uint32_t>(268 - ex) << 23);
+      const float back = ex > 244 ? 16777216.f : __uint_as_float(static_cast<uint32_t>(ex + 10) << 23);      // 2^24 / up
+#pragma unroll
+      for (int gr = 0; gr < GR; ++gr) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = unpack_bf16(raw[gr][c][e]);
+            f[2 * e] = v.x * up;
+            f[2 * e + 1] = v.y * up;
+          }
+          // step 2c: codes (0, 4) and, four bits up, (1, 5); step 2c + 1: (2, 6) and (3, 7)
+          qf[nt][gr * 4 + 2 * c][0] = pack_f16(f[0], f[4]);
+          qf[nt][gr * 4 + 2 * c][1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
+          qf[nt][gr * 4 + 2 * c + 1][0] = pack_f16(f[2], f[6]);
+          qf[nt][gr * 4 + 2 * c + 1][1] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {                      // lane 4 (2t + c) has head 2t + c
+        unscale[nt][c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c)) * p.scale_log2;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) qsum[nt][c][gr] = __shfl_sync(0xffffffffu, sum[gr], 4 * (2 * t + c)) * p.scale_log2;
+      }
+    }
+
+    float o[NT][KS][4], ones[NT][GR][2], lows[NT][GR][2], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[nt][c] = -INFINITY;
+        l[nt][c] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) ones[nt][gr][c] = lows[nt][gr][c] = 0.f;
+      }
+    }
+
+    for (; mine < seg_end && ok; mine += kV4Warps) {
+      const int stage = used % kV4Stages;
+      const int key0 = (at.tile + static_cast<int>(mine - seg)) * kV4Keys;
+      const int next_page = fetch_x < end ? page_of(fetch) : 0;      // on its way while this tile is worked on
+      ok = __all_sync(0xffffffffu, guard.wait(&bar[stage], (used / kV4Stages) & 1));
+      if (!ok) break;
+      const uint32_t kb = ring + stage * SM::kStage, vb = kb + 2 * SM::kBlock;
+      const bool tail = key0 + kV4Keys > len;
+
+      // scores of keys 16 sub + g, + 8
+      float s[NT][2][4];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const uint32_t b = kb + sub * SM::kBlock;
+        float acc[NT][GR][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][gr][e] = 0.f;
+        uint32_t w[2][2 * GR];                           // keys g, g + 8: chunks 2t, 2t + 1 of each group
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (D == 128) lds128(b + (g + 8 * r) * 64 + t * 16, w[r]);
+          else lds64(b + (g + 8 * r) * 32 + t * 8, w[r][0], w[r][1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int gr = 0; gr < GR; ++gr) {
+            const uint32_t x = w[0][c * GR + gr], y = w[1][c * GR + gr], x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(acc[nt][gr], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][gr * 4 + 2 * c][0],
+                      qf[nt][gr * 4 + 2 * c][1]);
+              mma_f16(acc[nt][gr], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
+                      qf[nt][gr * 4 + 2 * c + 1][0], qf[nt][gr * 4 + 2 * c + 1][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t pr[2];
+          if constexpr (GR == 2) lds64(b + 8 * D + (g + 8 * r) * 8, pr[0], pr[1]);
+          else pr[0] = lds32(b + 8 * D + (g + 8 * r) * 4);
+          const bool seen = key0 + 16 * sub + 8 * r + g < len;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float dot = low_half(pr[0]) * acc[nt][0][2 * r + c], add = high_half(pr[0]) * qsum[nt][c][0];
+              if constexpr (GR == 2) {
+                dot = fmaf(low_half(pr[1]), acc[nt][1][2 * r + c], dot);
+                add = fmaf(high_half(pr[1]), qsum[nt][c][1], add);
+              }
+              const float z = fmaf(unscale[nt][c], dot, add);
+              s[nt][sub][2 * r + c] = tail && !seen ? -INFINITY : z;
+            }
+          }
+        }
+      }
+      // the reference of the exponentials
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) mx[c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
+        if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + kV4Lazy || mx[1] > m[nt][1] + kV4Lazy)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int of = 4; of < 32; of <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], of));
+            const float m_new = fmaxf(m[nt][c], mx[c]);
+            const float alpha = m_new == -INFINITY ? 1.f : exp2f(m[nt][c] - m_new);
+            m[nt][c] = m_new;
+            l[nt][c] *= alpha;
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) {
+              ones[nt][gr][c] *= alpha;
+              lows[nt][gr][c] *= alpha;
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              o[nt][i][c] *= alpha;
+              o[nt][i][2 + c] *= alpha;
+            }
+          }
+        }
+      }
+      // probabilities, times the values' scales: operands of the second product
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const uint32_t b = vb + sub * SM::kBlock;
+        uint32_t pf[NT][GR][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t pr[2];
+          if constexpr (GR == 2) lds64(b + 8 * D + (g + 8 * r) * 8, pr[0], pr[1]);
+          else pr[0] = lds32(b + 8 * D + (g + 8 * r) * 4);
+          if (tail && key0 + 16 * sub + 8 * r + g >= len) pr[0] = pr[1] = 0u;       // what lies behind the last token may be anything
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float e[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float m_use = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+              e[c] = exp2f(s[nt][sub][2 * r + c] - m_use);
+              l[nt][c] += e[c];
+#pragma unroll
+              for (int gr = 0; gr < GR; ++gr) lows[nt][gr][c] = fmaf(e[c], high_half(pr[gr]), lows[nt][gr][c]);
+            }
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) {
+              const uint32_t packed = pack_bf16(e[0] * low_half(pr[gr]), e[1] * low_half(pr[gr]));
+              ones[nt][gr][0] += low_half(packed);
+              ones[nt][gr][1] += high_half(packed);
+              pf[nt][gr][r] = movmatrix(packed);
+            }
+          }
+        }
+        uint32_t w[4][2];                                // tokens 2t, 2t + 1, 2t + 8, 2t + 9: chunk g of each group
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a = b + (2 * t + (i & 1) + (i >> 1) * 8) * (D / 2) + g * (4 * GR);
+          if constexpr (GR == 2) lds64(a, w[i][0], w[i][1]);
+          else w[i][0] = lds32(a);
+        }
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {                  // dims 2i, 2i + 1 of the chunk
+            const uint32_t sel = i | ((4 + i) << 8);     // byte i of both tokens, each in the low byte of its half
+            const uint32_t x = __byte_perm(w[0][gr], w[1][gr], (sel & 0xf) | ((sel & 0xf) << 4) | (sel & 0xf00) | ((sel & 0xf00) << 4));
+            const uint32_t y = __byte_perm(w[2][gr], w[3][gr], (sel & 0xf) | ((sel & 0xf) << 4) | (sel & 0xf00) | ((sel & 0xf00) << 4));
+            const uint32_t a0 = (x & 0x000f000fu) | 0x43004300u, a1 = ((x >> 4) & 0x000f000fu) | 0x43004300u;
+            const uint32_t a2 = (y & 0x000f000fu) | 0x43004300u, a3 = ((y >> 4) & 0x000f000fu) | 0x43004300u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][gr * 4 + i], a0, a1, a2, a3, pf[nt][gr][0], pf[nt][gr][1]);
+          }
+        }
+      }
+      ++used;
+      __syncwarp();                                      // every lane has read the stage
+      if (fetch_x < end) {
+        issue(fetch, next_page, stage);
+        ++issued;
+        fetch_x += kV4Warps;
+        advance(fetch, kV4Warps);
+      }
+    }
+
+    // ---- the warps' sums together; l, ones and lows are of this lane's keys so far
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int of = 4; of < 32; of <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], of);
+#pragma unroll
+          for (int gr = 0; gr < GR; ++gr) {
+            ones[nt][gr][c] += __shfl_xor_sync(0xffffffffu, ones[nt][gr][c], of);
+            lows[nt][gr][c] += __shfl_xor_sync(0xffffffffu, lows[nt][gr][c], of);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          const float off = fmaf(-128.f, ones[nt][i / 4][c], lows[nt][i / 4][c]);
+          o[nt][i][c] += off;
+          o[nt][i][2 + c] += off;
+        }
+        if (g == 0) {
+          float* x = ml + (warp * 8 * NT + nt * 8 + 2 * t + c) * 2;
+          x[0] = m[nt][c];
+          x[1] = l[nt][c];
+        }
+      }
+    }
+    __syncthreads();
+    float top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kV4Warps; ++w) x = fmaxf(x, ml[(w * 8 * NT + nt * 8 + 2 * t + c) * 2]);
+        top[nt][c] = x;
+        const float f = m[nt][c] == -INFINITY ? 0.f : exp2f(m[nt][c] - x);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[nt][i][c] *= f;
+          o[nt][i][2 + c] *= f;
+        }
+      }
+    }
+    // sums[w][nt][head c][4 sums a lane at a time][lane]: eight dims of a group of one head are two pieces
+    auto piece = [&](int w, int nt, int gr, int c, int half) {
+      return reinterpret_cast<float4*>(sums) + (((w * NT + nt) * GR + gr) * 4 + c * 2 + half) * 32 + lane;
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int gr = 0; gr < GR; ++gr) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (warp >= 4)
+              *piece(warp - 4, nt, gr, c, half) = make_float4(o[nt][gr * 4 + 2 * half][c], o[nt][gr * 4 + 2 * half][2 + c],
+                                                              o[nt][gr * 4 + 2 * half + 1][c], o[nt][gr * 4 + 2 * half + 1][2 + c]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (warp < 4) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float4* x = piece(warp, nt, gr, c, half);
+              float4 v = *x;
+              v.x += o[nt][gr * 4 + 2 * half][c];
+              v.y += o[nt][gr * 4 + 2 * half][2 + c];
+              v.z += o[nt][gr * 4 + 2 * half + 1][c];
+              v.w += o[nt][gr * 4 + 2 * half + 1][2 + c];
+              *x = v;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    // a piece (four dims of a head) a thread: sum of the four, then the result or this share's part of it
+    const int slot = 2 * blockIdx.x + (seg == begin ? 0 : 1);
+    constexpr int kPieces = NT * GR * 4;
+    for (int x = warp; x < kPieces; x += kV4Warps) {
+      const int nt = x / (GR * 4), gr = x / 4 % GR, c = x / 2 % 2, half = x % 2;
+      const int h = 8 * nt + 2 * t + c, dim = gr * 64 + 8 * g + 4 * half;
+      float4 v = *piece(0, nt, gr, c, half);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float4 y = *piece(w, nt, gr, c, half);
+        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+      }
+      float mm = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kV4Warps; ++w) mm = fmaxf(mm, ml[(w * 8 * NT + h) * 2]);
+#pragma unroll
+      for (int w = 0; w < kV4Warps; ++w) {
+        const float mw = ml[(w * 8 * NT + h) * 2];
+        if (mw != -INFINITY) sum = fmaf(ml[(w * 8 * NT + h) * 2 + 1], exp2f(mw - mm), sum);
+      }
+      if (h < p.GP) {
+        if (whole) {
+          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;       // no keys: zeros
+          *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(at.seq) * p.Hq + head0 + h) * D + dim) =
+              make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 8 * NT + h) * D + dim) = v;
+          if (g == 0 && gr == 0 && half == 0) {
+            p.part_ml[(slot * 8 * NT + h) * 2] = mm;
+            p.part_ml[(slot * 8 * NT + h) * 2 + 1] = sum;
+          }
+        }
+      }
+    }
+    if (tid == 0 && at.tile == 0 && !whole)              // it ends with this share and goes on in the next
+      p.meta[blockIdx.x] = make_int4(at.seq, at.head, static_cast<int>((seg + at.n - 1) / share), slot);
+    __syncthreads();                                     // the pieces and factors have been read
+    at.tile += static_cast<int>(seg_end - seg);
+    if (at.tile == at.n) {
+      at.tile = 0;
+      if (++at.head == H) {
+        at.head = 0;
+        if (++at.seq < p.B) at.n = kv4_tiles(len_of(at.seq));
+      }
+    }
+    seg = seg_end;
+  }
+  // copies in flight land before the CTA ends, where the waits were given up
+  for (; used < issued; ++used) guard.land(&bar[used % kV4Stages], (used / kV4Stages) & 1);
+}
+
+// Joins the parts of a head group that several CTAs share: one CTA for each that starts one and does not end it.
+template <int D, int NT>
+__global__ void __launch_bounds__(D) kv4_join_kernel(const Kv4Params p) {
+  griddep_launch();
+  griddep_wait();
+  const int4 meta = p.meta[blockIdx.x];                  // sequence, head group, last CTA, slot of the first part
+  if (meta.x < 0) return;
+  const int h = blockIdx.y, hg = p.G / p.GP, d = threadIdx.x;
+  const int parts = meta.z - static_cast<int>(blockIdx.x) + 1;
+  auto slot_of = [&](int i) { return i == 0 ? meta.w : 2 * (static_cast<int>(blockIdx.x) + i); };
+  float m = -INFINITY;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[(slot_of(i) * 8 * NT + h) * 2]);
+  float sum = 0.f, v = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const int slot = slot_of(i);
+    const float mi = p.part_ml[(slot * 8 * NT + h) * 2];
+    const float f = mi == -INFINITY ? 0.f : exp2f(mi - m);
+    sum = fmaf(p.part_ml[(slot * 8 * NT + h) * 2 + 1], f, sum);
+    v = fmaf(p.part_o[(static_cast<int64_t>(slot) * 8 * NT + h) * D + d], f, v);
+  }
+  const int head = meta.y / hg * p.G + meta.y % hg * p.GP + h;
+  p.out[(static_cast<int64_t>(meta.x) * p.Hq + head) * D + d] = __float2bfloat16(v / sum);
+}
+
+template <int D, int NT>
+int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
+  using SM = Kv4Smem<D, NT>;
+  static PerDeviceOnce configured;
+  if (configured.need()) {
+    CUDA_CHECK_RET(cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
+    configured.done();
+  }
+  CUDA_CHECK_RET(launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(kV4Threads), SM::kBytes, st, p));
+  CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT>, dim3(ctas, p.GP), dim3(D), 0, st, p));
+  return 0;
+}
+
+// Pages of the sequences of a launch expanded to bf16 tiles [tile][Hkv][D / 64][64 tokens][64], as the prefill kernels read a cache with
+// pages of 64, and the tiles' table. Sequence s has ceil(len / 64) tiles, from the sum of those before it on. A CTA makes 16 tokens of a
+// head's keys or values. Memory-bound: 9 D / 16 bytes in, 2 D out a token.
+template <int D>
+__global__ void __launch_bounds__(128)
+kv4_expand_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ block_table,
+                  int max_blocks, const int32_t* __restrict__ seq_lens, int Hkv, int page_size, int64_t pages, int64_t tiles,
+                  __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int32_t* __restrict__ table, int max_tiles) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int G = D / 64, kBlock = 9 * D;
+  const int seq = blockIdx.y, blk = blockIdx.x;          // 16 tokens
+  const int len = seq_lens[seq];
+  if (blk * 16 >= (len + 63) / 64 * 64) return;          // a tile's last blocks are written too: zeros behind the last token
+  __shared__ int part[4];
+  int before = 0;
+  for (int s = threadIdx.x; s < seq; s += 128) before += (seq_lens[s] + 63) / 64;
+  before = __reduce_add_sync(0xffffffffu, before);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = before;
+  __syncthreads();
+  const int64_t tile = part[0] + part[1] + part[2] + part[3] + blk / 4;
+  if (tile >= tiles) return;                             // more tokens than the caller has made room for
+  if (threadIdx.x == 0 && blockIdx.z == 0 && blk % 4 == 0) table[static_cast<size_t>(seq) * max_tiles + blk / 4] = static_cast<int>(tile);
+  const int tok0 = blk * 16;
+  int64_t page = 0;
+  if (tok0 < len) page = min(static_cast<int64_t>(static_cast<uint32_t>(block_table[static_cast<size_t>(seq) * max_blocks + min(tok0 / page_size, max_blocks - 1)])),
+                            pages - 1);
+  const int heads2 = 2 * Hkv;
+  for (int hz = blockIdx.z; hz < heads2; hz += gridDim.z) {
+    const bool is_v = hz >= Hkv;
+    const int h = is_v ? hz - Hkv : hz;
+    const uint8_t* block = (is_v ? v_cache : k_cache) + ((page * Hkv + h) * (page_size / 16) + tok0 % page_size / 16) * kBlock;
+    __nv_bfloat16* out = (is_v ? v_out : k_out) + ((tile * Hkv + h) * G * 64 + blk % 4 * 16) * 64;
+#pragma unroll
+    for (int i = threadIdx.x; i < 16 * D / 8; i += 128) {
+      const int row = i / (D / 8), unit = i % (D / 8), group = unit % G, chunk = unit / G;
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (tok0 + row < len) {
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + row * (D / 2) + unit * 4);
+        const float2 pair = unpack_bf16(*reinterpret_cast<const uint32_t*>(block + 8 * D + (row * G + group) * 4));
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), pair.x, pair.y);
+        w = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+      }
+      *reinterpret_cast<uint4*>(out + (group * 64 + row) * 64 + chunk * 8) = w;
+    }
+  }
+}
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+// Bytes of scratch that gllm_kv4_decode needs on `ctas` CTAs.
+GLLM_EXPORT int64_t gllm_kv4_decode_scratch(int D, int ctas) {
+  return static_cast<int64_t>(ctas) * (2 * 16 * (D + 2) * 4 + 16);
+}
+
+// Attention of B sequences with one new token each over 4-bit caches of `pages` pages: q [B, Hq * D] (token stride q_ts), out [B, Hq, D]
+// contiguous; keys [0, seq_lens[s]) of each, zeros where there are none.
+GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const void* k_cache, const void* v_cache, int64_t pages,
+                                const void* block_table, int max_blocks, const void* seq_lens, int B, int Hq, int Hkv, int D,
+                                int page_size, float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
+  if (B <= 0) return 0;
+  auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || Hkv <= 0 || Hq % Hkv != 0 || q_ts % 8 != 0 || !al16(q) ||
+      !al16(out) || !al16(k_cache) || !al16(v_cache) || !al16(scratch) || pages <= 0 || ctas <= 0 ||
+      scratch_bytes < gllm_kv4_decode_scratch(D, ctas)) {
+    fprintf(stderr, "[gllm_b200] kv4_decode: unsupported D=%d page_size=%d Hq=%d Hkv=%d, or rows off 16-byte boundaries\n", D,
+            page_size, Hq, Hkv);
+    return 1;
+  }
+  Kv4Params p;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  p.q_ts = q_ts;
+  p.out = reinterpret_cast<__nv_bfloat16*>(out);
+  p.k_cache = reinterpret_cast<const uint8_t*>(k_cache);
+  p.v_cache = reinterpret_cast<const uint8_t*>(v_cache);
+  p.pages = pages;
+  p.block_table = reinterpret_cast<const int32_t*>(block_table);
+  p.seq_lens = reinterpret_cast<const int32_t*>(seq_lens);
+  p.B = B; p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.page_size = page_size;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part_o = reinterpret_cast<float*>(scratch);
+  p.part_ml = p.part_o + static_cast<int64_t>(ctas) * 2 * 16 * D;
+  p.meta = reinterpret_cast<int4*>(p.part_ml + static_cast<int64_t>(ctas) * 2 * 16 * 2);
+  p.waits = g_wait_config;
+  // as many query heads at a time as divide the kv head's: their codes are read once
+  p.GP = 1;
+  for (int d = 2; d <= 16 && d <= p.G; ++d)
+    if (p.G % d == 0) p.GP = d;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.GP <= 8) return D == 64 ? launch_kv4_decode<64, 1>(p, ctas, st) : launch_kv4_decode<128, 1>(p, ctas, st);
+  return D == 64 ? launch_kv4_decode<64, 2>(p, ctas, st) : launch_kv4_decode<128, 2>(p, ctas, st);
+}
+
+// Keys and values of B sequences from 4-bit caches to bf16 tiles k_out, v_out [tiles, Hkv, D / 64, 64, 64], sequence after sequence, each
+// rounded up to 64 tokens; table [B, max_tiles]: their tiles. max_len: the longest.
+GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const void* block_table, int max_blocks, const void* seq_lens,
+                                int B, int Hkv, int D, int page_size, int64_t pages, int64_t tiles, void* k_out, void* v_out,
+                                void* table, int max_tiles, int max_len, void* stream) {
+  if (B <= 0 || max_len <= 0) return 0;
+  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || pages <= 0 || B > 65535 ||
+      static_cast<int64_t>(max_tiles) * 64 < max_len) {
+    fprintf(stderr, "[gllm_b200] kv4_expand: unsupported D=%d page_size=%d, %d sequences\n", D, page_size, B);
+    return 1;
+  }
+  const int blocks = (max_len + 63) / 64 * 4;
+  const int per = static_cast<int64_t>(blocks) * B >= 4 * num_sms() ? 4 : 1;        // heads of a CTA: fewer and longer ones for long prompts
+  const dim3 grid(blocks, B, (2 * Hkv + per - 1) / per);
+  CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_expand_kernel<64> : kv4_expand_kernel<128>, grid, dim3(128), 0,
+                            reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint8_t*>(k_cache),
+                            reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(block_table), max_blocks,
+                            reinterpret_cast<const int32_t*>(seq_lens), Hkv, page_size, pages, tiles,
+                            reinterpret_cast<__nv_bfloat16*>(k_out), reinterpret_cast<__nv_bfloat16*>(v_out),
+                            reinterpret_cast<int32_t*>(table), max_tiles));
+  return 0;
+}

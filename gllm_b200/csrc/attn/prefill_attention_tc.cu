@@ -645,6 +645,22 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 
 // tensor map over the paged cache with ONE 64-wide slab per box ([page_size][64]), so that a KV tile can be
 // assembled slab-major ([D/64][keys][64]) — the layout both UMMA operand forms need (pages of 128 keys: two boxes)
+static int make_kv_slab_tmap(const void* base, int64_t num_pages, int Hkv, int D, int page_size, CUtensorMap* out) {
+  cuuint64_t dims[3] = {64, (cuuint64_t)page_size, (cuuint64_t)(num_pages * Hkv * (D / 64))};
+  cuuint64_t strides[2] = {128, (cuuint64_t)page_size * 128};
+  cuuint32_t box[3] = {64, (cuuint32_t)(page_size < 64 ? page_size : 64), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = get_encode_fn()(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "[gllm_b200] KV slab tensor-map encode failed (%d)\n", (int)r);
+    return 1;
+  }
+  return 0;
+}
+
+// The map of a cache that lives as long as the process is made once.
 static int get_kv_slab_tmap(const void* base, int64_t num_pages, int Hkv, int D, int page_size, CUtensorMap* out) {
   static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
   static std::mutex mu;
@@ -656,17 +672,7 @@ static int get_kv_slab_tmap(const void* base, int64_t num_pages, int Hkv, int D,
     return 0;
   }
   CUtensorMap m;
-  cuuint64_t dims[3] = {64, (cuuint64_t)page_size, (cuuint64_t)(num_pages * Hkv * (D / 64))};
-  cuuint64_t strides[2] = {128, (cuuint64_t)page_size * 128};
-  cuuint32_t box[3] = {64, (cuuint32_t)(page_size < 64 ? page_size : 64), 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    fprintf(stderr, "[gllm_b200] KV slab tensor-map encode failed (%d)\n", (int)r);
-    return 1;
-  }
+  if (make_kv_slab_tmap(base, num_pages, Hkv, D, page_size, &m)) return 1;
   cache.emplace(key, m);
   *out = m;
   return 0;
@@ -725,7 +731,7 @@ static int attn_prefill_tc_impl(const void* q, int64_t q_ts, void* out, const vo
                                 const void* q_start, int num_tokens, int num_seqs, int seq_offset, int max_q_len,
                                 int max_blocks, int Hq, int Hkv, int D, int page_size, float scale, int kv_tile,
                                 const void* sink, float softcap, void* stream, int window = 0, int64_t out_ts = 0,
-                                const AttnExtras& ex = AttnExtras()) {
+                                const AttnExtras& ex = AttnExtras(), bool keep_maps = true) {
   if (num_seqs <= 0 || max_q_len <= 0) return 0;
   if ((D != 64 && D != 128) || (kv_tile != 64 && kv_tile != 128) || page_size < 8 || kv_tile % page_size != 0 ||
       q_ts % 8 != 0 || (reinterpret_cast<uintptr_t>(q) & 15) != 0 ||
@@ -734,8 +740,9 @@ static int attn_prefill_tc_impl(const void* q, int64_t q_ts, void* out, const vo
     return 2;
   if (ex.dtab != nullptr && 64 % page_size != 0) return 2;
   CUtensorMap tk, tv;
-  if (get_kv_slab_tmap(k_cache, num_pages, Hkv, D, page_size, &tk)) return 1;
-  if (get_kv_slab_tmap(v_cache, num_pages, Hkv, D, page_size, &tv)) return 1;
+  const auto slab_tmap = keep_maps ? get_kv_slab_tmap : make_kv_slab_tmap;
+  if (slab_tmap(k_cache, num_pages, Hkv, D, page_size, &tk)) return 1;
+  if (slab_tmap(v_cache, num_pages, Hkv, D, page_size, &tv)) return 1;
   TcAttnParams p;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_ts = q_ts;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
@@ -781,6 +788,16 @@ GLLM_EXPORT int gllm_attn_prefill_tc(const void* q, int64_t q_ts, void* out, con
   return attn_prefill_tc_impl(q, q_ts, out, k_cache, v_cache, num_pages, block_table, seq_lens, q_start, num_tokens, num_seqs,
                               seq_offset, max_q_len, max_blocks, Hq, Hkv, D, page_size, scale, kv_tile, nullptr, 0.f,
                               stream);
+}
+
+// the same on keys and values that are there for this call only: tiles of 64 tokens [tiles, Hkv, D / 64, 64, 64] and their table
+// [num_seqs, max_tiles] (the expanded pages of a 4-bit cache)
+GLLM_EXPORT int gllm_attn_prefill_tc_tiles(const void* q, int64_t q_ts, void* out, const void* k_tiles, const void* v_tiles,
+                                           int64_t tiles, const void* table, int max_tiles, const void* seq_lens,
+                                           const void* q_start, int num_tokens, int num_seqs, int max_q_len, int Hq, int Hkv, int D,
+                                           float scale, void* stream) {
+  return attn_prefill_tc_impl(q, q_ts, out, k_tiles, v_tiles, tiles, table, seq_lens, q_start, num_tokens, num_seqs, 0, max_q_len,
+                              max_tiles, Hq, Hkv, D, 64, scale, 64, nullptr, 0.f, stream, 0, 0, AttnExtras(), false);
 }
 
 // the same causal attention with a per-head softmax sink (null = none) and a tanh cap on the scaled scores

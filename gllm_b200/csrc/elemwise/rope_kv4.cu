@@ -1,0 +1,284 @@
+// [per-head q / k RMSNorm] -> RoPE -> keys and values coded in 4 bits into their pages, in one pass over the projection's rows;
+// and the rows of such a cache read back.
+//
+// The cache (layout and rounding: ops/kv4.py): uint8 [pages, Hkv, page_size / 16, 9 D], blocks of 16 tokens: 16 rows of D / 2 bytes,
+// then 16 x D / 64 pairs (scale, low) of bf16. Each 64 dims y of a token's head:
+//   low = min y,  scale = bf16((max y - low) / 15),  code = min(15, rne((y - low) / scale)),  value = code * scale + low.
+// y is rounded to bf16 before it is coded (what a bf16 cache would hold), so low needs no rounding of its own. Many quotients
+// are ties (both sides are multiples of the same power of two), hence the IEEE division: a product with the reciprocal would
+// send them either way.
+//
+// Queries are rotated in place; the rotated keys go to the cache only.
+#include "../common/host_utils.h"
+#include "../common/ptx.cuh"
+#include "rope_common.cuh"
+
+namespace b200 {
+
+namespace {
+
+// where the block of `slot` starts in head 0 of its page, and the row in it; ok: the slot is one of the cache
+struct Kv4Place {
+  size_t block;
+  int row;
+  bool ok;
+};
+__device__ __forceinline__ Kv4Place kv4_place(int slot, int page_size, int64_t pages, int Hkv, int D) {
+  const int page = slot / page_size, off = slot - page * page_size;
+  return Kv4Place{(static_cast<size_t>(page) * Hkv * (page_size / 16) + off / 16) * (9 * D), off % 16, slot >= 0 && page < pages};
+}
+
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Eight bf16 values of a group that eight neighbouring lanes hold: this lane's codes and the group's pair. All lanes of the warp
+// take part. A NaN or an infinity (or a span beyond fp32) makes the scale a NaN, and so every value that is read back.
+__device__ __forceinline__ uint32_t kv4_encode(const uint32_t (&w)[4], uint32_t& pair) {
+  uint32_t lo = min_nan2(min_nan2(w[0], w[1]), min_nan2(w[2], w[3])), hi = max_nan2(max_nan2(w[0], w[1]), max_nan2(w[2], w[3]));
+  lo = min_nan2(lo, __byte_perm(lo, lo, 0x1032));
+  hi = max_nan2(hi, __byte_perm(hi, hi, 0x1032));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    lo = min_nan2(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan2(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const float low = __uint_as_float(lo << 16), high = __uint_as_float(hi << 16);
+  const __nv_bfloat16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f));
+  const float scale = __bfloat162float(scale16);
+  const bool fine = scale <= 3.3895e38f;                 // false for NaN as well
+  pair = (lo & 0xffff0000u) | (fine ? __bfloat16_as_ushort(scale16) : 0x7fffu);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 y = unpack_bf16(w[e]);
+    const float a = __fdiv_rn(__fsub_rn(y.x, low), scale), b = __fdiv_rn(__fsub_rn(y.y, low), scale);
+    codes |= __float2uint_rn(fminf(a, 15.f)) << (8 * e) | __float2uint_rn(fminf(b, 15.f)) << (8 * e + 4);
+  }
+  return fine && scale > 0.f ? codes : 0u;
+}
+
+// A lane holds eight dims of a head, L = D / 8 lanes a head, NB heads a lane group, all loaded before the first is worked on.
+template <int L, int NB>
+__global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const int64_t pages) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int D = 8 * L, G = D / 64, kHeadsPerWarp = 32 / L, kStep = 4 * kHeadsPerWarp;
+  const int t = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int gl = lane % L, e0 = gl * 8;
+  const int half = p.rot >> 1;
+  const int n_qk = p.Hq + p.Hkv, n_heads = n_qk + p.Hkv;
+  const int first = blockIdx.y * (kStep * NB) + warp * kHeadsPerWarp + lane / L;
+  uint8_t* kc = reinterpret_cast<uint8_t*>(p.k_cache);
+  uint8_t* vc = reinterpret_cast<uint8_t*>(p.v_cache);
+
+  uint4 raw[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int hh = first + n * kStep;
+    raw[n] = make_uint4(0u, 0u, 0u, 0u);
+    if (hh < n_heads) {
+      const __nv_bfloat16* src = hh < p.Hq ? p.q + t * p.q_ts + hh * p.q_hs
+                                 : hh < n_qk ? p.k + t * p.k_ts + (hh - p.Hq) * p.k_hs
+                                             : p.v + t * p.v_ts + (hh - n_qk) * p.v_hs;
+      raw[n] = *reinterpret_cast<const uint4*>(src + e0);
+    }
+  }
+  // this lane's rotation row: the pair of element e is (e0 + e) % half (NeoX) or (e0 + e) / 2 (neighbours)
+  float c[8], s[8];
+  const bool in_rot = e0 < p.rot, lo = e0 < half;
+  if (in_rot) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = p.neox ? e0 + e - (lo ? 0 : half) : (e0 + e) >> 1;
+      const int pos = p.sec0 != 0 ? p.positions[mrope_axis(i, p.sec0, p.sec1) * p.pos_stride + t] : p.positions[t];
+      const float* row = p.cos_sin + static_cast<size_t>(pos) * p.rot;
+      c[e] = row[i];
+      s[e] = row[half + i];
+    }
+  }
+  const int dl = half / 8;
+  const int partner = (lane & ~(L - 1)) | ((lo ? gl + dl : gl - dl) & (L - 1));
+  const Kv4Place at = kv4_place(p.slots[t], p.page_size, pages, p.Hkv, D);
+  const size_t head_stride = static_cast<size_t>(p.page_size / 16) * (9 * D);
+  const int group = e0 / 64, unit = (e0 % 64) / 8 * G + group;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int hh = first + n * kStep;
+    const bool is_q = hh < p.Hq, is_qk = hh < n_qk;
+    uint32_t w[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_bf16(w[e]);
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
+    }
+    const __nv_bfloat16* nw = is_q ? p.q_norm_w : p.k_norm_w;
+    if (p.q_norm_w != nullptr || p.k_norm_w != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (is_qk && nw != nullptr) {
+        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+        const uint4 wv = *reinterpret_cast<const uint4*>(nw + e0);
+        const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16(ww[e]);
+          // rounded to bf16 after the norm, as on a bf16 cache
+          x[2 * e] = __bfloat162float(__float2bfloat16(x[2 * e] * inv * f.x));
+          x[2 * e + 1] = __bfloat162float(__float2bfloat16(x[2 * e + 1] * inv * f.y));
+        }
+      }
+    }
+    if (p.rot > 0) {
+      // products and sum rounded one by one: a contraction would turn the last bit of some keys, and with it their codes
+      if (p.neox) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
+        if (in_rot && is_qk) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float a = __fmul_rn(x[e], c[e]), b = __fmul_rn(y[e], s[e]);
+            x[e] = lo ? __fsub_rn(a, b) : __fadd_rn(a, b);
+          }
+        }
+      } else if (in_rot && is_qk) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float a = x[e], b = x[e + 1];
+          x[e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+          x[e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+        }
+      }
+    }
+    if (is_qk) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+    }
+    uint32_t pair;
+    const uint32_t codes = kv4_encode(w, pair);
+    if (hh >= n_heads) continue;
+    if (is_q) {
+      *reinterpret_cast<uint4*>(p.q + t * p.q_ts + hh * p.q_hs + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if (at.ok) {
+      uint8_t* block = (is_qk ? kc + (hh - p.Hq) * head_stride : vc + (hh - n_qk) * head_stride) + at.block;
+      *reinterpret_cast<uint32_t*>(block + at.row * (D / 2) + unit * 4) = codes;
+      if (e0 % 64 == 0) *reinterpret_cast<uint32_t*>(block + 8 * D + (at.row * G + group) * 4) = pair;
+    }
+  }
+}
+
+// Rows of a 4-bit cache as bf16 (code * scale + low, rounded once); a lane makes eight dims. Memory-bound.
+template <int L>
+__global__ void __launch_bounds__(128)
+kv4_rows_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ slots,
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int T, int Hkv, int page_size, int64_t pages) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int D = 8 * L, G = D / 64;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
+  const int64_t row = i / L;                             // token, head, keys or values
+  if (row >= static_cast<int64_t>(T) * Hkv * 2) return;
+  const int unit = static_cast<int>(i % L), group = unit % G, e0 = 64 * group + unit / G * 8;
+  const bool is_v = row >= static_cast<int64_t>(T) * Hkv;
+  const int64_t th = is_v ? row - static_cast<int64_t>(T) * Hkv : row;
+  const int t = static_cast<int>(th / Hkv), h = static_cast<int>(th % Hkv);
+  const Kv4Place at = kv4_place(slots[t], page_size, pages, Hkv, D);
+  uint4 w = make_uint4(0u, 0u, 0u, 0u);
+  if (at.ok) {
+    const uint8_t* block = (is_v ? v_cache : k_cache) + at.block + h * (static_cast<size_t>(page_size / 16) * (9 * D));
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + at.row * (D / 2) + unit * 4);
+    const float2 pair = unpack_bf16(*reinterpret_cast<const uint32_t*>(block + 8 * D + (at.row * G + group) * 4));
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), pair.x, pair.y);
+    w = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  }
+  *reinterpret_cast<uint4*>((is_v ? v_out : k_out) + th * D + e0) = w;
+}
+
+template <int L>
+cudaError_t launch_rope_kv4(const RopeParams& p, int64_t pages, cudaStream_t st) {
+  constexpr int kStep = 4 * (32 / L);
+  const int n_heads = p.Hq + 2 * p.Hkv;
+  // many tokens: four heads a lane, fewer and longer blocks; a decode batch: one, so that it still fills the machine
+  if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 4)
+    return launch_pdl(rope_kv4_kernel<L, 4>, dim3(p.T, (n_heads + 4 * kStep - 1) / (4 * kStep)), dim3(128), 0, st, p, pages);
+  return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages);
+}
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+// As gllm_rope_kv_write, on 4-bit caches of `pages` pages; k is left as it is. Slots outside of the cache are left out. Rows, norm
+// weights and caches on 16-byte boundaries, D 64 or 128, pages of a multiple of 16 tokens, rot a multiple of 16 (of 8 for
+// neighbouring pairs).
+GLLM_EXPORT int gllm_rope_kv4_write(void* q, int64_t q_ts, int64_t q_hs, int Hq, const void* k, int64_t k_ts, int64_t k_hs, int Hkv,
+                                    const void* v, int64_t v_ts, int64_t v_hs, const void* q_norm_w, const void* k_norm_w,
+                                    const void* cos_sin, int D, int rot, int neox, int T, const void* positions,
+                                    const void* slots, float eps, void* k_cache, void* v_cache, int64_t pages, int sec0,
+                                    int sec1, int page_size, int64_t pos_stride, void* stream) {
+  if (T <= 0) return 0;
+  auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || rot < 0 || rot > D || rot % (neox ? 16 : 8) != 0 ||
+      ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs) & 7) != 0 || !al16(q) || !al16(k) || !al16(v) || !al16(q_norm_w) ||
+      !al16(k_norm_w) || !al16(k_cache) || !al16(v_cache)) {
+    fprintf(stderr, "[gllm_b200] rope_kv4_write: unsupported D=%d rot=%d page_size=%d, or rows off 16-byte boundaries\n", D, rot,
+            page_size);
+    return 1;
+  }
+  RopeParams p;
+  p.q = reinterpret_cast<__nv_bfloat16*>(q); p.q_ts = q_ts; p.q_hs = q_hs; p.Hq = Hq;
+  p.k = const_cast<__nv_bfloat16*>(reinterpret_cast<const __nv_bfloat16*>(k)); p.k_ts = k_ts; p.k_hs = k_hs; p.Hkv = Hkv;
+  p.v = reinterpret_cast<const __nv_bfloat16*>(v); p.v_ts = v_ts; p.v_hs = v_hs;
+  p.q_norm_w = reinterpret_cast<const __nv_bfloat16*>(q_norm_w);
+  p.k_norm_w = reinterpret_cast<const __nv_bfloat16*>(k_norm_w);
+  p.cos_sin = reinterpret_cast<const float*>(cos_sin);
+  p.D = D; p.rot = rot; p.neox = neox; p.T = T;
+  p.positions = reinterpret_cast<const int32_t*>(positions);
+  p.slots = reinterpret_cast<const int32_t*>(slots);
+  p.eps = eps;
+  p.k_cache = reinterpret_cast<__nv_bfloat16*>(k_cache);
+  p.v_cache = reinterpret_cast<__nv_bfloat16*>(v_cache);
+  p.sec0 = sec0; p.sec1 = sec1; p.page_size = page_size; p.pos_stride = pos_stride;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  CUDA_CHECK_RET(D == 64 ? launch_rope_kv4<8>(p, pages, st) : launch_rope_kv4<16>(p, pages, st));
+  return 0;
+}
+
+// k_out, v_out [T, Hkv, D] bf16: what the caches hold at `slots`; zeros for slots outside of the cache
+GLLM_EXPORT int gllm_kv4_rows(const void* k_cache, const void* v_cache, const void* slots, void* k_out, void* v_out, int T, int Hkv,
+                              int D, int page_size, int64_t pages, void* stream) {
+  if (T <= 0) return 0;
+  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0) {
+    fprintf(stderr, "[gllm_b200] kv4_rows: unsupported D=%d page_size=%d\n", D, page_size);
+    return 1;
+  }
+  const int64_t blocks = (static_cast<int64_t>(T) * Hkv * 2 * (D / 8) + 127) / 128;
+  if (blocks > 0x7fffffff) {
+    fprintf(stderr, "[gllm_b200] kv4_rows: %lld blocks\n", static_cast<long long>(blocks));
+    return 1;
+  }
+  CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_rows_kernel<8> : kv4_rows_kernel<16>, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
+                            reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint8_t*>(k_cache),
+                            reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(slots),
+                            reinterpret_cast<__nv_bfloat16*>(k_out), reinterpret_cast<__nv_bfloat16*>(v_out), T, Hkv, page_size,
+                            pages));
+  return 0;
+}

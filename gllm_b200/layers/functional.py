@@ -9,12 +9,17 @@ from typing import Optional
 
 import torch
 
-from gllm_b200.ops import ref
+from gllm_b200.ops import kv4, ref
 
 
 def _sm():
     from gllm_b200.ops import sm100
     return sm100
+
+
+def _kv4():
+    from gllm_b200.ops import sm100_kv4
+    return sm100_kv4
 
 
 def linear(x, w, bias=None, out=None):
@@ -115,7 +120,12 @@ def gather_rows(src, idx):
 
 def rope_kv_write(q, k, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w, eps, k_cache, v_cache, slots,
                   mrope_section=None):
+    """Per-head norm and rotation of q and k in place, keys and values into their pages. Caches held in 4 bits (uint8, layout:
+    `ops.kv4`) take the keys and values coded; k itself then stays as it is."""
     if q.is_cuda:
+        if kv4.held(k_cache):
+            return _kv4().rope_kv_write(q, k, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w, eps, k_cache, v_cache, slots,
+                                        mrope_section)
         return _sm().rope_kv_write(q, k, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w, eps, k_cache,
                                    v_cache, slots, mrope_section)
     return ref.rope_kv_write(q, k, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w, eps, k_cache,
@@ -123,7 +133,12 @@ def rope_kv_write(q, k, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w
 
 
 def paged_attention(q, k_cache, v_cache, inp, scale, num_q_heads, head_dim):
-    """`inp` is the worker's InputData (device batch state)."""
+    """`inp` is the worker's InputData (device batch state). The caches may be held in 4 bits."""
+    if q.is_cuda and kv4.held(k_cache):
+        lens = inp.batch.seq_lens if inp.batch is not None and not inp.padded_tokens else None
+        return _kv4().paged_attention(q, k_cache, v_cache, inp.block_table, inp.seq_lens, inp.query_start_loc, scale,
+                                      num_q_heads, head_dim, inp.padded_tokens or inp.num_decode_seqs,
+                                      inp.padded_tokens or inp.num_seqs, inp.max_q_len, inp.max_seq_len, host_lens=lens)
     if q.is_cuda:
         return _sm().paged_attention(q, k_cache, v_cache, inp.block_table, inp.seq_lens, inp.query_start_loc, scale,
                                      num_q_heads, head_dim, inp.padded_tokens or inp.num_decode_seqs,
@@ -131,6 +146,14 @@ def paged_attention(q, k_cache, v_cache, inp, scale, num_q_heads, head_dim):
                                      splits=inp.decode_splits)
     return ref.paged_attention(q, k_cache, v_cache, inp.block_table, inp.seq_lens, inp.query_start_loc, scale,
                                num_q_heads, head_dim)
+
+
+def kv_cache_rows(k_cache, v_cache, slots):
+    """(keys, values) [T, Hkv, D] bf16 that caches held in 4 bits have at `slots`: what `rope_kv_write` put there, as attention
+    sees it. Zeros for slots outside of the cache."""
+    if k_cache.is_cuda:
+        return _kv4().kv_cache_rows(k_cache, v_cache, slots)
+    return tuple(kv4.read_rows(c, slots).to(torch.bfloat16) for c in (k_cache, v_cache))
 
 
 def sample(logits, inp, seen_bits=None, seed=0, step=None):

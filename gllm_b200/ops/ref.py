@@ -13,6 +13,8 @@ from typing import List, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from gllm_b200.ops import kv4
+
 
 def kv_slab(head_dim: int) -> int:
     """Width of the innermost KV-cache slab (64 on the product path)."""
@@ -126,7 +128,13 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], p
                   k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
                   slots: Optional[torch.Tensor], mrope_section=None):
     """In place on q [T,Hq,D] and k [T,Hkv,D] (views allowed): optional per-head RMSNorm, RoPE,
-    then K/V scatter into the paged cache."""
+    then K/V scatter into the paged cache. On 4-bit caches (`ops.kv4`) k stays as it is."""
+    if kv4.held(k_cache):
+        keys = k.clone()
+        rope_kv_write(q, keys, v, positions, cos_sin, rot_dim, neox, q_norm_w, k_norm_w, eps, None, None, None, mrope_section)
+        kv4.write_rows(k_cache, slots, keys)
+        kv4.write_rows(v_cache, slots, v)
+        return
     dt = q.dtype
     qf, kf = q.float(), k.float()
     if q_norm_w is not None:
@@ -166,6 +174,10 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], p
 # ----------------------------------------------------------------------------------------------
 def gather_kv(cache: torch.Tensor, block_row: torch.Tensor, seq_len: int) -> torch.Tensor:
     """-> [seq_len, Hkv, D]"""
+    if kv4.held(cache):
+        page_size = kv4.geometry(cache)[2]
+        at = torch.arange(seq_len, device=cache.device)
+        return kv4.read_rows(cache, block_row.long()[at // page_size] * page_size + at % page_size)
     pages, hkv, nslab, page_size, w = cache.shape
     n_pages = (seq_len + page_size - 1) // page_size
     blk = cache[block_row[:n_pages].long()]  # [n, Hkv, nslab, page, W]

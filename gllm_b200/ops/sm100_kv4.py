@@ -1,0 +1,159 @@
+"""Python front-ends of the 4-bit cache kernels (csrc/elemwise/rope_kv4.cu, csrc/attn/kv4_attention.cu): rotary write, attention, rows
+read back. Layout: `ops.kv4`. Each function validates, allocates its output and its scratch and launches on the current stream; no fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from gllm_b200.ops import kv4, lib as _lib
+from gllm_b200.ops.lib import check, stream_ptr
+from gllm_b200.ops.sm100 import NUM_SMS, _BF16, _count, _p
+
+_DECODE_CTAS = 2 * NUM_SMS           # two fit an SM
+EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at a time (one sequence at least)
+
+
+def _declared():
+    L = _lib.load()
+    if L.gllm_kv4_decode.argtypes is None:
+        P, I, N, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+        L.gllm_rope_kv4_write.argtypes = [P, N, N, I, P, N, N, I, P, N, N, P, P, P, I, I, I, I, P, P, F, P, P, N, I, I, I, N, P]
+        L.gllm_kv4_rows.argtypes = [P, P, P, P, P, I, I, I, I, N, P]
+        L.gllm_kv4_decode_scratch.argtypes, L.gllm_kv4_decode_scratch.restype = [I, I], N
+        L.gllm_kv4_expand.argtypes = [P, P, P, I, P, I, I, I, I, N, N, P, P, P, I, I, P]
+        L.gllm_attn_prefill_tc_tiles.argtypes = [P, N, P, P, P, N, P, I, P, P, I, I, I, I, I, I, F, P]
+        L.gllm_kv4_decode.argtypes = [P, N, P, P, P, N, P, I, P, I, I, I, I, I, F, I, P, N, P]
+    return L
+
+
+def _pair(k_cache, v_cache):
+    geo = kv4.geometry(k_cache)
+    if kv4.geometry(v_cache) != geo:
+        raise ValueError(f"4-bit caches of unequal shape: {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    return geo
+
+
+def _index(t: torch.Tensor, what: str, dims: int = 1):
+    assert t.dtype == torch.int32 and t.dim() == dims and t.stride(-1) == 1, f"{what}: int32, contiguous rows"
+
+
+def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos_sin: Optional[torch.Tensor],
+                  rot_dim: int, neox: bool, q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], eps: float,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, mrope_section=None):
+    """`sm100.rope_kv_write` on 4-bit caches: q [T, Hq, D] is normed and rotated in place; k and v [T, Hkv, D] are read only. Rows (all three
+    may be strided views) lie on 16-byte boundaries; rot_dim is a multiple of 16, of 8 for neighbouring pairs."""
+    pages, heads, page_size, dim = _pair(k_cache, v_cache)
+    t, hq, d = q.shape
+    if v is None or slots is None:
+        raise ValueError("a 4-bit cache is written with keys, values and their slots")
+    assert q.dtype == k.dtype == v.dtype == _BF16 and q.stride(2) == k.stride(2) == v.stride(2) == 1
+    assert d == dim and k.shape == v.shape == (t, heads, d), (q.shape, k.shape, v.shape, tuple(k_cache.shape))
+    _index(slots, "slots")
+    assert slots.shape[0] >= t
+    rot = rot_dim if cos_sin is not None else 0
+    if rot:
+        assert cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1] == rot, (cos_sin.shape, rot)
+    if rot < 0 or rot > d or rot % (16 if neox else 8):
+        raise ValueError(f"a 4-bit cache takes rotations of a multiple of 16 dims (of 8 in neighbouring pairs): got {rot} of {d}")
+    for w in (q_norm_w, k_norm_w):
+        assert w is None or (w.dtype == _BF16 and w.shape == (d,) and w.is_contiguous())
+    rows = [x for x in (q, k, v) if x.numel()]
+    if any(x.data_ptr() % 16 or x.stride(0) % 8 or (x.shape[1] > 1 and x.stride(1) % 8) for x in rows) or \
+            any(w is not None and w.data_ptr() % 16 for w in (q_norm_w, k_norm_w)):
+        raise ValueError("rows and norm weights written to a 4-bit cache must lie on 16-byte boundaries")
+    if t == 0:
+        return
+    sec0 = sec1 = pos_stride = 0
+    if mrope_section is not None and positions.dim() == 2:
+        _index(positions, "positions", 2)
+        if len(mrope_section) > 3 and mrope_section[3]:       # interleaved; otherwise chunks (see sm100.rope_kv_write)
+            sec0, sec1 = -int(mrope_section[1]), int(mrope_section[2])
+        else:
+            sec0, sec1 = int(mrope_section[0]), int(mrope_section[1])
+        pos_stride = positions.stride(0)
+    else:
+        positions = positions[0] if positions.dim() == 2 else positions
+        _index(positions, "positions")
+    hs = [x.stride(1) if x.shape[1] > 1 else d for x in (q, k, v)]
+    check(_declared().gllm_rope_kv4_write(
+        _p(q), q.stride(0), hs[0], hq, _p(k), k.stride(0), hs[1], heads, _p(v), v.stride(0), hs[2], _p(q_norm_w), _p(k_norm_w),
+        _p(cos_sin) if rot else None, d, rot, 1 if neox else 0, t, _p(positions), _p(slots), float(eps), _p(k_cache), _p(v_cache),
+        pages, sec0, sec1, page_size, pos_stride, stream_ptr()), "rope_kv4_write")
+    _count()
+
+
+def kv_cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor):
+    """(keys, values) [T, Hkv, D] bf16 that 4-bit caches hold at `slots`; zeros for slots outside of the cache."""
+    pages, heads, page_size, d = _pair(k_cache, v_cache)
+    _index(slots, "slots")
+    t = slots.shape[0]
+    k, v = (torch.empty(t, heads, d, dtype=_BF16, device=k_cache.device) for _ in range(2))
+    check(_declared().gllm_kv4_rows(_p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), t, heads, d, page_size, pages, stream_ptr()),
+          "kv4_rows")
+    if t:
+        _count()
+    return k, v
+
+
+def expand_rounds(lens, token_bytes: int, limit: int = EXPAND_BYTES):
+    """(first, end, tiles of 64 tokens) of consecutive sequences whose expanded keys and values stay below `limit` bytes together, one
+    sequence at least. lens: their lengths, on the host."""
+    rounds, first, tiles = [], 0, 0
+    for s, n in enumerate(lens):
+        more = (int(n) + 63) // 64
+        if s > first and (tiles + more) * 64 * token_bytes > limit:
+            rounds.append((first, s, tiles))
+            first, tiles = s, 0
+        tiles += more
+    if len(lens) > first:
+        rounds.append((first, len(lens), tiles))
+    return rounds
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    query_start_loc: torch.Tensor, scale: float, num_q_heads: int, head_dim: int, num_decode_seqs: int,
+                    num_seqs: int, max_q_len: int, max_seq_len: int, out: Optional[torch.Tensor] = None, host_lens=None):
+    """`sm100.paged_attention` on 4-bit caches. Decoding sequences read the codes (csrc/attn/kv4_attention.cu). Prompt portions have their
+    sequences' keys and values expanded to bf16 first, EXPAND_BYTES of them at a time, and take the tcgen05 prefill kernel.
+    host_lens: the lengths [num_seqs] on the host; without them every prompt is given room for max_seq_len."""
+    pages, hkv, page_size, d = _pair(k_cache, v_cache)
+    t, hq = q.shape[0], num_q_heads
+    assert q.dtype == _BF16 and q.dim() == 2 and q.shape[1] >= hq * d and q.stride(1) == 1 and d == head_dim and hq % hkv == 0
+    _index(block_table, "block_table", 2)
+    _index(seq_lens, "seq_lens")
+    if q.numel() and (q.data_ptr() % 16 or q.stride(0) % 8):
+        raise ValueError("queries over a 4-bit cache must lie on 16-byte boundaries")
+    if out is None:
+        out = torch.empty(t, hq * d, dtype=_BF16, device=q.device)
+    assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
+    L, st, dev = _declared(), stream_ptr(), q.device
+    if num_decode_seqs > 0:
+        assert block_table.shape[0] >= num_decode_seqs and seq_lens.shape[0] >= num_decode_seqs and t >= num_decode_seqs
+        size = L.gllm_kv4_decode_scratch(d, _DECODE_CTAS)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)       # of this call: captured graphs and streams share none
+        check(L.gllm_kv4_decode(_p(q), q.stride(0), _p(out), _p(k_cache), _p(v_cache), pages, _p(block_table), block_table.stride(0),
+                                _p(seq_lens), num_decode_seqs, hq, hkv, d, page_size, float(scale), _DECODE_CTAS, _p(scratch), size,
+                                st), "kv4_decode")
+        _count(2)
+    prompts = num_seqs - num_decode_seqs
+    if prompts > 0 and max_q_len > 0:
+        _index(query_start_loc, "query_start_loc")
+        lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
+        for first, end, tiles in expand_rounds(lens, 4 * hkv * d):
+            if tiles == 0:
+                continue
+            a, n = num_decode_seqs + first, end - first
+            longest = int(max(lens[first:end]))
+            k, v = (torch.empty(tiles, hkv, d // 64, 64, 64, dtype=_BF16, device=dev) for _ in range(2))
+            max_tiles = (longest + 63) // 64
+            table = torch.empty(n, max_tiles, dtype=torch.int32, device=dev)
+            check(L.gllm_kv4_expand(_p(k_cache), _p(v_cache), _p(block_table[a:]), block_table.stride(0), _p(seq_lens[a:]), n, hkv, d,
+                                    page_size, pages, tiles, _p(k), _p(v), _p(table), max_tiles, longest, st), "kv4_expand")
+            check(L.gllm_attn_prefill_tc_tiles(_p(q), q.stride(0), _p(out), _p(k), _p(v), tiles, _p(table), max_tiles, _p(seq_lens[a:]),
+                                               _p(query_start_loc[a:]), t, n, max_q_len, hq, hkv, d, float(scale), st),
+                  "attn_prefill_tc_tiles")
+            _count(2)
+    return out
