@@ -12,6 +12,9 @@
 // CTAs took 3.2 us for 128 rows (and a barrier before it, because they land where the ring was); being read they take 2.1.
 //
 // Roles: warp 0 copies, warp 1 issues the products, warps 2-9 bring the sums from TMEM to shared memory; all add.
+//
+// With INT8 the operands are signed bytes, 128 of K in a block of 128 bytes, and the parts' sums integers: exact whatever their order.
+// The scales of rows and columns come in with the rounding (gemm_int8.cu has the rest of that product).
 #include <mutex>
 
 #include "../common/bounded.cuh"
@@ -23,11 +26,12 @@ namespace b200 {
 
 namespace {
 
-constexpr int kCW = 128, kCK = 64;                       // weight rows of a tile, depth of a K block (128 bytes)
+constexpr int kCW = 128, kCBytes = 128;                  // weight rows of a tile, bytes of a row's K block
 constexpr int kCEpi = 8, kCThreads = (2 + kCEpi) * 32;
 
 struct ClusterParams {
   ClusterGemm g;
+  const float *a_scale, *w_scale;                        // INT8
   WaitConfig waits;
   int bt, tiles_n, stages;                               // rows of A per tile (a multiple of 16), tiles across N, stages of the ring
   uint32_t tmem_cols;
@@ -49,9 +53,10 @@ struct Most {
   static constexpr int value = N;
 };
 
-template <bool GATED>
+template <bool GATED, bool INT8>
 __global__ void __launch_bounds__(kCThreads, 2)
-gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const ClusterParams p) {
+gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const ClusterParams p) {
+  constexpr int kCK = INT8 ? kCBytes : kCBytes / 2;      // values of a K block
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // barriers first: what follows is the ring, and the sums where the ring has been
@@ -63,7 +68,7 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   uint8_t* ring = smem + 1024;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int S = p.stages, BT = p.bt, stage_bytes = kCW * kCK * 2 + BT * kCK * 2;
+  const int S = p.stages, BT = p.bt, stage_bytes = (kCW + BT) * kCBytes;
   const uint32_t C = cluster_size(), rank = cluster_ctarank();
   const int tile = blockIdx.x / C, tn = tile % p.tiles_n, m0 = tile / p.tiles_n * BT;
   const int num_kb = (p.g.K + kCK - 1) / kCK;
@@ -88,10 +93,10 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     if (lane == 0) {
       auto load_w = [&](int i, int kb) {
         uint8_t* dst = ring + i * stage_bytes;
-        if constexpr (GATED) {                           // 64 gate rows, then their up rows; blocks of 128 alternate in the weight
-          const int f = tn * 64, row = f / 128 * 256 + f % 128;
+        if constexpr (GATED) {                           // 64 gate rows, then their up rows; blocks of 128 alternate in a bf16 weight
+          const int f = tn * 64, row = INT8 ? f : f / 128 * 256 + f % 128, up = row + (INT8 ? p.g.N / 2 : 128);
           tma_load_2d(dst, &tmap_w, &full_bar[i], kb * kCK, row, kEvictFirst);
-          tma_load_2d(dst + 64 * kCK * 2, &tmap_w, &full_bar[i], kb * kCK, row + 128, kEvictFirst);
+          tma_load_2d(dst + 64 * kCBytes, &tmap_w, &full_bar[i], kb * kCK, up, kEvictFirst);
         } else {
           tma_load_2d(dst, &tmap_w, &full_bar[i], kb * kCK, tn * kCW, kEvictFirst);
         }
@@ -111,7 +116,7 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
           mbar_expect_tx(&full_bar[s], stage_bytes);
           load_w(s, kb0 + it);
         }
-        tma_load_2d(ring + s * stage_bytes + kCW * kCK * 2, &tmap_x, &full_bar[s], (kb0 + it) * kCK, m0, kEvictLast);
+        tma_load_2d(ring + s * stage_bytes + kCW * kCBytes, &tmap_x, &full_bar[s], (kb0 + it) * kCK, m0, kEvictLast);
       }
       // copies in flight land before the sums take their place, whichever role gave up
       for (int i = max(0, it - S); i < it; ++i) guard.land(&full_bar[i % S], (i / S) & 1);
@@ -119,7 +124,7 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   } else if (warp == 1) {
     griddep_wait();                                      // A is copied behind it: the limit of the waits does not count the kernel before
     if (lane == 0) {
-      const uint32_t idesc = make_idesc_bf16(kCW, BT);
+      const uint32_t idesc = INT8 ? make_idesc_s8(kCW, BT) : make_idesc_bf16(kCW, BT);
       bool ok = guard.first(&full_bar[0]);
       for (int it = 0; it < kb1 - kb0 && ok; ++it) {
         const int s = it % S;
@@ -127,10 +132,12 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         if (!ok) break;
         tc_fence_after();
         const uint32_t w_addr = smem_u32(ring + s * stage_bytes);
-        const uint64_t dw = make_sw128_kmajor_desc(w_addr), dx = make_sw128_kmajor_desc(w_addr + kCW * kCK * 2);
+        const uint64_t dw = make_sw128_kmajor_desc(w_addr), dx = make_sw128_kmajor_desc(w_addr + kCW * kCBytes);
 #pragma unroll
-        for (int k = 0; k < kCK / 16; ++k)
-          umma_bf16<1>(tmem, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, (it | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < kCBytes / 32; ++k) {
+          if constexpr (INT8) umma_s8(tmem, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, (it | k) != 0 ? 1u : 0u);
+          else umma_bf16<1>(tmem, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, (it | k) != 0 ? 1u : 0u);
+        }
         umma_commit(&empty_bar[s]);
       }
       umma_commit(done);                                 // every product has finished: the ring is free
@@ -191,12 +198,29 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
 #pragma unroll
           for (int r = 1; r < P; ++r)
             if (r < static_cast<int>(C)) {
-              x[u][v][0].x += x[u][v][r].x; x[u][v][0].y += x[u][v][r].y;
-              x[u][v][0].z += x[u][v][r].z; x[u][v][0].w += x[u][v][r].w;
+              if constexpr (INT8) {
+                auto sum = [](float& a, float b) { a = __int_as_float(__float_as_int(a) + __float_as_int(b)); };
+                sum(x[u][v][0].x, x[u][v][r].x); sum(x[u][v][0].y, x[u][v][r].y);
+                sum(x[u][v][0].z, x[u][v][r].z); sum(x[u][v][0].w, x[u][v][r].w);
+              } else {
+                x[u][v][0].x += x[u][v][r].x; x[u][v][0].y += x[u][v][r].y;
+                x[u][v][0].z += x[u][v][r].z; x[u][v][0].w += x[u][v][r].w;
+              }
             }
         float y[4] = {x[u][0][0].x, x[u][0][0].y, x[u][0][0].z, x[u][0][0].w};
+        float up[4] = {x[u][V - 1][0].x, x[u][V - 1][0].y, x[u][V - 1][0].z, x[u][V - 1][0].w};
+        if constexpr (INT8) {
+          const float wy = col0 + w < out_N ? p.w_scale[col0 + w] : 0.f;
+          [[maybe_unused]] const float wu = GATED && col0 + w < out_N ? p.w_scale[out_N + col0 + w] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int m = m0 + (my_lo + f) * 4 + e;
+            const float as = m < p.g.M ? p.a_scale[m] : 0.f;
+            y[e] = static_cast<float>(__float_as_int(y[e])) * (as * wy);
+            if constexpr (GATED) up[e] = static_cast<float>(__float_as_int(up[e])) * (as * wu);
+          }
+        }
         if constexpr (GATED) {
-          const float up[4] = {x[u][V - 1][0].x, x[u][V - 1][0].y, x[u][V - 1][0].z, x[u][V - 1][0].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             y[e] = p.g.gelu ? gelu_tanh_fast(y[e]) * up[e] : y[e] / (1.f + __expf(-y[e])) * up[e];
@@ -229,9 +253,9 @@ gemm_bf16_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // ... and they this CTA's
 }
 
-template <bool GATED>
+template <bool GATED, bool INT8>
 int launch_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ClusterParams& p, int tiles, int parts, int smem, cudaStream_t st) {
-  auto kern = gemm_bf16_cluster_kernel<GATED>;
+  auto kern = gemm_cluster_kernel<GATED, INT8>;
   static PerDeviceOnce configured;
   if (configured.need()) {
     CUDA_CHECK_RET(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
@@ -249,12 +273,12 @@ namespace {
 constexpr int kAlone = 220 * 1024, kOfTwo = 108 * 1024, kMostOfTwo = 112 * 1024;
 
 int stages_of(int bt, int smem) {
-  const int n = (smem - 2048) / ((kCW + bt) * kCK * 2);
+  const int n = (smem - 2048) / ((kCW + bt) * kCBytes);
   return n > kClusterStages ? kClusterStages : n;
 }
 // the ring, or the sums and the rounded results that take its place
 int smem_of(int bt, int parts, bool gated, int stages) {
-  const int ring = stages * (kCW + bt) * kCK * 2, most = (bt / 4 + parts - 1) / parts;
+  const int ring = stages * (kCW + bt) * kCBytes, most = (bt / 4 + parts - 1) / parts;
   const int sums = bt * kCW * 4 + most * 4 * ((gated ? 64 : 128) + 8) * 2;
   return (ring > sums ? ring : sums) + 2048;
 }
@@ -323,7 +347,7 @@ const Slots* slots() {                                   // null: not known
 // x 2496, 256 rows 17, here 21; 9664 x 9472 64.7 and 55.7); (f) K in four parts there (4608 x 2368, 128 rows 11.5, here 12.6; 3072 x
 // 8192, 384 rows 25, here 30; with K below 4480 15.9 and 15.3); (g) a short K (11,008 x 960, 128 rows 9.7, here 11.3).
 static bool others_are_faster(int M, int N, int K, int bn, int split, const ClusterPlan& plan, int rounds) {
-  const int tiles_n = (N + kCW - 1) / kCW, sms = num_sms(), num_kb = (K + kCK - 1) / kCK, rows = (M + 127) / 128, spare = rows * 128 - M;
+  const int tiles_n = (N + kCW - 1) / kCW, sms = num_sms(), num_kb = (K + kCBytes / 2 - 1) / (kCBytes / 2), rows = (M + 127) / 128, spare = rows * 128 - M;
   if (M <= 32) return plan.parts == 1 && tiles_n <= sms && tiles_n * 8 > sms * 7;
   if (M <= 256 && ((plan.parts == 1 && M > 48 && spare <= 48) || (rounds > 1 && M > 216 && num_kb <= 48))) return true;
   if (bn == 0) return false;
@@ -334,7 +358,7 @@ static bool others_are_faster(int M, int N, int K, int bn, int split, const Clus
 }
 
 bool plan_gemm_cluster(int M, int N, int K, bool gated, int bn, int split, ClusterPlan* plan) {
-  const int tiles_n = (N + kCW - 1) / kCW, sms = num_sms(), num_kb = (K + kCK - 1) / kCK;
+  const int tiles_n = (N + kCW - 1) / kCW, sms = num_sms(), num_kb = (K + kCBytes / 2 - 1) / (kCBytes / 2);
   if (M > 512 || tiles_n >= 4 * sms) return false;
   if (M > 256 && (gated || N < 2560 || N > 4096 || K < 1536)) return false;
   if (tiles_n * 8 < sms && (M <= 4 || (M <= 8 && K >= 6144))) return false;
@@ -357,7 +381,7 @@ bool plan_gemm_cluster(int M, int N, int K, bool gated, int bn, int split, Clust
         const double ctas = static_cast<double>(tiles < side ? tiles : side) * parts;
         double drawing = per_sm == 1 ? ctas : 1.46 * ctas;                  // SMs that draw on the memory
         if (drawing > sms) drawing = sms;
-        const double copies = static_cast<double>(rounds) * per_sm * ((num_kb + parts - 1) / parts) * ((kCW + bt) * kCK * 2) * 1e-5;
+        const double copies = static_cast<double>(rounds) * per_sm * ((num_kb + parts - 1) / parts) * ((kCW + bt) * kCBytes) * 1e-5;
         const double memory = 2.0 * N * K / 6.36e6 * (1.0 + 0.25 * (sms / drawing - 1.0));
         const double t = (copies > memory ? copies : memory) + rounds * (4.4 + 0.005 * bt) + (parts > 1 ? 0.0026 * bt : 0.0) +
                          (per_sm == 2 ? 0.0018 * bt : 0.0);
@@ -371,23 +395,54 @@ bool plan_gemm_cluster(int M, int N, int K, bool gated, int bn, int split, Clust
   return best < 1e30 && (gated || !others_are_faster(M, N, K, bn, split, *plan, best_rounds));
 }
 
+int cluster_slots(int per_sm, int parts) {
+  const Slots* s = slots();
+  return s == nullptr ? 0 : s->n[per_sm][parts];
+}
+
+int cluster_smem(const ClusterPlan& plan, bool gated) {
+  const int stages = stages_of(plan.bt, plan.smem), smem = smem_of(plan.bt, plan.parts, gated, stages);
+  return stages < 2 || smem > 227 * 1024 ? 0 : smem;
+}
+
+static int set_up(ClusterParams& p, const ClusterPlan& plan, int* tiles) {
+  p.waits = g_wait_config;
+  p.bt = plan.bt;
+  p.tiles_n = (p.g.N + kCW - 1) / kCW;
+  p.stages = stages_of(p.bt, plan.smem);
+  *tiles = (p.g.M + plan.bt - 1) / plan.bt * p.tiles_n;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < static_cast<uint32_t>(p.bt)) p.tmem_cols *= 2;
+  return cluster_smem(plan, p.g.gated);
+}
+
 int gemm_bf16_cluster(const ClusterGemm& g, const ClusterPlan& plan, cudaStream_t st) {
   ClusterParams p;
   p.g = g;
-  p.waits = g_wait_config;
-  const int tiles_m = (g.M + plan.bt - 1) / plan.bt;
-  p.bt = plan.bt;
-  p.tiles_n = (g.N + kCW - 1) / kCW;
-  p.stages = stages_of(p.bt, plan.smem);
-  const int smem = smem_of(p.bt, plan.parts, g.gated, p.stages);
-  if (p.stages < 2 || smem > 227 * 1024) return 1;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < static_cast<uint32_t>(p.bt)) p.tmem_cols *= 2;
+  p.a_scale = p.w_scale = nullptr;
+  int tiles;
+  const int smem = set_up(p, plan, &tiles);
+  if (smem == 0) return 1;
   CUtensorMap tw, tx;
-  if (make_tmap_2d(&tw, g.W, g.N, g.K, g.ldw * 2, g.gated ? 64 : kCW, kCK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
-  if (make_tmap_2d(&tx, g.A, g.M, g.K, g.lda * 2, p.bt, kCK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
-  return g.gated ? launch_cluster<true>(tw, tx, p, tiles_m * p.tiles_n, plan.parts, smem, st)
-                 : launch_cluster<false>(tw, tx, p, tiles_m * p.tiles_n, plan.parts, smem, st);
+  if (make_tmap_2d(&tw, g.W, g.N, g.K, g.ldw * 2, g.gated ? 64 : kCW, kCBytes / 2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
+  if (make_tmap_2d(&tx, g.A, g.M, g.K, g.lda * 2, p.bt, kCBytes / 2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
+  return g.gated ? launch_cluster<true, false>(tw, tx, p, tiles, plan.parts, smem, st)
+                 : launch_cluster<false, false>(tw, tx, p, tiles, plan.parts, smem, st);
+}
+
+int gemm_int8_cluster(const ClusterGemmInt8& g, const ClusterPlan& plan, cudaStream_t st) {
+  ClusterParams p;
+  p.g = g.g;
+  p.a_scale = g.a_scale;
+  p.w_scale = g.w_scale;
+  int tiles;
+  const int smem = set_up(p, plan, &tiles);
+  if (smem == 0) return 1;
+  CUtensorMap tw, tx;
+  if (make_tmap_2d(&tw, p.g.W, p.g.N, p.g.K, p.g.ldw, p.g.gated ? 64 : kCW, kCBytes, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return 1;
+  if (make_tmap_2d(&tx, p.g.A, p.g.M, p.g.K, p.g.lda, p.bt, kCBytes, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return 1;
+  return p.g.gated ? launch_cluster<true, true>(tw, tx, p, tiles, plan.parts, smem, st)
+                   : launch_cluster<false, true>(tw, tx, p, tiles, plan.parts, smem, st);
 }
 
 }  // namespace b200
@@ -400,7 +455,7 @@ GLLM_EXPORT int gllm_gemm_bf16_cluster(const void* A, int64_t lda, const void* W
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   if (K % 8 != 0 || N % 8 != 0 || lda % 8 != 0 || ldw % 8 != 0 || ldc % 8 != 0 || (gated && (N % 256 != 0 || bias != nullptr)) ||
       ((reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(bias)) & 15) != 0 || bt % 16 != 0 || bt < 16 || bt > 256 || parts < 1 ||
-      parts > 8 || parts > (K + kCK - 1) / kCK) {
+      parts > 8 || parts > (K + kCBytes / 2 - 1) / (kCBytes / 2)) {
     fprintf(stderr, "[gllm_b200] gemm_bf16_cluster: M=%d N=%d K=%d with %d rows, %d parts\n", M, N, K, bt, parts);
     return 1;
   }

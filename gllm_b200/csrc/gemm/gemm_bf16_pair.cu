@@ -12,6 +12,9 @@
 // round out, and pairs that walk K out of step no longer share their reads of L2. 8192 x 16384 x 4096: 716 us, on single SMs 808;
 // 4096 x 6144 x 4096: 141 / 151; 8192 x 8192 x 256: 50 / 82 (with four warps to drain TMEM 58).
 //
+// With INT8 the operands are signed bytes (128 of K in a block of 128 bytes, twice the operations a block) and the sums integers; the scales of
+// rows and columns come in with the rounding (gemm_int8.cu has the rest of that product).
+//
 // Roles per CTA: warp 0 copies (both CTAs; every byte is counted by the leader's barrier of the stage), warp 1 issues products
 // (leader only) and commits to both CTAs' barriers, warps 2-9 drain TMEM (each CTA its own rows). Sums are double buffered: the
 // epilogue of a tile overlaps the products of the next.
@@ -26,16 +29,17 @@ namespace b200 {
 
 namespace {
 
-constexpr int kPBK = 64;             // 64 bf16 = 128 B = one swizzle atom row
+constexpr int kPBytes = 128;         // bytes of a row's K block: one swizzle atom row
 constexpr int kPEpi = 8;             // warps that drain TMEM
 constexpr int kPThreads = (2 + kPEpi) * 32;
 constexpr int kPBN = 256;            // columns of a tile (192: the same time per tile, 128: 1.6 times the time per column)
 constexpr int kPStages = 6;
-constexpr int kPABytes = 128 * kPBK * 2, kPStage = kPABytes + kPBN / 2 * kPBK * 2;
+constexpr int kPABytes = 128 * kPBytes, kPStage = kPABytes + kPBN / 2 * kPBytes;
 constexpr int kPSmem = kPStages * kPStage + 1024 + 256 + kPEpi * 4096;
 
 struct PairParams {
   PairGemm g;
+  const float *a_scale, *w_scale;    // INT8
   WaitConfig waits;
   int num_m, num_n;                  // tiles down, across
 };
@@ -50,10 +54,11 @@ __device__ __forceinline__ void tile_at(const PairParams& p, int t, int& mt, int
   mt = sweep * kSweep + r - nt * rows;
 }
 
-template <bool GATED>
+template <bool GATED, bool INT8>
 __global__ void __launch_bounds__(kPThreads, 1)
-gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const PairParams p) {
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const PairParams p) {
   constexpr int BN = kPBN, S = kPStages;
+  constexpr int kPBK = INT8 ? kPBytes : kPBytes / 2;     // values of a K block
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * kPStage);
@@ -92,6 +97,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_smem;
 
+  // this CTA's half of the tile's weight rows: gates and ups where an 8-bit weight is [gate rows ; up rows]
+  auto w_row = [&](int nt) {
+    return GATED && INT8 ? nt * (BN / 2) + static_cast<int>(rank) * (N / 2) : nt * BN + static_cast<int>(rank) * (BN / 2);
+  };
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0, pre = 0;
@@ -104,13 +113,13 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         for (uint32_t i = 0; i < pre; ++i) {
           if (rank == 0) mbar_expect_tx(&full_bar[i], 2 * kPStage);
           tma_load_2d_pair(smem + i * kPStage + kPABytes, &tmap_b, cluster_addr(&full_bar[i], 0),
-                           static_cast<int>(i) * kPBK, nt * BN + static_cast<int>(rank) * (BN / 2), kEvictNormal);
+                           static_cast<int>(i) * kPBK, w_row(nt), kEvictNormal);
         }
       }
       griddep_wait();
       for (int t = pair; t < num_tiles && ok; t += pairs) {
         tile_at(p, t, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * 128, n0 = nt * BN + static_cast<int>(rank) * (BN / 2);
+        const int m0 = mt * 256 + static_cast<int>(rank) * 128, n0 = w_row(nt);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
           const int s = it % S;
           uint8_t* sa = smem + s * kPStage;
@@ -155,7 +164,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   } else if (warp == 1) {
     griddep_wait();                                      // A is copied behind it: the limit of the waits does not count the kernel before
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16(256, BN);
+      constexpr uint32_t idesc = INT8 ? make_idesc_s8(256, BN) : make_idesc_bf16(256, BN);
       uint32_t it = 0, n = 0;
       bool ok = guard.first(&full_bar[0]);
       for (int t = pair; t < num_tiles && ok; t += pairs, ++n) {
@@ -171,8 +180,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           const uint32_t a_addr = smem_u32(smem + s * kPStage);
           const uint64_t da = make_sw128_kmajor_desc(a_addr), db = make_sw128_kmajor_desc(a_addr + kPABytes);
 #pragma unroll
-          for (int k = 0; k < kPBK / 16; ++k)
-            umma_bf16_pair(d_tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < kPBytes / 32; ++k) {
+            if constexpr (INT8) umma_s8_pair(d_tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            else umma_bf16_pair(d_tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          }
           umma_commit_pair(&empty_bar[s]);
         }
         if (ok) umma_commit_pair(&tmem_full[buf]);
@@ -206,6 +217,20 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         give_back();
         continue;
       }
+      const float a_scale = INT8 && row0 + lane < M ? p.a_scale[row0 + lane] : 0.f;      // of this lane's row
+      // eight sums as they are in TMEM, in fp32; w: the scales of their columns (a multiple of 8 of them is there)
+      auto sums8 = [&](const uint32_t* v, const float* w, bool in, float (&f)[8]) {
+        if constexpr (INT8) {
+          float4 s[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+          if (in) { s[0] = *reinterpret_cast<const float4*>(w); s[1] = *reinterpret_cast<const float4*>(w + 4); }
+          const float c[8] = {s[0].x, s[0].y, s[0].z, s[0].w, s[1].x, s[1].y, s[1].z, s[1].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(static_cast<int>(v[e])) * (a_scale * c[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[e]);
+        }
+      };
       // 32 rows x 64 columns at a time through shared memory, so that every store instruction writes whole 128-byte rows
       auto put = [&](int ch, const float (&f)[8]) {      // eight columns of this lane's row
         *reinterpret_cast<uint4*>(stg + lane * 128 + ((ch ^ (lane & 7)) * 16)) =
@@ -225,8 +250,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             for (int j = 0; j < 32; j += 8) {
               const int col = col0 + c + h * 32 + j;
               float f[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[h][j + e]);
+              sums8(&v[h][j], p.w_scale + col, col < out_N, f);
               if (p.g.bias != nullptr && col < out_N) {
                 const uint4 bv = *reinterpret_cast<const uint4*>(p.g.bias + col);
                 const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
@@ -250,10 +274,13 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             if (c + h + 32 >= (half + 1) * (OUT / 2)) give_back();
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
-              float f[8];
+              const int col = col0 + c + h + j;
+              float f[8], gf[8], uf[8];
+              sums8(&g[j], p.w_scale + col, col < out_N, gf);
+              sums8(&u[j], p.w_scale + out_N + col, col < out_N, uf);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float gv = __uint_as_float(g[j + e]), uv = __uint_as_float(u[j + e]);
+                const float gv = gf[e], uv = uf[e];
                 if (p.g.glu_limit > 0.f) {
                   const float gc = fminf(gv, p.g.glu_limit), uc = fminf(fmaxf(uv, -p.g.glu_limit), p.g.glu_limit);
                   f[e] = gc / (1.0f + __expf(-p.g.glu_alpha * gc)) * (uc + 1.0f);
@@ -289,9 +316,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   }
 }
 
-template <bool GATED>
+template <bool GATED, bool INT8>
 int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, PairParams p, cudaStream_t st) {
-  auto kern = gemm_bf16_pair_kernel<GATED>;
+  auto kern = gemm_pair_kernel<GATED, INT8>;
   static PerDeviceOnce configured;
   if (configured.need()) {
     CUDA_CHECK_RET(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem));
@@ -309,11 +336,24 @@ int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, PairParams p, cuda
 int gemm_bf16_pair(const PairGemm& g, cudaStream_t st) {
   PairParams p;
   p.g = g;
+  p.a_scale = p.w_scale = nullptr;
   p.waits = g_wait_config;
   CUtensorMap ta, tb;
-  if (make_tmap_2d(&ta, g.A, g.M, g.K, g.lda * 2, 128, kPBK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
-  if (make_tmap_2d(&tb, g.W, g.N, g.K, g.ldw * 2, kPBN / 2, kPBK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
-  return g.gated ? launch_pair<true>(ta, tb, p, st) : launch_pair<false>(ta, tb, p, st);
+  if (make_tmap_2d(&ta, g.A, g.M, g.K, g.lda * 2, 128, kPBytes / 2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
+  if (make_tmap_2d(&tb, g.W, g.N, g.K, g.ldw * 2, kPBN / 2, kPBytes / 2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)) return 1;
+  return g.gated ? launch_pair<true, false>(ta, tb, p, st) : launch_pair<false, false>(ta, tb, p, st);
+}
+
+int gemm_int8_pair(const PairGemmInt8& g, cudaStream_t st) {
+  PairParams p;
+  p.g = g.g;
+  p.a_scale = g.a_scale;
+  p.w_scale = g.w_scale;
+  p.waits = g_wait_config;
+  CUtensorMap ta, tb;
+  if (make_tmap_2d(&ta, p.g.A, p.g.M, p.g.K, p.g.lda, 128, kPBytes, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return 1;
+  if (make_tmap_2d(&tb, p.g.W, p.g.N, p.g.K, p.g.ldw, kPBN / 2, kPBytes, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return 1;
+  return p.g.gated ? launch_pair<true, true>(ta, tb, p, st) : launch_pair<false, true>(ta, tb, p, st);
 }
 
 }  // namespace b200

@@ -30,6 +30,21 @@ struct ClusterPlan {
 // would take instead (0: not that kernel).
 bool plan_gemm_cluster(int M, int N, int K, bool gated, int bn, int split, ClusterPlan* plan);
 
+// Clusters of `parts` CTAs, one or two CTAs per SM, that this device runs side by side (0: not known).
+int cluster_slots(int per_sm, int parts);
+
+// The 8-bit product of gemm_int8.cu in this form: K is counted in bytes, the leading dimensions are multiples of 16; scales per row of A [M] and
+// of W [N]. Gated: the weight is [gate rows ; up rows].
+struct ClusterGemmInt8 {
+  ClusterGemm g;
+  const float *a_scale, *w_scale;
+};
+
+// 0: launched
+int gemm_int8_cluster(const ClusterGemmInt8& g, const ClusterPlan& plan, cudaStream_t st);
+// the shared memory that a plan takes (0: none of the sizes in `plan` fit)
+int cluster_smem(const ClusterPlan& plan, bool gated);
+
 // 0: launched
 int gemm_bf16_cluster(const ClusterGemm& g, const ClusterPlan& plan, cudaStream_t st);
 

@@ -1,0 +1,153 @@
+// Products in 8-bit integers with a scale per token and per output channel:
+//
+//   a_t = max_k |x_tk|,  X_tk = rne(127 x_tk / a_t),  y_tn = (a_t / 127) s_n sum_k X_tk W_nk (+ b_n)  -> bf16
+//
+// x bf16, W int8 with fp32 scales s; gated: W = [gate rows ; up rows] and y = silu(gate) * up. The sums are int32, exact for K up to
+// 131,072 (127 x 128 x K < 2^31); scales, bias and gate are fp32, and y is rounded once.
+//
+// Two launches: the rows are quantised (here), then multiplied on the tensor cores (tcgen05.mma kind::i8) by one of two kernels:
+// prompts on pairs of SMs (gemm_bf16_pair.cu), decode batches with K cut over a cluster (gemm_bf16_cluster.cu), which copies its first
+// weights while the rows are quantised. `gllm_linear_int8` chooses by what their time is made of.
+#include "../common/host_utils.h"
+#include "../common/ptx.cuh"
+#include "gemm_cluster.h"
+#include "gemm_pair.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr float kQuantFloor = 7.888609052210118e-31f;    // 2^-100: rows below it become zeros
+
+// the larger of two pairs of magnitudes, as bits: NaN is above infinity
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
+
+// Eight bytes from eight bf16. The quotient 127 x / a is x / (a / 127) to the nearest, ties to even, as in exact arithmetic: its
+// estimate by the reciprocal is off by one only next to a tie, which the remainder shows (t - q a / 128 is exact: 15 bits each).
+__device__ __forceinline__ uint2 quant8(const uint4& raw, float a, float inv) {
+  constexpr float kMagic = 12582912.f;                   // 1.5 x 2^23: an integer added to it stands in the low bits
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  const float half = a * 0.00390625f;
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = (e & 1 ? __uint_as_float(w[e >> 1] & 0xffff0000u) : __uint_as_float(w[e >> 1] << 16)) * 0.9921875f;      // 127 / 128
+    float m = fmaf(t, inv, kMagic);
+    const float q = m - kMagic, r = fmaf(q * -0.0078125f, a, t);
+    if (fabsf(r) > half || (fabsf(r) == half && (__float_as_uint(m) & 1u))) m += copysignf(1.f, r);
+    b[e] = __float_as_uint(m);
+  }
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+// A row is T threads' (a warp's or a block's), eight values a piece, NV pieces a thread kept in registers; NV = 0: any length, read
+// twice.
+template <int T, int NV>
+__global__ void __launch_bounds__(256)
+int8_quant_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scales, int M, int K) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int kRows = 256 / T;
+  const int row = blockIdx.x * kRows + threadIdx.x / T, at = threadIdx.x % T, pieces = K / 8;
+  const bool in = row < M;
+  const __nv_bfloat16* src = x + static_cast<int64_t>(in ? row : 0) * ldx;
+  uint4 raw[NV > 0 ? NV : 1];
+  uint32_t most = 0;
+  auto take = [&](const uint4& v) { most = max_abs2(max_abs2(max_abs2(max_abs2(most, v.x), v.y), v.z), v.w); };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (in && at + i * T < pieces) raw[i] = *reinterpret_cast<const uint4*>(src + (at + i * T) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) take(raw[i]);
+  } else {
+    for (int i = at; i < pieces; i += T) take(*reinterpret_cast<const uint4*>(src + i * 8));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if constexpr (T > 32) {
+    __shared__ uint32_t part[T / 32];
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T / 32; ++i) most = __vmaxu2(most, part[i]);
+  }
+  if (!in) return;
+  const float found = __uint_as_float(max(most & 0xffffu, most >> 16) << 16);
+  const float a = found < kQuantFloor ? kQuantFloor : found;                 // a NaN stays one
+  const float inv = __fdiv_rn(128.f, a);
+  if (at == 0) scales[row] = __fdiv_rn(a, 127.f);
+  uint8_t* dst = q + static_cast<int64_t>(row) * K;
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at + i * T < pieces) *reinterpret_cast<uint2*>(dst + (at + i * T) * 8) = quant8(raw[i], a, inv);
+  } else {
+    for (int i = at; i < pieces; i += T) *reinterpret_cast<uint2*>(dst + i * 8) = quant8(*reinterpret_cast<const uint4*>(src + i * 8), a, inv);
+  }
+}
+
+int quant_rows(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, float* scales, int M, int K, cudaStream_t st) {
+  auto go = [&](auto kern, int rows) {
+    return launch_pdl(kern, dim3((M + rows - 1) / rows), dim3(256), 0, st, x, ldx, q, scales, M, K);
+  };
+  if (K <= 512) CUDA_CHECK_RET(go(int8_quant_rows_kernel<32, 2>, 8));
+  else if (K <= 1024) CUDA_CHECK_RET(go(int8_quant_rows_kernel<32, 4>, 8));
+  else if (K <= 4096) CUDA_CHECK_RET(go(int8_quant_rows_kernel<256, 2>, 1));
+  else if (K <= 8192) CUDA_CHECK_RET(go(int8_quant_rows_kernel<256, 4>, 1));
+  else if (K <= 16384) CUDA_CHECK_RET(go(int8_quant_rows_kernel<256, 8>, 1));
+  else CUDA_CHECK_RET(go(int8_quant_rows_kernel<256, 0>, 1));
+  return 0;
+}
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+// x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude / 127)
+GLLM_EXPORT int gllm_int8_quant_rows(const void* x, int64_t ldx, void* q, void* scales, int M, int K, void* stream) {
+  if (M <= 0 || K <= 0) return 0;
+  if (K % 16 != 0 || ldx % 8 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) {
+    fprintf(stderr, "[gllm_b200] int8_quant_rows: K %% 16 and rows on 16-byte boundaries required\n");
+    return 1;
+  }
+  return quant_rows(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<uint8_t*>(q), reinterpret_cast<float*>(scales), M,
+                    K, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// y [M, N] (gated: [M, N / 2]) of x [M, K] and W8 [N, K] int8 (contiguous) with w_scale [N]; xq [M, K] and x_scale [M] are scratch.
+// form: 0 = by size, 1 = pairs of SMs, 2 = clusters with bt rows of x a tile and K in `parts` (tests, tuning).
+GLLM_EXPORT int gllm_linear_int8(const void* x, int64_t ldx, void* xq, void* x_scale, const void* W8, const void* w_scale, void* C,
+                                 int64_t ldc, int M, int N, int K, const void* bias, int gated, int form, int bt, int parts, int smem,
+                                 void* stream) {
+  if (M <= 0 || N <= 0) return 0;
+  const int out_N = gated ? N / 2 : N;
+  if (K <= 0 || K % 16 != 0 || K > 131072 || N % 8 != 0 || out_N % 8 != 0 || (gated && (N % 2 != 0 || bias != nullptr)) || ldx % 8 != 0 ||
+      ldc % 8 != 0 || form < 0 || form > 2 ||
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W8) | reinterpret_cast<uintptr_t>(w_scale) |
+        reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(bias)) & 15) != 0 ||
+      (form == 2 && (bt % 16 != 0 || bt < 16 || bt > 256 || parts < 1 || parts > 8 || parts > (K + 127) / 128))) {
+    fprintf(stderr, "[gllm_b200] linear_int8: M=%d N=%d K=%d (K %% 16, K <= 131072, N %% 8, gated N %% 16; 16-byte boundaries)\n", M, N, K);
+    return 1;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (const int rc = quant_rows(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<uint8_t*>(xq),
+                                reinterpret_cast<float*>(x_scale), M, K, st))
+    return rc;
+  const float *as = reinterpret_cast<const float*>(x_scale), *ws = reinterpret_cast<const float*>(w_scale);
+  __nv_bfloat16* c = reinterpret_cast<__nv_bfloat16*>(C);
+  const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(bias);
+  ClusterPlan plan{bt, parts, smem};
+  if (form == 0) {
+    plan = ClusterPlan{(M < 256 ? M + 15 : 256) / 16 * 16, 1, 108 * 1024};
+    form = M <= 256 ? 2 : 1;
+  }
+  if (form == 2)
+    return gemm_int8_cluster(ClusterGemmInt8{ClusterGemm{xq, W8, K, K, c, ldc, M, N, K, b, gated != 0, 0}, as, ws}, plan, st);
+  return gemm_int8_pair(PairGemmInt8{PairGemm{xq, W8, K, K, c, ldc, M, N, K, b, gated, 0.f, 0.f, 0}, as, ws}, st);
+}

@@ -18,6 +18,14 @@ struct PairGemm {
   int gelu;                          // 1: the tanh form of gelu, 0: silu
 };
 
+// The 8-bit product of gemm_int8.cu in this form: leading dimensions in multiples of 16; scales per row of A [M] and of W [N]. Gated: the
+// weight is [gate rows ; up rows].
+struct PairGemmInt8 {
+  PairGemm g;
+  const float *a_scale, *w_scale;
+};
+int gemm_int8_pair(const PairGemmInt8& g, cudaStream_t st);
+
 // Needs K, N and the leading dimensions in multiples of 8, C and bias on 16-byte boundaries.
 int gemm_bf16_pair(const PairGemm& g, cudaStream_t st);
 

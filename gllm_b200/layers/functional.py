@@ -23,7 +23,14 @@ def _kv4():
 
 
 def linear(x, w, bias=None, out=None):
-    if isinstance(w, tuple):  # (e4m3 weight, fp32 block scale_inv): block-scaled fp8 GEMM
+    """x @ w.T (+ bias). A pair as weight: (e4m3 [N, K], fp32 block scale_inv), the block-scaled fp8 product, or (int8 [N, K], fp32 scale
+    [N]), the 8-bit product with a scale per token and output channel."""
+    if isinstance(w, tuple):
+        if w[0].dtype == torch.int8:
+            if x.is_cuda:
+                return _sm().linear_int8(x, w[0], w[1], bias, out=out)
+            y = ref.linear_int8(x, w[0], w[1], bias)
+            return y if out is None else out.copy_(y)
         if x.is_cuda:
             return _sm().linear_fp8_block(x, w[0], w[1], bias, out=out)
         return ref.linear_fp8_block(x, w[0], w[1], bias)
@@ -34,7 +41,13 @@ def linear(x, w, bias=None, out=None):
 
 def linear_silu_mul(x, w_interleaved, out=None, act="silu"):
     """act(gate) * up of one gate / up projection (rows interleaved per 128); `act`: "silu" | "gelu" (tanh form).
-    An fp8 weight is the pair (e4m3 [gate rows ; up rows], scale_inv), not interleaved; silu only."""
+    An fp8 or int8 weight is the pair (e4m3 or int8 [gate rows ; up rows], scales), not interleaved; silu only."""
+    if isinstance(w_interleaved, tuple) and w_interleaved[0].dtype == torch.int8:
+        assert act == "silu"
+        if x.is_cuda:
+            return _sm().linear_int8(x, *w_interleaved, out=out, silu=True)
+        y = ref.linear_int8(x, *w_interleaved, silu=True)
+        return y if out is None else out.copy_(y)
     if isinstance(w_interleaved, tuple):
         assert act == "silu" and out is None
         w8, ws = w_interleaved

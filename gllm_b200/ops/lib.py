@@ -90,6 +90,14 @@ def _declare(lib):
     sig("gllm_fp8_quant_group", [P, L, P, P, I, I, P, P])
     sig("gllm_moe_grouped_gemm_fp8", [P, P, P, P, P, L, I, I, I, I, I, P, P, I, P])
     sig("gllm_set_waits", [P, c_uint32])
+    sig("gllm_int8_quant_rows", [P, L, P, P, I, I, P])
+    sig("gllm_linear_int8", [P, L, P, P, P, P, P, L, I, I, I, P, I, I, I, I, I, P])
+    sig("gllm_rope_kv4_write", [P, L, L, I, P, L, L, I, P, L, L, P, P, P, I, I, I, I, P, P, F, P, P, L, I, I, I, L, P])
+    sig("gllm_kv4_rows", [P, P, P, P, P, I, I, I, I, L, P])
+    sig("gllm_kv4_decode_scratch", [I, I], L)
+    sig("gllm_kv4_decode", [P, L, P, P, P, L, P, I, P, I, I, I, I, I, F, I, P, L, P])
+    sig("gllm_kv4_expand", [P, P, P, I, P, I, I, I, I, L, L, P, P, P, I, I, P])
+    sig("gllm_attn_prefill_tc_tiles", [P, L, P, P, P, L, P, I, P, P, I, I, I, I, I, I, F, P])
     sig("gllm_gemm_fp8_block", [P, P, P, P, P, L, I, I, I, P, I, P])
 
 

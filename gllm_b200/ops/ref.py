@@ -458,6 +458,23 @@ def linear_fp8_block(x: torch.Tensor, w: torch.Tensor, w_scale_inv: torch.Tensor
     return y.to(x.dtype)
 
 
+def int8_quant_rows(x: torch.Tensor):
+    """(int8 [M, K], fp32 scales [M]): the largest magnitude of a row / 127, values to the nearest multiple, ties to even."""
+    a = x.float().abs().amax(1, keepdim=True)
+    q = torch.where(a > 0, torch.round(x.float() * 127 / a), 0.0)
+    return torch.nan_to_num(q).to(torch.int8), (a / 127)[:, 0]
+
+
+def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, silu: bool = False):
+    """8-bit product with a scale per token and output channel; `silu`: w8 is [gate rows ; up rows]."""
+    q, s = int8_quant_rows(x)
+    y = (q.double() @ w8.double().t()).float() * (s[:, None] * w_scale)
+    if silu:
+        gate, up = y.chunk(2, 1)
+        return (F.silu(gate) * up).to(x.dtype)
+    return (y if bias is None else y + bias.float()).to(x.dtype)
+
+
 def merge_attn_states(o1: torch.Tensor, lse1: torch.Tensor, o2: torch.Tensor, lse2: torch.Tensor):
     """LSE-weighted merge of two partial attention results. o [T,H,D], lse [T,H] (natural log)."""
     m = torch.maximum(lse1, lse2)

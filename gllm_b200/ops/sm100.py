@@ -515,6 +515,62 @@ def linear_fp8_block(x: torch.Tensor, w8: torch.Tensor, w_scale_inv: torch.Tenso
 
 
 # ----------------------------------------------------------------------------------------------
+# 8-bit integer products, a scale per token and per output channel
+# ----------------------------------------------------------------------------------------------
+INT8_MOST_K = 131072     # the int32 sums are exact up to here
+
+
+def _int8_rows(x: torch.Tensor):
+    assert x.dtype == _BF16 and x.dim() == 2 and x.stride(1) == 1
+    m, k = x.shape
+    if k % 16 or k == 0 or k > INT8_MOST_K:
+        raise ValueError(f"8-bit products take rows of a multiple of 16 values, at most {INT8_MOST_K}: got {k}")
+    if m and (x.data_ptr() % 16 or x.stride(0) % 8):
+        raise ValueError("rows of an 8-bit product must lie on 16-byte boundaries")
+    return m, k
+
+
+def int8_quant_rows(x: torch.Tensor):
+    """bf16 [M, K] -> (int8 [M, K], fp32 scales [M]): a row's scale is its largest magnitude / 127, values are rounded to the nearest
+    multiple, ties to even. A row that holds a NaN or an infinity has such a scale."""
+    m, k = _int8_rows(x)
+    q = torch.empty(m, k, dtype=torch.int8, device=x.device)
+    s = torch.empty(m, dtype=torch.float32, device=x.device)
+    if m:
+        check(_lib.load().gllm_int8_quant_rows(_p(x), x.stride(0), _p(q), _p(s), m, k, stream_ptr()), "int8_quant_rows")
+        _count()
+    return q, s
+
+
+def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None, silu: bool = False, plan: Optional[tuple] = None) -> torch.Tensor:
+    """x bf16 [M, K] (rows quantised here, `int8_quant_rows`); w8 int8 [N, K], w_scale fp32 [N] -> bf16 [M, N] (+ bias). `silu`: w8 is
+    [gate rows ; up rows] and the result silu(gate) * up [M, N / 2]. `plan`: a form by name (csrc/gemm/gemm_int8.cu) instead of the
+    one chosen by size."""
+    m, k = _int8_rows(x)
+    n = w8.shape[0]
+    assert w8.dtype == torch.int8 and w8.is_contiguous() and w8.shape == (n, k), (w8.dtype, w8.shape, k)
+    assert w_scale.dtype == torch.float32 and w_scale.shape == (n,) and w_scale.is_contiguous()
+    assert bias is None or (bias.dtype == _BF16 and bias.shape == (n,) and bias.is_contiguous())
+    n_out = n // 2 if silu else n
+    if n % 8 or n_out % 8 or n == 0 or (silu and bias is not None):
+        raise ValueError(f"8-bit products take a multiple of 8 columns (gated: of 16, and no bias): got {n}")
+    if out is None:
+        out = torch.empty(m, n_out, dtype=_BF16, device=x.device)
+    assert out.dtype == _BF16 and out.shape == (m, n_out) and out.stride(1) == 1
+    if any(t is not None and t.data_ptr() % 16 for t in (w8, w_scale, bias)) or (m and (out.data_ptr() % 16 or out.stride(0) % 8)):
+        raise ValueError("weights, scales, bias and results of an 8-bit product must lie on 16-byte boundaries")
+    if m == 0:
+        return out
+    scratch = torch.empty(m * k + 4 * m, dtype=torch.uint8, device=x.device)     # k % 16: the scales lie on 16-byte boundaries
+    form, bt, parts, smem = plan or (0, 0, 0, 0)
+    check(_lib.load().gllm_linear_int8(_p(x), x.stride(0), scratch.data_ptr(), scratch.data_ptr() + m * k, _p(w8), _p(w_scale), _p(out),
+                                       out.stride(0), m, n, k, _p(bias), int(silu), form, bt, parts, smem, stream_ptr()), "linear_int8")
+    _count(2)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
 # multi-head latent attention (DeepSeek): absorbed MQA over the paged latent cache
 # ----------------------------------------------------------------------------------------------
 def mla_rope_cache(q_pe: torch.Tensor, q_full: Optional[torch.Tensor], k_pe: torch.Tensor, kv_c: torch.Tensor,

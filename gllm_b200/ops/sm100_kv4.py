@@ -3,7 +3,6 @@ read back. Layout: `ops.kv4`. Each function validates, allocates its output and 
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import torch
@@ -14,19 +13,6 @@ from gllm_b200.ops.sm100 import NUM_SMS, _BF16, _count, _p
 
 _DECODE_CTAS = 2 * NUM_SMS           # two fit an SM
 EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at a time (one sequence at least)
-
-
-def _declared():
-    L = _lib.load()
-    if L.gllm_kv4_decode.argtypes is None:
-        P, I, N, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-        L.gllm_rope_kv4_write.argtypes = [P, N, N, I, P, N, N, I, P, N, N, P, P, P, I, I, I, I, P, P, F, P, P, N, I, I, I, N, P]
-        L.gllm_kv4_rows.argtypes = [P, P, P, P, P, I, I, I, I, N, P]
-        L.gllm_kv4_decode_scratch.argtypes, L.gllm_kv4_decode_scratch.restype = [I, I], N
-        L.gllm_kv4_expand.argtypes = [P, P, P, I, P, I, I, I, I, N, N, P, P, P, I, I, P]
-        L.gllm_attn_prefill_tc_tiles.argtypes = [P, N, P, P, P, N, P, I, P, P, I, I, I, I, I, I, F, P]
-        L.gllm_kv4_decode.argtypes = [P, N, P, P, P, N, P, I, P, I, I, I, I, I, F, I, P, N, P]
-    return L
 
 
 def _pair(k_cache, v_cache):
@@ -78,7 +64,7 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         positions = positions[0] if positions.dim() == 2 else positions
         _index(positions, "positions")
     hs = [x.stride(1) if x.shape[1] > 1 else d for x in (q, k, v)]
-    check(_declared().gllm_rope_kv4_write(
+    check(_lib.load().gllm_rope_kv4_write(
         _p(q), q.stride(0), hs[0], hq, _p(k), k.stride(0), hs[1], heads, _p(v), v.stride(0), hs[2], _p(q_norm_w), _p(k_norm_w),
         _p(cos_sin) if rot else None, d, rot, 1 if neox else 0, t, _p(positions), _p(slots), float(eps), _p(k_cache), _p(v_cache),
         pages, sec0, sec1, page_size, pos_stride, stream_ptr()), "rope_kv4_write")
@@ -91,7 +77,7 @@ def kv_cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
     _index(slots, "slots")
     t = slots.shape[0]
     k, v = (torch.empty(t, heads, d, dtype=_BF16, device=k_cache.device) for _ in range(2))
-    check(_declared().gllm_kv4_rows(_p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), t, heads, d, page_size, pages, stream_ptr()),
+    check(_lib.load().gllm_kv4_rows(_p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), t, heads, d, page_size, pages, stream_ptr()),
           "kv4_rows")
     if t:
         _count()
@@ -129,7 +115,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if out is None:
         out = torch.empty(t, hq * d, dtype=_BF16, device=q.device)
     assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
-    L, st, dev = _declared(), stream_ptr(), q.device
+    L, st, dev = _lib.load(), stream_ptr(), q.device
     if num_decode_seqs > 0:
         assert block_table.shape[0] >= num_decode_seqs and seq_lens.shape[0] >= num_decode_seqs and t >= num_decode_seqs
         size = L.gllm_kv4_decode_scratch(d, _DECODE_CTAS)

@@ -1,0 +1,187 @@
+"""8-bit products with scales per token and output channel against their definition in 64 bits (GPU)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F64 = torch.bfloat16, torch.float64
+DEV = "cuda"
+
+
+def quantised(x):
+    """(whole numbers, unit) per row in 64 bits: x 127 / max to the nearest, ties to even."""
+    x = x.to(F64)
+    a = x.abs().amax(1, keepdim=True)
+    a = torch.where(a == 0, 1.0, a)
+    near = 127 * x.abs() / a                               # 15 by 8 bits: fp64 has every tie exactly
+    return torch.round(near) * x.sign(), a / 127
+
+
+def product(x, w8, ws, bias=None, silu=False):
+    """-> (y, tolerance), fp64. Integer sums are exact; a sum to fp32, the scale of the row, that of the row and column and their
+    product with it are one rounding of 2^-24 each; the bias another. With the gate: those of its two factors (its own slope is at most 1.1,
+    the exponential and the division good to 2^-21), then the result's 2^-8."""
+    q, unit = quantised(x)
+    y = (q @ w8.to(F64).t()) * unit * ws.to(F64)
+    if silu:
+        g, u = y.chunk(2, 1)
+        y = g * torch.sigmoid(g) * u
+        slack = 2 ** -22 * 1.1 * g.abs() * u.abs() + 2 ** -22 * y.abs() + 2 ** -20 * y.abs()
+    else:
+        slack = 2 ** -22 * y.abs()
+        if bias is not None:
+            slack = slack + 2 ** -23 * bias.to(F64).abs()
+            y = y + bias.to(F64)
+    return y, 2 ** -8 * (y.abs() + slack) + slack + 1e-30
+
+
+def _inputs(m, n, k, seed=0):
+    torch.manual_seed(seed + m + n + k)
+    x = (torch.randn(m, k, device=DEV) * (0.05 + 5 * torch.rand(m, 1, device=DEV))).to(BF16)
+    w8 = torch.randint(-128, 128, (n, k), device=DEV, dtype=torch.int8)
+    ws = (0.5 + torch.rand(n, device=DEV)) * 0.01
+    return x, w8, ws
+
+
+@pytest.mark.parametrize("m,k", [(1, 16), (3, 512), (9, 528), (5, 1024), (70, 2048), (2, 4096), (33, 5008), (4, 12288), (3, 28672), (2, 131072)])
+def test_rows_are_quantised_to_the_nearest(m, k):
+    from gllm_b200.ops import sm100
+    torch.manual_seed(k)
+    x = (torch.randn(m, k + 8, device=DEV) * 3).to(BF16)[:, 8:]             # rows of a wider tensor
+    x[0, 0] = 254 * 2.0 ** -4                                               # 127 / 2^k: many quotients are ties
+    x[0, 1:] = torch.randint(-254, 255, (k - 1,), device=DEV).to(BF16) * 2.0 ** -4
+    q, s = sm100.int8_quant_rows(x)
+    want, unit = quantised(x)
+    assert torch.equal(q.to(F64), want)
+    torch.testing.assert_close(s.to(F64), unit[:, 0], rtol=2 ** -24, atol=0)
+
+
+def test_rows_of_zeros_tiny_rows_and_rows_that_are_no_numbers():
+    from gllm_b200.ops import sm100
+    x = torch.randn(6, 64, device=DEV).to(BF16)
+    x[0], x[1] = 0.0, x[1] * 2.0 ** -110
+    x[2, 5], x[3, 9] = float("nan"), float("inf")
+    x[4] *= 2.0 ** 120
+    q, s = sm100.int8_quant_rows(x)
+    assert (q[:2] == 0).all() and torch.isfinite(s[:2]).all() and not torch.isfinite(s[2:4]).any()
+    want, unit = quantised(x[4:])
+    assert torch.equal(q[4:].to(F64), want)
+    w8, ws = torch.ones(16, 64, device=DEV, dtype=torch.int8), torch.ones(16, device=DEV)
+    y = sm100.linear_int8(x, w8, ws)
+    assert (y[:2] == 0).all() and not torch.isfinite(y[2:4]).any() and torch.isfinite(y[4:]).all()
+
+
+SHAPES = [(1, 8, 16), (1, 6144, 4096), (2, 136, 80), (17, 264, 1040), (48, 1024, 4096), (64, 4096, 512), (130, 392, 272), (255, 2048, 1024),
+          (257, 640, 400), (300, 1000, 2064), (777, 1280, 1024), (1030, 520, 144)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_product(m, n, k, with_bias):
+    from gllm_b200.layers import functional as Fn
+    x, w8, ws = _inputs(m, n, k)
+    bias = torch.randn(n, device=DEV).to(BF16) if with_bias else None
+    y = Fn.linear(x, (w8, ws), bias)
+    want, tol = product(x, w8, ws, bias)
+    assert y.dtype == BF16 and ((y.to(F64) - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(m, 2 * n, k) for m, n, k in SHAPES])
+def test_gated_product(m, n, k):
+    from gllm_b200.layers import functional as Fn
+    x, w8, ws = _inputs(m, n, k)
+    ws = ws / k ** 0.5 * 0.3
+    y = Fn.linear_silu_mul(x, (w8, ws))
+    want, tol = product(x, w8, ws, silu=True)
+    assert y.shape == (m, n // 2) and ((y.to(F64) - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("plan", [(1, 0, 0, 0), (2, 16, 1, 108 * 1024), (2, 64, 3, 108 * 1024), (2, 32, 8, 220 * 1024), (2, 256, 2, 220 * 1024),
+                                  (2, 112, 5, 108 * 1024)])
+@pytest.mark.parametrize("silu", [False, True])
+def test_forms_by_name(plan, silu):
+    """Every form at a size that the choice by size would give to another: the same bits, since the sums are integers."""
+    from gllm_b200.ops import sm100
+    x, w8, ws = _inputs(139, 1104, 1168)
+    ws = ws * 0.01
+    y = sm100.linear_int8(x, w8, ws, silu=silu, plan=plan)
+    want, tol = product(x, w8, ws, silu=silu)
+    assert ((y.to(F64) - want).abs() <= tol).all()
+    assert torch.equal(y, sm100.linear_int8(x, w8, ws, silu=silu))
+
+
+@pytest.mark.parametrize("m", [3, 300])
+def test_largest_sums_are_exact(m):
+    """127 x -128 over the longest rows: 2.13e9, next to the end of int32."""
+    from gllm_b200.ops import sm100
+    k = sm100.INT8_MOST_K
+    x = torch.full((m, k), 3.0, device=DEV).to(BF16)
+    w8 = torch.full((16, k), -128, device=DEV, dtype=torch.int8)
+    w8[3] = 127
+    ws = torch.full((16,), 2.0 ** -20, device=DEV)
+    y = sm100.linear_int8(x, w8, ws)
+    want, tol = product(x, w8, ws)
+    assert ((y.to(F64) - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m", [5, 400])
+def test_strided_rows_results_in_place_and_rows_behind(m):
+    from gllm_b200.ops import sm100
+    x, w8, ws = _inputs(m, 264, 256)
+    wide = torch.randn(m, 512, device=DEV).to(BF16)
+    wide[:, 128:384] = x
+    out = torch.full((m + 3, 512), 7.0, dtype=BF16, device=DEV)
+    y = sm100.linear_int8(wide[:, 128:384], w8, ws, out=out[:m, 64:328])
+    want, tol = product(x, w8, ws)
+    assert y.data_ptr() == out[:m, 64:328].data_ptr() and ((y.to(F64) - want).abs() <= tol).all()
+    assert (out[m:] == 7).all() and (out[:, :64] == 7).all() and (out[:, 328:] == 7).all()
+
+
+def test_no_rows():
+    from gllm_b200.ops import sm100
+    _, w8, ws = _inputs(1, 64, 64)
+    assert sm100.linear_int8(torch.empty(0, 64, dtype=BF16, device=DEV), w8, ws).shape == (0, 64)
+    assert sm100.int8_quant_rows(torch.empty(0, 64, dtype=BF16, device=DEV))[0].shape == (0, 64)
+
+
+def test_captured_products_on_two_streams():
+    """Two graphs replayed at once: each has its quantised rows in memory of its own."""
+    from gllm_b200.ops import sm100
+    runs = []
+    for m in (7, 600):
+        x, w8, ws = _inputs(m, 1024, 2048, seed=m)
+        out = torch.empty(m, 1024, dtype=BF16, device=DEV)
+        sm100.linear_int8(x, w8, ws, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            sm100.linear_int8(x, w8, ws, out=out)
+        runs.append((graph, x, w8, ws, out, torch.cuda.Stream()))
+    for turn in range(3):
+        for graph, x, w8, ws, out, stream in runs:
+            x.copy_(torch.randn_like(x.float()).to(BF16))
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, x, w8, ws, out, stream in runs:
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for graph, x, w8, ws, out, stream in runs:
+            want, tol = product(x, w8, ws)
+            assert ((out.to(F64) - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("plan", [(1, 0, 0, 0), (2, 64, 2, 108 * 1024)])
+def test_waits_that_run_out_are_reported(plan):
+    from gllm_b200.ops import lib as _lib, sm100
+    x, w8, ws = _inputs(300, 1024, 4096)
+    assert sm100.waits_given_up() == 0
+    try:
+        _lib.watch_waits(0)
+        sm100.linear_int8(x, w8, ws, plan=plan)
+        torch.cuda.synchronize()
+        assert _lib.waits_gave_up(clear=True)
+    finally:
+        _lib.watch_waits()
+    want, tol = product(x, w8, ws)
+    assert ((sm100.linear_int8(x, w8, ws, plan=plan).to(F64) - want).abs() <= tol).all() and not _lib.waits_gave_up()
