@@ -7,11 +7,12 @@
 // so the codes go into the matrix instructions as they are and scales and low ends stay outside: four fused operations a score, two a
 // probability, instead of one or two for each of the D values of a key.
 //
-// Codes as 16-bit operands: a nibble at bits 0 (or 4) of an fp16 is the subnormal c 2^-24 (or 16 c 2^-24), exact, and the matrix
-// instructions take subnormals: one AND for two codes. Queries are scaled by a power of two to the upper end of fp16 (by a
-// further 1/16 where a nibble stands four bits up); eleven bits hold their eight. The values' codes meet probabilities of any
-// size, so there they are bf16: 0x4300 | c is 128 + c, and 128 times the sum of the (rounded) probabilities, which one more product with
-// ones gives, comes off again at the end: fp32 sums lose 2^-19 of the result to it, rounding the probabilities to bf16 2^-9.
+// Codes as 16-bit operands: a byte of two codes in an fp16 is the subnormal (c0 + 16 c1) 2^-24, and with its lower half cleared 16 c1 2^-24,
+// both exact, and the matrix instructions take subnormals: four ANDs or byte moves for eight codes, and what belongs to c0 alone comes
+// off the other operand (keys: q0 c0 + q1 c1 = q0 b + (q1 / 16 - q0) u, the second factor rounded to 2^-11) or off the sums
+// (values: four of fp32's bits). Queries are scaled by a power of two to the upper end of fp16. Probabilities times scales are rounded to
+// fp16 (2^-11 of each): the exponentials' reference is the head's maximum plus the logarithm of the largest scale met so far, so that
+// they stay below 2^14, and what vanishes below 2^-25 is 2^-32 of the largest that can stand beside it.
 //
 // Keys are the rows of the products (m16n8k16: 16 keys x 8 query heads, then 16 dims x 8 heads), so eight query heads of
 // one kv head fill an instruction. A lane (g, t) = (lane / 4, lane % 4) holds
@@ -25,8 +26,7 @@
 // its tiles in turn and sum up in shared memory where a sequence's head ends; what a share has of a head that goes on in another
 // CTA goes to scratch, and a second kernel joins it.
 //
-// The reference of a head's exponentials follows its maximum only when a score passes it by 2^8 (one vote instead of three
-// shuffles a tile).
+// The reference follows only when a score passes the head's maximum by 2^8 or a scale the largest one (one vote instead of shuffles).
 #include "../common/bounded.cuh"
 #include "attn_common.cuh"
 
@@ -36,7 +36,8 @@ namespace {
 
 constexpr int kV4Warps = 8, kV4Threads = kV4Warps * 32, kV4Keys = 32, kV4Stages = 2;
 constexpr int kV4Lens = 256;                             // lengths that a CTA keeps in shared memory, from its first sequence on
-constexpr float kV4Lazy = 8.f;
+constexpr float kV4Lazy = 8.f;                           // scores pass the maximum that the reference is taken from by no more than this
+constexpr float kV4Room = 6.f;                           // and exponentials times scales stay below 2^(kV4Lazy + kV4Room)
 
 struct Kv4Params {
   const __nv_bfloat16* q;
@@ -44,10 +45,12 @@ struct Kv4Params {
   __nv_bfloat16* out;                                    // [B, Hq, D]
   const uint8_t* k_cache;
   const uint8_t* v_cache;
-  int64_t pages;
+  uint32_t last_page;
   const int32_t* block_table;
   const int32_t* seq_lens;
-  int B, max_blocks, Hq, Hkv, G, GP, page_size;          // GP query heads (at most 8 NT) of the G of a kv head at a time
+  int B, max_blocks, Hq, Hkv, G, GP;                     // GP query heads (at most 8 NT) of the G of a kv head at a time
+  int page_blocks;                                       // blocks of 16 tokens in a page
+  uint32_t page_magic;                                   // floor(b / page_blocks) = umulhi(b, page_magic), exact while b x page_blocks < 2^32 (0: one block)
   float scale_log2;
   float* part_o;                                         // [2 CTAs, 8 NT, D]
   float* part_ml;                                        // [2 CTAs, 8 NT, 2]
@@ -85,12 +88,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -182,81 +179,78 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   __syncthreads();
   auto len_of = [&](int s) { return s - seq0 < kV4Lens ? lens[s - seq0] : p.seq_lens[s]; };
 
-  struct Place {                                         // of a tile in the row
-    int seq, head, tile, n;
-  };
-  const int first_in = static_cast<int>(begin - static_cast<int64_t>(words[2]) * H);
-  Place at;
+  const int first_in = static_cast<int>(begin - static_cast<int64_t>(words[2]) * H), tiles = static_cast<int>(end - begin);
+  const int hg = p.G / p.GP;
+  struct Place {                                         // a head group of a sequence
+    int seq, head, len, n;
+  } at;
   at.seq = seq0;
-  at.n = kv4_tiles(len_of(seq0));
+  at.len = len_of(seq0);
+  at.n = kv4_tiles(at.len);
   at.head = first_in / at.n;
-  at.tile = first_in - at.head * at.n;
-  auto advance = [&](Place& x, int by) {
-    x.tile += by;
-    while (x.tile >= x.n) {
-      x.tile -= x.n;
-      if (++x.head == H) {
-        x.head = 0;
-        if (++x.seq >= p.B) {                            // behind the last tile: never used
-          x.seq = p.B - 1;
-          x.tile = 0;
-          return;
-        }
-        x.n = kv4_tiles(len_of(x.seq));
-      }
-    }
+  int at_tile = first_in - at.head * at.n;               // the first tile of the segment that is worked on
+  auto next_head = [&](Place& x) {                       // behind the last one: never used
+    if (++x.head < H) return;
+    x.head = 0;
+    if (++x.seq >= p.B) return;
+    x.len = len_of(x.seq);
+    x.n = kv4_tiles(x.len);
   };
 
-  // ---- copies: lanes 0-3 have a block each, (keys, values) x 16 tokens
+  // ---- copies. The warp's tiles are the share's warp-th, (warp + 8)-th ...; eight of them are prepared at a time, a block a lane: tile
+  // lane / 4, keys or values, 16 tokens. A table entry that is no page reads another one.
   const uint32_t ring = smem_u32(smem) + warp * (kV4Stages * SM::kStage);
   uint64_t* bar = bars + warp * kV4Stages;
-  const int64_t head_bytes = static_cast<int64_t>(p.page_size / 16) * SM::kBlock;
-  const int hg = p.G / p.GP;
-  auto page_of = [&](const Place& x) {                   // lane's page of this tile; a table entry that is no page reads another one
-    const int tok = x.tile * kV4Keys + (lane & 1) * 16;
-    if (lane >= 4 || tok >= len_of(x.seq)) return 0;
-    return p.block_table[static_cast<size_t>(x.seq) * p.max_blocks + min(tok / p.page_size, p.max_blocks - 1)];
-  };
-  auto issue = [&](const Place& x, int page, int stage) {
-    const int len = len_of(x.seq), blocks = min(2, (len - x.tile * kV4Keys + 15) / 16);
-    if (blocks <= 0) {                                   // an empty sequence
-      if (lane == 0) mbar_arrive(&bar[stage]);
-      return;
+  const uint32_t my_tiles = static_cast<uint32_t>(max(0, (tiles - warp + kV4Warps - 1) / kV4Warps));
+  Place fetch = at;                                      // of this lane's next block
+  int fetch_x = warp + kV4Warps * (lane >> 2), fetch_tile = at_tile + fetch_x;
+  const uint8_t* src = nullptr;
+  int blocks = 0;                                        // of this lane's tile (none: an empty sequence)
+  auto prepare = [&] {
+    while (fetch_tile >= fetch.n && fetch.seq < p.B) {
+      fetch_tile -= fetch.n;
+      next_head(fetch);
     }
-    if (lane == 0) mbar_expect_tx(&bar[stage], blocks * 2 * SM::kBlock);
-    __syncwarp();
-    const int sub = lane & 1;
-    if (lane < 4 && sub < blocks) {
-      const int64_t in_range = min(static_cast<int64_t>(static_cast<uint32_t>(page)), p.pages - 1);
-      const int in_page = (x.tile * kV4Keys + sub * 16) % p.page_size / 16;
-      const uint8_t* src = (lane & 2 ? p.v_cache : p.k_cache) + (in_range * p.Hkv + x.head / hg) * head_bytes + in_page * SM::kBlock;
-      bulk_load(ring + stage * SM::kStage + lane * SM::kBlock, src, SM::kBlock, &bar[stage]);
+    blocks = 0;
+    if (fetch_x < tiles) {
+      const int blk = 2 * fetch_tile + (lane & 1);
+      blocks = min(2, (fetch.len - fetch_tile * kV4Keys + 15) / 16);
+      if ((lane & 1) < blocks) {
+        const int i = p.page_magic != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(blk), p.page_magic)) : blk;
+        const uint32_t page = min(static_cast<uint32_t>(p.block_table[static_cast<size_t>(fetch.seq) * p.max_blocks + min(i, p.max_blocks - 1)]),
+                                  p.last_page);
+        src = (lane & 2 ? p.v_cache : p.k_cache) +
+              ((static_cast<uint64_t>(page) * p.Hkv + fetch.head / hg) * p.page_blocks + (blk - i * p.page_blocks)) * SM::kBlock;
+      }
     }
+    fetch_x += 8 * kV4Warps;
+    fetch_tile += 8 * kV4Warps;
   };
-
-  Place fetch = at;                                      // the next tile to copy
-  int64_t fetch_x = begin + warp;
-  advance(fetch, warp);
   uint32_t issued = 0, used = 0;
-#pragma unroll
-  for (int s = 0; s < kV4Stages; ++s) {
-    if (fetch_x < end) {
-      issue(fetch, page_of(fetch), s);
-      ++issued;
-      fetch_x += kV4Warps;
-      advance(fetch, kV4Warps);
+  auto issue = [&](int stage) {
+    if ((issued & 7u) == 0) prepare();
+    if (static_cast<uint32_t>(lane >> 2) == (issued & 7u)) {
+      if ((lane & 3) == 0) {
+        if (blocks > 0) mbar_expect_tx(&bar[stage], blocks * 2 * SM::kBlock);
+        else mbar_arrive(&bar[stage]);
+      }
+      if ((lane & 1) < blocks) bulk_load(ring + stage * SM::kStage + (lane & 3) * SM::kBlock, src, SM::kBlock, &bar[stage]);
     }
-  }
+    ++issued;
+  };
+#pragma unroll
+  for (int s = 0; s < kV4Stages; ++s)
+    if (issued < my_tiles) issue(s);
 
   // ---- segment by segment (the tiles of one head group of one sequence)
-  int64_t mine = begin + warp;                           // this warp's next tile
+  int mine = warp;                                       // this warp's next tile of the share
   bool ok = true;
-  if (guard.cfg.limit_ns == 0) ok = __all_sync(0xffffffffu, mine >= end || guard.first(&bar[0]));
-  int64_t seg = begin;
-  while (seg < end) {
-    const int64_t seg_end = min(end, seg + (at.n - at.tile));
-    const bool whole = at.tile == 0 && seg_end - seg == at.n;
-    const int len = len_of(at.seq);
+  if (guard.cfg.limit_ns == 0) ok = __all_sync(0xffffffffu, mine >= tiles || guard.first(&bar[0]));
+  int seg = 0;
+  while (seg < tiles) {
+    const int seg_end = min(tiles, seg + (at.n - at_tile));
+    const bool whole = at_tile == 0 && seg_end - seg == at.n;
+    const int len = at.len;
     const int head0 = at.head / hg * p.G + at.head % hg * p.GP;
     const __nv_bfloat16* q = p.q + at.seq * p.q_ts + static_cast<int64_t>(head0) * D;
 
@@ -306,11 +300,13 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
             f[2 * e] = v.x * up;
             f[2 * e + 1] = v.y * up;
           }
-          // step 2c: codes (0, 4) and, four bits up, (1, 5); step 2c + 1: (2, 6) and (3, 7)
-          qf[nt][gr * 4 + 2 * c][0] = pack_f16(f[0], f[4]);
-          qf[nt][gr * 4 + 2 * c][1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
-          qf[nt][gr * 4 + 2 * c + 1][0] = pack_f16(f[2], f[6]);
-          qf[nt][gr * 4 + 2 * c + 1][1] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
+          // step 2c: bytes 0 and 2 (codes 0, 1 and 4, 5); step 2c + 1: bytes 1 and 3. With the byte b = c0 + 16 c1 and its upper part
+          // u = 16 c1: q0 c0 + q1 c1 = q0 b + (q1 / 16 - q0) u
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            qf[nt][gr * 4 + 2 * c + i][0] = pack_f16(f[2 * i], f[2 * i + 4]);
+            qf[nt][gr * 4 + 2 * c + i][1] = pack_f16(fmaf(f[2 * i + 1], 0.0625f, -f[2 * i]), fmaf(f[2 * i + 5], 0.0625f, -f[2 * i + 4]));
+          }
         }
       }
 #pragma unroll
@@ -321,7 +317,9 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       }
     }
 
-    float o[NT][KS][4], ones[NT][GR][2], lows[NT][GR][2], m[NT][2], l[NT][2];
+    // o: sums of bytes (even dim + 16 odd dim) and of their upper parts (16 odd dim), in units of 2^-24; o, l and lows relative to
+    // 2^base, base = maximum (m) + log2 of the largest scale (top_scale) - kV4Room
+    float o[NT][KS][4], lows[NT][GR][2], m[NT][2], l[NT][2], base[NT][2], top_scale = 8.6736174e-19f;      // 2^-60: scales below it count as that
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -331,16 +329,15 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         m[nt][c] = -INFINITY;
-        l[nt][c] = 0.f;
+        l[nt][c] = base[nt][c] = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) ones[nt][gr][c] = lows[nt][gr][c] = 0.f;
+        for (int gr = 0; gr < GR; ++gr) lows[nt][gr][c] = 0.f;
       }
     }
 
     for (; mine < seg_end && ok; mine += kV4Warps) {
       const int stage = used % kV4Stages;
-      const int key0 = (at.tile + static_cast<int>(mine - seg)) * kV4Keys;
-      const int next_page = fetch_x < end ? page_of(fetch) : 0;      // on its way while this tile is worked on
+      const int key0 = (at_tile + mine - seg) * kV4Keys;
       ok = __all_sync(0xffffffffu, guard.wait(&bar[stage], (used / kV4Stages) & 1));
       if (!ok) break;
       const uint32_t kb = ring + stage * SM::kStage, vb = kb + 2 * SM::kBlock;
@@ -368,13 +365,13 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t x = w[0][c * GR + gr], y = w[1][c * GR + gr], x8 = x >> 8, y8 = y >> 8;
+            const uint32_t x = w[0][c * GR + gr], y = w[1][c * GR + gr];
+            const uint32_t x0 = x & 0x00ff00ffu, y0 = y & 0x00ff00ffu, x1 = __byte_perm(x, 0u, 0x4341), y1 = __byte_perm(y, 0u, 0x4341);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(acc[nt][gr], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][gr * 4 + 2 * c][0],
-                      qf[nt][gr * 4 + 2 * c][1]);
-              mma_f16(acc[nt][gr], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
-                      qf[nt][gr * 4 + 2 * c + 1][0], qf[nt][gr * 4 + 2 * c + 1][1]);
+              mma_f16(acc[nt][gr], x0, y0, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][gr * 4 + 2 * c][0], qf[nt][gr * 4 + 2 * c][1]);
+              mma_f16(acc[nt][gr], x1, y1, x1 & 0x00f000f0u, y1 & 0x00f000f0u, qf[nt][gr * 4 + 2 * c + 1][0],
+                      qf[nt][gr * 4 + 2 * c + 1][1]);
             }
           }
         }
@@ -383,7 +380,6 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
           uint32_t pr[2];
           if constexpr (GR == 2) lds64(b + 8 * D + (g + 8 * r) * 8, pr[0], pr[1]);
           else pr[0] = lds32(b + 8 * D + (g + 8 * r) * 4);
-          const bool seen = key0 + 16 * sub + 8 * r + g < len;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -393,32 +389,64 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
                 dot = fmaf(low_half(pr[1]), acc[nt][1][2 * r + c], dot);
                 add = fmaf(high_half(pr[1]), qsum[nt][c][1], add);
               }
-              const float z = fmaf(unscale[nt][c], dot, add);
-              s[nt][sub][2 * r + c] = tail && !seen ? -INFINITY : z;
+              s[nt][sub][2 * r + c] = fmaf(unscale[nt][c], dot, add);
             }
           }
         }
       }
+      // the values' scales and low ends; what lies behind the last token may be anything
+      uint32_t vp[2][2][GR];
+      float scale_max = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t (&pr)[GR] = vp[i / 2][i % 2];
+        const uint32_t at_pair = vb + i / 2 * SM::kBlock + 8 * D + (g + 8 * (i % 2)) * (4 * GR);
+        if constexpr (GR == 2) lds64(at_pair, pr[0], pr[1]);
+        else pr[0] = lds32(at_pair);
+      }
+      if (tail) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key0 + 8 * i + g >= len) {
+            vp[i / 2][i % 2][0] = vp[i / 2][i % 2][GR - 1] = 0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][i / 2][i % 2 * 2] = s[nt][i / 2][i % 2 * 2 + 1] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) scale_max = fmaxf(scale_max, low_half(vp[i / 2][i % 2][gr]));
       // the reference of the exponentials
+      float mx[NT][2];
+      bool follow = scale_max > top_scale;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float mx[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) mx[c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
-        if (__any_sync(0xffffffffu, mx[0] > m[nt][0] + kV4Lazy || mx[1] > m[nt][1] + kV4Lazy)) {
+        for (int c = 0; c < 2; ++c) {
+          mx[nt][c] = fmaxf(fmaxf(s[nt][0][c], s[nt][0][2 + c]), fmaxf(s[nt][1][c], s[nt][1][2 + c]));
+          follow = follow || mx[nt][c] > m[nt][c] + kV4Lazy;
+        }
+      }
+      if (__any_sync(0xffffffffu, follow)) {
+        // the next power of two: the reference moves by whole steps
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(scale_max, top_scale)));
+        top_scale = __uint_as_float(min((bits + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
+        const float room = static_cast<float>(static_cast<int>(__float_as_uint(top_scale) >> 23) - 127) - kV4Room;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int of = 4; of < 32; of <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], of));
-            const float m_new = fmaxf(m[nt][c], mx[c]);
-            const float alpha = m_new == -INFINITY ? 1.f : exp2f(m[nt][c] - m_new);
+            for (int of = 4; of < 32; of <<= 1) mx[nt][c] = fmaxf(mx[nt][c], __shfl_xor_sync(0xffffffffu, mx[nt][c], of));
+            const float m_new = fmaxf(m[nt][c], mx[nt][c]);
+            const float to = m_new == -INFINITY ? 0.f : m_new + room;
+            const float alpha = m[nt][c] == -INFINITY ? 0.f : exp2f(base[nt][c] - to);       // nothing is there yet where m is -inf
             m[nt][c] = m_new;
+            base[nt][c] = to;
             l[nt][c] *= alpha;
 #pragma unroll
-            for (int gr = 0; gr < GR; ++gr) {
-              ones[nt][gr][c] *= alpha;
-              lows[nt][gr][c] *= alpha;
-            }
+            for (int gr = 0; gr < GR; ++gr) lows[nt][gr][c] *= alpha;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
               o[nt][i][c] *= alpha;
@@ -434,28 +462,19 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         uint32_t pf[NT][GR][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          uint32_t pr[2];
-          if constexpr (GR == 2) lds64(b + 8 * D + (g + 8 * r) * 8, pr[0], pr[1]);
-          else pr[0] = lds32(b + 8 * D + (g + 8 * r) * 4);
-          if (tail && key0 + 16 * sub + 8 * r + g >= len) pr[0] = pr[1] = 0u;       // what lies behind the last token may be anything
+          const uint32_t (&pr)[GR] = vp[sub][r];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float e[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float m_use = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-              e[c] = exp2f(s[nt][sub][2 * r + c] - m_use);
+              e[c] = exp2f(s[nt][sub][2 * r + c] - base[nt][c]);
               l[nt][c] += e[c];
 #pragma unroll
               for (int gr = 0; gr < GR; ++gr) lows[nt][gr][c] = fmaf(e[c], high_half(pr[gr]), lows[nt][gr][c]);
             }
 #pragma unroll
-            for (int gr = 0; gr < GR; ++gr) {
-              const uint32_t packed = pack_bf16(e[0] * low_half(pr[gr]), e[1] * low_half(pr[gr]));
-              ones[nt][gr][0] += low_half(packed);
-              ones[nt][gr][1] += high_half(packed);
-              pf[nt][gr][r] = movmatrix(packed);
-            }
+            for (int gr = 0; gr < GR; ++gr) pf[nt][gr][r] = movmatrix(pack_f16(e[0] * low_half(pr[gr]), e[1] * low_half(pr[gr])));
           }
         }
         uint32_t w[4][2];                                // tokens 2t, 2t + 1, 2t + 8, 2t + 9: chunk g of each group
@@ -468,28 +487,23 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {                  // dims 2i, 2i + 1 of the chunk
-            const uint32_t sel = i | ((4 + i) << 8);     // byte i of both tokens, each in the low byte of its half
-            const uint32_t x = __byte_perm(w[0][gr], w[1][gr], (sel & 0xf) | ((sel & 0xf) << 4) | (sel & 0xf00) | ((sel & 0xf00) << 4));
-            const uint32_t y = __byte_perm(w[2][gr], w[3][gr], (sel & 0xf) | ((sel & 0xf) << 4) | (sel & 0xf00) | ((sel & 0xf00) << 4));
-            const uint32_t a0 = (x & 0x000f000fu) | 0x43004300u, a1 = ((x >> 4) & 0x000f000fu) | 0x43004300u;
-            const uint32_t a2 = (y & 0x000f000fu) | 0x43004300u, a3 = ((y >> 4) & 0x000f000fu) | 0x43004300u;
+          for (int i = 0; i < 2; ++i) {                  // bytes 2i, 2i + 1 of the chunk: dims 4i .. 4i + 3
+            const uint32_t x = __byte_perm(w[0][gr], w[1][gr], i == 0 ? 0x5410 : 0x7632), y = __byte_perm(w[2][gr], w[3][gr], i == 0 ? 0x5410 : 0x7632);
+            const uint32_t x0 = x & 0x00ff00ffu, y0 = y & 0x00ff00ffu, x1 = __byte_perm(x, 0u, 0x4341), y1 = __byte_perm(y, 0u, 0x4341);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][gr * 4 + i], a0, a1, a2, a3, pf[nt][gr][0], pf[nt][gr][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][gr * 4 + 2 * i], x0, x & 0x00f000f0u, y0, y & 0x00f000f0u, pf[nt][gr][0], pf[nt][gr][1]);
+              mma_f16(o[nt][gr * 4 + 2 * i + 1], x1, x1 & 0x00f000f0u, y1, y1 & 0x00f000f0u, pf[nt][gr][0], pf[nt][gr][1]);
+            }
           }
         }
       }
       ++used;
       __syncwarp();                                      // every lane has read the stage
-      if (fetch_x < end) {
-        issue(fetch, next_page, stage);
-        ++issued;
-        fetch_x += kV4Warps;
-        advance(fetch, kV4Warps);
-      }
+      if (issued < my_tiles) issue(stage);
     }
 
-    // ---- the warps' sums together; l, ones and lows are of this lane's keys so far
+    // ---- the warps' sums together; l and lows are of this lane's keys so far
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -498,26 +512,22 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         for (int of = 4; of < 32; of <<= 1) {
           l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], of);
 #pragma unroll
-          for (int gr = 0; gr < GR; ++gr) {
-            ones[nt][gr][c] += __shfl_xor_sync(0xffffffffu, ones[nt][gr][c], of);
-            lows[nt][gr][c] += __shfl_xor_sync(0xffffffffu, lows[nt][gr][c], of);
-          }
+          for (int gr = 0; gr < GR; ++gr) lows[nt][gr][c] += __shfl_xor_sync(0xffffffffu, lows[nt][gr][c], of);
         }
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          const float off = fmaf(-128.f, ones[nt][i / 4][c], lows[nt][i / 4][c]);
-          o[nt][i][c] += off;
-          o[nt][i][2 + c] += off;
+          o[nt][i][c] = fmaf(o[nt][i][c] - o[nt][i][2 + c], 16777216.f, lows[nt][i / 4][c]);
+          o[nt][i][2 + c] = fmaf(o[nt][i][2 + c], 1048576.f, lows[nt][i / 4][c]);
         }
+        if (m[nt][c] == -INFINITY) base[nt][c] = -INFINITY;          // no keys: no part in the join
         if (g == 0) {
           float* x = ml + (warp * 8 * NT + nt * 8 + 2 * t + c) * 2;
-          x[0] = m[nt][c];
+          x[0] = base[nt][c];
           x[1] = l[nt][c];
         }
       }
     }
     __syncthreads();
-    float top[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -525,8 +535,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         float x = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kV4Warps; ++w) x = fmaxf(x, ml[(w * 8 * NT + nt * 8 + 2 * t + c) * 2]);
-        top[nt][c] = x;
-        const float f = m[nt][c] == -INFINITY ? 0.f : exp2f(m[nt][c] - x);
+        const float f = base[nt][c] == -INFINITY ? 0.f : exp2f(base[nt][c] - x);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           o[nt][i][c] *= f;
@@ -577,7 +586,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     }
     __syncthreads();
     // a piece (four dims of a head) a thread: sum of the four, then the result or this share's part of it
-    const int slot = 2 * blockIdx.x + (seg == begin ? 0 : 1);
+    const int slot = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
     constexpr int kPieces = NT * GR * 4;
     for (int x = warp; x < kPieces; x += kV4Warps) {
       const int nt = x / (GR * 4), gr = x / 4 % GR, c = x / 2 % 2, half = x % 2;
@@ -610,17 +619,11 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         }
       }
     }
-    if (tid == 0 && at.tile == 0 && !whole)              // it ends with this share and goes on in the next
-      p.meta[blockIdx.x] = make_int4(at.seq, at.head, static_cast<int>((seg + at.n - 1) / share), slot);
+    if (tid == 0 && at_tile == 0 && !whole)              // it ends with this share and goes on in the next
+      p.meta[blockIdx.x] = make_int4(at.seq, at.head, static_cast<int>((begin + seg + at.n - 1) / share), slot);
     __syncthreads();                                     // the pieces and factors have been read
-    at.tile += static_cast<int>(seg_end - seg);
-    if (at.tile == at.n) {
-      at.tile = 0;
-      if (++at.head == H) {
-        at.head = 0;
-        if (++at.seq < p.B) at.n = kv4_tiles(len_of(at.seq));
-      }
-    }
+    at_tile = 0;                                         // only a share's last segment ends before its head group does
+    next_head(at);
     seg = seg_end;
   }
   // copies in flight land before the CTA ends, where the waits were given up
@@ -733,7 +736,7 @@ GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const vo
                                 int page_size, float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (B <= 0) return 0;
   auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || Hkv <= 0 || Hq % Hkv != 0 || q_ts % 8 != 0 || !al16(q) ||
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || Hkv <= 0 || Hq % Hkv != 0 || q_ts % 8 != 0 || !al16(q) ||
       !al16(out) || !al16(k_cache) || !al16(v_cache) || !al16(scratch) || pages <= 0 || ctas <= 0 ||
       scratch_bytes < gllm_kv4_decode_scratch(D, ctas)) {
     fprintf(stderr, "[gllm_b200] kv4_decode: unsupported D=%d page_size=%d Hq=%d Hkv=%d, or rows off 16-byte boundaries\n", D,
@@ -746,10 +749,12 @@ GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const vo
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
   p.k_cache = reinterpret_cast<const uint8_t*>(k_cache);
   p.v_cache = reinterpret_cast<const uint8_t*>(v_cache);
-  p.pages = pages;
+  p.last_page = static_cast<uint32_t>(pages < 0x80000000ll ? pages - 1 : 0x7fffffffll);
   p.block_table = reinterpret_cast<const int32_t*>(block_table);
   p.seq_lens = reinterpret_cast<const int32_t*>(seq_lens);
-  p.B = B; p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.page_size = page_size;
+  p.B = B; p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
+  p.page_blocks = page_size / 16;
+  p.page_magic = p.page_blocks == 1 ? 0u : static_cast<uint32_t>((0x100000000ull + p.page_blocks - 1) / p.page_blocks);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part_o = reinterpret_cast<float*>(scratch);
   p.part_ml = p.part_o + static_cast<int64_t>(ctas) * 2 * 16 * D;
@@ -770,7 +775,7 @@ GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const 
                                 int B, int Hkv, int D, int page_size, int64_t pages, int64_t tiles, void* k_out, void* v_out,
                                 void* table, int max_tiles, int max_len, void* stream) {
   if (B <= 0 || max_len <= 0) return 0;
-  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || pages <= 0 || B > 65535 ||
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || pages <= 0 || B > 65535 ||
       static_cast<int64_t>(max_tiles) * 64 < max_len) {
     fprintf(stderr, "[gllm_b200] kv4_expand: unsupported D=%d page_size=%d, %d sequences\n", D, page_size, B);
     return 1;

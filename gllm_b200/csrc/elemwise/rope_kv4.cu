@@ -227,7 +227,7 @@ cudaError_t launch_rope_kv4(const RopeParams& p, int64_t pages, cudaStream_t st)
 using namespace b200;
 
 // As gllm_rope_kv_write, on 4-bit caches of `pages` pages; k is left as it is. Slots outside of the cache are left out. Rows, norm
-// weights and caches on 16-byte boundaries, D 64 or 128, pages of a multiple of 16 tokens, rot a multiple of 16 (of 8 for
+// weights and caches on 16-byte boundaries, D 64 or 128, pages of a multiple of 16 tokens up to 512, rot a multiple of 16 (of 8 for
 // neighbouring pairs).
 GLLM_EXPORT int gllm_rope_kv4_write(void* q, int64_t q_ts, int64_t q_hs, int Hq, const void* k, int64_t k_ts, int64_t k_hs, int Hkv,
                                     const void* v, int64_t v_ts, int64_t v_hs, const void* q_norm_w, const void* k_norm_w,
@@ -236,7 +236,7 @@ GLLM_EXPORT int gllm_rope_kv4_write(void* q, int64_t q_ts, int64_t q_hs, int Hq,
                                     int sec1, int page_size, int64_t pos_stride, void* stream) {
   if (T <= 0) return 0;
   auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0 || rot < 0 || rot > D || rot % (neox ? 16 : 8) != 0 ||
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || rot < 0 || rot > D || rot % (neox ? 16 : 8) != 0 ||
       ((q_ts | q_hs | k_ts | k_hs | v_ts | v_hs) & 7) != 0 || !al16(q) || !al16(k) || !al16(v) || !al16(q_norm_w) ||
       !al16(k_norm_w) || !al16(k_cache) || !al16(v_cache)) {
     fprintf(stderr, "[gllm_b200] rope_kv4_write: unsupported D=%d rot=%d page_size=%d, or rows off 16-byte boundaries\n", D, rot,
@@ -266,7 +266,7 @@ GLLM_EXPORT int gllm_rope_kv4_write(void* q, int64_t q_ts, int64_t q_hs, int Hq,
 GLLM_EXPORT int gllm_kv4_rows(const void* k_cache, const void* v_cache, const void* slots, void* k_out, void* v_out, int T, int Hkv,
                               int D, int page_size, int64_t pages, void* stream) {
   if (T <= 0) return 0;
-  if ((D != 64 && D != 128) || page_size <= 0 || page_size % 16 != 0) {
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0) {
     fprintf(stderr, "[gllm_b200] kv4_rows: unsupported D=%d page_size=%d\n", D, page_size);
     return 1;
   }

@@ -19,20 +19,21 @@ import functools
 import torch
 
 BLOCK = 16
+MOST_PAGE = 512          # tokens; the attention kernel divides by it with one multiplication
 HEAD_DIMS = (64, 128)
 
 
 def cache_shape(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int):
-    if head_dim not in HEAD_DIMS or page_size <= 0 or page_size % BLOCK:
-        raise ValueError(f"a 4-bit cache holds heads of 64 or 128 in pages of a multiple of {BLOCK} tokens: got heads of "
-                         f"{head_dim}, pages of {page_size}")
+    if head_dim not in HEAD_DIMS or not BLOCK <= page_size <= MOST_PAGE or page_size % BLOCK:
+        raise ValueError(f"a 4-bit cache holds heads of 64 or 128 in pages of a multiple of {BLOCK} tokens up to {MOST_PAGE}: got heads "
+                         f"of {head_dim}, pages of {page_size}")
     return (num_pages, num_kv_heads, page_size // BLOCK, 9 * head_dim)
 
 
 def geometry(cache: torch.Tensor):
     """(pages, kv heads, page_size, head_dim) of a 4-bit cache."""
     if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[3] % 9 or cache.shape[3] // 9 not in HEAD_DIMS or \
-            not cache.is_contiguous():
+            not 1 <= cache.shape[2] <= MOST_PAGE // BLOCK or not cache.is_contiguous():
         raise ValueError(f"not a 4-bit cache: {cache.dtype} {tuple(cache.shape)}")
     return cache.shape[0], cache.shape[1], cache.shape[2] * BLOCK, cache.shape[3] // 9
 

@@ -38,12 +38,13 @@ def turned(x, w, cos, sin, rot, neox, eps):
 def attention(q, rows, lens, news, scale, hkv, rounded):
     """q [T, Hq, D]; rows: per sequence the bf16 (keys, values) [len, Hkv, D] that were coded; -> (result, tolerance) [T, Hq, D] fp64.
 
-    The tolerance counts roundings: half a step of bf16 is 2^-8 of a value. Results are rounded once (2^-8 |o|) and probabilities once
-    (2^-8 of what they bring in: sum p s c in the form on codes, whose low ends are added in fp32, and sum p |v| over expanded tiles).
-    Scores are fp32 sums of at most 128 products, good to 2^-22 of the sum of their magnitudes, some 2^-17 at the sizes here; with
-    expanded tiles (`rounded`) every key and value is rounded too: six standard deviations of 64 or 128 independent
-    roundings (uniform within half a step: 2^-8 / sqrt 3) in a score, 2^-8 sum p |v| for the values. The form on codes sums 128 + c and takes
-    128 sum(p s) off: at most len / 128 additions of a warp, each good to 2^-23 of 143 sum(p s)."""
+    The tolerance counts roundings: half a step of bf16 is 2^-8 of a value, of fp16 2^-11. Results are rounded once (2^-8 |o|) and
+    probabilities once: in the form on codes, times their scales, to fp16 (2^-11 of sum p s c; the low ends are added in fp32), over expanded
+    tiles to bf16 (2^-8 of sum p |v|). Scores are fp32 sums of at most 128 products, good to 2^-22 of the sum of their magnitudes, some
+    2^-17 at the sizes here; with expanded tiles (`rounded`) every key and value is rounded too: six standard deviations of 64 or
+    128 independent roundings (uniform within half a step: 2^-8 / sqrt 3) in a score, 2^-8 sum p |v| for the values. The form on codes rounds half of its factors of
+    queries to fp16: likewise, with 2^-11, in the codes' part of a score. A product of it that is below fp16's normal numbers is good to 2^-25 where the largest that can stand beside it is 2^6 and more: 2^-31
+    of it a key."""
     out, tol = [], []
     at = 0
     for (k, v), n, new in zip(rows, lens, news):
@@ -68,8 +69,10 @@ def attention(q, rows, lens, news, scale, hkv, rounded):
             slack = (2 * 2 ** -8 + 2 * dz + 2 ** -16) * size
         else:
             steps = torch.einsum("hgqk,khd->qhgd", p, (s * c).flatten(-2))
-            units = torch.einsum("hgqk,khd->qhgd", p, s.expand(-1, -1, -1, 64).flatten(-2))
-            slack = (2 ** -8) * steps + (n / 128 + 2) * 2 ** -23 * 143 * units + 2 ** -16 * (size + steps)
+            spread = torch.einsum("qhgd,khd->hgqk", qq.square(), c.flatten(-2).square() * s.expand(-1, -1, -1, 64).flatten(-2).square()).sqrt()
+            dz = (6 * 2 ** -11 / math.sqrt(3) * spread * scale).amax(-1).permute(2, 0, 1)[..., None]
+            least = 2 ** -31 * 15 * n * s.amax((0, 2, 3))[None, :, None, None] * p.amax(-1).permute(2, 0, 1)[..., None]
+            slack = 2 ** -11 * steps + least + (2 ** -16 + 2 * dz) * (size + steps)
         out.append(o.flatten(1, 2))
         tol.append((slack + 2 ** -8 * o.abs()).flatten(1, 2) * 1.01)
     return torch.cat(out), torch.cat(tol)

@@ -112,7 +112,7 @@ def test_rounds_of_expansion():
     assert sm100_kv4.expand_rounds([], 1) == [] and sm100_kv4.expand_rounds([0, 0], 1) == [(0, 2, 0)]
 
 
-@pytest.mark.parametrize("d,page", [(32, 16), (96, 16), (256, 16), (64, 8), (128, 24), (128, 0)])
+@pytest.mark.parametrize("d,page", [(32, 16), (96, 16), (256, 16), (64, 8), (128, 24), (128, 0), (64, 528)])
 def test_shapes_that_a_cache_does_not_take(d, page):
     with pytest.raises(ValueError):
         kv4.cache_shape(4, 2, d, page)

@@ -180,6 +180,22 @@ def test_decode_over_the_range_of_queries(size):
     assert ((got.view_as(want).double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("loud", [1.0, 2.0 ** 12, 2.0 ** -12])
+def test_decode_of_values_of_very_different_sizes(loud):
+    """One token's values are `loud` times the others', and it is not what the queries look for, or all that they look for."""
+    lens, hq, hkv, d = [333, 64], 8, 2, 128
+    torch.manual_seed(5)
+    caches, rows, table = _filled(lens, hkv, d, 16)
+    for i, at in ((0, 300), (1, 5)):
+        rows[i][1][at] = (rows[i][1][at].float() * loud).to(BF16)
+        kv4.write_rows(caches[1], (table[i, at // 16] * 16 + at % 16).view(1), rows[i][1][at:at + 1])
+    q = torch.randn(2, hq * d, device=DEV).to(BF16)
+    q[1] = (rows[1][0][5].float() * (2.0 if loud < 1 else -0.2)).to(BF16).repeat_interleave(hq // hkv, 0).flatten()
+    got = _attend(q, caches, table, lens, [1, 1], 2, hq, hkv, d)
+    want, tol = U.attention(q.view(2, hq, d), rows, lens, [1, 1], d ** -0.5, hkv, False)
+    assert ((got.view_as(want).double() - want).abs() <= tol).all()
+
+
 def test_decode_of_a_key_that_is_no_number():
     lens, hq, hkv, d = [90, 40], 4, 2, 128
     caches, rows, table = _filled(lens, hkv, d, 16)
