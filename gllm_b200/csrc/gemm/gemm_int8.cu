@@ -103,6 +103,56 @@ int quant_rows(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, float* scales, i
   return 0;
 }
 
+// The faster form of a product of this size: true with a plan for the cluster kernel, false for the pairs. Fitted to 933 products (1 to 700
+// rows, weights of 512 to 57,344 rows and 640 to 28,672 columns, a third gated; every plan timed with cold weights, the rows'
+// quantiser included). A plan costs what is more of its copies (an SM takes 100 KB per us) and its weights (6.36 TB/s, less where few
+// SMs draw), and a fixed sum a round, which counts as 14 us here, more than the 0.8 us that it takes: a second round is rarely worth it.
+// The choice takes 1.5 % longer than the best plan on average (27 of 933 over 10 %, 1.42 at worst). Against the pairs both are estimated in
+// us; the choice between them loses 0.4 % (19 over 10 %, 1.28 at worst); the pairs win 91 of the 933, all but a few over 256 rows. Some, pairs and
+// chosen, us: 1 row of 6144 x 4096 18.6 and 8.8, 64 rows 24,576 x 4096 gated 33.9 and 24.8, 64 of 4096 x 12,288 37.5 and 18.4, 256 of 6144 x
+// 4096 19.7 and 19.1, 777 of 10,240 x 8192 71.7 and 80.1.
+bool plan_int8(int M, int N, int K, bool gated, ClusterPlan* plan) {
+  if (M > 1024) return false;
+  const int sms = num_sms(), num_kb = (K + 127) / 128, tiles_n = (N + 127) / 128;
+  const double bytes = static_cast<double>(N) * K / 6.36e6;
+  double best = 1e30, takes = 1e30;
+  for (int tm = 1; tm <= 8; ++tm) {
+    const int bt = ((M + tm - 1) / tm + 15) / 16 * 16;
+    if (bt > 256) continue;
+    if (tm > 1 && bt < 32) break;
+    for (const int parts : {1, 2, 3, 4, 6, 8}) {
+      if (parts > 1 && parts * 2 > num_kb) break;
+      const int side = cluster_slots(1, parts) - (parts == 3 ? 2 : 0);      // of three, fewer run at once than the query says
+      if (side <= 0) continue;
+      for (int per_sm = 1; per_sm <= 2; ++per_sm) {
+        const ClusterPlan one{bt, parts, per_sm == 1 ? 220 * 1024 : 108 * 1024};
+        const int stages = (one.smem - 2048) / ((128 + bt) * 128);
+        if (stages < per_sm + 1 || cluster_smem(one, gated) == 0) continue;
+        const int tiles = tiles_n * ((M + bt - 1) / bt), rounds = (tiles + side * per_sm - 1) / (side * per_sm);
+        const double ctas = static_cast<double>(tiles < side * per_sm ? tiles : side * per_sm) * parts;
+        const double copies = static_cast<double>(rounds) * per_sm * ((num_kb + parts - 1) / parts) * ((128 + bt) * 128) * 1e-5;
+        auto drawn = [&](double share, double less) {                       // ... by so many SMs
+          const double n = per_sm == 1 ? ctas : share * ctas;
+          return bytes * (1.0 + less * (sms / (n < sms ? n : sms) - 1.0));
+        };
+        auto most = [](double a, double b) { return a > b ? a : b; };
+        const double memory = drawn(0.92, 0.3);
+        const double t = most(copies, memory) + 0.018 * (copies < memory ? copies : memory) + rounds * (14.3 + 0.0054 * bt) +
+                         (per_sm == 2 ? 0.0014 * bt : 0.0);
+        if (t < best) {
+          best = t;
+          takes = most(0.924 * copies, drawn(0.38, 0.1)) + rounds * (0.76 + 0.0434 * bt) + 4.1;
+          *plan = one;
+        }
+      }
+    }
+  }
+  if (best == 1e30) return false;
+  const int tiles = ((M + 255) / 256) * ((N + 255) / 256), rounds = (tiles + sms / 2 - 1) / (sms / 2);
+  const double products = rounds * (0.297 * num_kb + 0.08), memory = 1.95 * bytes;
+  return takes < 1.1 * ((products > memory ? products : memory) + 8.5);
+}
+
 }  // namespace
 
 }  // namespace b200
@@ -143,10 +193,7 @@ GLLM_EXPORT int gllm_linear_int8(const void* x, int64_t ldx, void* xq, void* x_s
   __nv_bfloat16* c = reinterpret_cast<__nv_bfloat16*>(C);
   const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(bias);
   ClusterPlan plan{bt, parts, smem};
-  if (form == 0) {
-    plan = ClusterPlan{(M < 256 ? M + 15 : 256) / 16 * 16, 1, 108 * 1024};
-    form = M <= 256 ? 2 : 1;
-  }
+  if (form == 0) form = plan_int8(M, N, K, gated != 0, &plan) ? 2 : 1;
   if (form == 2)
     return gemm_int8_cluster(ClusterGemmInt8{ClusterGemm{xq, W8, K, K, c, ldc, M, N, K, b, gated != 0, 0}, as, ws}, plan, st);
   return gemm_int8_pair(PairGemmInt8{PairGemm{xq, W8, K, K, c, ldc, M, N, K, b, gated, 0.f, 0.f, 0}, as, ws}, st);
