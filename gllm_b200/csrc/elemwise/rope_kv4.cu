@@ -5,8 +5,7 @@
 // then 16 x D / 64 pairs (scale, low) of bf16. Each 64 dims y of a token's head:
 //   low = min y,  scale = bf16((max y - low) / 15),  code = min(15, rne((y - low) / scale)),  value = code * scale + low.
 // y is rounded to bf16 before it is coded (what a bf16 cache would hold), so low needs no rounding of its own. Many quotients
-// are ties (both sides are multiples of the same power of two), hence the IEEE division: a product with the reciprocal would
-// send them either way.
+// are ties (both sides are multiples of the same power of two), which a product with the reciprocal alone would send either way.
 //
 // Queries are rotated in place; the rotated keys go to the cache only.
 #include "../common/host_utils.h"
@@ -39,31 +38,59 @@ __device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Eight bf16 values of a group that eight neighbouring lanes hold: this lane's codes and the group's pair. All lanes of the warp
-// take part. A NaN or an infinity (or a span beyond fp32) makes the scale a NaN, and so every value that is read back.
-__device__ __forceinline__ uint32_t kv4_encode(const uint32_t (&w)[4], uint32_t& pair) {
-  uint32_t lo = min_nan2(min_nan2(w[0], w[1]), min_nan2(w[2], w[3])), hi = max_nan2(max_nan2(w[0], w[1]), max_nan2(w[2], w[3]));
+// The ends of a group from those of a lane's values (bf16 pairs): O neighbouring lanes hold the group, all of the warp take part.
+template <int O>
+__device__ __forceinline__ void kv4_ends(uint32_t& lo, uint32_t& hi) {
   lo = min_nan2(lo, __byte_perm(lo, lo, 0x1032));
   hi = max_nan2(hi, __byte_perm(hi, hi, 0x1032));
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
+  for (int o = O / 2; o > 0; o >>= 1) {
     lo = min_nan2(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = max_nan2(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const float low = __uint_as_float(lo << 16), high = __uint_as_float(hi << 16);
-  const __nv_bfloat16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f));
-  const float scale = __bfloat162float(scale16);
-  const bool fine = scale <= 3.3895e38f;                 // false for NaN as well
-  pair = (lo & 0xffff0000u) | (fine ? __bfloat16_as_ushort(scale16) : 0x7fffu);
-  uint32_t codes = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 y = unpack_bf16(w[e]);
-    const float a = __fdiv_rn(__fsub_rn(y.x, low), scale), b = __fdiv_rn(__fsub_rn(y.y, low), scale);
-    codes |= __float2uint_rn(fminf(a, 15.f)) << (8 * e) | __float2uint_rn(fminf(b, 15.f)) << (8 * e + 4);
-  }
-  return fine && scale > 0.f ? codes : 0u;
 }
+__device__ __forceinline__ uint32_t min4(const uint32_t (&w)[4]) { return min_nan2(min_nan2(w[0], w[1]), min_nan2(w[2], w[3])); }
+__device__ __forceinline__ uint32_t max4(const uint32_t (&w)[4]) { return max_nan2(max_nan2(w[0], w[1]), max_nan2(w[2], w[3])); }
+
+// A group's pair from its ends, and what its codes are made with. A NaN or an infinity (or a span beyond fp32) makes the scale a
+// NaN, and so every value that is read back.
+struct Kv4Group {
+  float low, scale, inv;
+  uint32_t pair;
+  __device__ __forceinline__ Kv4Group(uint32_t lo, uint32_t hi) {
+    low = __uint_as_float(lo << 16);
+    const float high = __uint_as_float(hi << 16);
+    const __nv_bfloat16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f));
+    scale = __bfloat162float(scale16);
+    const bool fine = scale <= 3.3895e38f;               // false for NaN as well
+    pair = (lo & 0xffff0000u) | (fine ? __bfloat16_as_ushort(scale16) : 0x7fffu);
+    if (!(fine && scale > 0.f)) scale = 0.f;
+    inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;     // no scale: codes of 0
+  }
+  // Eight codes. The quotient's estimate by the reciprocal is off by one only next to a tie, which the remainder y - low - q scale shows (it
+  // is exact): half a dozen operations instead of an IEEE division's dozen and more.
+  __device__ __forceinline__ uint32_t codes(const uint32_t (&w)[4]) const {
+    constexpr float kMagic = 12582912.f;                 // 1.5 x 2^23: an integer added to it stands in the low bits
+    const float half = 0.5f * scale;
+    float q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = __fsub_rn(e & 1 ? __uint_as_float(w[e >> 1] & 0xffff0000u) : __uint_as_float(w[e >> 1] << 16), low);
+      const float m = fmaf(d, inv, kMagic);
+      q[e] = m - kMagic;
+      const float r = fmaf(-q[e], scale, d);
+      if (fabsf(r) > __uint_as_float(__float_as_uint(half) - (__float_as_uint(m) & 1u))) q[e] += copysignf(1.f, r);
+      q[e] = fminf(q[e], 15.f);
+    }
+    // four codes are a number below 2^16
+    const float a = fmaf(q[3], 4096.f, fmaf(q[2], 256.f, fmaf(q[1], 16.f, q[0] + kMagic)));
+    const float b = fmaf(q[7], 4096.f, fmaf(q[6], 256.f, fmaf(q[5], 16.f, q[4] + kMagic)));
+    return inv > 0.f ? __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410) : 0u;
+  }
+};
+
+__device__ __forceinline__ uint8_t* kc_of(const RopeParams& p) { return reinterpret_cast<uint8_t*>(p.k_cache); }
+__device__ __forceinline__ uint8_t* vc_of(const RopeParams& p) { return reinterpret_cast<uint8_t*>(p.v_cache); }
 
 // A lane holds eight dims of a head, L = D / 8 lanes a head, NB heads a lane group, all loaded before the first is worked on.
 template <int L, int NB>
@@ -77,8 +104,6 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
   const int half = p.rot >> 1;
   const int n_qk = p.Hq + p.Hkv, n_heads = n_qk + p.Hkv;
   const int first = blockIdx.y * (kStep * NB) + warp * kHeadsPerWarp + lane / L;
-  uint8_t* kc = reinterpret_cast<uint8_t*>(p.k_cache);
-  uint8_t* vc = reinterpret_cast<uint8_t*>(p.v_cache);
 
   uint4 raw[NB];
 #pragma unroll
@@ -168,15 +193,142 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
     }
-    uint32_t pair;
-    const uint32_t codes = kv4_encode(w, pair);
-    if (hh >= n_heads) continue;
+    if (is_q) *reinterpret_cast<uint4*>(p.q + t * p.q_ts + hh * p.q_hs + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (__all_sync(0xffffffffu, is_q)) continue;
+    uint32_t low = min4(w), high = max4(w);
+    kv4_ends<8>(low, high);
+    const Kv4Group made(low, high);
+    if (!is_q && hh < n_heads && at.ok) {
+      uint8_t* block = (is_qk ? kc_of(p) + (hh - p.Hq) * head_stride : vc_of(p) + (hh - n_qk) * head_stride) + at.block;
+      *reinterpret_cast<uint32_t*>(block + at.row * (D / 2) + unit * 4) = made.codes(w);
+      if (e0 % 64 == 0) *reinterpret_cast<uint32_t*>(block + 8 * D + (at.row * G + group) * 4) = made.pair;
+    }
+  }
+}
+
+// NeoX rotation of whole heads (rot = D), the common form: a lane holds eight dims of the lower half and their partners of the upper
+// one, L = D / 16 lanes a head, so that nothing is exchanged for the rotation; heads of 128: its two words are neighbours in the cache.
+template <int L, int NB>
+__global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, const int64_t pages) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int D = 16 * L, H = D / 2, G = D / 64, kHeadsPerWarp = 32 / L, kStep = 4 * kHeadsPerWarp;
+  const int t = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % L, e0 = gl * 8;
+  const int n_qk = p.Hq + p.Hkv, n_heads = n_qk + p.Hkv;
+  const int first = blockIdx.y * (kStep * NB) + warp * kHeadsPerWarp + lane / L;
+
+  uint4 raw[NB][2];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int hh = first + n * kStep;
+    raw[n][0] = raw[n][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (hh < n_heads) {
+      const __nv_bfloat16* src = hh < p.Hq ? p.q + t * p.q_ts + hh * p.q_hs
+                                 : hh < n_qk ? p.k + t * p.k_ts + (hh - p.Hq) * p.k_hs
+                                             : p.v + t * p.v_ts + (hh - n_qk) * p.v_hs;
+      raw[n][0] = *reinterpret_cast<const uint4*>(src + e0);
+      raw[n][1] = *reinterpret_cast<const uint4*>(src + H + e0);
+    }
+  }
+  float c[8], s[8];
+  const float* row = p.cos_sin + static_cast<size_t>(p.positions[t]) * D + e0;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float4 cv = *reinterpret_cast<const float4*>(row + 4 * g), sv = *reinterpret_cast<const float4*>(row + H + 4 * g);
+    c[4 * g] = cv.x; c[4 * g + 1] = cv.y; c[4 * g + 2] = cv.z; c[4 * g + 3] = cv.w;
+    s[4 * g] = sv.x; s[4 * g + 1] = sv.y; s[4 * g + 2] = sv.z; s[4 * g + 3] = sv.w;
+  }
+  const Kv4Place at = kv4_place(p.slots[t], p.page_size, pages, p.Hkv, D);
+  const size_t head_stride = static_cast<size_t>(p.page_size / 16) * (9 * D);
+  const bool norm = p.q_norm_w != nullptr || p.k_norm_w != nullptr;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int hh = first + n * kStep;
+    const bool is_q = hh < p.Hq, is_qk = hh < n_qk;
+    uint32_t w[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i][0] = raw[n][i].x; w[i][1] = raw[n][i].y; w[i][2] = raw[n][i].z; w[i][3] = raw[n][i].w;
+    }
+    if (__any_sync(0xffffffffu, is_qk)) {
+      float x[2][8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_bf16(w[i][e]);
+          x[i][2 * e] = f.x;
+          x[i][2 * e + 1] = f.y;
+        }
+      }
+      if (norm) {
+        float ss = 0.f, upper = 0.f;                     // apart: the order of the sums is the other kernel's, and so are the bits
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ss += x[0][e] * x[0][e];
+          upper += x[1][e] * x[1][e];
+        }
+        ss += upper;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const __nv_bfloat16* nw = is_q ? p.q_norm_w : p.k_norm_w;
+        if (is_qk && nw != nullptr) {
+          const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 wv = *reinterpret_cast<const uint4*>(nw + i * H + e0);
+            const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_bf16(ww[e]);
+              x[i][2 * e] = __bfloat162float(__float2bfloat16(x[i][2 * e] * inv * f.x));
+              x[i][2 * e + 1] = __bfloat162float(__float2bfloat16(x[i][2 * e + 1] * inv * f.y));
+            }
+          }
+        }
+      }
+      if (is_qk) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float r[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {                  // rounded one by one, as above
+            const int i = 2 * e + j;
+            r[0][j] = __fsub_rn(__fmul_rn(x[0][i], c[i]), __fmul_rn(x[1][i], s[i]));
+            r[1][j] = __fadd_rn(__fmul_rn(x[1][i], c[i]), __fmul_rn(x[0][i], s[i]));
+          }
+          w[0][e] = pack_bf16(r[0][0], r[0][1]);
+          w[1][e] = pack_bf16(r[1][0], r[1][1]);
+        }
+      }
+    }
     if (is_q) {
-      *reinterpret_cast<uint4*>(p.q + t * p.q_ts + hh * p.q_hs + e0) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else if (at.ok) {
-      uint8_t* block = (is_qk ? kc + (hh - p.Hq) * head_stride : vc + (hh - n_qk) * head_stride) + at.block;
-      *reinterpret_cast<uint32_t*>(block + at.row * (D / 2) + unit * 4) = codes;
-      if (e0 % 64 == 0) *reinterpret_cast<uint32_t*>(block + 8 * D + (at.row * G + group) * 4) = pair;
+      __nv_bfloat16* dst = p.q + t * p.q_ts + hh * p.q_hs + e0;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+      *reinterpret_cast<uint4*>(dst + H) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+    }
+    if (__all_sync(0xffffffffu, is_q)) continue;
+    const bool stored = !is_q && hh < n_heads && at.ok;
+    uint8_t* block = is_q || !at.ok ? nullptr : (is_qk ? kc_of(p) + (hh - p.Hq) * head_stride : vc_of(p) + (hh - n_qk) * head_stride) + at.block;
+    if constexpr (G == 2) {                              // the halves are the groups
+      uint32_t lo[2] = {min4(w[0]), min4(w[1])}, hi[2] = {max4(w[0]), max4(w[1])};
+      kv4_ends<L>(lo[0], hi[0]);
+      kv4_ends<L>(lo[1], hi[1]);
+      const Kv4Group a(lo[0], hi[0]), b(lo[1], hi[1]);
+      if (stored) {
+        *reinterpret_cast<uint2*>(block + at.row * (D / 2) + gl * 8) = make_uint2(a.codes(w[0]), b.codes(w[1]));
+        if (gl == 0) *reinterpret_cast<uint2*>(block + 8 * D + at.row * 8) = make_uint2(a.pair, b.pair);
+      }
+    } else {
+      uint32_t lo = min_nan2(min4(w[0]), min4(w[1])), hi = max_nan2(max4(w[0]), max4(w[1]));
+      kv4_ends<L>(lo, hi);
+      const Kv4Group a(lo, hi);
+      if (stored) {
+        *reinterpret_cast<uint32_t*>(block + at.row * (D / 2) + gl * 4) = a.codes(w[0]);
+        *reinterpret_cast<uint32_t*>(block + at.row * (D / 2) + (gl + L) * 4) = a.codes(w[1]);
+        if (gl == 0) *reinterpret_cast<uint32_t*>(block + 8 * D + at.row * 4) = a.pair;
+      }
     }
   }
 }
@@ -220,6 +372,15 @@ cudaError_t launch_rope_kv4(const RopeParams& p, int64_t pages, cudaStream_t st)
   return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages);
 }
 
+template <int L>
+cudaError_t launch_rope_kv4_pair(const RopeParams& p, int64_t pages, cudaStream_t st) {
+  constexpr int kStep = 4 * (32 / L);
+  const int n_heads = p.Hq + 2 * p.Hkv;
+  if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 2)
+    return launch_pdl(rope_kv4_pair_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages);
+  return launch_pdl(rope_kv4_pair_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages);
+}
+
 }  // namespace
 
 }  // namespace b200
@@ -258,7 +419,10 @@ GLLM_EXPORT int gllm_rope_kv4_write(void* q, int64_t q_ts, int64_t q_hs, int Hq,
   p.v_cache = reinterpret_cast<__nv_bfloat16*>(v_cache);
   p.sec0 = sec0; p.sec1 = sec1; p.page_size = page_size; p.pos_stride = pos_stride;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  CUDA_CHECK_RET(D == 64 ? launch_rope_kv4<8>(p, pages, st) : launch_rope_kv4<16>(p, pages, st));
+  if (neox && rot == D && sec0 == 0 && al16(cos_sin))
+    CUDA_CHECK_RET(D == 64 ? launch_rope_kv4_pair<4>(p, pages, st) : launch_rope_kv4_pair<8>(p, pages, st));
+  else
+    CUDA_CHECK_RET(D == 64 ? launch_rope_kv4<8>(p, pages, st) : launch_rope_kv4<16>(p, pages, st));
   return 0;
 }
 

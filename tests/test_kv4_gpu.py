@@ -79,6 +79,18 @@ def test_write_with_norms(t, hq, hkv, d, rot, neox, norms):
     assert torch.equal(vals, U.values(x.v).float().to(BF16))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t", [3, 900])
+def test_write_in_both_forms_gives_the_same_bits(t, d):
+    """Three equal rows of positions take the form with a lane per eight dims, one row the one with both halves of a pair in a lane."""
+    from gllm_b200.ops import sm100_kv4
+    x = _write_inputs(t, 16, 8, d, d, 16, "qk")
+    other, q0 = [c.clone() for c in x.caches], x.q.clone()
+    sm100_kv4.rope_kv_write(x.q, x.k, x.v, x.pos, x.cs, d, True, *x.w, 1e-6, *x.caches, x.slots)
+    sm100_kv4.rope_kv_write(q0, x.k, x.v, x.pos.expand(3, -1).contiguous(), x.cs, d, True, *x.w, 1e-6, *other, x.slots, [d // 4, d // 8, d // 8])
+    assert torch.equal(x.q, q0) and all(torch.equal(a, b) for a, b in zip(x.caches, other))
+
+
 @pytest.mark.parametrize("section", [[8, 12, 12], [16, 8, 8], [12, 10, 10, True]])
 def test_write_with_three_position_rows(section):
     from gllm_b200.ops import sm100_kv4
