@@ -12,14 +12,23 @@ import torch
 from gllm_b200.ops import kv4, ref
 
 
+_modules = {}      # imported on first use: a lookup a call instead of the import statement
+
+
 def _sm():
-    from gllm_b200.ops import sm100
-    return sm100
+    m = _modules.get("sm100")
+    if m is None:
+        from gllm_b200.ops import sm100 as m
+        _modules["sm100"] = m
+    return m
 
 
 def _kv4():
-    from gllm_b200.ops import sm100_kv4
-    return sm100_kv4
+    m = _modules.get("kv4")
+    if m is None:
+        from gllm_b200.ops import sm100_kv4 as m
+        _modules["kv4"] = m
+    return m
 
 
 def linear(x, w, bias=None, out=None):

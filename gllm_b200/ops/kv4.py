@@ -30,12 +30,20 @@ def cache_shape(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int
     return (num_pages, num_kv_heads, page_size // BLOCK, 9 * head_dim)
 
 
+@functools.lru_cache(maxsize=256)
+def _sizes(shape):
+    """(pages, kv heads, page_size, head_dim) of a shape, or None if it is no 4-bit cache's."""
+    if len(shape) != 4 or shape[3] % 9 or shape[3] // 9 not in HEAD_DIMS or not 1 <= shape[2] <= MOST_PAGE // BLOCK:
+        return None
+    return shape[0], shape[1], shape[2] * BLOCK, shape[3] // 9
+
+
 def geometry(cache: torch.Tensor):
     """(pages, kv heads, page_size, head_dim) of a 4-bit cache."""
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[3] % 9 or cache.shape[3] // 9 not in HEAD_DIMS or \
-            not 1 <= cache.shape[2] <= MOST_PAGE // BLOCK or not cache.is_contiguous():
+    sizes = _sizes(cache.shape)
+    if sizes is None or cache.dtype != torch.uint8 or not cache.is_contiguous():
         raise ValueError(f"not a 4-bit cache: {cache.dtype} {tuple(cache.shape)}")
-    return cache.shape[0], cache.shape[1], cache.shape[2] * BLOCK, cache.shape[3] // 9
+    return sizes
 
 
 def held(cache) -> bool:

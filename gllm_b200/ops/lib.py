@@ -195,6 +195,14 @@ def stream_ptr() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def on_this_device(*tensors):
+    """Raises unless every tensor (None: left out) lies on the current device, whose stream the launch goes to."""
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"a tensor on {t.device} for a launch on cuda:{here}")
+
+
 def check(rc: int, what: str):
     if rc != 0:
         raise RuntimeError(f"gllm_b200 kernel launch failed: {what} (rc={rc})")

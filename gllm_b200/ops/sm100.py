@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from gllm_b200.ops import lib as _lib
-from gllm_b200.ops.lib import GemmComm, check, stream_ptr
+from gllm_b200.ops.lib import GemmComm, check, on_this_device, stream_ptr
 
 _BF16 = torch.bfloat16
 NUM_SMS = 148
@@ -521,8 +521,11 @@ INT8_MOST_K = 131072     # the int32 sums are exact up to here
 
 
 def _int8_rows(x: torch.Tensor):
-    assert x.dtype == _BF16 and x.dim() == 2 and x.stride(1) == 1
     m, k = x.shape
+    ld, one = x.stride()
+    if x.dtype is _BF16 and one == 1 and 0 < k <= INT8_MOST_K and (k | x.data_ptr() | 2 * ld) % 16 == 0:
+        return m, k
+    assert x.dtype == _BF16 and x.stride(1) == 1
     if k % 16 or k == 0 or k > INT8_MOST_K:
         raise ValueError(f"8-bit products take rows of a multiple of 16 values, at most {INT8_MOST_K}: got {k}")
     if m and (x.data_ptr() % 16 or x.stride(0) % 8):
@@ -537,6 +540,7 @@ def int8_quant_rows(x: torch.Tensor):
     q = torch.empty(m, k, dtype=torch.int8, device=x.device)
     s = torch.empty(m, dtype=torch.float32, device=x.device)
     if m:
+        on_this_device(x)
         check(_lib.load().gllm_int8_quant_rows(_p(x), x.stride(0), _p(q), _p(s), m, k, stream_ptr()), "int8_quant_rows")
         _count()
     return q, s
@@ -549,23 +553,32 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
     one chosen by size."""
     m, k = _int8_rows(x)
     n = w8.shape[0]
-    assert w8.dtype == torch.int8 and w8.is_contiguous() and w8.shape == (n, k), (w8.dtype, w8.shape, k)
-    assert w_scale.dtype == torch.float32 and w_scale.shape == (n,) and w_scale.is_contiguous()
-    assert bias is None or (bias.dtype == _BF16 and bias.shape == (n,) and bias.is_contiguous())
     n_out = n // 2 if silu else n
-    if n % 8 or n_out % 8 or n == 0 or (silu and bias is not None):
-        raise ValueError(f"8-bit products take a multiple of 8 columns (gated: of 16, and no bias): got {n}")
     if out is None:
         out = torch.empty(m, n_out, dtype=_BF16, device=x.device)
-    assert out.dtype == _BF16 and out.shape == (m, n_out) and out.stride(1) == 1
-    if any(t is not None and t.data_ptr() % 16 for t in (w8, w_scale, bias)) or (m and (out.data_ptr() % 16 or out.stride(0) % 8)):
-        raise ValueError("weights, scales, bias and results of an 8-bit product must lie on 16-byte boundaries")
+    w_at, s_at, o_at, ldc = w8.data_ptr(), w_scale.data_ptr(), out.data_ptr(), out.stride(0)
+    b_at = None if bias is None else bias.data_ptr()
+    if not (w8.dtype is torch.int8 and w8.shape == (n, k) and w8.is_contiguous() and w_scale.dtype is torch.float32 and
+            w_scale.shape == (n,) and w_scale.stride(0) == 1 and out.dtype is _BF16 and out.shape == (m, n_out) and
+            out.stride(1) == 1 and (w_at | s_at | o_at | (b_at or 0) | 2 * ldc | 2 * n_out | 2 * n) % 16 == 0 and n > 0 and
+            (bias is None or (not silu and bias.dtype is _BF16 and bias.shape == (n,) and bias.stride(0) == 1))):
+        # not the common call: what is wrong with it, if anything is
+        assert w8.dtype == torch.int8 and w8.is_contiguous() and w8.shape == (n, k), (w8.dtype, w8.shape, k)
+        assert w_scale.dtype == torch.float32 and w_scale.shape == (n,) and w_scale.is_contiguous()
+        assert bias is None or (bias.dtype == _BF16 and bias.shape == (n,) and bias.is_contiguous())
+        if n % 8 or n_out % 8 or n == 0 or (silu and bias is not None):
+            raise ValueError(f"8-bit products take a multiple of 8 columns (gated: of 16, and no bias): got {n}")
+        assert out.dtype == _BF16 and out.shape == (m, n_out) and out.stride(1) == 1
+        if w_at % 16 or s_at % 16 or (b_at or 0) % 16 or (m and (o_at % 16 or ldc % 8)):
+            raise ValueError("weights, scales, bias and results of an 8-bit product must lie on 16-byte boundaries")
     if m == 0:
         return out
+    on_this_device(x, w8, w_scale, out, bias)
     scratch = torch.empty(m * k + 4 * m, dtype=torch.uint8, device=x.device)     # k % 16: the scales lie on 16-byte boundaries
+    xq = scratch.data_ptr()
     form, bt, parts, smem = plan or (0, 0, 0, 0)
-    check(_lib.load().gllm_linear_int8(_p(x), x.stride(0), scratch.data_ptr(), scratch.data_ptr() + m * k, _p(w8), _p(w_scale), _p(out),
-                                       out.stride(0), m, n, k, _p(bias), int(silu), form, bt, parts, smem, stream_ptr()), "linear_int8")
+    check(_lib.load().gllm_linear_int8(x.data_ptr(), x.stride(0), xq, xq + m * k, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,
+                                       smem, stream_ptr()), "linear_int8")
     _count(2)
     return out
 

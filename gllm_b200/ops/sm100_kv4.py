@@ -3,13 +3,14 @@ read back. Layout: `ops.kv4`. Each function validates, allocates its output and 
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
 from gllm_b200.ops import kv4, lib as _lib
-from gllm_b200.ops.lib import check, stream_ptr
-from gllm_b200.ops.sm100 import NUM_SMS, _BF16, _count, _p
+from gllm_b200.ops.lib import check, on_this_device, stream_ptr
+from gllm_b200.ops.sm100 import NUM_SMS, _BF16, _count
 
 _DECODE_CTAS = 2 * NUM_SMS           # two fit an SM
 EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at a time (one sequence at least)
@@ -17,7 +18,7 @@ EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at
 
 def _pair(k_cache, v_cache):
     geo = kv4.geometry(k_cache)
-    if kv4.geometry(v_cache) != geo:
+    if v_cache.shape != k_cache.shape or kv4.geometry(v_cache) != geo:
         raise ValueError(f"4-bit caches of unequal shape: {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     return geo
 
@@ -26,48 +27,72 @@ def _index(t: torch.Tensor, what: str, dims: int = 1):
     assert t.dtype == torch.int32 and t.dim() == dims and t.stride(-1) == 1, f"{what}: int32, contiguous rows"
 
 
+def _check_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope):
+    """Raises for arguments that `rope_kv_write` does not take."""
+    t, hq, d = q.shape
+    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride()
+    at = q.data_ptr() | k.data_ptr() | v.data_ptr()
+    norms = True
+    for w in (q_norm_w, k_norm_w):
+        if w is not None:
+            at |= w.data_ptr()
+            norms = norms and w.dtype is _BF16 and w.shape == (d,) and w.stride(0) == 1
+    if norms and q.dtype is k.dtype is v.dtype is _BF16 and qd == kd == vd == 1 and d == dim and k.shape == v.shape == (t, heads, d) and \
+            slots.dtype is positions.dtype is torch.int32 and slots.dim() == positions.dim() == 1 and not mrope and \
+            slots.shape[0] >= t and positions.shape[0] >= t and slots.stride(0) == positions.stride(0) == 1 and \
+            0 <= rot <= d and rot % 16 == 0 and (at | 2 * (qt | qh | kt | kh | vt | vh)) % 16 == 0 and \
+            (rot == 0 or (cos_sin.dtype is torch.float32 and cos_sin.shape[1] == rot and cos_sin.is_contiguous())):
+        return                                                # the common call; what follows says what is wrong with others
+    assert q.dtype == k.dtype == v.dtype == _BF16 and q.stride(2) == k.stride(2) == v.stride(2) == 1
+    assert d == dim and k.shape == v.shape == (t, heads, d), (q.shape, k.shape, v.shape, heads, dim)
+    _index(slots, "slots")
+    assert slots.shape[0] >= t
+    if rot < 0 or rot > d or rot % (16 if neox else 8):
+        raise ValueError(f"a 4-bit cache takes rotations of a multiple of 16 dims (of 8 in neighbouring pairs): got {rot} of {d}")
+    if rot:
+        assert cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1] == rot, (cos_sin.shape, rot)
+    for w in (q_norm_w, k_norm_w):
+        assert w is None or (w.dtype == _BF16 and w.shape == (d,) and w.is_contiguous())
+    _index(positions, "positions", 2 if mrope else 1)
+    assert positions.shape[-1] >= t
+    rows = [x for x in (q, k, v) if x.numel()]
+    if any(x.data_ptr() % 16 or x.stride(0) % 8 or (x.shape[1] > 1 and x.stride(1) % 8) for x in rows) or \
+            any(w is not None and w.data_ptr() % 16 for w in (q_norm_w, k_norm_w)):
+        raise ValueError("rows and norm weights written to a 4-bit cache must lie on 16-byte boundaries")
+
+
 def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos_sin: Optional[torch.Tensor],
                   rot_dim: int, neox: bool, q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], eps: float,
                   k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, mrope_section=None):
     """`sm100.rope_kv_write` on 4-bit caches: q [T, Hq, D] is normed and rotated in place; k and v [T, Hkv, D] are read only. Rows (all three
     may be strided views) lie on 16-byte boundaries; rot_dim is a multiple of 16, of 8 for neighbouring pairs."""
     pages, heads, page_size, dim = _pair(k_cache, v_cache)
-    t, hq, d = q.shape
     if v is None or slots is None:
         raise ValueError("a 4-bit cache is written with keys, values and their slots")
-    assert q.dtype == k.dtype == v.dtype == _BF16 and q.stride(2) == k.stride(2) == v.stride(2) == 1
-    assert d == dim and k.shape == v.shape == (t, heads, d), (q.shape, k.shape, v.shape, tuple(k_cache.shape))
-    _index(slots, "slots")
-    assert slots.shape[0] >= t
+    t, hq, d = q.shape
     rot = rot_dim if cos_sin is not None else 0
-    if rot:
-        assert cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1] == rot, (cos_sin.shape, rot)
-    if rot < 0 or rot > d or rot % (16 if neox else 8):
-        raise ValueError(f"a 4-bit cache takes rotations of a multiple of 16 dims (of 8 in neighbouring pairs): got {rot} of {d}")
-    for w in (q_norm_w, k_norm_w):
-        assert w is None or (w.dtype == _BF16 and w.shape == (d,) and w.is_contiguous())
-    rows = [x for x in (q, k, v) if x.numel()]
-    if any(x.data_ptr() % 16 or x.stride(0) % 8 or (x.shape[1] > 1 and x.stride(1) % 8) for x in rows) or \
-            any(w is not None and w.data_ptr() % 16 for w in (q_norm_w, k_norm_w)):
-        raise ValueError("rows and norm weights written to a 4-bit cache must lie on 16-byte boundaries")
+    mrope = mrope_section is not None and positions.dim() == 2
+    if not mrope and positions.dim() == 2:
+        positions = positions[0]
+    _check_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope)
     if t == 0:
         return
+    on_this_device(q, k, v, positions, slots, k_cache, v_cache, cos_sin, q_norm_w, k_norm_w)
     sec0 = sec1 = pos_stride = 0
-    if mrope_section is not None and positions.dim() == 2:
-        _index(positions, "positions", 2)
+    if mrope:
         if len(mrope_section) > 3 and mrope_section[3]:       # interleaved; otherwise chunks (see sm100.rope_kv_write)
             sec0, sec1 = -int(mrope_section[1]), int(mrope_section[2])
         else:
             sec0, sec1 = int(mrope_section[0]), int(mrope_section[1])
         pos_stride = positions.stride(0)
-    else:
-        positions = positions[0] if positions.dim() == 2 else positions
-        _index(positions, "positions")
-    hs = [x.stride(1) if x.shape[1] > 1 else d for x in (q, k, v)]
+    (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+    if heads == 1:                                            # the stride of a dimension of one may be anything
+        kh = vh = d
     check(_lib.load().gllm_rope_kv4_write(
-        _p(q), q.stride(0), hs[0], hq, _p(k), k.stride(0), hs[1], heads, _p(v), v.stride(0), hs[2], _p(q_norm_w), _p(k_norm_w),
-        _p(cos_sin) if rot else None, d, rot, 1 if neox else 0, t, _p(positions), _p(slots), float(eps), _p(k_cache), _p(v_cache),
-        pages, sec0, sec1, page_size, pos_stride, stream_ptr()), "rope_kv4_write")
+        q.data_ptr(), qt, qh if hq > 1 else d, hq, k.data_ptr(), kt, kh, heads, v.data_ptr(), vt, vh,
+        None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr(),
+        cos_sin.data_ptr() if rot else None, d, rot, 1 if neox else 0, t, positions.data_ptr(), slots.data_ptr(), eps,
+        k_cache.data_ptr(), v_cache.data_ptr(), pages, sec0, sec1, page_size, pos_stride, stream_ptr()), "rope_kv4_write")
     _count()
 
 
@@ -75,13 +100,19 @@ def kv_cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
     """(keys, values) [T, Hkv, D] bf16 that 4-bit caches hold at `slots`; zeros for slots outside of the cache."""
     pages, heads, page_size, d = _pair(k_cache, v_cache)
     _index(slots, "slots")
+    on_this_device(k_cache, v_cache, slots)
     t = slots.shape[0]
-    k, v = (torch.empty(t, heads, d, dtype=_BF16, device=k_cache.device) for _ in range(2))
-    check(_lib.load().gllm_kv4_rows(_p(k_cache), _p(v_cache), _p(slots), _p(k), _p(v), t, heads, d, page_size, pages, stream_ptr()),
-          "kv4_rows")
+    k, v = torch.empty(2, t, heads, d, dtype=_BF16, device=k_cache.device).unbind(0)
+    check(_lib.load().gllm_kv4_rows(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, heads, d,
+                                    page_size, pages, stream_ptr()), "kv4_rows")
     if t:
         _count()
     return k, v
+
+
+@functools.lru_cache(maxsize=None)
+def _decode_scratch(d: int) -> int:
+    return _lib.load().gllm_kv4_decode_scratch(d, _DECODE_CTAS)
 
 
 def expand_rounds(lens, token_bytes: int, limit: int = EXPAND_BYTES):
@@ -115,31 +146,35 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if out is None:
         out = torch.empty(t, hq * d, dtype=_BF16, device=q.device)
     assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
+    on_this_device(q, out, k_cache, v_cache, block_table, seq_lens)
     L, st, dev = _lib.load(), stream_ptr(), q.device
     if num_decode_seqs > 0:
         assert block_table.shape[0] >= num_decode_seqs and seq_lens.shape[0] >= num_decode_seqs and t >= num_decode_seqs
-        size = L.gllm_kv4_decode_scratch(d, _DECODE_CTAS)
+        size = _decode_scratch(d)
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)       # of this call: captured graphs and streams share none
-        check(L.gllm_kv4_decode(_p(q), q.stride(0), _p(out), _p(k_cache), _p(v_cache), pages, _p(block_table), block_table.stride(0),
-                                _p(seq_lens), num_decode_seqs, hq, hkv, d, page_size, float(scale), _DECODE_CTAS, _p(scratch), size,
-                                st), "kv4_decode")
+        check(L.gllm_kv4_decode(q.data_ptr(), q.stride(0), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages,
+                                block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), num_decode_seqs, hq, hkv, d,
+                                page_size, scale, _DECODE_CTAS, scratch.data_ptr(), size, st), "kv4_decode")
         _count(2)
     prompts = num_seqs - num_decode_seqs
     if prompts > 0 and max_q_len > 0:
         _index(query_start_loc, "query_start_loc")
+        on_this_device(query_start_loc)
         lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
         for first, end, tiles in expand_rounds(lens, 4 * hkv * d):
             if tiles == 0:
                 continue
             a, n = num_decode_seqs + first, end - first
             longest = int(max(lens[first:end]))
-            k, v = (torch.empty(tiles, hkv, d // 64, 64, 64, dtype=_BF16, device=dev) for _ in range(2))
+            k, v = torch.empty(2, tiles, hkv, d // 64, 64, 64, dtype=_BF16, device=dev).unbind(0)
             max_tiles = (longest + 63) // 64
             table = torch.empty(n, max_tiles, dtype=torch.int32, device=dev)
-            check(L.gllm_kv4_expand(_p(k_cache), _p(v_cache), _p(block_table[a:]), block_table.stride(0), _p(seq_lens[a:]), n, hkv, d,
-                                    page_size, pages, tiles, _p(k), _p(v), _p(table), max_tiles, longest, st), "kv4_expand")
-            check(L.gllm_attn_prefill_tc_tiles(_p(q), q.stride(0), _p(out), _p(k), _p(v), tiles, _p(table), max_tiles, _p(seq_lens[a:]),
-                                               _p(query_start_loc[a:]), t, n, max_q_len, hq, hkv, d, float(scale), st),
+            lens_at, k_at, v_at, table_at = seq_lens.data_ptr() + 4 * a, k.data_ptr(), v.data_ptr(), table.data_ptr()
+            check(L.gllm_kv4_expand(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.stride(0),
+                                    block_table.stride(0), lens_at, n, hkv, d, page_size, pages, tiles, k_at, v_at, table_at, max_tiles,
+                                    longest, st), "kv4_expand")
+            check(L.gllm_attn_prefill_tc_tiles(q.data_ptr(), q.stride(0), out.data_ptr(), k_at, v_at, tiles, table_at, max_tiles, lens_at,
+                                               query_start_loc.data_ptr() + 4 * a, t, n, max_q_len, hq, hkv, d, scale, st),
                   "attn_prefill_tc_tiles")
             _count(2)
     return out

@@ -302,6 +302,21 @@ def test_attention_refuses():
         sm100_kv4.paged_attention(q[:, :256].contiguous(), caches[0], caches[1][:1], table, _i32([20]), None, 1.0, 4, 64, 1, 1, 1, 20)
 
 
+def test_tensors_elsewhere_are_refused():
+    from gllm_b200.ops import sm100, sm100_kv4
+    caches, rows, table = _filled([20], 2, 64, 16)
+    q = torch.randn(1, 4 * 64, device=DEV).to(BF16)
+    with pytest.raises(ValueError):
+        sm100_kv4.paged_attention(q, *caches, table.cpu(), _i32([20]), None, 1.0, 4, 64, 1, 1, 1, 20)
+    with pytest.raises(ValueError):
+        sm100_kv4.kv_cache_rows(*caches, torch.zeros(3, dtype=torch.int32))
+    x = _write_inputs(4, 2, 2, 64, 64, 16, "")
+    with pytest.raises(ValueError):
+        sm100_kv4.rope_kv_write(x.q, x.k, x.v, x.pos.cpu(), x.cs, 64, True, None, None, 1e-6, *x.caches, x.slots)
+    with pytest.raises(ValueError):
+        sm100.linear_int8(q, torch.zeros(16, 256, dtype=torch.int8), torch.ones(16, device=DEV))
+
+
 def test_waits_that_run_out_are_reported():
     from gllm_b200.ops import lib as _lib, sm100
     lens, hq, hkv, d = [4000, 300], 8, 2, 128
