@@ -35,7 +35,8 @@ namespace b200 {
 namespace {
 
 constexpr int kV4Warps = 8, kV4Threads = kV4Warps * 32, kV4Keys = 32, kV4Stages = 2;
-constexpr int kV4Lens = 256;                             // lengths that a CTA keeps in shared memory, from its first sequence on
+static_assert(kV4Threads == 256);
+constexpr int kV4Lens = kV4Threads;                             // lengths that a CTA keeps in shared memory, from its first sequence on
 constexpr float kV4Lazy = 8.f;                           // scores pass the maximum that the reference is taken from by no more than this
 constexpr float kV4Room = 6.f;                           // and exponentials times scales stay below 2^(kV4Lazy + kV4Room)
 
@@ -149,10 +150,12 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     }
     return x + before;
   };
-  int all = 0;
+  // up to one sequence a thread, one pass has it all; beyond that the first counts, the second finds this CTA's
+  int all = 0, mine_len = 0, mine_upto = 0;
   for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
     int total;
-    block_scan(s0 + tid < p.B ? kv4_tiles(p.seq_lens[s0 + tid]) : 0, total);
+    mine_len = s0 + tid < p.B ? p.seq_lens[s0 + tid] : 0;
+    mine_upto = block_scan(s0 + tid < p.B ? kv4_tiles(mine_len) : 0, total);
     all += total;
   }
   const int64_t work = static_cast<int64_t>(all) * H;
@@ -163,9 +166,10 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   {
     int base = 0;                                        // tiles of one head group before this round
     for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
-      int total;
-      const int n = s0 + tid < p.B ? kv4_tiles(p.seq_lens[s0 + tid]) : 0;
-      const int upto = block_scan(n, total) + base;
+      int total = 0;
+      if (p.B > kV4Threads) mine_len = s0 + tid < p.B ? p.seq_lens[s0 + tid] : 0;
+      const int n = s0 + tid < p.B ? kv4_tiles(mine_len) : 0;
+      const int upto = (p.B > kV4Threads ? block_scan(n, total) : mine_upto) + base;
       if (begin >= static_cast<int64_t>(upto - n) * H && begin < static_cast<int64_t>(upto) * H) {
         words[1] = s0 + tid;
         words[2] = upto - n;
@@ -175,7 +179,11 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     __syncthreads();
   }
   const int seq0 = words[1];
-  for (int i = tid; i < kV4Lens; i += kV4Threads) lens[i] = seq0 + i < p.B ? p.seq_lens[seq0 + i] : 0;
+  if (p.B > kV4Threads) {
+    for (int i = tid; i < kV4Lens; i += kV4Threads) lens[i] = seq0 + i < p.B ? p.seq_lens[seq0 + i] : 0;
+  } else if (tid >= seq0) {
+    lens[tid - seq0] = mine_len;                         // kV4Lens == kV4Threads
+  }
   __syncthreads();
   auto len_of = [&](int s) { return s - seq0 < kV4Lens ? lens[s - seq0] : p.seq_lens[s]; };
 
@@ -630,29 +638,49 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   for (; used < issued; ++used) guard.land(&bar[used % kV4Stages], (used / kV4Stages) & 1);
 }
 
-// Joins the parts of a head group that several CTAs share: one CTA for each that starts one and does not end it.
+// Joins the parts of a head group that several CTAs share: one CTA for each that starts one and does not end it. A thread has four dims of a
+// head; factors and sums of several parts are on their way at a time.
+constexpr int kV4JoinThreads = 256;
 template <int D, int NT>
-__global__ void __launch_bounds__(D) kv4_join_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(kV4JoinThreads) kv4_join_kernel(const Kv4Params p) {
   griddep_launch();
   griddep_wait();
   const int4 meta = p.meta[blockIdx.x];                  // sequence, head group, last CTA, slot of the first part
   if (meta.x < 0) return;
-  const int h = blockIdx.y, hg = p.G / p.GP, d = threadIdx.x;
-  const int parts = meta.z - static_cast<int>(blockIdx.x) + 1;
-  auto slot_of = [&](int i) { return i == 0 ? meta.w : 2 * (static_cast<int>(blockIdx.x) + i); };
-  float m = -INFINITY;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[(slot_of(i) * 8 * NT + h) * 2]);
-  float sum = 0.f, v = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const int slot = slot_of(i);
-    const float mi = p.part_ml[(slot * 8 * NT + h) * 2];
-    const float f = mi == -INFINITY ? 0.f : exp2f(mi - m);
-    sum = fmaf(p.part_ml[(slot * 8 * NT + h) * 2 + 1], f, sum);
-    v = fmaf(p.part_o[(static_cast<int64_t>(slot) * 8 * NT + h) * D + d], f, v);
+  const int hg = p.G / p.GP, parts = meta.z - static_cast<int>(blockIdx.x) + 1;
+  const int head0 = meta.y / hg * p.G + meta.y % hg * p.GP;
+  for (int i = threadIdx.x; i < p.GP * (D / 4); i += kV4JoinThreads) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int n0 = 0; n0 < parts; n0 += 4) {
+      float2 ml[4];
+      float4 o[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {                      // behind the last part: that one again, with no weight
+        const int part = min(n0 + n, parts - 1), slot = part == 0 ? meta.w : 2 * (static_cast<int>(blockIdx.x) + part);
+        ml[n] = *reinterpret_cast<const float2*>(p.part_ml + (slot * 8 * NT + h) * 2);
+        o[n] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot) * 8 * NT + h) * D + d);
+      }
+      float m_new = m;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) m_new = fmaxf(m_new, ml[n].x);
+      const float old = m == -INFINITY ? 0.f : exp2f(m - m_new);
+      m = m_new;
+      sum *= old; v.x *= old; v.y *= old; v.z *= old; v.w *= old;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (n0 + n >= parts) break;
+        const float f = ml[n].x == -INFINITY ? 0.f : exp2f(ml[n].x - m);
+        sum = fmaf(ml[n].y, f, sum);
+        v.x = fmaf(o[n].x, f, v.x); v.y = fmaf(o[n].y, f, v.y);
+        v.z = fmaf(o[n].z, f, v.z); v.w = fmaf(o[n].w, f, v.w);
+      }
+    }
+    const float inv = 1.f / sum;
+    *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(meta.x) * p.Hq + head0 + h) * D + d) =
+        make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
   }
-  const int head = meta.y / hg * p.G + meta.y % hg * p.GP + h;
-  p.out[(static_cast<int64_t>(meta.x) * p.Hq + head) * D + d] = __float2bfloat16(v / sum);
 }
 
 template <int D, int NT>
@@ -664,7 +692,7 @@ int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
     configured.done();
   }
   CUDA_CHECK_RET(launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(kV4Threads), SM::kBytes, st, p));
-  CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT>, dim3(ctas, p.GP), dim3(D), 0, st, p));
+  CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT>, dim3(ctas), dim3(kV4JoinThreads), 0, st, p));
   return 0;
 }
 

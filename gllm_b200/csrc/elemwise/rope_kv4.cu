@@ -7,6 +7,8 @@
 // y is rounded to bf16 before it is coded (what a bf16 cache would hold), so low needs no rounding of its own. Many quotients
 // are ties (both sides are multiples of the same power of two), which a product with the reciprocal alone would send either way.
 //
+// What bounds it: issue slots. 4096 tokens x (32 + 8 + 8) heads of 128 with norms: @PAIR@ us; with IEEE divisions in every lane 80.
+//
 // Queries are rotated in place; the rotated keys go to the cache only.
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
@@ -52,6 +54,13 @@ __device__ __forceinline__ void kv4_ends(uint32_t& lo, uint32_t& hi) {
 __device__ __forceinline__ uint32_t min4(const uint32_t (&w)[4]) { return min_nan2(min_nan2(w[0], w[1]), min_nan2(w[2], w[3])); }
 __device__ __forceinline__ uint32_t max4(const uint32_t (&w)[4]) { return max_nan2(max_nan2(w[0], w[1]), max_nan2(w[2], w[3])); }
 
+// A quotient to the nearest from an estimate of the reciprocal: the remainder of the first estimate is exact, and adding its share leaves
+// an error far below half a step (Markstein). So a quotient that is a tie between two codes comes out as one.
+__device__ __forceinline__ float quotient(float d, float s, float inv) {
+  const float q = __fmul_rn(d, inv);
+  return fmaf(fmaf(-q, s, d), inv, q);
+}
+
 // A group's pair from its ends, and what its codes are made with. A NaN or an infinity (or a span beyond fp32) makes the scale a
 // NaN, and so every value that is read back.
 struct Kv4Group {
@@ -60,32 +69,23 @@ struct Kv4Group {
   __device__ __forceinline__ Kv4Group(uint32_t lo, uint32_t hi) {
     low = __uint_as_float(lo << 16);
     const float high = __uint_as_float(hi << 16);
-    const __nv_bfloat16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f));
+    const __nv_bfloat16 scale16 = __float2bfloat16_rn(quotient(__fsub_rn(high, low), 15.f, 1.f / 15.f));
     scale = __bfloat162float(scale16);
     const bool fine = scale <= 3.3895e38f;               // false for NaN as well
     pair = (lo & 0xffff0000u) | (fine ? __bfloat16_as_ushort(scale16) : 0x7fffu);
-    if (!(fine && scale > 0.f)) scale = 0.f;
-    inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;     // no scale: codes of 0
+    inv = fine && scale > 0.f ? __fdividef(1.f, scale) : 0.f;       // no scale: codes of 0
   }
-  // Eight codes. The quotient's estimate by the reciprocal is off by one only next to a tie, which the remainder y - low - q scale shows (it
-  // is exact): half a dozen operations instead of an IEEE division's dozen and more.
+  // Eight codes. The scale is at least (1 - 2^-8) / 15 of the span, so none is over 15.
   __device__ __forceinline__ uint32_t codes(const uint32_t (&w)[4]) const {
     constexpr float kMagic = 12582912.f;                 // 1.5 x 2^23: an integer added to it stands in the low bits
-    const float half = 0.5f * scale;
-    float q[8];
+    uint32_t v = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 7; e >= 0; --e) {
       const float d = __fsub_rn(e & 1 ? __uint_as_float(w[e >> 1] & 0xffff0000u) : __uint_as_float(w[e >> 1] << 16), low);
-      const float m = fmaf(d, inv, kMagic);
-      q[e] = m - kMagic;
-      const float r = fmaf(-q[e], scale, d);
-      if (fabsf(r) > __uint_as_float(__float_as_uint(half) - (__float_as_uint(m) & 1u))) q[e] += copysignf(1.f, r);
-      q[e] = fminf(q[e], 15.f);
+      v = v * 16u + __float_as_uint(__fadd_rn(quotient(d, scale, inv), kMagic));
     }
-    // four codes are a number below 2^16
-    const float a = fmaf(q[3], 4096.f, fmaf(q[2], 256.f, fmaf(q[1], 16.f, q[0] + kMagic)));
-    const float b = fmaf(q[7], 4096.f, fmaf(q[6], 256.f, fmaf(q[5], 16.f, q[4] + kMagic)));
-    return inv > 0.f ? __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410) : 0u;
+    // sum of 16^e (kMagic's bits) mod 2^32: 0x4b400000 (1 + 16 + 256), the rest is shifted out
+    return inv > 0.f ? v - (0x4b400000u + 0xb4000000u + 0x40000000u) : 0u;
   }
 };
 
@@ -94,7 +94,7 @@ __device__ __forceinline__ uint8_t* vc_of(const RopeParams& p) { return reinterp
 
 // A lane holds eight dims of a head, L = D / 8 lanes a head, NB heads a lane group, all loaded before the first is worked on.
 template <int L, int NB>
-__global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const int64_t pages) {
+__global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const int64_t pages, const int wide) {
   griddep_launch();
   griddep_wait();
   constexpr int D = 8 * L, G = D / 64, kHeadsPerWarp = 32 / L, kStep = 4 * kHeadsPerWarp;
@@ -120,7 +120,22 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
   // this lane's rotation row: the pair of element e is (e0 + e) % half (NeoX) or (e0 + e) / 2 (neighbours)
   float c[8], s[8];
   const bool in_rot = e0 < p.rot, lo = e0 < half;
-  if (in_rot) {
+  if (in_rot && p.sec0 == 0 && wide) {
+    const float* row = p.cos_sin + static_cast<size_t>(p.positions[t]) * p.rot;
+    if (p.neox) {
+      const int i = e0 - (lo ? 0 : half);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 cv = *reinterpret_cast<const float4*>(row + i + 4 * g), sv = *reinterpret_cast<const float4*>(row + half + i + 4 * g);
+        c[4 * g] = cv.x; c[4 * g + 1] = cv.y; c[4 * g + 2] = cv.z; c[4 * g + 3] = cv.w;
+        s[4 * g] = sv.x; s[4 * g + 1] = sv.y; s[4 * g + 2] = sv.z; s[4 * g + 3] = sv.w;
+      }
+    } else {
+      const float4 cv = *reinterpret_cast<const float4*>(row + e0 / 2), sv = *reinterpret_cast<const float4*>(row + half + e0 / 2);
+      c[0] = c[1] = cv.x; c[2] = c[3] = cv.y; c[4] = c[5] = cv.z; c[6] = c[7] = cv.w;
+      s[0] = s[1] = sv.x; s[2] = s[3] = sv.y; s[4] = s[5] = sv.z; s[6] = s[7] = sv.w;
+    }
+  } else if (in_rot) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = p.neox ? e0 + e - (lo ? 0 : half) : (e0 + e) >> 1;
@@ -162,8 +177,9 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
         for (int e = 0; e < 4; ++e) {
           const float2 f = unpack_bf16(ww[e]);
           // rounded to bf16 after the norm, as on a bf16 cache
-          x[2 * e] = __bfloat162float(__float2bfloat16(x[2 * e] * inv * f.x));
-          x[2 * e + 1] = __bfloat162float(__float2bfloat16(x[2 * e + 1] * inv * f.y));
+          const float2 y = unpack_bf16(pack_bf16(x[2 * e] * inv * f.x, x[2 * e + 1] * inv * f.y));
+          x[2 * e] = y.x;
+          x[2 * e + 1] = y.y;
         }
       }
     }
@@ -282,8 +298,9 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = unpack_bf16(ww[e]);
-              x[i][2 * e] = __bfloat162float(__float2bfloat16(x[i][2 * e] * inv * f.x));
-              x[i][2 * e + 1] = __bfloat162float(__float2bfloat16(x[i][2 * e + 1] * inv * f.y));
+              const float2 y = unpack_bf16(pack_bf16(x[i][2 * e] * inv * f.x, x[i][2 * e + 1] * inv * f.y));
+              x[i][2 * e] = y.x;
+              x[i][2 * e + 1] = y.y;
             }
           }
         }
@@ -333,43 +350,59 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
   }
 }
 
-// Rows of a 4-bit cache as bf16 (code * scale + low, rounded once); a lane makes eight dims. Memory-bound.
-template <int L>
+// Rows of a 4-bit cache as bf16 (code * scale + low, rounded once): a lane makes the eight dims of a unit of the keys and of the values, of two
+// heads where there are as many, all loaded before the first is worked on. Memory-bound.
+template <int L, int NB>
 __global__ void __launch_bounds__(128)
 kv4_rows_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ slots,
                 __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int T, int Hkv, int page_size, int64_t pages) {
   griddep_launch();
   griddep_wait();
   constexpr int D = 8 * L, G = D / 64;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
-  const int64_t row = i / L;                             // token, head, keys or values
-  if (row >= static_cast<int64_t>(T) * Hkv * 2) return;
+  const int groups = (Hkv + NB - 1) / NB;                // of heads
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x, row = i / L;
+  if (row >= static_cast<int64_t>(T) * groups) return;
   const int unit = static_cast<int>(i % L), group = unit % G, e0 = 64 * group + unit / G * 8;
-  const bool is_v = row >= static_cast<int64_t>(T) * Hkv;
-  const int64_t th = is_v ? row - static_cast<int64_t>(T) * Hkv : row;
-  const int t = static_cast<int>(th / Hkv), h = static_cast<int>(th % Hkv);
+  const int t = static_cast<int>(row / groups), h0 = static_cast<int>(row % groups) * NB;
   const Kv4Place at = kv4_place(slots[t], page_size, pages, Hkv, D);
-  uint4 w = make_uint4(0u, 0u, 0u, 0u);
-  if (at.ok) {
-    const uint8_t* block = (is_v ? v_cache : k_cache) + at.block + h * (static_cast<size_t>(page_size / 16) * (9 * D));
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + at.row * (D / 2) + unit * 4);
-    const float2 pair = unpack_bf16(*reinterpret_cast<const uint32_t*>(block + 8 * D + (at.row * G + group) * 4));
-    float f[8];
+  const size_t head_stride = static_cast<size_t>(page_size / 16) * (9 * D);
+  uint32_t codes[NB][2], pair[NB][2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), pair.x, pair.y);
-    w = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  for (int n = 0; n < NB; ++n) {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      codes[n][kv] = pair[n][kv] = 0u;                   // stands for zeros
+      if (at.ok && h0 + n < Hkv) {
+        const uint8_t* block = (kv ? v_cache : k_cache) + at.block + (h0 + n) * head_stride;
+        codes[n][kv] = *reinterpret_cast<const uint32_t*>(block + at.row * (D / 2) + unit * 4);
+        pair[n][kv] = *reinterpret_cast<const uint32_t*>(block + 8 * D + (at.row * G + group) * 4);
+      }
+    }
   }
-  *reinterpret_cast<uint4*>((is_v ? v_out : k_out) + th * D + e0) = w;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (h0 + n >= Hkv) break;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const float2 p = unpack_bf16(pair[n][kv]);
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes[n][kv] >> (4 * e)) & 15u), p.x, p.y);
+      *reinterpret_cast<uint4*>((kv ? v_out : k_out) + (static_cast<int64_t>(t) * Hkv + h0 + n) * D + e0) =
+          make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    }
+  }
 }
 
 template <int L>
 cudaError_t launch_rope_kv4(const RopeParams& p, int64_t pages, cudaStream_t st) {
   constexpr int kStep = 4 * (32 / L);
   const int n_heads = p.Hq + 2 * p.Hkv;
-  // many tokens: four heads a lane, fewer and longer blocks; a decode batch: one, so that it still fills the machine
-  if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 4)
-    return launch_pdl(rope_kv4_kernel<L, 4>, dim3(p.T, (n_heads + 4 * kStep - 1) / (4 * kStep)), dim3(128), 0, st, p, pages);
-  return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages);
+  const int wide = (reinterpret_cast<uintptr_t>(p.cos_sin) & 15) == 0 && p.rot % 8 == 0;       // rotation rows in pieces of 16 bytes
+  // many tokens: several heads a lane, fewer and longer blocks; a decode batch: one, so that it still fills the machine
+  if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 2)
+    return launch_pdl(rope_kv4_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages, wide);
+  return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages, wide);
 }
 
 template <int L>
@@ -434,15 +467,16 @@ GLLM_EXPORT int gllm_kv4_rows(const void* k_cache, const void* v_cache, const vo
     fprintf(stderr, "[gllm_b200] kv4_rows: unsupported D=%d page_size=%d\n", D, page_size);
     return 1;
   }
-  const int64_t blocks = (static_cast<int64_t>(T) * Hkv * 2 * (D / 8) + 127) / 128;
+  const int nb = static_cast<int64_t>(T) * Hkv >= 4096 ? 2 : 1;             // one head a lane where that does not fill the machine
+  const int64_t blocks = (static_cast<int64_t>(T) * ((Hkv + nb - 1) / nb) * (D / 8) + 127) / 128;
   if (blocks > 0x7fffffff) {
     fprintf(stderr, "[gllm_b200] kv4_rows: %lld blocks\n", static_cast<long long>(blocks));
     return 1;
   }
-  CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_rows_kernel<8> : kv4_rows_kernel<16>, dim3(static_cast<unsigned>(blocks)), dim3(128), 0,
-                            reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint8_t*>(k_cache),
-                            reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(slots),
-                            reinterpret_cast<__nv_bfloat16*>(k_out), reinterpret_cast<__nv_bfloat16*>(v_out), T, Hkv, page_size,
-                            pages));
+  auto kern = D == 64 ? (nb == 2 ? kv4_rows_kernel<8, 2> : kv4_rows_kernel<8, 1>) : (nb == 2 ? kv4_rows_kernel<16, 2> : kv4_rows_kernel<16, 1>);
+  CUDA_CHECK_RET(launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, reinterpret_cast<cudaStream_t>(stream),
+                            reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache),
+                            reinterpret_cast<const int32_t*>(slots), reinterpret_cast<__nv_bfloat16*>(k_out),
+                            reinterpret_cast<__nv_bfloat16*>(v_out), T, Hkv, page_size, pages));
   return 0;
 }
