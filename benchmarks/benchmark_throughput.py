@@ -32,6 +32,8 @@ def main():
     ap.add_argument("--enable-prefix-caching", action="store_true")
     ap.add_argument("--max-cuda-graph-bs", type=int, default=512)
     ap.add_argument("--tp-mode", default="fused", choices=["fused", "nccl"])
+    ap.add_argument("--kv-cache-dtype", default=None, choices=["auto", "int4"])
+    ap.add_argument("--quantization", default=None, choices=["int8"])
     ap.add_argument("--output-json", default=None)
     args = ap.parse_args()
     from gllm_b200 import LLM
@@ -39,7 +41,8 @@ def main():
     llm = LLM(args.model_path, load_format=args.load_format, tp_size=args.tp, pp_size=args.pp, maxp=args.maxp,
               maxd=args.maxd, gpu_memory_util=args.gpu_memory_util, schedule_method=args.schedule_method,
               enable_prefix_caching=args.enable_prefix_caching, max_cuda_graph_bs=args.max_cuda_graph_bs,
-              model_max_length=2048 + 16, tp_mode=args.tp_mode, log_stats=False)
+              model_max_length=2048 + 16, tp_mode=args.tp_mode, log_stats=False, kv_cache_dtype=args.kv_cache_dtype,
+              quantization=args.quantization)
     vocab = llm.loader.config["vocab_size"]
     if args.dataset:
         prompts, outs = from_sharegpt_file(args.dataset, llm.tokenizer, args.num_prompts, args.seed)

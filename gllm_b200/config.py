@@ -46,6 +46,8 @@ class EngineConfig:
     log_stats: bool = True
     tokenizer_path: Optional[str] = None
     dtype: Optional[str] = None               # override the checkpoint's compute dtype (bfloat16 | float32)
+    kv_cache_dtype: Optional[str] = None      # "int4": keys and values held in 4 bits (ops/kv4.py); None: the compute dtype
+    quantization: Optional[str] = None        # "int8": 8-bit linears, weights quantised per output channel while loading
     num_state_slots: Optional[int] = None     # recurrent-state slots (models with per-sequence state); None: auto
 
     @property

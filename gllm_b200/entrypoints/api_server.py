@@ -295,6 +295,10 @@ def make_parser() -> argparse.ArgumentParser:
     p.add_argument("--tp-mode", type=str, default="fused", choices=["fused", "nccl"])
     p.add_argument("--dtype", type=str, default=None, choices=["bfloat16", "float32"],
                    help="override the checkpoint's compute dtype (float32: layer-list decoders only)")
+    p.add_argument("--kv-cache-dtype", type=str, default=None, choices=["auto", "int4"],
+                   help="int4: keys and values held in 4 bits (heads of 64 or 128)")
+    p.add_argument("--quantization", type=str, default=None, choices=["int8"],
+                   help="int8: 8-bit linears, weights quantised per output channel while loading")
     p.add_argument("--num-state-slots", type=int, default=None,
                    help="recurrent-state slots = most sequences running at once (models with per-sequence state)")
     return p
@@ -313,7 +317,8 @@ def engine_kwargs(args) -> dict:
                 max_cuda_graph_bs=args.max_cuda_graph_bs, model_max_length=args.model_max_length,
                 mm_processor_min_pixels=args.mm_processor_min_pixels,
                 mm_processor_max_pixels=args.mm_processor_max_pixels, tp_mode=args.tp_mode,
-                dtype=args.dtype, num_state_slots=args.num_state_slots)
+                dtype=args.dtype, num_state_slots=args.num_state_slots, kv_cache_dtype=args.kv_cache_dtype,
+                quantization=args.quantization)
 
 
 async def run_server(app, host: str, port: int):

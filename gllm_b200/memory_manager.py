@@ -19,25 +19,34 @@ from typing import Dict, List, Optional
 import torch
 
 from gllm_b200.id_allocator import IDAllocator
+from gllm_b200.ops import kv4
 from gllm_b200.ops.ref import kv_cache_shape
 from gllm_b200.sequence import Sequence
 
 
 class KVCache:
-    """Device storage: per-layer K and V tensors (or one latent tensor per layer for MLA)."""
+    """Device storage: per-layer K and V tensors (or one latent tensor per layer for MLA). `four_bit`: held in 4 bits (`ops.kv4`)."""
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, kv_head_num: int, kv_head_dim: int,
-                 dtype: torch.dtype, device, use_mla: bool = False):
+                 dtype: torch.dtype, device, use_mla: bool = False, four_bit: bool = False):
         self.num_layers, self.num_pages, self.page_size = num_layers, num_pages, page_size
         self.kv_head_num, self.kv_head_dim, self.use_mla = kv_head_num, kv_head_dim, use_mla
         heads = 1 if use_mla else kv_head_num
-        shape = kv_cache_shape(num_pages, heads, kv_head_dim, page_size)
+        if four_bit:
+            if use_mla:
+                raise ValueError("a latent cache is not held in 4 bits")
+            shape, dtype = kv4.cache_shape(num_pages, heads, kv_head_dim, page_size), torch.uint8
+        else:
+            shape = kv_cache_shape(num_pages, heads, kv_head_dim, page_size)
         # zero-init: masked / padded positions must hold finite values (attention multiplies them by 0)
         self.k_cache = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
         self.v_cache = [] if use_mla else [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
 
     @staticmethod
-    def bytes_per_page(num_layers, page_size, kv_head_num, kv_head_dim, dtype_bytes, use_mla=False) -> int:
+    def bytes_per_page(num_layers, page_size, kv_head_num, kv_head_dim, dtype_bytes, use_mla=False, four_bit=False) -> int:
+        if four_bit:
+            _, _, blocks, block = kv4.cache_shape(1, kv_head_num, kv_head_dim, page_size)
+            return 2 * num_layers * kv_head_num * blocks * block
         if use_mla:
             return num_layers * page_size * kv_head_dim * dtype_bytes
         return 2 * num_layers * page_size * kv_head_num * kv_head_dim * dtype_bytes

@@ -19,7 +19,7 @@ from gllm_b200.utils.logging import logger
 
 
 class ModelLoader:
-    def __init__(self, model_path, load_format: str = "auto", dtype: Optional[str] = None):
+    def __init__(self, model_path, load_format: str = "auto", dtype: Optional[str] = None, quantization: Optional[str] = None):
         self.model_path = model_path
         self.load_format = load_format
         self.config = self.load_config(model_path)
@@ -27,6 +27,10 @@ class ModelLoader:
             self.config["architectures"] = [self.config["architecture"]]   # single-name form of the key
         if dtype is not None:
             self.config["torch_dtype"] = dtype
+        if quantization not in (None, "int8"):
+            raise ValueError(f"quantization is None or 'int8': got {quantization!r}")
+        if quantization is not None:
+            self.config["weights_int8"] = True
         self.generation_config = self.load_generation_config(model_path)
         self.architecture = self.config["architectures"][0]
         self.use_mla = self.architecture in ("DeepseekV2ForCausalLM", "DeepseekV3ForCausalLM") and \

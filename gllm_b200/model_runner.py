@@ -25,6 +25,7 @@ from gllm_b200.input_data import BatchArrays, InputData
 from gllm_b200.layers import functional as Fn
 from gllm_b200.memory_manager import HybridCache, KVCache
 from gllm_b200.model_loader import ModelLoader
+from gllm_b200.ops import kv4
 from gllm_b200.ops.lib import raise_if_waits_gave_up, watch_waits
 from gllm_b200.parallel import state as ps
 from gllm_b200.parallel.tp import make_tp_comm
@@ -52,7 +53,7 @@ class StepResult:
 class ModelRunner:
     def __init__(self, cfg: EngineConfig, loader: Optional[ModelLoader] = None):
         self.cfg = cfg
-        self.loader = loader or ModelLoader(cfg.model_path, cfg.load_format, dtype=cfg.dtype)
+        self.loader = loader or ModelLoader(cfg.model_path, cfg.load_format, dtype=cfg.dtype, quantization=cfg.quantization)
         self.page_size = cfg.page_size
         self.max_num_batched_tokens = cfg.max_num_batched_tokens
         self.max_running_seqs = cfg.max_running_seqs
@@ -99,8 +100,9 @@ class ModelRunner:
         if self.hybrid and self.model.has_state:
             # one slot per running sequence + the padding slot; the scheduler admits a sequence only with a slot
             self.num_state_slots = (cfg.num_state_slots or min(max(self.max_running_seqs, 1), 256)) + 1
+        self.four_bit = self._four_bit_cache()
         want_fused = cfg.tp_mode == "fused" and cfg.tp_size > 1 and is_cuda
-        why_not = "fp8 block-scaled linears" if getattr(self.spec, "quant", None) is not None else \
+        why_not = f"{self.spec.quant} linears" if getattr(self.spec, "quant", None) is not None else \
             "DeepStack (Qwen3-VL) feature injection" if getattr(self.model, "num_deepstack", 0) else None
         if want_fused and why_not:
             logger.warning("tp_mode=fused is not available with %s: tensor-parallel collectives run on NCCL", why_not)
@@ -144,10 +146,22 @@ class ModelRunner:
         else:
             kvh, kvd = self.kv_shape()
             self.kv_cache = KVCache(self.model.num_layers, self.num_pages, self.page_size, kvh, kvd, dt, self.device,
-                                    use_mla=self.loader.use_mla)
+                                    use_mla=self.loader.use_mla, four_bit=self.four_bit)
         if is_cuda and not cfg.disable_cuda_graph:
             self.capture_graphs()
         return self
+
+    def _four_bit_cache(self) -> bool:
+        """Whether the cache is held in 4 bits; raises where the model or the page size does not allow what was asked for."""
+        if self.cfg.kv_cache_dtype in (None, "auto"):
+            return False
+        if self.cfg.kv_cache_dtype != "int4":
+            raise ValueError(f"kv_cache_dtype is None, 'auto' or 'int4': got {self.cfg.kv_cache_dtype!r}")
+        if self.hybrid or self.loader.use_mla:
+            raise ValueError(f"{self.loader.architecture}: a 4-bit cache holds the keys and values of decoders with paged "
+                             "grouped-query attention")
+        kv4.cache_shape(1, *self.kv_shape(), self.page_size)
+        return True
 
     def kv_shape(self):
         if self.loader.use_mla:
@@ -174,7 +188,8 @@ class ModelRunner:
             return self._hybrid_num_pages()
         kvh, kvd = self.kv_shape()
         per_page = KVCache.bytes_per_page(self.model.num_layers, self.page_size, kvh, kvd,
-                                          torch.empty(0, dtype=self.spec.dtype).element_size(), self.loader.use_mla)
+                                          torch.empty(0, dtype=self.spec.dtype).element_size(), self.loader.use_mla,
+                                          four_bit=self.four_bit)
         if self.device.type != "cuda":
             num = cfg.num_cpu_pages
         elif cfg.num_gpu_pages is not None:
@@ -184,6 +199,9 @@ class ModelRunner:
             free, _ = torch.cuda.mem_get_info(self.device)
             # what the layers allocate beside the cache, and the probe, which runs without one, has not seen
             free -= getattr(self.model, "step_scratch_bytes", lambda max_len: 0)(self.model_max_length)
+            if self.four_bit:
+                from gllm_b200.ops import sm100_kv4
+                free -= sm100_kv4.scratch_bytes(kvh, kvd, self.model_max_length)
             num = int((max(free, 0) // max(per_page, 1)) * cfg.gpu_memory_util)
         if ps.get_world_size() > 1 and torch.distributed.is_initialized():
             all_n = [None] * ps.get_world_size()
@@ -269,6 +287,7 @@ class ModelRunner:
         from gllm_b200.ops import sm100
         if not self.hybrid:
             kvh, _ = self.kv_shape()
+        if not self.hybrid and not self.four_bit:         # attention over a 4-bit cache takes its scratch per call
             sm100.reserve_attn_workspace(self.device, max(self.capture_sizes or [1]),
                                          self.model.layers[0].attn.num_heads if len(self.model.layers) else 1,
                                          self.model.head_dim)

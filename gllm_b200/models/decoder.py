@@ -75,7 +75,8 @@ class ModelSpec:
     names: Dict[str, str] = field(default_factory=dict)
     eos_token_id: Optional[object] = None
     extra: dict = field(default_factory=dict)
-    quant: Optional[str] = None  # "fp8": block-scaled e4m3 linears (HF quantization_config, 128x128 blocks)
+    # "fp8": block-scaled e4m3 linears (HF quantization_config, 128x128 blocks); "int8": 8-bit linears, a scale per output channel
+    quant: Optional[str] = None
 
     def is_moe_layer(self, layer_id: int) -> bool:
         if self.moe is None:
@@ -108,7 +109,12 @@ def _param(*shape, dtype, device, std=0.02, fill=None):
 
 
 def _linear_params(n: int, k: int, spec: ModelSpec, device):
-    """(weight, scale_inv | None): bf16 [n, k], or e4m3 [n, k] + fp32 block scales for fp8 checkpoints."""
+    """(weight, scale_inv | None): bf16 [n, k], or e4m3 [n, k] + fp32 block scales for fp8 checkpoints, or int8 [n, k] + fp32 [n]."""
+    if spec.quant == "int8":
+        if n % 8 or k % 16:
+            raise ValueError(f"an 8-bit linear of {n} x {k}: rows come in multiples of 8, columns of 16")
+        return (nn.Parameter(torch.zeros(n, k, dtype=torch.int8, device=device), requires_grad=False),
+                nn.Parameter(torch.ones(n, dtype=torch.float32, device=device), requires_grad=False))
     if spec.quant == "fp8" and k % 128 == 0:      # activations are quantised per 128-wide K group
         w = nn.Parameter(torch.zeros(n, k, dtype=torch.float8_e4m3fn, device=device), requires_grad=False)
         s = nn.Parameter(torch.ones((n + 127) // 128, (k + 127) // 128, dtype=torch.float32, device=device),
@@ -122,12 +128,43 @@ def _qw(w, s):
     return w if s is None else (w, s)
 
 
-def _store_linear(w_param, s_param, w: torch.Tensor):
+def _linear_weight(reader, name: str, quant: Optional[str]):
+    """A checkpoint's linear weight: a tensor, or, where it is held in 8 bits, (int8 [N, K], fp32 scales [N, 1])."""
+    if quant == "int8" and reader.has(name + "_scale"):
+        return reader.get_raw(name), reader.get_raw(name + "_scale").float().reshape(-1, 1)
+    return reader.get(name)
+
+
+def _by_rows(fn, *ws):
+    """fn of weights that it takes rows of: of the values and of the scales where they are pairs."""
+    pairs = [isinstance(w, tuple) for w in ws]
+    if not any(pairs):
+        return fn(*ws)
+    if not all(pairs):
+        raise ValueError("projections that are multiplied together, some held in 8 bits and some not")
+    return fn(*(w[0] for w in ws)), fn(*(w[1] for w in ws))
+
+
+def _by_cols(fn, w):
+    """fn of a weight that it takes columns of: every output channel keeps its scale."""
+    return (fn(w[0]), w[1]) if isinstance(w, tuple) else fn(w)
+
+
+def _store_linear(w_param, s_param, w):
     """Copy a (sharded) weight into its parameter; fp8 parameters are block-quantised here (128x128 blocks,
     scale_inv = amax / 448). Re-quantising the de-quantised tensor of an fp8 checkpoint is lossless as long
     as shard boundaries fall on block boundaries (they do: head_dim 128, intermediate % 128 == 0)."""
     if s_param is None:
         w_param.data.copy_(w)
+        return
+    if w_param.dtype == torch.int8:      # pairs as they are; other weights quantised per output channel, scale = amax / 127
+        if not isinstance(w, tuple):
+            w = w.float()
+            s = (w.abs().amax(1, keepdim=True) / 127).clamp_min(1e-12)
+            w = torch.round(w / s).to(torch.int8), s
+        assert w[0].dtype == torch.int8 and w[0].shape == w_param.shape and w[1].shape == (w_param.shape[0], 1), (w[0].shape, w[1].shape)
+        w_param.data.copy_(w[0])
+        s_param.data.copy_(w[1][:, 0])
         return
     w = w.float()
     n, k = w.shape
@@ -194,10 +231,10 @@ class DenseMLP(nn.Module):
         tp = ps.get_tp_size() if shard else 1
         assert intermediate % tp == 0
         self.inter = intermediate // tp
-        fp8 = spec is not None and spec.quant == "fp8"
-        # fused SiLU-gate epilogue needs the gate/up rows interleaved per 128 (bf16 kernel only)
-        self.fused_act = self.inter % 128 == 0 and not fp8
-        if fp8:
+        quantised = spec is not None and spec.quant in ("fp8", "int8")
+        # fused SiLU-gate epilogue needs the gate/up rows interleaved per 128 (bf16 kernel only; the others take them as they are)
+        self.fused_act = self.inter % 128 == 0 and not quantised
+        if quantised:
             self.gate_up_w, self.gate_up_ws = _linear_params(2 * self.inter, hidden, spec, device)
             self.down_w, self.down_ws = _linear_params(hidden, self.inter, spec, device)
         else:
@@ -422,6 +459,10 @@ class CausalLM(nn.Module):
         for name, p in self.named_parameters():
             if name.endswith("norm_w"):
                 p.data.fill_(1.0)
+            elif p.dtype == torch.int8:
+                p.data.copy_(torch.randn(p.shape, device=p.device, generator=None if p.is_cuda else g).mul_(32).round_().clamp_(-127, 127))
+            elif name.endswith("_ws") and p.dim() == 1:
+                p.data.fill_(0.02 / 32)
             elif p.dim() == 1:
                 p.data.zero_()
             elif name.endswith("router_w") or name.endswith("shared_gate_w"):
@@ -486,14 +527,14 @@ class CausalLM(nn.Module):
 
     def _load_attention(self, reader, pre, nm, at: Attention):
         spec, tp, tr, d = self.spec, self.tp_size, self.tp_rank, self.spec.head_dim
+        sizes = [spec.num_heads * d, spec.num_kv_heads * d, spec.num_kv_heads * d]
         if "qkv_fused" in nm:  # ChatGLM: one [ (hq + 2 hkv) * D, H ] tensor
-            w = reader.get(pre + nm["qkv_fused"] + ".weight")
-            q, k, v = w.split([spec.num_heads * d, spec.num_kv_heads * d, spec.num_kv_heads * d], dim=0)
+            w = _linear_weight(reader, pre + nm["qkv_fused"] + ".weight", spec.quant)
+            q, k, v = (_by_rows(lambda x, i=i: x.split(sizes, dim=0)[i], w) for i in range(3))
         else:
-            q = reader.get(pre + nm["q"] + ".weight")
-            k = reader.get(pre + nm["k"] + ".weight")
-            v = reader.get(pre + nm["v"] + ".weight")
-        _store_linear(at.qkv_w, at.qkv_ws, wu.shard_qkv(q, k, v, spec.num_heads, spec.num_kv_heads, d, tr, tp))
+            q, k, v = (_linear_weight(reader, pre + nm[x] + ".weight", spec.quant) for x in ("q", "k", "v"))
+        _store_linear(at.qkv_w, at.qkv_ws,
+                      _by_rows(lambda *ws: wu.shard_qkv(*ws, spec.num_heads, spec.num_kv_heads, d, tr, tp), q, k, v))
         if at.qkv_b is not None:
             if "qkv_fused" in nm:
                 b = reader.get(pre + nm["qkv_fused"] + ".bias")
@@ -501,7 +542,8 @@ class CausalLM(nn.Module):
             else:
                 qb, kb, vb = (reader.get(pre + nm[x] + ".bias") for x in ("q", "k", "v"))
             at.qkv_b.data.copy_(wu.shard_qkv(qb, kb, vb, spec.num_heads, spec.num_kv_heads, d, tr, tp))
-        _store_linear(at.o_w, at.o_ws, wu.shard_cols(reader.get(pre + nm["o"] + ".weight"), tr, tp))
+        _store_linear(at.o_w, at.o_ws, _by_cols(lambda w: wu.shard_cols(w, tr, tp),
+                                                _linear_weight(reader, pre + nm["o"] + ".weight", spec.quant)))
         if at.o_b is not None:
             at.o_b.data.copy_(reader.get(pre + nm["o"] + ".bias"))
         if at.q_norm_w is not None:
@@ -511,10 +553,11 @@ class CausalLM(nn.Module):
     def _load_dense_mlp(self, reader, pre, nm, mlp: DenseMLP):
         tp, tr = self.tp_size, self.tp_rank
         if "gate_up_fused" in nm:  # ChatGLM dense_h_to_4h = [gate; up]
-            w = reader.get(pre + nm["gate_up_fused"] + ".weight")
-            gate, up = w.chunk(2, dim=0)
+            w = _linear_weight(reader, pre + nm["gate_up_fused"] + ".weight", self.spec.quant)
+            gate, up = (_by_rows(lambda x, i=i: x.chunk(2, dim=0)[i], w) for i in range(2))
         else:
-            gate = reader.get(pre + nm["gate"] + ".weight")
-            up = reader.get(pre + nm["up"] + ".weight")
-        mlp.set_gate_up(wu.shard_gate_up(gate, up, tr, tp))
-        _store_linear(mlp.down_w, mlp.down_ws, wu.shard_cols(reader.get(pre + nm["down"] + ".weight"), tr, tp))
+            gate = _linear_weight(reader, pre + nm["gate"] + ".weight", self.spec.quant)
+            up = _linear_weight(reader, pre + nm["up"] + ".weight", self.spec.quant)
+        mlp.set_gate_up(_by_rows(lambda *ws: wu.shard_gate_up(*ws, tr, tp), gate, up))
+        _store_linear(mlp.down_w, mlp.down_ws, _by_cols(lambda w: wu.shard_cols(w, tr, tp),
+                                                        _linear_weight(reader, pre + nm["down"] + ".weight", self.spec.quant)))

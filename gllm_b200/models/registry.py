@@ -38,6 +38,26 @@ def _dtype(cfg) -> torch.dtype:
     return _DTYPES.get(d, torch.bfloat16)
 
 
+def _int8_checkpoint(qc: dict) -> bool:
+    """Whether a `quantization_config` describes 8-bit linears with a scale per output channel and one per token, formed as it comes."""
+    if qc.get("quant_method") != "compressed-tensors" or qc.get("format") != "int-quantized":
+        return False
+    groups = list((qc.get("config_groups") or {}).values())
+    if len(groups) != 1:
+        return False
+    w, x = (groups[0].get(k) or {} for k in ("weights", "input_activations"))
+    return all(p.get("num_bits") == 8 and p.get("type") == "int" and p.get("symmetric", True) for p in (w, x)) and \
+        w.get("strategy") == "channel" and x.get("strategy") == "token" and bool(x.get("dynamic"))
+
+
+def _quant(cfg: HFConfig):
+    """How the linears of a checkpoint are held: "fp8", "int8" or None (as the compute dtype)."""
+    qc = cfg.get("quantization_config") or {}
+    if qc.get("quant_method") == "fp8" and list(qc.get("weight_block_size") or []) == [128, 128]:
+        return "fp8"
+    return "int8" if cfg.get("weights_int8") or _int8_checkpoint(qc) else None
+
+
 def _base_spec(cfg: HFConfig, arch: str, **kw) -> ModelSpec:
     heads = cfg["num_attention_heads"]
     hidden = cfg["hidden_size"]
@@ -57,9 +77,7 @@ def _base_spec(cfg: HFConfig, arch: str, **kw) -> ModelSpec:
         max_position=cfg.get("max_position_embeddings", 8192), rope_theta=rope_theta,
         rope_scaling=dict(rope_scaling) if rope_scaling else None, dtype=_dtype(cfg),
         eos_token_id=cfg.get("eos_token_id"))
-    qc = cfg.get("quantization_config") or {}
-    if qc.get("quant_method") == "fp8" and list(qc.get("weight_block_size") or []) == [128, 128]:
-        spec.quant = "fp8"
+    spec.quant = _quant(cfg)
     for k, v in kw.items():
         setattr(spec, k, v)
     return spec
@@ -128,7 +146,8 @@ def spec_chatglm(cfg):
         intermediate_size=cfg["ffn_hidden_size"], vocab_size=cfg.get("padded_vocab_size", cfg.get("vocab_size")),
         rms_eps=cfg.get("layernorm_epsilon", 1e-5), qkv_bias=bool(cfg.get("add_qkv_bias", False)),
         max_position=cfg.get("seq_length", 8192), rope_theta=10000.0 * cfg.get("rope_ratio", 1.0),
-        rot_dim=head_dim // 2, rope_neox=False, dtype=_dtype(cfg), eos_token_id=cfg.get("eos_token_id"))
+        rot_dim=head_dim // 2, rope_neox=False, dtype=_dtype(cfg), eos_token_id=cfg.get("eos_token_id"),
+        quant="int8" if _quant(cfg) == "int8" else None)
     spec.names = {
         "embed": "transformer.embedding.word_embeddings.weight",
         "final_norm": "transformer.encoder.final_layernorm.weight",
@@ -143,6 +162,8 @@ def spec_chatglm(cfg):
 def _build_decoder(spec_fn):
     def build(cfg, device):
         from gllm_b200.layers.moe import make_moe_block
+        if _quant(cfg) == "int8" and spec_fn(cfg).moe is not None:
+            raise ValueError(f"{cfg['architectures'][0]}: routed experts have no 8-bit form")
         return CausalLM(spec_fn(cfg), device, moe_factory=make_moe_block)
     return build
 
@@ -237,4 +258,7 @@ def build_model(cfg: HFConfig, device):
     arch = cfg["architectures"][0]
     if arch not in ARCHITECTURES:
         raise ValueError(f"unsupported architecture {arch}; supported: {sorted(ARCHITECTURES)}")
-    return ARCHITECTURES[arch](cfg, device)
+    model = ARCHITECTURES[arch](cfg, device)
+    if (cfg.get("weights_int8") or _quant(cfg) == "int8") and getattr(model.spec, "quant", None) != "int8":
+        raise ValueError(f"{arch}{' in fp8' if _quant(cfg) == 'fp8' else ''} has no 8-bit linears")
+    return model

@@ -60,9 +60,9 @@ def _order(dim: int):
 
 
 def encode(x: torch.Tensor):
-    """Rows [..., D] -> (codes [..., D / 2], pairs [..., D / 16]), bytes."""
+    """Rows [..., D] (rounded to bf16 first) -> (codes [..., D / 2], pairs [..., D / 16]), bytes."""
     d = x.shape[-1]
-    y = x.float().unflatten(-1, (d // 64, 64))
+    y = x.to(torch.bfloat16).float().unflatten(-1, (d // 64, 64))
     low, high = y.amin(-1, keepdim=True), y.amax(-1, keepdim=True)
     scale = ((high - low) / 15).to(torch.bfloat16).float()
     scale = torch.where(torch.isfinite(scale), scale, torch.nan)

@@ -115,6 +115,11 @@ def _decode_scratch(d: int) -> int:
     return _lib.load().gllm_kv4_decode_scratch(d, _DECODE_CTAS)
 
 
+def scratch_bytes(kv_heads: int, d: int, max_len: int) -> int:
+    """The most that one step's `paged_attention` allocates beside its result: expanded tiles of prompts, parts of decoding sequences."""
+    return max(EXPAND_BYTES, 4 * kv_heads * d * (max_len + 63)) + _DECODE_CTAS * (2 * 16 * (d + 2) * 4 + 16) + (1 << 20)
+
+
 def expand_rounds(lens, token_bytes: int, limit: int = EXPAND_BYTES):
     """(first, end, tiles of 64 tokens) of consecutive sequences whose expanded keys and values stay below `limit` bytes together, one
     sequence at least. lens: their lengths, on the host."""
