@@ -21,9 +21,9 @@
 //   scores: keys g, g + 8 of heads 2t, 2t + 1; movmatrix turns the probabilities into the second product's operand
 //
 // A warp walks tiles of 32 keys by itself: it copies them (cp.async.bulk, one contiguous block of 9 D bytes for 16 tokens' keys or
-// values) into its own ring, two tiles deep. The tiles of all sequences and heads lie in one row, which is cut into equal
-// shares, one per CTA, on the device: ragged batches and few long sequences fill the machine alike. The eight warps of a CTA take
-// its tiles in turn and sum up in shared memory where a sequence's head ends; what a share has of a head that goes on in another
+// values) into its own ring, two tiles deep. The tiles of all sequences and heads lie in one row, which is cut into equal shares on the
+// device, for CTAs and then for their warps: ragged batches, many short sequences and few long ones fill the machine alike. A head that
+// lies in one warp's share is finished there; the warps of a CTA add their parts of others up at its end, once; what goes on in another
 // CTA goes to scratch, and a second kernel joins it.
 //
 // The reference follows only when a score passes the head's maximum by 2^8 or a scale the largest one (one vote instead of shuffles).
@@ -64,9 +64,10 @@ struct Kv4Smem {
   static constexpr int kBlock = 9 * D;                   // 16 tokens' keys or values
   static constexpr int kStage = 4 * kBlock;
   static constexpr int kRing = kV4Warps * kV4Stages * kStage;
-  static constexpr int kSums = 4 * 32 * (D / 16 * 4 * NT) * 4;    // four warps' sums
-  static constexpr int kMl = kV4Warps * 8 * NT * 2 * 4;
-  static constexpr int kBytes = kRing + kSums + kMl + kV4Lens * 4 + kV4Warps * kV4Stages * 8 + 64;
+  static constexpr int kSums = kV4Warps * 32 * (D / 16 * 4 * NT) * 4;
+  static_assert(kSums / kV4Warps <= kV4Stages * kStage, "a warp's last part takes its ring's place");
+  static constexpr int kMl = 2 * kV4Warps * 8 * NT * 2 * 4;
+  static constexpr int kBytes = kRing + kSums + kMl + kV4Lens * 4 + kV4Warps * (kV4Stages * 8 + 32) + 64;
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -114,11 +115,13 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   constexpr int GR = D / 64;                             // groups of a head
   constexpr int KS = D / 16;                             // 16-dim steps of the first product, and dim tiles of the second
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sums = reinterpret_cast<float*>(smem + SM::kRing);
-  float* ml = reinterpret_cast<float*>(smem + SM::kRing + SM::kSums);              // [warp][head][m, l]
+  constexpr int kPieces = NT * GR * 4;                   // of a part: four sums a lane
+  float4* firsts = reinterpret_cast<float4*>(smem + SM::kRing);                    // [warp][piece][lane]: parts that an earlier warp starts
+  float* ml = reinterpret_cast<float*>(smem + SM::kRing + SM::kSums);              // [first or last][warp][head][base, l]
   int* lens = reinterpret_cast<int*>(smem + SM::kRing + SM::kSums + SM::kMl);
   uint64_t* bars = reinterpret_cast<uint64_t*>(lens + kV4Lens);
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + kV4Warps * kV4Stages);      // gave up, first sequence, its first tile
+  int4* info = reinterpret_cast<int4*>(bars + kV4Warps * kV4Stages);               // [first or last][warp] (sequence or -1, head group, ends, last CTA)
+  uint32_t* words = reinterpret_cast<uint32_t*>(info + 2 * kV4Warps);              // gave up, first sequence, its first tile
   const WaitGuard guard{words, p.waits};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
@@ -205,22 +208,32 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     x.n = kv4_tiles(x.len);
   };
 
-  // ---- copies. The warp's tiles are the share's warp-th, (warp + 8)-th ...; eight of them are prepared at a time, a block a lane: tile
-  // lane / 4, keys or values, 16 tokens. A table entry that is no page reads another one.
+  auto settle = [&](Place& x, int& tile) {               // tile counted from x's first: into the head group that it lies in
+    while (tile >= x.n && x.seq < p.B) {
+      tile -= x.n;
+      next_head(x);
+    }
+  };
+  // This warp's part [my_begin, my_end) of the share.
+  const int per_warp = (tiles + kV4Warps - 1) / kV4Warps, my_begin = min(tiles, warp * per_warp), my_end = min(tiles, my_begin + per_warp);
+  const uint32_t my_tiles = static_cast<uint32_t>(my_end - my_begin);
+  at_tile += my_begin;
+  settle(at, at_tile);
+  if (lane < 2) info[lane * kV4Warps + warp] = make_int4(-1, 0, 0, 0);
+  __syncwarp();
+
+  // ---- copies. Eight of the warp's tiles are prepared at a time, a block a lane: tile lane / 4, keys or values, 16 tokens. A table entry
+  // that is no page reads another one.
   const uint32_t ring = smem_u32(smem) + warp * (kV4Stages * SM::kStage);
   uint64_t* bar = bars + warp * kV4Stages;
-  const uint32_t my_tiles = static_cast<uint32_t>(max(0, (tiles - warp + kV4Warps - 1) / kV4Warps));
   Place fetch = at;                                      // of this lane's next block
-  int fetch_x = warp + kV4Warps * (lane >> 2), fetch_tile = at_tile + fetch_x;
+  int fetch_x = my_begin + (lane >> 2), fetch_tile = at_tile + (lane >> 2);
   const uint8_t* src = nullptr;
   int blocks = 0;                                        // of this lane's tile (none: an empty sequence)
   auto prepare = [&] {
-    while (fetch_tile >= fetch.n && fetch.seq < p.B) {
-      fetch_tile -= fetch.n;
-      next_head(fetch);
-    }
+    settle(fetch, fetch_tile);
     blocks = 0;
-    if (fetch_x < tiles) {
+    if (fetch_x < my_end) {
       const int blk = 2 * fetch_tile + (lane & 1);
       blocks = min(2, (fetch.len - fetch_tile * kV4Keys + 15) / 16);
       if ((lane & 1) < blocks) {
@@ -231,8 +244,8 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
               ((static_cast<uint64_t>(page) * p.Hkv + fetch.head / hg) * p.page_blocks + (blk - i * p.page_blocks)) * SM::kBlock;
       }
     }
-    fetch_x += 8 * kV4Warps;
-    fetch_tile += 8 * kV4Warps;
+    fetch_x += 8;
+    fetch_tile += 8;
   };
   uint32_t issued = 0, used = 0;
   auto issue = [&](int stage) {
@@ -251,13 +264,11 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     if (issued < my_tiles) issue(s);
 
   // ---- segment by segment (the tiles of one head group of one sequence)
-  int mine = warp;                                       // this warp's next tile of the share
   bool ok = true;
-  if (guard.cfg.limit_ns == 0) ok = __all_sync(0xffffffffu, mine >= tiles || guard.first(&bar[0]));
-  int seg = 0;
-  while (seg < tiles) {
-    const int seg_end = min(tiles, seg + (at.n - at_tile));
-    const bool whole = at_tile == 0 && seg_end - seg == at.n;
+  if (guard.cfg.limit_ns == 0) ok = __all_sync(0xffffffffu, my_tiles == 0 || guard.first(&bar[0]));
+  int seg = my_begin;
+  while (seg < my_end) {
+    const int seg_end = min(my_end, seg + (at.n - at_tile));
     const int len = at.len;
     const int head0 = at.head / hg * p.G + at.head % hg * p.GP;
     const __nv_bfloat16* q = p.q + at.seq * p.q_ts + static_cast<int64_t>(head0) * D;
@@ -343,9 +354,9 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       }
     }
 
-    for (; mine < seg_end && ok; mine += kV4Warps) {
+    for (int tile = at_tile; tile < at_tile + seg_end - seg && ok; ++tile) {
       const int stage = used % kV4Stages;
-      const int key0 = (at_tile + mine - seg) * kV4Keys;
+      const int key0 = tile * kV4Keys;
       ok = __all_sync(0xffffffffu, guard.wait(&bar[stage], (used / kV4Stages) & 1));
       if (!ok) break;
       const uint32_t kb = ring + stage * SM::kStage, vb = kb + 2 * SM::kBlock;
@@ -511,7 +522,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       if (issued < my_tiles) issue(stage);
     }
 
-    // ---- the warps' sums together; l and lows are of this lane's keys so far
+    // ---- the head group's end, or this warp's: l and lows are of this lane's keys so far
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -527,112 +538,91 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
           o[nt][i][c] = fmaf(o[nt][i][c] - o[nt][i][2 + c], 16777216.f, lows[nt][i / 4][c]);
           o[nt][i][2 + c] = fmaf(o[nt][i][2 + c], 1048576.f, lows[nt][i / 4][c]);
         }
-        if (m[nt][c] == -INFINITY) base[nt][c] = -INFINITY;          // no keys: no part in the join
-        if (g == 0) {
-          float* x = ml + (warp * 8 * NT + nt * 8 + 2 * t + c) * 2;
-          x[0] = base[nt][c];
-          x[1] = l[nt][c];
-        }
+        if (m[nt][c] == -INFINITY) base[nt][c] = -INFINITY;          // no keys: no part in a sum
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kV4Warps; ++w) x = fmaxf(x, ml[(w * 8 * NT + nt * 8 + 2 * t + c) * 2]);
-        const float f = base[nt][c] == -INFINITY ? 0.f : exp2f(base[nt][c] - x);
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          o[nt][i][c] *= f;
-          o[nt][i][2 + c] *= f;
-        }
-      }
-    }
-    // sums[w][nt][head c][4 sums a lane at a time][lane]: eight dims of a group of one head are two pieces
-    auto piece = [&](int w, int nt, int gr, int c, int half) {
-      return reinterpret_cast<float4*>(sums) + (((w * NT + nt) * GR + gr) * 4 + c * 2 + half) * 32 + lane;
-    };
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int gr = 0; gr < GR; ++gr) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (warp >= 4)
-              *piece(warp - 4, nt, gr, c, half) = make_float4(o[nt][gr * 4 + 2 * half][c], o[nt][gr * 4 + 2 * half][2 + c],
-                                                              o[nt][gr * 4 + 2 * half + 1][c], o[nt][gr * 4 + 2 * half + 1][2 + c]);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    if (warp < 4) {
+    const bool starts = at_tile == 0, ends = at_tile + seg_end - seg == at.n;
+    if (starts && ends) {                                // all of it: eight dims of a group of heads 2t, 2t + 1 a lane
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) {
+        for (int c = 0; c < 2; ++c) {
+          const int h = 8 * nt + 2 * t + c;
+          const float inv = l[nt][c] > 0.f || l[nt][c] != l[nt][c] ? 1.f / l[nt][c] : 0.f;       // no keys: zeros
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int gr = 0; gr < GR; ++gr) {
+            uint32_t w[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float4* x = piece(warp, nt, gr, c, half);
-              float4 v = *x;
-              v.x += o[nt][gr * 4 + 2 * half][c];
-              v.y += o[nt][gr * 4 + 2 * half][2 + c];
-              v.z += o[nt][gr * 4 + 2 * half + 1][c];
-              v.w += o[nt][gr * 4 + 2 * half + 1][2 + c];
-              *x = v;
-            }
+            for (int i = 0; i < 4; ++i) w[i] = pack_bf16(o[nt][gr * 4 + i][c] * inv, o[nt][gr * 4 + i][2 + c] * inv);
+            if (h < p.GP)
+              *reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(at.seq) * p.Hq + head0 + h) * D + gr * 64 + 8 * g) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
+    } else {
+      // a part: what does not start here goes to `firsts` (a warp's first part), what does is the warp's last and takes its ring's place
+      float4* to = starts ? reinterpret_cast<float4*>(smem + warp * (kV4Stages * SM::kStage)) : firsts + warp * kPieces * 32;
+      float* to_ml = ml + ((starts ? kV4Warps : 0) + warp) * 16 * NT;
+      if (lane == 0)
+        info[(starts ? kV4Warps : 0) + warp] = make_int4(at.seq, at.head, ends ? 1 : 0, starts ? static_cast<int>((begin + seg + at.n - 1) / share) : 0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (g == 0) *reinterpret_cast<float2*>(to_ml + (nt * 8 + 2 * t + c) * 2) = make_float2(base[nt][c], l[nt][c]);
+#pragma unroll
+          for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              to[((nt * GR + gr) * 4 + c * 2 + half) * 32 + lane] =
+                  make_float4(o[nt][gr * 4 + 2 * half][c], o[nt][gr * 4 + 2 * half][2 + c], o[nt][gr * 4 + 2 * half + 1][c],
+                              o[nt][gr * 4 + 2 * half + 1][2 + c]);
+        }
+      }
     }
-    __syncthreads();
-    // a piece (four dims of a head) a thread: sum of the four, then the result or this share's part of it
-    const int slot = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
-    constexpr int kPieces = NT * GR * 4;
+    at_tile = 0;                                         // only a warp's last head group ends after it does
+    next_head(at);
+    seg = seg_end;
+  }
+  __syncthreads();
+  // ---- the parts of this CTA's warps: a row starts with a warp's last part, or with what the CTA before began, and goes on through
+  // the first parts of the warps behind. Four dims of a head a thread.
+  for (int row = -1; row < kV4Warps; ++row) {
+    if (row >= 0 && info[kV4Warps + row].x < 0) continue;
+    int last = row;                                      // the last warp with a part
+    bool done = false;
+    while (!done && last + 1 < kV4Warps && info[last + 1].x >= 0) done = info[++last].z != 0;
+    if (row < 0 && last < 0) continue;
+    const int4 what = row < 0 ? info[0] : info[kV4Warps + row];
+    const int head0 = what.y / hg * p.G + what.y % hg * p.GP, slot = 2 * static_cast<int>(blockIdx.x) + (row < 0 ? 0 : 1);
     for (int x = warp; x < kPieces; x += kV4Warps) {
       const int nt = x / (GR * 4), gr = x / 4 % GR, c = x / 2 % 2, half = x % 2;
       const int h = 8 * nt + 2 * t + c, dim = gr * 64 + 8 * g + 4 * half;
-      float4 v = *piece(0, nt, gr, c, half);
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        const float4 y = *piece(w, nt, gr, c, half);
-        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-      }
-      float mm = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kV4Warps; ++w) mm = fmaxf(mm, ml[(w * 8 * NT + h) * 2]);
-#pragma unroll
-      for (int w = 0; w < kV4Warps; ++w) {
-        const float mw = ml[(w * 8 * NT + h) * 2];
-        if (mw != -INFINITY) sum = fmaf(ml[(w * 8 * NT + h) * 2 + 1], exp2f(mw - mm), sum);
+      float top = -INFINITY, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = max(row, 0); w <= last; ++w)
+        top = fmaxf(top, ml[((w == row ? kV4Warps : 0) + w) * 16 * NT + h * 2]);
+      for (int w = max(row, 0); w <= last; ++w) {
+        const float2 y = *reinterpret_cast<const float2*>(ml + ((w == row ? kV4Warps : 0) + w) * 16 * NT + h * 2);
+        const float4* from = w == row ? reinterpret_cast<const float4*>(smem + w * (kV4Stages * SM::kStage)) : firsts + w * kPieces * 32;
+        const float4 z = from[x * 32 + lane];
+        const float f = y.x == -INFINITY ? 0.f : exp2f(y.x - top);
+        sum = fmaf(y.y, f, sum);
+        v.x = fmaf(z.x, f, v.x); v.y = fmaf(z.y, f, v.y); v.z = fmaf(z.z, f, v.z); v.w = fmaf(z.w, f, v.w);
       }
       if (h < p.GP) {
-        if (whole) {
-          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;       // no keys: zeros
-          *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(at.seq) * p.Hq + head0 + h) * D + dim) =
+        if (row >= 0 && done) {
+          const float inv = 1.f / sum;
+          *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(what.x) * p.Hq + head0 + h) * D + dim) =
               make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
         } else {
           *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 8 * NT + h) * D + dim) = v;
-          if (g == 0 && gr == 0 && half == 0) {
-            p.part_ml[(slot * 8 * NT + h) * 2] = mm;
-            p.part_ml[(slot * 8 * NT + h) * 2 + 1] = sum;
-          }
+          if (g == 0 && gr == 0 && half == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 8 * NT + h) * 2) = make_float2(top, sum);
         }
       }
     }
-    if (tid == 0 && at_tile == 0 && !whole)              // it ends with this share and goes on in the next
-      p.meta[blockIdx.x] = make_int4(at.seq, at.head, static_cast<int>((begin + seg + at.n - 1) / share), slot);
-    __syncthreads();                                     // the pieces and factors have been read
-    at_tile = 0;                                         // only a share's last segment ends before its head group does
-    next_head(at);
-    seg = seg_end;
+    if (row >= 0 && !done && tid == 0) p.meta[blockIdx.x] = make_int4(what.x, what.y, what.w, slot);     // goes on in the next share
   }
   // copies in flight land before the CTA ends, where the waits were given up
   for (; used < issued; ++used) guard.land(&bar[used % kV4Stages], (used / kV4Stages) & 1);
