@@ -629,47 +629,68 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
 }
 
 // Joins the parts of a head group that several CTAs share: one CTA for each that starts one and does not end it. A thread has four dims of a
-// head; factors and sums of several parts are on their way at a time.
-constexpr int kV4JoinThreads = 256;
-template <int D, int NT>
-__global__ void __launch_bounds__(kV4JoinThreads) kv4_join_kernel(const Kv4Params p) {
+// head and every WAYS-th part; three parts' sums are on their way at a time. Four ways where few head groups have many parts (one sequence
+// of 80 thousand, 64 / 8 heads: 45 -> 38 us in all), one where many have two (64 of some 500: 21 us, 23 in four).
+template <int D, int NT, int WAYS>
+__global__ void __launch_bounds__(256 * WAYS) kv4_join_kernel(const Kv4Params p) {
+  __shared__ float4 sums[WAYS][256];
+  __shared__ float2 tops[WAYS][256];
   griddep_launch();
   griddep_wait();
   const int4 meta = p.meta[blockIdx.x];                  // sequence, head group, last CTA, slot of the first part
   if (meta.x < 0) return;
   const int hg = p.G / p.GP, parts = meta.z - static_cast<int>(blockIdx.x) + 1;
-  const int head0 = meta.y / hg * p.G + meta.y % hg * p.GP;
-  for (int i = threadIdx.x; i < p.GP * (D / 4); i += kV4JoinThreads) {
-    const int h = i / (D / 4), d = i % (D / 4) * 4;
+  const int head0 = meta.y / hg * p.G + meta.y % hg * p.GP, way = WAYS == 1 ? 0 : threadIdx.x / 256, at = threadIdx.x % 256;
+  for (int i0 = 0; i0 < p.GP * (D / 4); i0 += 256) {
+    const int i = i0 + at, h = i / (D / 4), d = i % (D / 4) * 4;
+    const bool in = h < p.GP;
     float m = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int n0 = 0; n0 < parts; n0 += 4) {
-      float2 ml[4];
-      float4 o[4];
+    for (int n0 = way; in && n0 < parts; n0 += 3 * WAYS) {
+      float2 ml[3];
+      float4 o[3];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {                      // behind the last part: that one again, with no weight
-        const int part = min(n0 + n, parts - 1), slot = part == 0 ? meta.w : 2 * (static_cast<int>(blockIdx.x) + part);
+      for (int n = 0; n < 3; ++n) {                      // behind the last part: that one again, with no weight
+        const int part = min(n0 + n * WAYS, parts - 1), slot = part == 0 ? meta.w : 2 * (static_cast<int>(blockIdx.x) + part);
         ml[n] = *reinterpret_cast<const float2*>(p.part_ml + (slot * 8 * NT + h) * 2);
         o[n] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot) * 8 * NT + h) * D + d);
       }
-      float m_new = m;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) m_new = fmaxf(m_new, ml[n].x);
-      const float old = m == -INFINITY ? 0.f : exp2f(m - m_new);
+      const float m_new = fmaxf(fmaxf(m, ml[0].x), fmaxf(ml[1].x, ml[2].x)), old = m == -INFINITY ? 0.f : exp2f(m - m_new);
       m = m_new;
       sum *= old; v.x *= old; v.y *= old; v.z *= old; v.w *= old;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (n0 + n >= parts) break;
+      for (int n = 0; n < 3; ++n) {
+        if (n0 + n * WAYS >= parts) break;
         const float f = ml[n].x == -INFINITY ? 0.f : exp2f(ml[n].x - m);
         sum = fmaf(ml[n].y, f, sum);
         v.x = fmaf(o[n].x, f, v.x); v.y = fmaf(o[n].y, f, v.y);
         v.z = fmaf(o[n].z, f, v.z); v.w = fmaf(o[n].w, f, v.w);
       }
     }
-    const float inv = 1.f / sum;
-    *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(meta.x) * p.Hq + head0 + h) * D + d) =
-        make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+    if constexpr (WAYS > 1) {
+      __syncthreads();
+      sums[way][at] = v;
+      tops[way][at] = make_float2(m, sum);
+      __syncthreads();
+    }
+    if (way == 0 && in) {
+      float top = m;
+#pragma unroll
+      for (int w = 1; w < WAYS; ++w) top = fmaxf(top, tops[w][at].x);
+      const float mine = m == -INFINITY ? 0.f : exp2f(m - top);
+      sum *= mine; v.x *= mine; v.y *= mine; v.z *= mine; v.w *= mine;
+#pragma unroll
+      for (int w = 1; w < WAYS; ++w) {
+        const float2 y = tops[w][at];
+        const float4 z = sums[w][at];
+        const float f = y.x == -INFINITY ? 0.f : exp2f(y.x - top);
+        sum = fmaf(y.y, f, sum);
+        v.x = fmaf(z.x, f, v.x); v.y = fmaf(z.y, f, v.y); v.z = fmaf(z.z, f, v.z); v.w = fmaf(z.w, f, v.w);
+      }
+      const float inv = 1.f / sum;
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(meta.x) * p.Hq + head0 + h) * D + d) =
+          make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+    }
   }
 }
 
@@ -682,7 +703,8 @@ int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
     configured.done();
   }
   CUDA_CHECK_RET(launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(kV4Threads), SM::kBytes, st, p));
-  CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT>, dim3(ctas), dim3(kV4JoinThreads), 0, st, p));
+  if (static_cast<int64_t>(p.B) * (p.Hq / p.GP) * 6 < ctas) CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT, 4>, dim3(ctas), dim3(1024), 0, st, p));
+  else CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT, 1>, dim3(ctas), dim3(256), 0, st, p));
   return 0;
 }
 
