@@ -31,7 +31,7 @@ def cache_shape(num_pages: int, num_kv_heads: int, head_dim: int, page_size: int
 
 
 @functools.lru_cache(maxsize=256)
-def _sizes(shape):
+def sizes(shape):
     """(pages, kv heads, page_size, head_dim) of a shape, or None if it is no 4-bit cache's."""
     if len(shape) != 4 or shape[3] % 9 or shape[3] // 9 not in HEAD_DIMS or not 1 <= shape[2] <= MOST_PAGE // BLOCK:
         return None
@@ -40,10 +40,10 @@ def _sizes(shape):
 
 def geometry(cache: torch.Tensor):
     """(pages, kv heads, page_size, head_dim) of a 4-bit cache."""
-    sizes = _sizes(cache.shape)
-    if sizes is None or cache.dtype != torch.uint8 or not cache.is_contiguous():
+    geo = sizes(cache.shape)
+    if geo is None or cache.dtype != torch.uint8 or not cache.is_contiguous():
         raise ValueError(f"not a 4-bit cache: {cache.dtype} {tuple(cache.shape)}")
-    return sizes
+    return geo
 
 
 def held(cache) -> bool:

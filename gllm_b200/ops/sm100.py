@@ -555,7 +555,7 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
     n = w8.shape[0]
     n_out = n // 2 if silu else n
     if out is None:
-        out = torch.empty(m, n_out, dtype=_BF16, device=x.device)
+        out = x.new_empty((m, n_out))
     w_at, s_at, o_at, ldc = w8.data_ptr(), w_scale.data_ptr(), out.data_ptr(), out.stride(0)
     b_at = None if bias is None else bias.data_ptr()
     if not (w8.dtype is torch.int8 and w8.shape == (n, k) and w8.is_contiguous() and w_scale.dtype is torch.float32 and
@@ -574,7 +574,7 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
     if m == 0:
         return out
     on_this_device(x, w8, w_scale, out, bias)
-    scratch = torch.empty(m * k + 4 * m, dtype=torch.uint8, device=x.device)     # k % 16: the scales lie on 16-byte boundaries
+    scratch = w8.new_empty(m * k + 4 * m)        # k % 16: the scales lie on 16-byte boundaries
     xq = scratch.data_ptr()
     form, bt, parts, smem = plan or (0, 0, 0, 0)
     check(_lib.load().gllm_linear_int8(x.data_ptr(), x.stride(0), xq, xq + m * k, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,

@@ -17,8 +17,14 @@ EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at
 
 
 def _pair(k_cache, v_cache):
-    geo = kv4.geometry(k_cache)
-    if v_cache.shape != k_cache.shape or kv4.geometry(v_cache) != geo:
+    """(pages, kv heads, page_size, head_dim) of a layer's caches."""
+    shape = k_cache.shape
+    geo = kv4.sizes(shape)
+    if geo is not None and k_cache.dtype is v_cache.dtype is torch.uint8 and v_cache.shape == shape and k_cache.is_contiguous() and \
+            v_cache.is_contiguous():
+        return geo
+    geo = kv4.geometry(k_cache)                               # raises for what is no cache
+    if kv4.geometry(v_cache) != geo:
         raise ValueError(f"4-bit caches of unequal shape: {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     return geo
 
@@ -27,22 +33,9 @@ def _index(t: torch.Tensor, what: str, dims: int = 1):
     assert t.dtype == torch.int32 and t.dim() == dims and t.stride(-1) == 1, f"{what}: int32, contiguous rows"
 
 
-def _check_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope):
-    """Raises for arguments that `rope_kv_write` does not take."""
+def _refuse_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope):
+    """Raises for arguments that `rope_kv_write` does not take (the common ones do not come here)."""
     t, hq, d = q.shape
-    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride()
-    at = q.data_ptr() | k.data_ptr() | v.data_ptr()
-    norms = True
-    for w in (q_norm_w, k_norm_w):
-        if w is not None:
-            at |= w.data_ptr()
-            norms = norms and w.dtype is _BF16 and w.shape == (d,) and w.stride(0) == 1
-    if norms and q.dtype is k.dtype is v.dtype is _BF16 and qd == kd == vd == 1 and d == dim and k.shape == v.shape == (t, heads, d) and \
-            slots.dtype is positions.dtype is torch.int32 and slots.dim() == positions.dim() == 1 and not mrope and \
-            slots.shape[0] >= t and positions.shape[0] >= t and slots.stride(0) == positions.stride(0) == 1 and \
-            0 <= rot <= d and rot % 16 == 0 and (at | 2 * (qt | qh | kt | kh | vt | vh)) % 16 == 0 and \
-            (rot == 0 or (cos_sin.dtype is torch.float32 and cos_sin.shape[1] == rot and cos_sin.is_contiguous())):
-        return                                                # the common call; what follows says what is wrong with others
     assert q.dtype == k.dtype == v.dtype == _BF16 and q.stride(2) == k.stride(2) == v.stride(2) == 1
     assert d == dim and k.shape == v.shape == (t, heads, d), (q.shape, k.shape, v.shape, heads, dim)
     _index(slots, "slots")
@@ -71,10 +64,29 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         raise ValueError("a 4-bit cache is written with keys, values and their slots")
     t, hq, d = q.shape
     rot = rot_dim if cos_sin is not None else 0
-    mrope = mrope_section is not None and positions.dim() == 2
-    if not mrope and positions.dim() == 2:
-        positions = positions[0]
-    _check_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope)
+    mrope = False
+    if positions.dim() == 2:
+        mrope = mrope_section is not None
+        if not mrope:
+            positions = positions[0]
+    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride()
+    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    ends = q_at | k_at | v_at | 2 * (qt | qh | kt | kh | vt | vh)
+    qw_at = kw_at = None
+    common = not mrope and d == dim and qd == kd == vd == 1 and rot % 16 == 0 and 0 <= rot <= d
+    if q_norm_w is not None:
+        qw_at = q_norm_w.data_ptr()
+        ends |= qw_at
+        common = common and q_norm_w.dtype is _BF16 and q_norm_w.numel() == d and q_norm_w.is_contiguous()
+    if k_norm_w is not None:
+        kw_at = k_norm_w.data_ptr()
+        ends |= kw_at
+        common = common and k_norm_w.dtype is _BF16 and k_norm_w.numel() == d and k_norm_w.is_contiguous()
+    if not (common and ends % 16 == 0 and q.dtype is k.dtype is v.dtype is _BF16 and k.shape == v.shape == (t, heads, d) and
+            slots.dtype is positions.dtype is torch.int32 and slots.dim() == positions.dim() == 1 and slots.numel() >= t and
+            positions.numel() >= t and slots.is_contiguous() and positions.is_contiguous() and
+            (rot == 0 or (cos_sin.dtype is torch.float32 and cos_sin.shape[1] == rot and cos_sin.is_contiguous()))):
+        _refuse_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope)
     if t == 0:
         return
     on_this_device(q, k, v, positions, slots, k_cache, v_cache, cos_sin, q_norm_w, k_norm_w)
@@ -85,14 +97,12 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         else:
             sec0, sec1 = int(mrope_section[0]), int(mrope_section[1])
         pos_stride = positions.stride(0)
-    (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
     if heads == 1:                                            # the stride of a dimension of one may be anything
         kh = vh = d
     check(_lib.load().gllm_rope_kv4_write(
-        q.data_ptr(), qt, qh if hq > 1 else d, hq, k.data_ptr(), kt, kh, heads, v.data_ptr(), vt, vh,
-        None if q_norm_w is None else q_norm_w.data_ptr(), None if k_norm_w is None else k_norm_w.data_ptr(),
-        cos_sin.data_ptr() if rot else None, d, rot, 1 if neox else 0, t, positions.data_ptr(), slots.data_ptr(), eps,
-        k_cache.data_ptr(), v_cache.data_ptr(), pages, sec0, sec1, page_size, pos_stride, stream_ptr()), "rope_kv4_write")
+        q_at, qt, qh if hq > 1 else d, hq, k_at, kt, kh, heads, v_at, vt, vh, qw_at, kw_at, cos_sin.data_ptr() if rot else None, d, rot,
+        neox, t, positions.data_ptr(), slots.data_ptr(), eps, k_cache.data_ptr(), v_cache.data_ptr(), pages, sec0, sec1, page_size,
+        pos_stride, stream_ptr()), "rope_kv4_write")
     _count()
 
 
@@ -102,10 +112,11 @@ def kv_cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
     _index(slots, "slots")
     on_this_device(k_cache, v_cache, slots)
     t = slots.shape[0]
-    k, v = torch.empty(2, t, heads, d, dtype=_BF16, device=k_cache.device).unbind(0)
-    check(_lib.load().gllm_kv4_rows(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, heads, d,
-                                    page_size, pages, stream_ptr()), "kv4_rows")
+    k = k_cache.new_empty((t, heads, d), dtype=_BF16)
+    v = torch.empty_like(k)
     if t:
+        check(_lib.load().gllm_kv4_rows(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, heads,
+                                        d, page_size, pages, stream_ptr()), "kv4_rows")
         _count()
     return k, v
 
@@ -120,7 +131,7 @@ def scratch_bytes(kv_heads: int, d: int, max_len: int) -> int:
     return max(EXPAND_BYTES, 4 * kv_heads * d * (max_len + 63)) + _DECODE_CTAS * (2 * 16 * (d + 2) * 4 + 16) + (1 << 20)
 
 
-def expand_rounds(lens, token_bytes: int, limit: int = EXPAND_BYTES):
+def expand_rounds(lens, token_bytes: int, limit: int):
     """(first, end, tiles of 64 tokens) of consecutive sequences whose expanded keys and values stay below `limit` bytes together, one
     sequence at least. lens: their lengths, on the host."""
     rounds, first, tiles = [], 0, 0
@@ -142,44 +153,47 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequences' keys and values expanded to bf16 first, EXPAND_BYTES of them at a time, and take the tcgen05 prefill kernel.
     host_lens: the lengths [num_seqs] on the host; without them every prompt is given room for max_seq_len."""
     pages, hkv, page_size, d = _pair(k_cache, v_cache)
-    t, hq = q.shape[0], num_q_heads
-    assert q.dtype == _BF16 and q.dim() == 2 and q.shape[1] >= hq * d and q.stride(1) == 1 and d == head_dim and hq % hkv == 0
+    (t, width), (q_ts, one), hq = q.shape, q.stride(), num_q_heads
+    assert q.dtype is _BF16 and width >= hq * d and one == 1 and d == head_dim and hq % hkv == 0
     _index(block_table, "block_table", 2)
     _index(seq_lens, "seq_lens")
-    if q.numel() and (q.data_ptr() % 16 or q.stride(0) % 8):
+    assert block_table.shape[0] >= num_seqs and seq_lens.shape[0] >= num_seqs and t >= num_decode_seqs
+    q_at = q.data_ptr()
+    if (q_at | 2 * q_ts) % 16 and t:
         raise ValueError("queries over a 4-bit cache must lie on 16-byte boundaries")
     if out is None:
-        out = torch.empty(t, hq * d, dtype=_BF16, device=q.device)
-    assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
+        out = q.new_empty((t, hq * d))
+    else:
+        assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
     on_this_device(q, out, k_cache, v_cache, block_table, seq_lens)
-    L, st, dev = _lib.load(), stream_ptr(), q.device
+    L, st = _lib.load(), stream_ptr()
+    pitch = block_table.stride(0)
+    k_at, v_at, out_at, table_at, lens_at = k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
     if num_decode_seqs > 0:
-        assert block_table.shape[0] >= num_decode_seqs and seq_lens.shape[0] >= num_decode_seqs and t >= num_decode_seqs
         size = _decode_scratch(d)
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)       # of this call: captured graphs and streams share none
-        check(L.gllm_kv4_decode(q.data_ptr(), q.stride(0), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages,
-                                block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), num_decode_seqs, hq, hkv, d,
-                                page_size, scale, _DECODE_CTAS, scratch.data_ptr(), size, st), "kv4_decode")
+        scratch = k_cache.new_empty(size)                     # of this call: captured graphs and streams share none
+        check(L.gllm_kv4_decode(q_at, q_ts, out_at, k_at, v_at, pages, table_at, pitch, lens_at, num_decode_seqs, hq, hkv, d, page_size,
+                                scale, _DECODE_CTAS, scratch.data_ptr(), size, st), "kv4_decode")
         _count(2)
     prompts = num_seqs - num_decode_seqs
     if prompts > 0 and max_q_len > 0:
         _index(query_start_loc, "query_start_loc")
         on_this_device(query_start_loc)
         lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
-        for first, end, tiles in expand_rounds(lens, 4 * hkv * d):
+        start_at = query_start_loc.data_ptr()
+        for first, end, tiles in expand_rounds(lens, 4 * hkv * d, EXPAND_BYTES):
             if tiles == 0:
                 continue
             a, n = num_decode_seqs + first, end - first
             longest = int(max(lens[first:end]))
-            k, v = torch.empty(2, tiles, hkv, d // 64, 64, 64, dtype=_BF16, device=dev).unbind(0)
+            k = q.new_empty((tiles, hkv, d // 64, 64, 64))
+            v = torch.empty_like(k)
             max_tiles = (longest + 63) // 64
-            table = torch.empty(n, max_tiles, dtype=torch.int32, device=dev)
-            lens_at, k_at, v_at, table_at = seq_lens.data_ptr() + 4 * a, k.data_ptr(), v.data_ptr(), table.data_ptr()
-            check(L.gllm_kv4_expand(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.stride(0),
-                                    block_table.stride(0), lens_at, n, hkv, d, page_size, pages, tiles, k_at, v_at, table_at, max_tiles,
-                                    longest, st), "kv4_expand")
-            check(L.gllm_attn_prefill_tc_tiles(q.data_ptr(), q.stride(0), out.data_ptr(), k_at, v_at, tiles, table_at, max_tiles, lens_at,
-                                               query_start_loc.data_ptr() + 4 * a, t, n, max_q_len, hq, hkv, d, scale, st),
+            table = seq_lens.new_empty((n, max_tiles))
+            check(L.gllm_kv4_expand(k_at, v_at, table_at + 4 * a * pitch, pitch, lens_at + 4 * a, n, hkv, d, page_size, pages, tiles,
+                                    k.data_ptr(), v.data_ptr(), table.data_ptr(), max_tiles, longest, st), "kv4_expand")
+            check(L.gllm_attn_prefill_tc_tiles(q_at, q_ts, out_at, k.data_ptr(), v.data_ptr(), tiles, table.data_ptr(), max_tiles,
+                                               lens_at + 4 * a, start_at + 4 * a, t, n, max_q_len, hq, hkv, d, scale, st),
                   "attn_prefill_tc_tiles")
             _count(2)
     return out

@@ -109,7 +109,7 @@ def test_ref_attention():
 def test_rounds_of_expansion():
     assert sm100_kv4.expand_rounds([64, 65, 1], 10, limit=64 * 10 * 3) == [(0, 2, 3), (2, 3, 1)]
     assert sm100_kv4.expand_rounds([1000, 10], 1, limit=1) == [(0, 1, 16), (1, 2, 1)]       # one at least
-    assert sm100_kv4.expand_rounds([], 1) == [] and sm100_kv4.expand_rounds([0, 0], 1) == [(0, 2, 0)]
+    assert sm100_kv4.expand_rounds([], 1, 1) == [] and sm100_kv4.expand_rounds([0, 0], 1, 1) == [(0, 2, 0)]
 
 
 @pytest.mark.parametrize("d,page", [(32, 16), (96, 16), (256, 16), (64, 8), (128, 24), (128, 0), (64, 528)])
