@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int hh = first + n * kStep;
+    if (hh - lane / L >= n_heads) break;                 // none for the whole warp
     const bool is_q = hh < p.Hq, is_qk = hh < n_qk;
     uint32_t w[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
     float x[8];
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int hh = first + n * kStep;
+    if (hh - lane / L >= n_heads) break;                 // none for the whole warp
     const bool is_q = hh < p.Hq, is_qk = hh < n_qk;
     uint32_t w[2][4];
 #pragma unroll
