@@ -709,52 +709,59 @@ int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
 }
 
 // Pages of the sequences of a launch expanded to bf16 tiles [tile][Hkv][D / 64][64 tokens][64], as the prefill kernels read a cache with
-// pages of 64, and the tiles' table. Sequence s has ceil(len / 64) tiles, from the sum of those before it on. A CTA makes 16 tokens of a
-// head's keys or values. Memory-bound: 9 D / 16 bytes in, 2 D out a token.
+// pages of 64, and the tiles' table. Sequence s has ceil(len / 64) tiles, from the sum of those before it on. A CTA makes a tile of a
+// head's keys or values, zeros behind the last token; a thread has several units of eight dims on their way. Memory-bound: 9 D / 16 bytes in,
+// 2 D out a token.
+constexpr int kV4ExpandThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kV4ExpandThreads)
 kv4_expand_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ block_table,
                   int max_blocks, const int32_t* __restrict__ seq_lens, int Hkv, int page_size, int64_t pages, int64_t tiles,
                   __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int32_t* __restrict__ table, int max_tiles) {
   griddep_launch();
   griddep_wait();
-  constexpr int G = D / 64, kBlock = 9 * D;
-  const int seq = blockIdx.y, blk = blockIdx.x;          // 16 tokens
+  constexpr int G = D / 64, kBlock = 9 * D, kUnits = D / 8, kN = 64 * kUnits / kV4ExpandThreads;
+  const int seq = blockIdx.y, in_seq = blockIdx.x;       // tile of the sequence
   const int len = seq_lens[seq];
-  if (blk * 16 >= (len + 63) / 64 * 64) return;          // a tile's last blocks are written too: zeros behind the last token
-  __shared__ int part[4];
+  if (in_seq * 64 >= len) return;
+  __shared__ int part[kV4ExpandThreads / 32];
   int before = 0;
-  for (int s = threadIdx.x; s < seq; s += 128) before += (seq_lens[s] + 63) / 64;
+  for (int s = threadIdx.x; s < seq; s += kV4ExpandThreads) before += (seq_lens[s] + 63) / 64;
   before = __reduce_add_sync(0xffffffffu, before);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = before;
   __syncthreads();
-  const int64_t tile = part[0] + part[1] + part[2] + part[3] + blk / 4;
+  int64_t tile = in_seq;
+#pragma unroll
+  for (int w = 0; w < kV4ExpandThreads / 32; ++w) tile += part[w];
   if (tile >= tiles) return;                             // more tokens than the caller has made room for
-  if (threadIdx.x == 0 && blockIdx.z == 0 && blk % 4 == 0) table[static_cast<size_t>(seq) * max_tiles + blk / 4] = static_cast<int>(tile);
-  const int tok0 = blk * 16;
-  int64_t page = 0;
-  if (tok0 < len) page = min(static_cast<int64_t>(static_cast<uint32_t>(block_table[static_cast<size_t>(seq) * max_blocks + min(tok0 / page_size, max_blocks - 1)])),
-                            pages - 1);
-  const int heads2 = 2 * Hkv;
-  for (int hz = blockIdx.z; hz < heads2; hz += gridDim.z) {
-    const bool is_v = hz >= Hkv;
-    const int h = is_v ? hz - Hkv : hz;
-    const uint8_t* block = (is_v ? v_cache : k_cache) + ((page * Hkv + h) * (page_size / 16) + tok0 % page_size / 16) * kBlock;
-    __nv_bfloat16* out = (is_v ? v_out : k_out) + ((tile * Hkv + h) * G * 64 + blk % 4 * 16) * 64;
+  if (threadIdx.x == 0 && blockIdx.z == 0) table[static_cast<size_t>(seq) * max_tiles + in_seq] = static_cast<int>(tile);
+  const bool is_v = static_cast<int>(blockIdx.z) >= Hkv;
+  const int h = is_v ? blockIdx.z - Hkv : blockIdx.z;
+  const uint8_t* cache = is_v ? v_cache : k_cache;
+  __nv_bfloat16* out = (is_v ? v_out : k_out) + (tile * Hkv + h) * G * 64 * 64;
+  const int32_t* row = block_table + static_cast<size_t>(seq) * max_blocks;
+  uint32_t codes[kN], pair[kN];
 #pragma unroll
-    for (int i = threadIdx.x; i < 16 * D / 8; i += 128) {
-      const int row = i / (D / 8), unit = i % (D / 8), group = unit % G, chunk = unit / G;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (tok0 + row < len) {
-        const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + row * (D / 2) + unit * 4);
-        const float2 pair = unpack_bf16(*reinterpret_cast<const uint32_t*>(block + 8 * D + (row * G + group) * 4));
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes >> (4 * e)) & 15u), pair.x, pair.y);
-        w = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-      }
-      *reinterpret_cast<uint4*>(out + (group * 64 + row) * 64 + chunk * 8) = w;
+  for (int n = 0; n < kN; ++n) {
+    const int i = threadIdx.x + n * kV4ExpandThreads, r = i / kUnits, unit = i % kUnits, tok = in_seq * 64 + r;
+    codes[n] = pair[n] = 0u;                             // stands for zeros
+    if (tok < len) {
+      const int at = tok / page_size, off = tok - at * page_size;
+      const int64_t page = min(static_cast<int64_t>(static_cast<uint32_t>(row[min(at, max_blocks - 1)])), pages - 1);
+      const uint8_t* block = cache + ((page * Hkv + h) * (page_size / 16) + off / 16) * kBlock;
+      codes[n] = *reinterpret_cast<const uint32_t*>(block + off % 16 * (D / 2) + unit * 4);
+      pair[n] = *reinterpret_cast<const uint32_t*>(block + 8 * D + (off % 16 * G + unit % G) * 4);
     }
+  }
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    const int i = threadIdx.x + n * kV4ExpandThreads, r = i / kUnits, unit = i % kUnits;
+    const float2 p = unpack_bf16(pair[n]);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes[n] >> (4 * e)) & 15u), p.x, p.y);
+    *reinterpret_cast<uint4*>(out + (unit % G * 64 + r) * 64 + unit / G * 8) =
+        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
   }
 }
 
@@ -815,15 +822,13 @@ GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const 
                                 int B, int Hkv, int D, int page_size, int64_t pages, int64_t tiles, void* k_out, void* v_out,
                                 void* table, int max_tiles, int max_len, void* stream) {
   if (B <= 0 || max_len <= 0) return 0;
-  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || pages <= 0 || B > 65535 ||
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || pages <= 0 || B > 65535 || Hkv > 32767 ||
       static_cast<int64_t>(max_tiles) * 64 < max_len) {
     fprintf(stderr, "[gllm_b200] kv4_expand: unsupported D=%d page_size=%d, %d sequences\n", D, page_size, B);
     return 1;
   }
-  const int blocks = (max_len + 63) / 64 * 4;
-  const int per = static_cast<int64_t>(blocks) * B >= 4 * num_sms() ? 4 : 1;        // heads of a CTA: fewer and longer ones for long prompts
-  const dim3 grid(blocks, B, (2 * Hkv + per - 1) / per);
-  CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_expand_kernel<64> : kv4_expand_kernel<128>, grid, dim3(128), 0,
+  const dim3 grid((max_len + 63) / 64, B, 2 * Hkv);
+  CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_expand_kernel<64> : kv4_expand_kernel<128>, grid, dim3(kV4ExpandThreads), 0,
                             reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint8_t*>(k_cache),
                             reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(block_table), max_blocks,
                             reinterpret_cast<const int32_t*>(seq_lens), Hkv, page_size, pages, tiles,

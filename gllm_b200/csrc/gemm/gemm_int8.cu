@@ -7,7 +7,8 @@
 //
 // Two launches: the rows are quantised (here), then multiplied on the tensor cores (tcgen05.mma kind::i8) by one of two kernels:
 // prompts on pairs of SMs (gemm_bf16_pair.cu), decode batches with K cut over a cluster (gemm_bf16_cluster.cu), which copies its first
-// weights while the rows are quantised. `gllm_linear_int8` chooses by what their time is made of.
+// weights while the rows are quantised. `gllm_linear_int8` chooses by what their time is made of. (Rows quantised in every CTA of the
+// cluster kernel, to save the launch: 10.0 us for one row of 6144 x 4096 instead of 9.1, 12.8 for four, 16 for eight.)
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
 #include "gemm_cluster.h"
