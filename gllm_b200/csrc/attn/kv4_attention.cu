@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     }
   };
   // This warp's part [my_begin, my_end) of the share.
-  const int per_warp = (tiles + kV4Warps - 1) / kV4Warps, my_begin = min(tiles, warp * per_warp), my_end = min(tiles, my_begin + per_warp);
+  const int each = tiles / kV4Warps, over = tiles % kV4Warps;        // the first ones have one more: a warp without tiles has none behind it
+  const int my_begin = warp * each + min(warp, over), my_end = my_begin + each + (warp < over ? 1 : 0);
   const uint32_t my_tiles = static_cast<uint32_t>(my_end - my_begin);
   at_tile += my_begin;
   settle(at, at_tile);
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(256 * WAYS) kv4_join_kernel(const Kv4Params p)
 template <int D, int NT>
 int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
   using SM = Kv4Smem<D, NT>;
+  if (NT > 1 && ctas > 1) ctas /= 2;                     // one fits an SM
   static PerDeviceOnce configured;
   if (configured.need()) {
     CUDA_CHECK_RET(cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
