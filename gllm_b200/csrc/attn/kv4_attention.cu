@@ -589,13 +589,17 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   __syncthreads();
   // ---- the parts of this CTA's warps: a row starts with a warp's last part, or with what the CTA before began, and goes on through
   // the first parts of the warps behind. Four dims of a head a thread.
-  for (int row = -1; row < kV4Warps; ++row) {
-    if (row >= 0 && info[kV4Warps + row].x < 0) continue;
-    int last = row;                                      // the last warp with a part
-    bool done = false;
-    while (!done && last + 1 < kV4Warps && info[last + 1].x >= 0) done = info[++last].z != 0;
-    if (row < 0 && last < 0) continue;
-    const int4 what = row < 0 ? info[0] : info[kV4Warps + row];
+  static_assert(kV4Warps == 8);
+  const int4 mine = lane < 2 * kV4Warps ? info[lane] : make_int4(-1, 0, 0, 0);
+  const uint32_t parts = __ballot_sync(0xffffffffu, mine.x >= 0), ending = __ballot_sync(0xffffffffu, mine.x >= 0 && mine.z != 0) & 0xffu;
+  for (uint32_t rows = (parts >> 8) << 1 | (parts & 1u); rows != 0; rows &= rows - 1) {        // bit 0: what the CTA before began
+    const int row = __ffs(rows) - 2;
+    const uint32_t behind = (parts & 0xffu) >> (row + 1), stops = ending >> (row + 1);
+    const int run = __ffs(~behind) - 1, stop = __ffs(stops);                 // first parts in a row, place of the one that ends (from 1 on)
+    const bool done = stop != 0 && stop <= run;
+    const int last = row + (done ? stop : run), at_info = row < 0 ? 0 : kV4Warps + row;          // the last warp with a part
+    const int4 what = make_int4(__shfl_sync(0xffffffffu, mine.x, at_info), __shfl_sync(0xffffffffu, mine.y, at_info), 0,
+                                __shfl_sync(0xffffffffu, mine.w, at_info));
     const int head0 = what.y / hg * p.G + what.y % hg * p.GP, slot = 2 * static_cast<int>(blockIdx.x) + (row < 0 ? 0 : 1);
     for (int x = warp; x < kPieces; x += kV4Warps) {
       const int nt = x / (GR * 4), gr = x / 4 % GR, c = x / 2 % 2, half = x % 2;
