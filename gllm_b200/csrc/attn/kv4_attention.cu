@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   if (tid == 0) *guard.dead = 0;
   if (tid < kV4Warps * kV4Stages) mbar_init(&bars[tid], 1);
   fence_mbar_init();
+  __syncthreads();
   griddep_launch();
   griddep_wait();
 
@@ -153,20 +154,60 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
     }
     return x + before;
   };
-  // up to one sequence a thread, one pass has it all; beyond that the first counts, the second finds this CTA's
-  int all = 0, mine_len = 0, mine_upto = 0;
-  for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
-    int total;
-    mine_len = s0 + tid < p.B ? p.seq_lens[s0 + tid] : 0;
-    mine_upto = block_scan(s0 + tid < p.B ? kv4_tiles(mine_len) : 0, total);
-    all += total;
-  }
-  const int64_t work = static_cast<int64_t>(all) * H;
-  const int64_t share = max((work + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kV4Warps));
-  const int64_t begin = share * blockIdx.x, end = min(begin + share, work);
+  int all = 0, mine_len = 0, mine_upto = 0, seq0, tiles0;      // all tiles of a head group, this CTA's first sequence and the tiles before it
+  int64_t share, begin, end;
+  auto cut = [&] {
+    const int64_t work = static_cast<int64_t>(all) * H;
+    share = max((work + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kV4Warps));
+    begin = share * blockIdx.x;
+    end = min(begin + share, work);
+  };
   if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if (begin >= work) return;
-  {
+  if (p.B <= 64) {
+    // few sequences: every warp for itself, without barriers (a lone sequence of 700: 8.6 -> 8.3 us)
+    int len[2], n[2], upto[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      len[i] = lane + 32 * i < p.B ? p.seq_lens[lane + 32 * i] : 0;
+      n[i] = lane + 32 * i < p.B ? kv4_tiles(len[i]) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      upto[i] = n[i];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto[i], o);
+        if (lane >= o) upto[i] += y;
+      }
+      upto[i] += all;
+      all = __shfl_sync(0xffffffffu, upto[i], 31);
+    }
+    cut();
+    if (begin >= end) return;
+    seq0 = tiles0 = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t here = __ballot_sync(0xffffffffu, begin >= static_cast<int64_t>(upto[i] - n[i]) * H && begin < static_cast<int64_t>(upto[i]) * H);
+      if (here != 0) {
+        const int from = __ffs(here) - 1;
+        seq0 = 32 * i + from;
+        tiles0 = __shfl_sync(0xffffffffu, upto[i] - n[i], from);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i >= seq0) lens[lane + 32 * i - seq0] = len[i];        // every warp the same
+    __syncwarp();
+  } else {
+    // up to one sequence a thread, one pass has it all; beyond that the first counts, the second finds this CTA's
+    for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
+      int total;
+      mine_len = s0 + tid < p.B ? p.seq_lens[s0 + tid] : 0;
+      mine_upto = block_scan(s0 + tid < p.B ? kv4_tiles(mine_len) : 0, total);
+      all += total;
+    }
+    cut();
+    if (begin >= end) return;
     int base = 0;                                        // tiles of one head group before this round
     for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
       int total = 0;
@@ -180,17 +221,18 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       base += total;
     }
     __syncthreads();
+    seq0 = words[1];
+    tiles0 = words[2];
+    if (p.B > kV4Threads) {
+      for (int i = tid; i < kV4Lens; i += kV4Threads) lens[i] = seq0 + i < p.B ? p.seq_lens[seq0 + i] : 0;
+    } else if (tid >= seq0) {
+      lens[tid - seq0] = mine_len;                       // kV4Lens == kV4Threads
+    }
+    __syncthreads();
   }
-  const int seq0 = words[1];
-  if (p.B > kV4Threads) {
-    for (int i = tid; i < kV4Lens; i += kV4Threads) lens[i] = seq0 + i < p.B ? p.seq_lens[seq0 + i] : 0;
-  } else if (tid >= seq0) {
-    lens[tid - seq0] = mine_len;                         // kV4Lens == kV4Threads
-  }
-  __syncthreads();
   auto len_of = [&](int s) { return s - seq0 < kV4Lens ? lens[s - seq0] : p.seq_lens[s]; };
 
-  const int first_in = static_cast<int>(begin - static_cast<int64_t>(words[2]) * H), tiles = static_cast<int>(end - begin);
+  const int first_in = static_cast<int>(begin - static_cast<int64_t>(tiles0) * H), tiles = static_cast<int>(end - begin);
   const int hg = p.G / p.GP;
   struct Place {                                         // a head group of a sequence
     int seq, head, len, n;
