@@ -162,8 +162,6 @@ def spec_chatglm(cfg):
 def _build_decoder(spec_fn):
     def build(cfg, device):
         from gllm_b200.layers.moe import make_moe_block
-        if _quant(cfg) == "int8" and spec_fn(cfg).moe is not None:
-            raise ValueError(f"{cfg['architectures'][0]}: routed experts have no 8-bit form")
         return CausalLM(spec_fn(cfg), device, moe_factory=make_moe_block)
     return build
 
@@ -261,4 +259,6 @@ def build_model(cfg: HFConfig, device):
     model = ARCHITECTURES[arch](cfg, device)
     if (cfg.get("weights_int8") or _quant(cfg) == "int8") and getattr(model.spec, "quant", None) != "int8":
         raise ValueError(f"{arch}{' in fp8' if _quant(cfg) == 'fp8' else ''} has no 8-bit linears")
+    if getattr(model.spec, "quant", None) == "int8" and model.spec.moe is not None:
+        raise ValueError(f"{arch}: routed experts have no 8-bit form")
     return model

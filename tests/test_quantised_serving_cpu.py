@@ -93,8 +93,19 @@ def test_pages_of_a_4_bit_cache():
     assert c.k_cache[1].dtype == torch.uint8 and kv4.geometry(c.v_cache[0]) == (5, 8, 32, 64)
 
 
+def _vl_moe():
+    text = tiny("Qwen3MoeForCausalLM", hidden_size=128, head_dim=64, num_experts=4, num_experts_per_tok=2, moe_intermediate_size=64)
+    text["rope_scaling"] = {"mrope_section": [12, 10, 10], "mrope_interleaved": True}
+    vision = dict(depth=1, hidden_size=32, num_heads=2, intermediate_size=64, patch_size=16, spatial_merge_size=2, temporal_patch_size=2,
+                  num_position_embeddings=16, deepstack_visual_indexes=[0], in_channels=3, out_hidden_size=128)
+    return registry.HFConfig({"architectures": ["Qwen3VLMoeForConditionalGeneration"], "text_config": text, "vision_config": vision,
+                              "torch_dtype": "float32", "image_token_id": 5, "video_token_id": 6, "vision_start_token_id": 7,
+                              "weights_int8": True})
+
+
 @pytest.mark.parametrize("make", [
     lambda: registry.build_model(_cfg("Qwen3MoeForCausalLM", num_experts=4, num_experts_per_tok=2, moe_intermediate_size=64, weights_int8=True), "cpu"),
+    lambda: registry.build_model(_vl_moe(), "cpu"),
     lambda: registry.build_model(_cfg(weights_int8=True, quantization_config={"quant_method": "fp8", "weight_block_size": [128, 128]}), "cpu"),
     lambda: registry.build_model(registry.HFConfig(tiny("Qwen3ForCausalLM", hidden_size=120, head_dim=64, weights_int8=True)), "cpu"),
     lambda: ModelLoader(tiny(), quantization="int3"),
