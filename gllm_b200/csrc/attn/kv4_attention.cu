@@ -49,6 +49,7 @@ struct Kv4Params {
   uint32_t last_page;
   const int32_t* block_table;
   const int32_t* seq_lens;
+  int64_t pitch;                                         // between the rows of the block table, which has max_blocks columns
   int B, max_blocks, Hq, Hkv, G, GP;                     // GP query heads (at most 8 NT) of the G of a kv head at a time
   int page_blocks;                                       // blocks of 16 tokens in a page
   uint32_t page_magic;                                   // floor(b / page_blocks) = umulhi(b, page_magic), exact while b x page_blocks < 2^32 (0: one block)
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       blocks = min(2, (fetch.len - fetch_tile * kV4Keys + 15) / 16);
       if ((lane & 1) < blocks) {
         const int i = p.page_magic != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(blk), p.page_magic)) : blk;
-        const uint32_t page = min(static_cast<uint32_t>(p.block_table[static_cast<size_t>(fetch.seq) * p.max_blocks + min(i, p.max_blocks - 1)]),
+        const uint32_t page = min(static_cast<uint32_t>(p.block_table[fetch.seq * p.pitch + min(i, p.max_blocks - 1)]),
                                   p.last_page);
         src = (lane & 2 ? p.v_cache : p.k_cache) +
               ((static_cast<uint64_t>(page) * p.Hkv + fetch.head / hg) * p.page_blocks + (blk - i * p.page_blocks)) * SM::kBlock;
@@ -764,7 +765,7 @@ constexpr int kV4ExpandThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kV4ExpandThreads)
 kv4_expand_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ block_table,
-                  int max_blocks, const int32_t* __restrict__ seq_lens, int Hkv, int page_size, int64_t pages, int64_t tiles,
+                  int64_t pitch, int max_blocks, const int32_t* __restrict__ seq_lens, int Hkv, int page_size, int64_t pages, int64_t tiles,
                   __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int32_t* __restrict__ table, int max_tiles) {
   griddep_launch();
   griddep_wait();
@@ -787,7 +788,7 @@ kv4_expand_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
   const int h = is_v ? blockIdx.z - Hkv : blockIdx.z;
   const uint8_t* cache = is_v ? v_cache : k_cache;
   __nv_bfloat16* out = (is_v ? v_out : k_out) + (tile * Hkv + h) * G * 64 * 64;
-  const int32_t* row = block_table + static_cast<size_t>(seq) * max_blocks;
+  const int32_t* row = block_table + seq * pitch;
   uint32_t codes[kN], pair[kN];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
@@ -827,15 +828,15 @@ GLLM_EXPORT int64_t gllm_kv4_decode_scratch(int D, int ctas) {
 // Attention of B sequences with one new token each over 4-bit caches of `pages` pages: q [B, Hq * D] (token stride q_ts), out [B, Hq, D]
 // contiguous; keys [0, seq_lens[s]) of each, zeros where there are none.
 GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const void* k_cache, const void* v_cache, int64_t pages,
-                                const void* block_table, int max_blocks, const void* seq_lens, int B, int Hq, int Hkv, int D,
-                                int page_size, float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
+                                const void* block_table, int64_t pitch, int max_blocks, const void* seq_lens, int B, int Hq, int Hkv,
+                                int D, int page_size, float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (B <= 0) return 0;
   auto al16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || Hkv <= 0 || Hq % Hkv != 0 || q_ts % 8 != 0 || !al16(q) ||
-      !al16(out) || !al16(k_cache) || !al16(v_cache) || !al16(scratch) || pages <= 0 || ctas <= 0 ||
+      !al16(out) || !al16(k_cache) || !al16(v_cache) || !al16(scratch) || pages <= 0 || max_blocks <= 0 || ctas <= 0 ||
       scratch_bytes < gllm_kv4_decode_scratch(D, ctas)) {
-    fprintf(stderr, "[gllm_b200] kv4_decode: unsupported D=%d page_size=%d Hq=%d Hkv=%d, or rows off 16-byte boundaries\n", D,
-            page_size, Hq, Hkv);
+    fprintf(stderr, "[gllm_b200] kv4_decode: unsupported D=%d page_size=%d Hq=%d Hkv=%d (%lld pages, %d a sequence), or rows off 16-byte boundaries\n",
+            D, page_size, Hq, Hkv, static_cast<long long>(pages), max_blocks);
     return 1;
   }
   Kv4Params p;
@@ -847,7 +848,7 @@ GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const vo
   p.last_page = static_cast<uint32_t>(pages < 0x80000000ll ? pages - 1 : 0x7fffffffll);
   p.block_table = reinterpret_cast<const int32_t*>(block_table);
   p.seq_lens = reinterpret_cast<const int32_t*>(seq_lens);
-  p.B = B; p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
+  p.pitch = pitch; p.B = B; p.max_blocks = max_blocks; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.page_blocks = page_size / 16;
   p.page_magic = p.page_blocks == 1 ? 0u : static_cast<uint32_t>((0x100000000ull + p.page_blocks - 1) / p.page_blocks);
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -866,11 +867,11 @@ GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const vo
 
 // Keys and values of B sequences from 4-bit caches to bf16 tiles k_out, v_out [tiles, Hkv, D / 64, 64, 64], sequence after sequence, each
 // rounded up to 64 tokens; table [B, max_tiles]: their tiles. max_len: the longest.
-GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const void* block_table, int max_blocks, const void* seq_lens,
-                                int B, int Hkv, int D, int page_size, int64_t pages, int64_t tiles, void* k_out, void* v_out,
+GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const void* block_table, int64_t pitch, int max_blocks,
+                                const void* seq_lens, int B, int Hkv, int D, int page_size, int64_t pages, int64_t tiles, void* k_out, void* v_out,
                                 void* table, int max_tiles, int max_len, void* stream) {
   if (B <= 0 || max_len <= 0) return 0;
-  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || pages <= 0 || B > 65535 || Hkv > 32767 ||
+  if ((D != 64 && D != 128) || page_size < 16 || page_size > 512 || page_size % 16 != 0 || pages <= 0 || max_blocks <= 0 || B > 65535 || Hkv > 32767 ||
       static_cast<int64_t>(max_tiles) * 64 < max_len) {
     fprintf(stderr, "[gllm_b200] kv4_expand: unsupported D=%d page_size=%d, %d sequences\n", D, page_size, B);
     return 1;
@@ -878,7 +879,7 @@ GLLM_EXPORT int gllm_kv4_expand(const void* k_cache, const void* v_cache, const 
   const dim3 grid((max_len + 63) / 64, B, 2 * Hkv);
   CUDA_CHECK_RET(launch_pdl(D == 64 ? kv4_expand_kernel<64> : kv4_expand_kernel<128>, grid, dim3(kV4ExpandThreads), 0,
                             reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint8_t*>(k_cache),
-                            reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(block_table), max_blocks,
+                            reinterpret_cast<const uint8_t*>(v_cache), reinterpret_cast<const int32_t*>(block_table), pitch, max_blocks,
                             reinterpret_cast<const int32_t*>(seq_lens), Hkv, page_size, pages, tiles,
                             reinterpret_cast<__nv_bfloat16*>(k_out), reinterpret_cast<__nv_bfloat16*>(v_out),
                             reinterpret_cast<int32_t*>(table), max_tiles));

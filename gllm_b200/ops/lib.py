@@ -95,8 +95,8 @@ def _declare(lib):
     sig("gllm_rope_kv4_write", [P, L, L, I, P, L, L, I, P, L, L, P, P, P, I, I, I, I, P, P, F, P, P, L, I, I, I, L, P])
     sig("gllm_kv4_rows", [P, P, P, P, P, I, I, I, I, L, P])
     sig("gllm_kv4_decode_scratch", [I, I], L)
-    sig("gllm_kv4_decode", [P, L, P, P, P, L, P, I, P, I, I, I, I, I, F, I, P, L, P])
-    sig("gllm_kv4_expand", [P, P, P, I, P, I, I, I, I, L, L, P, P, P, I, I, P])
+    sig("gllm_kv4_decode", [P, L, P, P, P, L, P, L, I, P, I, I, I, I, I, F, I, P, L, P])
+    sig("gllm_kv4_expand", [P, P, P, L, I, P, I, I, I, I, L, L, P, P, P, I, I, P])
     sig("gllm_attn_prefill_tc_tiles", [P, L, P, P, P, L, P, I, P, P, I, I, I, I, I, I, F, P])
     sig("gllm_gemm_fp8_block", [P, P, P, P, P, L, I, I, I, P, I, P])
 

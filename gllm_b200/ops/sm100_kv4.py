@@ -151,7 +151,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     num_seqs: int, max_q_len: int, max_seq_len: int, out: Optional[torch.Tensor] = None, host_lens=None):
     """`sm100.paged_attention` on 4-bit caches. Decoding sequences read the codes (csrc/attn/kv4_attention.cu). Prompt portions have their
     sequences' keys and values expanded to bf16 first, EXPAND_BYTES of them at a time, and take the tcgen05 prefill kernel.
-    host_lens: the lengths [num_seqs] on the host; without them every prompt is given room for max_seq_len."""
+    host_lens: the lengths [num_seqs] on the host, no shorter than those on the device; without them every prompt is given room for
+    max_seq_len, and while a graph is captured for all that its row of the table holds."""
     pages, hkv, page_size, d = _pair(k_cache, v_cache)
     (t, width), (q_ts, one), hq = q.shape, q.stride(), num_q_heads
     assert q.dtype is _BF16 and width >= hq * d and one == 1 and d == head_dim and hq % hkv == 0
@@ -167,32 +168,39 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
     on_this_device(q, out, k_cache, v_cache, block_table, seq_lens)
     L, st = _lib.load(), stream_ptr()
-    pitch = block_table.stride(0)
+    pitch, width = block_table.stride(0), block_table.shape[1]
     k_at, v_at, out_at, table_at, lens_at = k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
     if num_decode_seqs > 0:
         size = _decode_scratch(d)
         scratch = k_cache.new_empty(size)                     # of this call: captured graphs and streams share none
-        check(L.gllm_kv4_decode(q_at, q_ts, out_at, k_at, v_at, pages, table_at, pitch, lens_at, num_decode_seqs, hq, hkv, d, page_size,
+        check(L.gllm_kv4_decode(q_at, q_ts, out_at, k_at, v_at, pages, table_at, pitch, width, lens_at, num_decode_seqs, hq, hkv, d, page_size,
                                 scale, _DECODE_CTAS, scratch.data_ptr(), size, st), "kv4_decode")
         _count(2)
     prompts = num_seqs - num_decode_seqs
     if prompts > 0 and max_q_len > 0:
         _index(query_start_loc, "query_start_loc")
         on_this_device(query_start_loc)
-        lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
+        if torch.cuda.is_current_stream_capturing():          # replayed at other lengths
+            lens = [width * page_size] * prompts
+        else:
+            lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
         start_at = query_start_loc.data_ptr()
         for first, end, tiles in expand_rounds(lens, 4 * hkv * d, EXPAND_BYTES):
             if tiles == 0:
                 continue
             a, n = num_decode_seqs + first, end - first
             longest = int(max(lens[first:end]))
-            k = q.new_empty((tiles, hkv, d // 64, 64, 64))
-            v = torch.empty_like(k)
-            max_tiles = (longest + 63) // 64
-            table = seq_lens.new_empty((n, max_tiles))
-            check(L.gllm_kv4_expand(k_at, v_at, table_at + 4 * a * pitch, pitch, lens_at + 4 * a, n, hkv, d, page_size, pages, tiles,
-                                    k.data_ptr(), v.data_ptr(), table.data_ptr(), max_tiles, longest, st), "kv4_expand")
-            check(L.gllm_attn_prefill_tc_tiles(q_at, q_ts, out_at, k.data_ptr(), v.data_ptr(), tiles, table.data_ptr(), max_tiles,
+            # the tiles' table, keys, values. The table comes first: a sequence that is longer than its room (not what the caller said)
+            # has entries read behind it, which lie in the keys, and tiles that do not exist, which are read as zeros
+            max_tiles, tile = (longest + 63) // 64, hkv * d * 128
+            head = (4 * n * max_tiles + 255) // 256 * 256
+            room = k_cache.new_empty(head + 2 * tiles * tile)
+            t_at = room.data_ptr()
+            kt_at = t_at + head
+            vt_at = kt_at + tiles * tile
+            check(L.gllm_kv4_expand(k_at, v_at, table_at + 4 * a * pitch, pitch, width, lens_at + 4 * a, n, hkv, d, page_size, pages, tiles,
+                                    kt_at, vt_at, t_at, max_tiles, longest, st), "kv4_expand")
+            check(L.gllm_attn_prefill_tc_tiles(q_at, q_ts, out_at, kt_at, vt_at, tiles, t_at, max_tiles,
                                                lens_at + 4 * a, start_at + 4 * a, t, n, max_q_len, hq, hkv, d, scale, st),
                   "attn_prefill_tc_tiles")
             _count(2)

@@ -290,6 +290,53 @@ def test_decode_captured_and_replayed_with_other_lengths_beside_another_graph():
             assert ((out.view_as(want).double() - want).abs() <= tol).all()
 
 
+def test_prompts_captured_and_replayed_with_other_lengths():
+    """A graph has room for what its block table holds, whatever the lengths were when it was captured."""
+    from gllm_b200.ops import sm100_kv4
+    hq, hkv, d, news = 4, 2, 64, [1, 30, 70]
+    caches, rows, table = _filled([512] * 3, hkv, d, 16)
+    q = torch.randn(sum(news), hq * d, device=DEV).to(BF16)
+    n, starts = _i32([5, 40, 70]), _i32([0, 1, 31, 101])
+    out = torch.empty(sum(news), hq * d, dtype=BF16, device=DEV)
+
+    def call():
+        sm100_kv4.paged_attention(q, *caches, table, n, starts, d ** -0.5, hq, d, 1, 3, 70, 70, out=out, host_lens=[5, 40, 70])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lens in ([5, 40, 70], [400, 512, 333], [1, 30, 512]):
+        n.copy_(_i32(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, at, rounded in ((0, 1, 0, False), (1, 3, 1, True)):
+            want, tol = U.attention(q[at:sum(news[:b])].view(-1, hq, d), rows[a:b], lens[a:b], news[a:b], d ** -0.5, hkv, rounded)
+            assert ((out[at:sum(news[:b])].view_as(want).double() - want).abs() <= tol).all(), (lens, a)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [1, 40, 3]])
+def test_tables_that_are_views(news):
+    """Rows of a wider table, and one row for all sequences."""
+    hq, hkv, d, lens, tokens, first = 4, 2, 64, [40, 100, 77], sum(news), news[0]
+    caches, rows, table = _filled([112] * 3, hkv, d, 16)
+    q = torch.randn(tokens, hq * d, device=DEV).to(BF16)
+    decodes = 3 if max(news) == 1 else 1
+    wide = torch.full((3, 21), 0x7fffffff, dtype=torch.int32, device=DEV)
+    wide[:, 13:] = table
+    for t, r in ((wide[:, 13:], rows), (table[1:2].expand(3, -1), [rows[1]] * 3)):
+        got = _attend(q, caches, t, lens, news, decodes, hq, hkv, d).view(-1, hq, d).double()
+        for a, b, rounded in ((0, decodes, False), (decodes, 3, True)):
+            at = slice(sum(news[:a]), sum(news[:b]))
+            if a < b:
+                want, tol = U.attention(q[at].view(-1, hq, d), r[a:b], lens[a:b], news[a:b], d ** -0.5, hkv, rounded)
+                assert ((got[at] - want).abs() <= tol).all()
+
+
 def test_attention_refuses():
     from gllm_b200.ops import sm100_kv4
     caches, rows, table = _filled([20], 2, 64, 16)
