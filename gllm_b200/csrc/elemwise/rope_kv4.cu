@@ -12,11 +12,29 @@
 // Queries are rotated in place; the rotated keys go to the cache only.
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
+#include "../seq/seq_common.cuh"
 #include "rope_common.cuh"
 
 namespace b200 {
 
 namespace {
+
+using seqk::add2;
+using seqk::f2;
+using seqk::fma2;
+using seqk::mul2;
+using seqk::pk;
+
+__device__ __forceinline__ f2 both(float a) { return pk(a, a); }
+// a + b of products that are rounded by themselves. The compiler makes one rounding of product and sum where it sees them, and of a factor
+// that it knows to be one, so `one` comes with the launch (-one: a - b).
+__device__ __forceinline__ f2 plus2(f2 a, f2 b, f2 one) { return fma2(b, one, a); }
+__device__ __forceinline__ f2 unpack2(uint32_t w) { return pk(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t pack2(f2 v) {
+  float a, b;
+  seqk::un(v, a, b);
+  return pack_bf16(a, b);
+}
 
 // where the block of `slot` starts in head 0 of its page, and the row in it; ok: the slot is one of the cache
 struct Kv4Place {
@@ -80,21 +98,39 @@ struct Kv4Group {
     constexpr float kMagic = 12582912.f;                 // 1.5 x 2^23: an integer added to it stands in the low bits
     uint32_t v = 0;
 #pragma unroll
-    for (int e = 7; e >= 0; --e) {
-      const float d = __fsub_rn(e & 1 ? __uint_as_float(w[e >> 1] & 0xffff0000u) : __uint_as_float(w[e >> 1] << 16), low);
-      v = v * 16u + __float_as_uint(__fadd_rn(quotient(d, scale, inv), kMagic));
+    for (int e = 3; e >= 0; --e) {
+      const f2 d = add2(unpack2(w[e]), both(-low)), q = mul2(d, both(inv));
+      float a, b;
+      seqk::un(add2(fma2(fma2(q, both(-scale), d), both(inv), q), both(kMagic)), a, b);           // `quotient`, two at a time
+      v = (v * 16u + __float_as_uint(b)) * 16u + __float_as_uint(a);
     }
     // sum of 16^e (kMagic's bits) mod 2^32: 0x4b400000 (1 + 16 + 256), the rest is shifted out
     return inv > 0.f ? v - (0x4b400000u + 0xb4000000u + 0x40000000u) : 0u;
   }
 };
 
+__device__ __forceinline__ float squares(const f2 (&x)[4]) {
+  f2 v = mul2(x[0], x[0]);
+#pragma unroll
+  for (int e = 1; e < 4; ++e) v = fma2(x[e], x[e], v);
+  float a, b;
+  seqk::un(v, a, b);
+  return a + b;
+}
+// x inv w, rounded to bf16 as on a bf16 cache
+__device__ __forceinline__ void normed(f2 (&x)[4], float inv, const __nv_bfloat16* w) {
+  const uint4 v = *reinterpret_cast<const uint4*>(w);
+  const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = unpack2(pack2(mul2(mul2(x[e], both(inv)), unpack2(ww[e]))));
+}
+
 __device__ __forceinline__ uint8_t* kc_of(const RopeParams& p) { return reinterpret_cast<uint8_t*>(p.k_cache); }
 __device__ __forceinline__ uint8_t* vc_of(const RopeParams& p) { return reinterpret_cast<uint8_t*>(p.v_cache); }
 
 // A lane holds eight dims of a head, L = D / 8 lanes a head, NB heads a lane group, all loaded before the first is worked on.
 template <int L, int NB>
-__global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const int64_t pages, const int wide) {
+__global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const int64_t pages, const int wide, const float one) {
   griddep_launch();
   griddep_wait();
   constexpr int D = 8 * L, G = D / 64, kHeadsPerWarp = 32 / L, kStep = 4 * kHeadsPerWarp;
@@ -118,7 +154,8 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
     }
   }
   // this lane's rotation row: the pair of element e is (e0 + e) % half (NeoX) or (e0 + e) / 2 (neighbours)
-  float c[8], s[8];
+  const f2 plus = both(one), minus = both(-one);
+  f2 c[4], s[4];
   const bool in_rot = e0 < p.rot, lo = e0 < half;
   if (in_rot && p.sec0 == 0 && wide) {
     const float* row = p.cos_sin + static_cast<size_t>(p.positions[t]) * p.rot;
@@ -127,22 +164,28 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 cv = *reinterpret_cast<const float4*>(row + i + 4 * g), sv = *reinterpret_cast<const float4*>(row + half + i + 4 * g);
-        c[4 * g] = cv.x; c[4 * g + 1] = cv.y; c[4 * g + 2] = cv.z; c[4 * g + 3] = cv.w;
-        s[4 * g] = sv.x; s[4 * g + 1] = sv.y; s[4 * g + 2] = sv.z; s[4 * g + 3] = sv.w;
+        c[2 * g] = pk(cv.x, cv.y); c[2 * g + 1] = pk(cv.z, cv.w);
+        s[2 * g] = pk(sv.x, sv.y); s[2 * g + 1] = pk(sv.z, sv.w);
       }
     } else {
       const float4 cv = *reinterpret_cast<const float4*>(row + e0 / 2), sv = *reinterpret_cast<const float4*>(row + half + e0 / 2);
-      c[0] = c[1] = cv.x; c[2] = c[3] = cv.y; c[4] = c[5] = cv.z; c[6] = c[7] = cv.w;
-      s[0] = s[1] = sv.x; s[2] = s[3] = sv.y; s[4] = s[5] = sv.z; s[6] = s[7] = sv.w;
+      c[0] = both(cv.x); c[1] = both(cv.y); c[2] = both(cv.z); c[3] = both(cv.w);
+      s[0] = both(sv.x); s[1] = both(sv.y); s[2] = both(sv.z); s[3] = both(sv.w);
     }
   } else if (in_rot) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = p.neox ? e0 + e - (lo ? 0 : half) : (e0 + e) >> 1;
-      const int pos = p.sec0 != 0 ? p.positions[mrope_axis(i, p.sec0, p.sec1) * p.pos_stride + t] : p.positions[t];
-      const float* row = p.cos_sin + static_cast<size_t>(pos) * p.rot;
-      c[e] = row[i];
-      s[e] = row[half + i];
+    for (int e = 0; e < 4; ++e) {
+      float cs[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = p.neox ? e0 + 2 * e + j - (lo ? 0 : half) : (e0 + 2 * e) >> 1;
+        const int pos = p.sec0 != 0 ? p.positions[mrope_axis(i, p.sec0, p.sec1) * p.pos_stride + t] : p.positions[t];
+        const float* row = p.cos_sin + static_cast<size_t>(pos) * p.rot;
+        cs[0][j] = row[i];
+        cs[1][j] = row[half + i];
+      }
+      c[e] = pk(cs[0][0], cs[0][1]);
+      s[e] = pk(cs[1][0], cs[1][1]);
     }
   }
   const int dl = half / 8;
@@ -156,59 +199,42 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
     if (hh - lane / L >= n_heads) break;                 // none for the whole warp
     const bool is_q = hh < p.Hq, is_qk = hh < n_qk;
     uint32_t w[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
-    float x[8];
+    f2 x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack_bf16(w[e]);
-      x[2 * e] = f.x;
-      x[2 * e + 1] = f.y;
-    }
+    for (int e = 0; e < 4; ++e) x[e] = unpack2(w[e]);
     const __nv_bfloat16* nw = is_q ? p.q_norm_w : p.k_norm_w;
     if (p.q_norm_w != nullptr || p.k_norm_w != nullptr) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+      float ss = squares(x);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (is_qk && nw != nullptr) {
-        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-        const uint4 wv = *reinterpret_cast<const uint4*>(nw + e0);
-        const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16(ww[e]);
-          // rounded to bf16 after the norm, as on a bf16 cache
-          const float2 y = unpack_bf16(pack_bf16(x[2 * e] * inv * f.x, x[2 * e + 1] * inv * f.y));
-          x[2 * e] = y.x;
-          x[2 * e + 1] = y.y;
-        }
-      }
+      if (is_qk && nw != nullptr) normed(x, rsqrtf(ss * (1.f / D) + p.eps), nw + e0);
     }
     if (p.rot > 0) {
       // products and sum rounded one by one: a contraction would turn the last bit of some keys, and with it their codes
       if (p.neox) {
-        float y[8];
+        f2 y[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
+        for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
         if (in_rot && is_qk) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = __fmul_rn(x[e], c[e]), b = __fmul_rn(y[e], s[e]);
-            x[e] = lo ? __fsub_rn(a, b) : __fadd_rn(a, b);
+          for (int e = 0; e < 4; ++e) {
+            const f2 a = mul2(x[e], c[e]), b = mul2(y[e], s[e]);
+            x[e] = plus2(a, b, lo ? minus : plus);
           }
         }
       } else if (in_rot && is_qk) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float a = x[e], b = x[e + 1];
-          x[e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-          x[e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+        for (int e = 0; e < 4; ++e) {                    // (a c - b s, b c + a s): the halves of c and of s are equal
+          float a, b, si, same;
+          seqk::un(x[e], a, b);
+          seqk::un(s[e], si, same);
+          x[e] = plus2(mul2(x[e], c[e]), mul2(pk(b, a), pk(-si, si)), plus);
         }
       }
     }
     if (is_qk) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+      for (int e = 0; e < 4; ++e) w[e] = pack2(x[e]);
     }
     if (is_q) *reinterpret_cast<uint4*>(p.q + t * p.q_ts + hh * p.q_hs + e0) = make_uint4(w[0], w[1], w[2], w[3]);
     if (__all_sync(0xffffffffu, is_q)) continue;
@@ -226,7 +252,7 @@ __global__ void __launch_bounds__(128) rope_kv4_kernel(const RopeParams p, const
 // NeoX rotation of whole heads (rot = D), the common form: a lane holds eight dims of the lower half and their partners of the upper
 // one, L = D / 16 lanes a head, so that nothing is exchanged for the rotation; heads of 128: its two words are neighbours in the cache.
 template <int L, int NB>
-__global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, const int64_t pages) {
+__global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, const int64_t pages, const float one) {
   griddep_launch();
   griddep_wait();
   constexpr int D = 16 * L, H = D / 2, G = D / 64, kHeadsPerWarp = 32 / L, kStep = 4 * kHeadsPerWarp;
@@ -248,13 +274,14 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
       raw[n][1] = *reinterpret_cast<const uint4*>(src + H + e0);
     }
   }
-  float c[8], s[8];
+  const f2 plus = both(one), minus = both(-one);
+  f2 c[4], s[4];
   const float* row = p.cos_sin + static_cast<size_t>(p.positions[t]) * D + e0;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     const float4 cv = *reinterpret_cast<const float4*>(row + 4 * g), sv = *reinterpret_cast<const float4*>(row + H + 4 * g);
-    c[4 * g] = cv.x; c[4 * g + 1] = cv.y; c[4 * g + 2] = cv.z; c[4 * g + 3] = cv.w;
-    s[4 * g] = sv.x; s[4 * g + 1] = sv.y; s[4 * g + 2] = sv.z; s[4 * g + 3] = sv.w;
+    c[2 * g] = pk(cv.x, cv.y); c[2 * g + 1] = pk(cv.z, cv.w);
+    s[2 * g] = pk(sv.x, sv.y); s[2 * g + 1] = pk(sv.z, sv.w);
   }
   const Kv4Place at = kv4_place(p.slots[t], p.page_size, pages, p.Hkv, D);
   const size_t head_stride = static_cast<size_t>(p.page_size / 16) * (9 * D);
@@ -270,55 +297,28 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
       w[i][0] = raw[n][i].x; w[i][1] = raw[n][i].y; w[i][2] = raw[n][i].z; w[i][3] = raw[n][i].w;
     }
     if (__any_sync(0xffffffffu, is_qk)) {
-      float x[2][8];
+      f2 x[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_bf16(w[i][e]);
-          x[i][2 * e] = f.x;
-          x[i][2 * e + 1] = f.y;
-        }
+        for (int e = 0; e < 4; ++e) x[i][e] = unpack2(w[i][e]);
       }
       if (norm) {
-        float ss = 0.f, upper = 0.f;                     // apart: the order of the sums is the other kernel's, and so are the bits
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss += x[0][e] * x[0][e];
-          upper += x[1][e] * x[1][e];
-        }
-        ss += upper;
+        float ss = squares(x[0]) + squares(x[1]);        // the order of the sums is the other kernel's, and so are the bits
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const __nv_bfloat16* nw = is_q ? p.q_norm_w : p.k_norm_w;
         if (is_qk && nw != nullptr) {
           const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 wv = *reinterpret_cast<const uint4*>(nw + i * H + e0);
-            const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack_bf16(ww[e]);
-              const float2 y = unpack_bf16(pack_bf16(x[i][2 * e] * inv * f.x, x[i][2 * e + 1] * inv * f.y));
-              x[i][2 * e] = y.x;
-              x[i][2 * e + 1] = y.y;
-            }
-          }
+          normed(x[0], inv, nw + e0);
+          normed(x[1], inv, nw + H + e0);
         }
       }
       if (is_qk) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float r[2][2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {                  // rounded one by one, as above
-            const int i = 2 * e + j;
-            r[0][j] = __fsub_rn(__fmul_rn(x[0][i], c[i]), __fmul_rn(x[1][i], s[i]));
-            r[1][j] = __fadd_rn(__fmul_rn(x[1][i], c[i]), __fmul_rn(x[0][i], s[i]));
-          }
-          w[0][e] = pack_bf16(r[0][0], r[0][1]);
-          w[1][e] = pack_bf16(r[1][0], r[1][1]);
+        for (int e = 0; e < 4; ++e) {                    // rounded one by one, as above
+          w[0][e] = pack2(plus2(mul2(x[0][e], c[e]), mul2(x[1][e], s[e]), minus));
+          w[1][e] = pack2(plus2(mul2(x[1][e], c[e]), mul2(x[0][e], s[e]), plus));
         }
       }
     }
@@ -403,8 +403,8 @@ cudaError_t launch_rope_kv4(const RopeParams& p, int64_t pages, cudaStream_t st)
   const int wide = (reinterpret_cast<uintptr_t>(p.cos_sin) & 15) == 0 && p.rot % 8 == 0;       // rotation rows in pieces of 16 bytes
   // many tokens: several heads a lane, fewer and longer blocks; a decode batch: one, so that it still fills the machine
   if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 2)
-    return launch_pdl(rope_kv4_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages, wide);
-  return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages, wide);
+    return launch_pdl(rope_kv4_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages, wide, 1.f);
+  return launch_pdl(rope_kv4_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages, wide, 1.f);
 }
 
 template <int L>
@@ -412,8 +412,8 @@ cudaError_t launch_rope_kv4_pair(const RopeParams& p, int64_t pages, cudaStream_
   constexpr int kStep = 4 * (32 / L);
   const int n_heads = p.Hq + 2 * p.Hkv;
   if (static_cast<int64_t>(p.T) * n_heads >= static_cast<int64_t>(num_sms()) * 16 * kStep * 2)
-    return launch_pdl(rope_kv4_pair_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages);
-  return launch_pdl(rope_kv4_pair_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages);
+    return launch_pdl(rope_kv4_pair_kernel<L, 2>, dim3(p.T, (n_heads + 2 * kStep - 1) / (2 * kStep)), dim3(128), 0, st, p, pages, 1.f);
+  return launch_pdl(rope_kv4_pair_kernel<L, 1>, dim3(p.T, (n_heads + kStep - 1) / kStep), dim3(128), 0, st, p, pages, 1.f);
 }
 
 }  // namespace
