@@ -55,6 +55,18 @@ def test_rows_are_quantised_to_the_nearest(m, k):
     torch.testing.assert_close(s.to(F64), unit[:, 0], rtol=2 ** -24, atol=0)
 
 
+@pytest.mark.parametrize("power", [-90, 0, 117])
+def test_every_quotient_of_two_bf16(power):
+    """Each largest magnitude beside each other value that does not vanish, ties among them: a bf16 has eight bits."""
+    from gllm_b200.ops import sm100
+    bits = torch.arange(128, 256, device=DEV, dtype=F64)
+    below = torch.cat([bits * 2.0 ** -e for e in range(1, 10)])
+    x = torch.cat([bits[:, None], torch.minimum(bits[None], bits[:, None]), -below.expand(128, -1), torch.zeros(128, 15, device=DEV)], 1)
+    x = (x * 2.0 ** power).to(BF16)
+    q, s = sm100.int8_quant_rows(x)
+    assert torch.equal(q.to(F64), torch.round(x.to(F64) * 127 / x[:, :1].to(F64))) and (q == 127).any(1).all()
+
+
 def test_rows_of_zeros_tiny_rows_and_rows_that_are_no_numbers():
     from gllm_b200.ops import sm100
     x = torch.randn(6, 64, device=DEV).to(BF16)
