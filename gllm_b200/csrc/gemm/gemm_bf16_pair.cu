@@ -13,9 +13,10 @@
 // 4096 x 6144 x 4096: 141 / 151; 8192 x 8192 x 256: 50 / 82 (with four warps to drain TMEM 58).
 //
 // With INT8 the operands are signed bytes (128 of K in a block of 128 bytes, twice the operations a block) and the sums integers; the scales of
-// rows and columns come in with the rounding (gemm_int8.cu has the rest of that product). 4096 x 24,576 x 4096 gated, quantiser included: 264
-// us, 3.1 PFLOP/s, 1.9 times what the library reaches in bf16. Cutting K of the tiles that are left for a last round, parts added
-// up through L2, gains nothing here either: 777 x 10,240 x 8192 75.9 us for 75.4, 4096 x 6144 x 4096 91 for 85.
+// rows and columns come in with the rounding (gemm_int8.cu has the rest of that product). 4096 x 24,576 x 4096 gated: 241 us, 3.4 POP/s, tensor
+// pipe 95 %; with the quantiser 261, 1.9 times what the library reaches in bf16. Without gain: tiles of 192 columns (the same time a tile: 777 x 10,240 x
+// 8192 68.9 for 72.8, others 10 to 40 % slower), K of the tiles left for a last round cut (75.9 for 75.4, 4096 x 6144 x 4096 91 for 85), the last
+// 9 rows of the 777 by themselves on clusters (74).
 //
 // Roles per CTA: warp 0 copies (both CTAs; every byte is counted by the leader's barrier of the stage), warp 1 issues products
 // (leader only) and commits to both CTAs' barriers, warps 2-9 drain TMEM (each CTA its own rows). Sums are double buffered: the
