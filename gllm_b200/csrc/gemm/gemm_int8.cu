@@ -5,55 +5,21 @@
 // x bf16, W int8 with fp32 scales s; gated: W = [gate rows ; up rows] and y = silu(gate) * up. The sums are int32, exact for K up to
 // 131,072 (127 x 128 x K < 2^31); scales, bias and gate are fp32, and y is rounded once.
 //
-// Two launches: the rows are quantised (here), then multiplied on the tensor cores (tcgen05.mma kind::i8) by one of two kernels:
+// A row or two (up to four where K is short) are multiplied while they are read (gemv_int8.cu). Otherwise two launches: the rows are
+// quantised (here), then multiplied on the tensor cores (tcgen05.mma kind::i8) by one of two kernels:
 // prompts on pairs of SMs (gemm_bf16_pair.cu), decode batches with K cut over a cluster (gemm_bf16_cluster.cu), which copies its first
 // weights while the rows are quantised. `gllm_linear_int8` chooses by what their time is made of. (Rows quantised in every CTA of the
 // cluster kernel, to save the launch: 10.0 us for one row of 6144 x 4096 instead of 9.1, 12.8 for four, 16 for eight.)
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
-#include "../seq/seq_common.cuh"
 #include "gemm_cluster.h"
 #include "gemm_pair.h"
+#include "gemv_int8.h"
+#include "int8_rows.cuh"
 
 namespace b200 {
 
 namespace {
-
-constexpr float kQuantFloor = 7.888609052210118e-31f;    // 2^-100: rows below it become zeros
-
-// the larger of two pairs of magnitudes, as bits: NaN is above infinity
-__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
-
-// Eight bytes from eight bf16. The quotient 127 x / a to the nearest, ties to even, as in exact arithmetic, two at a time: the remainder of the
-// first estimate is exact (the compiler may not fuse it away: its terms are no product and sum of one), and adding its share leaves an error far
-// below what lies between a quotient that is no tie and the tie next to it, while a tie comes out as one.
-// (x and a have eight bits each: the distance is 1 / 510 of the last place's unit of x, the error 2^-22 of the quotient.) 4096 rows of 4096 take 11.5 us, with one value an instruction and ties told by their remainders 18.1.
-struct Quant8 {
-  seqk::f2 inv, minus;                                   // 128 / a and -a / 128
-  uint32_t keep;                                         // no bits of rows that are not finite: codes of 0, the scale says the rest
-  __device__ __forceinline__ explicit Quant8(float a) {
-    const float i = __fdiv_rn(128.f, a);
-    inv = seqk::pk(i, i);
-    minus = seqk::pk(a * -0.0078125f, a * -0.0078125f);
-    keep = a <= 3.3895e38f ? 0xffffffffu : 0u;
-  }
-  __device__ __forceinline__ uint2 operator()(const uint4& raw) const {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    uint32_t b[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const seqk::f2 t = seqk::mul2(seqk::pk(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)),
-                                    seqk::pk(0.9921875f, 0.9921875f));          // 127 / 128: exact
-      const seqk::f2 q = seqk::mul2(t, inv);
-      float lo, hi;
-      seqk::un(seqk::add2(seqk::fma2(seqk::fma2(q, minus, t), inv, q), seqk::pk(12582912.f, 12582912.f)), lo, hi);
-      b[2 * e] = __float_as_uint(lo);                    // 1.5 x 2^23: an integer added to it stands in the low bits
-      b[2 * e + 1] = __float_as_uint(hi);
-    }
-    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & keep,
-                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410) & keep);
-  }
-};
 
 // A row is T threads' (a warp's or a block's), eight values a piece, NV pieces a thread kept in registers; NV = 0: any length, read
 // twice.
@@ -68,7 +34,6 @@ int8_quant_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t
   const __nv_bfloat16* src = x + static_cast<int64_t>(in ? row : 0) * ldx;
   uint4 raw[NV > 0 ? NV : 1];
   uint32_t most = 0;
-  auto take = [&](const uint4& v) { most = max_abs2(max_abs2(max_abs2(max_abs2(most, v.x), v.y), v.z), v.w); };
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -76,9 +41,9 @@ int8_quant_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t
       if (in && at + i * T < pieces) raw[i] = *reinterpret_cast<const uint4*>(src + (at + i * T) * 8);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) take(raw[i]);
+    for (int i = 0; i < NV; ++i) most = max_abs2(most, raw[i]);
   } else {
-    for (int i = at; i < pieces; i += T) take(*reinterpret_cast<const uint4*>(src + i * 8));
+    for (int i = at; i < pieces; i += T) most = max_abs2(most, *reinterpret_cast<const uint4*>(src + i * 8));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -90,8 +55,7 @@ int8_quant_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t
     for (int i = 0; i < T / 32; ++i) most = __vmaxu2(most, part[i]);
   }
   if (!in) return;
-  const float found = __uint_as_float(max(most & 0xffffu, most >> 16) << 16);
-  const float a = found < kQuantFloor ? kQuantFloor : found;                 // a NaN stays one
+  const float a = largest(most);
   const Quant8 quant(a);
   if (at == 0) scales[row] = __fdiv_rn(a, 127.f);
   uint8_t* dst = q + static_cast<int64_t>(row) * K;
@@ -123,7 +87,7 @@ int quant_rows(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, float* scales, i
 // SMs draw), and a fixed sum a round, which counts as 14 us here, more than the 0.8 us that it takes: a second round is rarely worth it.
 // The choice takes 1.5 % longer than the best plan on average (27 of 933 over 10 %, 1.42 at worst). Against the pairs both are estimated in
 // us; the choice between them loses 0.4 % (19 over 10 %, 1.28 at worst); the pairs win 91 of the 933, all but a few over 256 rows. Some, pairs and
-// chosen, us: 1 row of 6144 x 4096 18.6 and 8.8, 64 rows 24,576 x 4096 gated 33.9 and 24.8, 64 of 4096 x 12,288 37.5 and 18.4, 256 of 6144 x
+// chosen, us: 64 rows 24,576 x 4096 gated 33.9 and 24.8, 64 of 4096 x 12,288 37.5 and 18.4, 256 of 6144 x
 // 4096 19.7 and 19.1, 777 of 10,240 x 8192 71.7 and 80.1.
 bool plan_int8(int M, int N, int K, bool gated, ClusterPlan* plan) {
   if (M > 1024) return false;
@@ -184,15 +148,19 @@ GLLM_EXPORT int gllm_int8_quant_rows(const void* x, int64_t ldx, void* q, void* 
                     K, reinterpret_cast<cudaStream_t>(stream));
 }
 
-// y [M, N] (gated: [M, N / 2]) of x [M, K] and W8 [N, K] int8 (contiguous) with w_scale [N]; xq [M, K] and x_scale [M] are scratch.
-// form: 0 = by size, 1 = pairs of SMs, 2 = clusters with bt rows of x a tile and K in `parts` (tests, tuning).
+// Whether the form that is taken for M rows needs no scratch.
+GLLM_EXPORT int gllm_int8_rows_inside(int M, int K) { return gemv_int8_takes(M, K) ? 1 : 0; }
+
+// y [M, N] (gated: [M, N / 2]) of x [M, K] and W8 [N, K] int8 (contiguous) with w_scale [N]; xq [M, K] and x_scale [M] are scratch (null
+// where gllm_int8_rows_inside says so).
+// form: 0 = by size, 1 = pairs of SMs, 2 = clusters with bt rows of x a tile and K in `parts`, 3 = a few rows (tests, tuning).
 GLLM_EXPORT int gllm_linear_int8(const void* x, int64_t ldx, void* xq, void* x_scale, const void* W8, const void* w_scale, void* C,
                                  int64_t ldc, int M, int N, int K, const void* bias, int gated, int form, int bt, int parts, int smem,
                                  void* stream) {
   if (M <= 0 || N <= 0) return 0;
   const int out_N = gated ? N / 2 : N;
   if (K <= 0 || K % 16 != 0 || K > 131072 || N % 8 != 0 || out_N % 8 != 0 || (gated && (N % 2 != 0 || bias != nullptr)) || ldx % 8 != 0 ||
-      ldc % 8 != 0 || form < 0 || form > 2 ||
+      ldc % 8 != 0 || form < 0 || form > 3 || (form == 3 && !gemv_int8_fits(M, K)) ||
       ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W8) | reinterpret_cast<uintptr_t>(w_scale) |
         reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(bias)) & 15) != 0 ||
       (form == 2 && (bt % 16 != 0 || bt < 16 || bt > 256 || parts < 1 || parts > 8 || parts > (K + 127) / 128))) {
@@ -200,6 +168,15 @@ GLLM_EXPORT int gllm_linear_int8(const void* x, int64_t ldx, void* xq, void* x_s
     return 1;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (form == 0 && gemv_int8_takes(M, K)) form = 3;
+  if (form == 3)
+    return gemv_int8(GemvInt8{reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<const uint8_t*>(W8),
+                              reinterpret_cast<const float*>(w_scale), reinterpret_cast<__nv_bfloat16*>(C), ldc,
+                              reinterpret_cast<const __nv_bfloat16*>(bias), N, K}, M, gated != 0, st);
+  if (xq == nullptr || x_scale == nullptr) {
+    fprintf(stderr, "[gllm_b200] linear_int8: no room for the quantised rows\n");
+    return 1;
+  }
   if (const int rc = quant_rows(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<uint8_t*>(xq),
                                 reinterpret_cast<float*>(x_scale), M, K, st))
     return rc;

@@ -90,6 +90,7 @@ def _declare(lib):
     sig("gllm_fp8_quant_group", [P, L, P, P, I, I, P, P])
     sig("gllm_moe_grouped_gemm_fp8", [P, P, P, P, P, L, I, I, I, I, I, P, P, I, P])
     sig("gllm_set_waits", [P, c_uint32])
+    sig("gllm_int8_rows_inside", [I, I])
     sig("gllm_int8_quant_rows", [P, L, P, P, I, I, P])
     sig("gllm_linear_int8", [P, L, P, P, P, P, P, L, I, I, I, P, I, I, I, I, I, P])
     sig("gllm_rope_kv4_write", [P, L, L, I, P, L, L, I, P, L, L, P, P, P, I, I, I, I, P, P, F, P, P, L, I, I, I, L, P])

@@ -6,6 +6,7 @@ CUDA stream. No fallback: if the library is missing on a GPU box this raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -546,6 +547,12 @@ def int8_quant_rows(x: torch.Tensor):
     return q, s
 
 
+@functools.lru_cache(maxsize=None)
+def _int8_rows_inside(m: int, k: int) -> bool:
+    """Whether the product quantises so few rows by itself."""
+    return bool(_lib.load().gllm_int8_rows_inside(m, k))
+
+
 def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None, silu: bool = False, plan: Optional[tuple] = None) -> torch.Tensor:
     """x bf16 [M, K] (rows quantised here, `int8_quant_rows`); w8 int8 [N, K], w_scale fp32 [N] -> bf16 [M, N] (+ bias). `silu`: w8 is
@@ -574,12 +581,16 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
     if m == 0:
         return out
     on_this_device(x, w8, w_scale, out, bias)
-    scratch = w8.new_empty(m * k + 4 * m)        # k % 16: the scales lie on 16-byte boundaries
-    xq = scratch.data_ptr()
     form, bt, parts, smem = plan or (0, 0, 0, 0)
-    check(_lib.load().gllm_linear_int8(x.data_ptr(), x.stride(0), xq, xq + m * k, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,
+    xq_at = xs_at = None
+    inside = form == 3 or form == 0 and m <= 4 and _int8_rows_inside(m, k)
+    if not inside:
+        scratch = w8.new_empty(m * k + 4 * m)    # k % 16: the scales lie on 16-byte boundaries
+        xq_at = scratch.data_ptr()
+        xs_at = xq_at + m * k
+    check(_lib.load().gllm_linear_int8(x.data_ptr(), x.stride(0), xq_at, xs_at, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,
                                        smem, stream_ptr()), "linear_int8")
-    _count(2)
+    _count(1 if inside else 2)
     return out
 
 

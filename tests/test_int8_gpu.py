@@ -107,6 +107,33 @@ def test_gated_product(m, n, k):
     assert y.shape == (m, n // 2) and ((y.to(F64) - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+@pytest.mark.parametrize("n,k", [(16, 16), (48, 528), (2384, 80), (4768, 2064), (272, 4096), (1040, 4112), (64, 12288), (48, 40960)])
+@pytest.mark.parametrize("silu", [False, True])
+def test_few_rows_give_the_bits_of_the_other_forms(m, n, k, silu):
+    """Sums are exact and the same operations follow. More units than warps, fewer than SMs, K that ends inside a warp's loads."""
+    from gllm_b200.ops import sm100
+    x, w8, ws = _inputs(m, n, k)
+    wide = torch.zeros(m, k + 8, dtype=BF16, device=DEV)
+    wide[:, 8:] = x
+    ws = ws / k ** 0.5 * 0.3 if silu else ws
+    bias = None if silu else torch.randn(n, device=DEV).to(BF16)
+    y = sm100.linear_int8(wide[:, 8:], w8, ws, bias, silu=silu, plan=(3, 0, 0, 0))
+    want, tol = product(x, w8, ws, bias, silu=silu)
+    assert ((y.to(F64) - want).abs() <= tol).all()
+    assert torch.equal(y, sm100.linear_int8(x, w8, ws, bias, silu=silu, plan=(1, 0, 0, 0)))
+    assert torch.equal(y, sm100.linear_int8(x, w8, ws, bias, silu=silu))
+
+
+def test_few_rows_that_are_no_numbers():
+    from gllm_b200.ops import sm100
+    x, w8, ws = _inputs(4, 16, 64)
+    x[0], x[1, 5], x[2, 9] = 0.0, float("nan"), float("inf")
+    y = sm100.linear_int8(x, w8, ws, plan=(3, 0, 0, 0))
+    want, tol = product(x[3:], w8, ws)
+    assert (y[0] == 0).all() and torch.isnan(y[1:3]).all() and ((y[3:].to(F64) - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("plan", [(1, 0, 0, 0), (2, 16, 1, 108 * 1024), (2, 64, 3, 108 * 1024), (2, 32, 8, 220 * 1024), (2, 256, 2, 220 * 1024),
                                   (2, 112, 5, 108 * 1024)])
 @pytest.mark.parametrize("silu", [False, True])
