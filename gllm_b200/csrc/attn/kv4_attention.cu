@@ -28,10 +28,11 @@
 //
 // The reference follows only when a score passes the head's maximum by 2^8 or a scale the largest one (one vote instead of shuffles).
 //
-// What bounds it: bytes beside the ALU. Four sequences of up to 60,000 tokens, 64 / 8 heads of 128: 191 MB in 47.8 us, join included; longer
-// contexts add at 5.8 TB/s (copies without arithmetic: 6.8), and some 13 us are the start (4 to the first data), the uneven ends of the SMs
-// (6) and the join. 576 warp instructions a tile of 32 keys: ALU 52 %, issue slots 56 %, tensor pipe 24 %. 64 sequences of up to 2500 (32 / 8): 39.3
-// us; one of 700: 8.3, latency. Without gain: the base folded into the scores, six warps with 168 registers.
+// What bounds it: bytes beside the ALU. Four sequences of up to 60,000 tokens, 64 / 8 heads of 128: 191 MB in 45.5 us, join included (with two
+// CTAs of eight warps an SM 47.8); longer contexts add at 5.8 TB/s (copies without arithmetic: 6.8), and some 11 us are the start (4 to the
+// first data), uneven ends and the join. 576 warp instructions a tile of 32 keys: ALU 52 %, issue slots 56 %, tensor pipe 24 %. 64 sequences of up
+// to 2500 (32 / 8): 39.3 us; one of 700: 8.2, latency. Without gain: the base folded into the scores, 12 warps with 168 registers, larger shares
+// for some CTAs.
 #include "../common/bounded.cuh"
 #include "attn_common.cuh"
 
@@ -39,9 +40,8 @@ namespace b200 {
 
 namespace {
 
-constexpr int kV4Warps = 8, kV4Threads = kV4Warps * 32, kV4Keys = 32, kV4Stages = 2;
-static_assert(kV4Threads == 256);
-constexpr int kV4Lens = kV4Threads;                             // lengths that a CTA keeps in shared memory, from its first sequence on
+constexpr int kV4Keys = 32, kV4Stages = 2, kV4Least = 8;      // tiles of a CTA's share, at least
+constexpr int kV4Snap = 1;                               // tiles by which a cut moves to a head group's start or end (two: 256 x 75 16.5 for 18.5 us, all others longer, by up to 5 %)
 constexpr float kV4Lazy = 8.f;                           // scores pass the maximum that the reference is taken from by no more than this
 constexpr float kV4Room = 6.f;                           // and exponentials times scales stay below 2^(kV4Lazy + kV4Room)
 
@@ -67,6 +67,10 @@ struct Kv4Params {
 
 template <int D, int NT>
 struct Kv4Smem {
+  // As many warps as registers allow, in one CTA: of two CTAs on an SM the first had the better of the second (its warps were done after 32 us, the
+  // other's after 37), where all of one get on alike.
+  static constexpr int kV4Warps = NT == 1 ? 16 : 8, kV4Threads = kV4Warps * 32;
+  static constexpr int kV4Lens = kV4Threads;             // lengths that a CTA keeps in shared memory, from its first sequence on
   static constexpr int kBlock = 9 * D;                   // 16 tokens' keys or values
   static constexpr int kStage = 4 * kBlock;
   static constexpr int kRing = kV4Warps * kV4Stages * kStage;
@@ -116,8 +120,9 @@ __device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(
 __device__ __forceinline__ int kv4_tiles(int len) { return max(1, (len + kV4Keys - 1) / kV4Keys); }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kernel(const Kv4Params p) {
   using SM = Kv4Smem<D, NT>;
+  constexpr int kV4Warps = SM::kV4Warps, kV4Threads = SM::kV4Threads, kV4Lens = SM::kV4Lens;
   constexpr int GR = D / 64;                             // groups of a head
   constexpr int KS = D / 16;                             // 16-dim steps of the first product, and dim tiles of the second
   extern __shared__ __align__(128) uint8_t smem[];
@@ -164,7 +169,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   int64_t share, begin, end;
   auto cut = [&] {
     const int64_t work = static_cast<int64_t>(all) * H;
-    share = max((work + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kV4Warps));
+    share = max((work + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kV4Least));
     begin = share * blockIdx.x;
     end = min(begin + share, work);
   };
@@ -264,10 +269,33 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   };
   // This warp's part [my_begin, my_end) of the share.
   const int each = tiles / kV4Warps, over = tiles % kV4Warps;        // the first ones have one more: a warp without tiles has none behind it
-  const int my_begin = warp * each + min(warp, over), my_end = my_begin + each + (warp < over ? 1 : 0);
-  const uint32_t my_tiles = static_cast<uint32_t>(my_end - my_begin);
+  int my_begin = warp * each + min(warp, over), my_end = my_begin + each + (warp < over ? 1 : 0);
   at_tile += my_begin;
   settle(at, at_tile);
+  // A cut that lies next to a head group's start or end moves there, where warps have two tiles and more: a part less (256 sequences of some 75:
+  // 22.3 -> 18.6 us).
+  const bool snap = share >= 2 * kV4Warps;
+  auto moves = [&](int n, int tile) {
+    return !snap ? 0 : tile <= kV4Snap && 2 * tile <= n ? -tile : n - tile <= kV4Snap ? n - tile : 0;
+  };
+  if (snap) {
+    Place stop = at;
+    int stop_tile = at_tile + (my_end - my_begin);
+    settle(stop, stop_tile);
+    if (stop.seq < p.B) my_end += moves(stop.n, stop_tile);
+    if (at.seq < p.B) {
+      const int by = moves(at.n, at_tile);
+      my_begin += by;
+      at_tile += by;
+      settle(at, at_tile);
+    }
+  }
+  const uint32_t my_tiles = static_cast<uint32_t>(my_end - my_begin);
+  auto last_cta = [&](int64_t stop, int n) {             // the CTA that ends a head group of n tiles up to `stop`
+    const int64_t cta = (stop - 1) / share;
+    const int tile = n - static_cast<int>(stop - cta * share);         // where its share begins, from the group's start
+    return static_cast<int>(tile > 0 && moves(n, tile) > 0 ? cta - 1 : cta);
+  };
   if (lane < 2) info[lane * kV4Warps + warp] = make_int4(-1, 0, 0, 0);
   __syncwarp();
 
@@ -614,7 +642,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
       float4* to = starts ? reinterpret_cast<float4*>(smem + warp * (kV4Stages * SM::kStage)) : firsts + warp * kPieces * 32;
       float* to_ml = ml + ((starts ? kV4Warps : 0) + warp) * 16 * NT;
       if (lane == 0)
-        info[(starts ? kV4Warps : 0) + warp] = make_int4(at.seq, at.head, ends ? 1 : 0, starts ? static_cast<int>((begin + seg + at.n - 1) / share) : 0);
+        info[(starts ? kV4Warps : 0) + warp] = make_int4(at.seq, at.head, ends ? 1 : 0, starts ? last_cta(begin + seg + at.n, at.n) : 0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -637,19 +665,23 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
   __syncthreads();
   // ---- the parts of this CTA's warps: a row starts with a warp's last part, or with what the CTA before began, and goes on through
   // the first parts of the warps behind. Four dims of a head a thread.
-  static_assert(kV4Warps == 8);
+  constexpr uint32_t kAll = (1u << kV4Warps) - 1;
+  static_assert(2 * kV4Warps <= 32);
   const int4 mine = lane < 2 * kV4Warps ? info[lane] : make_int4(-1, 0, 0, 0);
-  const uint32_t parts = __ballot_sync(0xffffffffu, mine.x >= 0), ending = __ballot_sync(0xffffffffu, mine.x >= 0 && mine.z != 0) & 0xffu;
-  for (uint32_t rows = (parts >> 8) << 1 | (parts & 1u); rows != 0; rows &= rows - 1) {        // bit 0: what the CTA before began
+  const uint32_t parts = __ballot_sync(0xffffffffu, mine.x >= 0), ending = __ballot_sync(0xffffffffu, mine.x >= 0 && mine.z != 0) & kAll;
+  constexpr int kTeam = kPieces < kV4Warps ? kPieces : kV4Warps, kTeams = kV4Warps / kTeam;       // as many warps as a row has pieces
+  int turn = 0;
+  for (uint32_t rows = (parts >> kV4Warps) << 1 | (parts & 1u); rows != 0; rows &= rows - 1) {        // bit 0: what the CTA before began
     const int row = __ffs(rows) - 2;
-    const uint32_t behind = (parts & 0xffu) >> (row + 1), stops = ending >> (row + 1);
+    if (turn++ % kTeams != warp / kTeam) continue;
+    const uint32_t behind = (parts & kAll) >> (row + 1), stops = ending >> (row + 1);
     const int run = __ffs(~behind) - 1, stop = __ffs(stops);                 // first parts in a row, place of the one that ends (from 1 on)
     const bool done = stop != 0 && stop <= run;
     const int last = row + (done ? stop : run), at_info = row < 0 ? 0 : kV4Warps + row;          // the last warp with a part
     const int4 what = make_int4(__shfl_sync(0xffffffffu, mine.x, at_info), __shfl_sync(0xffffffffu, mine.y, at_info), 0,
                                 __shfl_sync(0xffffffffu, mine.w, at_info));
     const int head0 = what.y / hg * p.G + what.y % hg * p.GP, slot = 2 * static_cast<int>(blockIdx.x) + (row < 0 ? 0 : 1);
-    for (int x = warp; x < kPieces; x += kV4Warps) {
+    for (int x = warp % kTeam; x < kPieces; x += kTeam) {
       const int nt = x / (GR * 4), gr = x / 4 % GR, c = x / 2 % 2, half = x % 2;
       const int h = 8 * nt + 2 * t + c, dim = gr * 64 + 8 * g + 4 * half;
       float top = -INFINITY, sum = 0.f;
@@ -675,7 +707,7 @@ __global__ void __launch_bounds__(kV4Threads, NT == 1 ? 2 : 1) kv4_decode_kernel
         }
       }
     }
-    if (row >= 0 && !done && tid == 0) p.meta[blockIdx.x] = make_int4(what.x, what.y, what.w, slot);     // goes on in the next share
+    if (row >= 0 && !done && warp % kTeam == 0 && lane == 0) p.meta[blockIdx.x] = make_int4(what.x, what.y, what.w, slot);     // goes on in the next share
   }
   // copies in flight land before the CTA ends, where the waits were given up
   for (; used < issued; ++used) guard.land(&bar[used % kV4Stages], (used / kV4Stages) & 1);
@@ -750,14 +782,13 @@ __global__ void __launch_bounds__(256 * WAYS) kv4_join_kernel(const Kv4Params p)
 template <int D, int NT>
 int launch_kv4_decode(const Kv4Params& p, int ctas, cudaStream_t st) {
   using SM = Kv4Smem<D, NT>;
-  if (NT > 1 && ctas > 1) ctas /= 2;                     // one fits an SM
   static PerDeviceOnce configured;
   if (configured.need()) {
     CUDA_CHECK_RET(cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
     configured.done();
   }
-  CUDA_CHECK_RET(launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(kV4Threads), SM::kBytes, st, p));
-  if (static_cast<int64_t>(p.B) * (p.Hq / p.GP) * 6 < ctas) CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT, 4>, dim3(ctas), dim3(1024), 0, st, p));
+  CUDA_CHECK_RET(launch_pdl(kv4_decode_kernel<D, NT>, dim3(ctas), dim3(SM::kV4Threads), SM::kBytes, st, p));
+  if (static_cast<int64_t>(p.B) * (p.Hq / p.GP) * 3 < ctas) CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT, 4>, dim3(ctas), dim3(1024), 0, st, p));
   else CUDA_CHECK_RET(launch_pdl(kv4_join_kernel<D, NT, 1>, dim3(ctas), dim3(256), 0, st, p));
   return 0;
 }

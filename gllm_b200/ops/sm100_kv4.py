@@ -12,7 +12,7 @@ from gllm_b200.ops import kv4, lib as _lib
 from gllm_b200.ops.lib import check, on_this_device, stream_ptr
 from gllm_b200.ops.sm100 import NUM_SMS, _BF16, _count
 
-_DECODE_CTAS = 2 * NUM_SMS           # two fit an SM
+_DECODE_CTAS = NUM_SMS               # one an SM
 EXPAND_BYTES = 1 << 30               # bf16 keys and values that prompts have at a time (one sequence at least)
 
 

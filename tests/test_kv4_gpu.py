@@ -166,7 +166,7 @@ def test_decode(lens, hq, hkv, d, page):
     assert ((got.view_as(want).double() - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("b,longest,hq,hkv,d", [(300, 90, 4, 2, 64), (700, 40, 8, 1, 128), (3, 30000, 8, 2, 128), (1, 50000, 16, 1, 64), (64, 1500, 8, 8, 128)])
+@pytest.mark.parametrize("b,longest,hq,hkv,d", [(300, 90, 4, 2, 64), (700, 40, 8, 1, 128), (256, 100, 32, 8, 128), (1100, 150, 4, 2, 64), (3, 30000, 8, 2, 128), (1, 50000, 16, 1, 64), (64, 1500, 8, 8, 128)])
 def test_decode_of_many_and_of_long_sequences(b, longest, hq, hkv, d):
     rng = np.random.RandomState(b)
     lens = rng.randint(1, longest + 1, b).tolist()
@@ -241,6 +241,20 @@ def test_prompts_without_lengths_on_the_host():
     q = torch.randn(sum(news), hq * d, device=DEV).to(BF16)
     args = (q, *caches, table, _i32(lens), _i32([0, 20, 120, 121]), 0.1, hq, d, 0, 3, 100, 190)
     assert torch.equal(sm100_kv4.paged_attention(*args), sm100_kv4.paged_attention(*args, host_lens=lens))
+
+
+def test_decode_of_more_sequences_than_a_block_keeps_lengths_of():
+    """A sequence of one tile is never cut, so it has the same bits in any batch."""
+    b, d = 90000, 64
+    caches, rows, table = _filled([16], 1, d, 16)
+    lens = np.random.RandomState(0).randint(0, 17, b).tolist()
+    q = torch.randn(b, d, device=DEV).to(BF16)
+    got = _attend(q, caches, table.expand(b, -1), lens, [1] * b, b, 1, 1, d)
+    for at in (0, 44000, b - 300):
+        part = _attend(q[at:at + 300], caches, table.expand(300, -1), lens[at:at + 300], [1] * 300, 300, 1, 1, d)
+        assert torch.equal(got[at:at + 300], part)
+    want, tol = U.attention(q[:40].view(40, 1, d), rows * 40, lens[:40], [1] * 40, d ** -0.5, 1, False)
+    assert ((got[:40].view_as(want).double() - want).abs() <= tol).all()
 
 
 def test_rows_behind_the_last_sequence_stay():
