@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
     }
     cut();
     if (begin >= end) return;
-    int base = 0;                                        // tiles of one head group before this round
+    int base = 0;                                        // tiles of one head group before these sequences
     for (int s0 = 0; s0 < p.B; s0 += kV4Threads) {
       int total = 0;
       if (p.B > kV4Threads) mine_len = s0 + tid < p.B ? p.seq_lens[s0 + tid] : 0;

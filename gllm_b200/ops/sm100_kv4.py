@@ -136,7 +136,7 @@ def expand_rounds(lens, token_bytes: int, limit: int):
     sequence at least. lens: their lengths, on the host."""
     rounds, first, tiles = [], 0, 0
     for s, n in enumerate(lens):
-        more = (int(n) + 63) // 64
+        more = (n + 63) // 64
         if s > first and (tiles + more) * 64 * token_bytes > limit:
             rounds.append((first, s, tiles))
             first, tiles = s, 0
@@ -184,12 +184,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             lens = [width * page_size] * prompts
         else:
             lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
+            lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
         start_at = query_start_loc.data_ptr()
         for first, end, tiles in expand_rounds(lens, 4 * hkv * d, EXPAND_BYTES):
             if tiles == 0:
                 continue
             a, n = num_decode_seqs + first, end - first
-            longest = int(max(lens[first:end]))
+            longest = max(lens[first:end])
             # the tiles' table, keys, values. The table comes first: a sequence that is longer than its room (not what the caller said)
             # has entries read behind it, which lie in the keys, and tiles that do not exist, which are read as zeros
             max_tiles, tile = (longest + 63) // 64, hkv * d * 128
