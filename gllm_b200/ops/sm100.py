@@ -522,27 +522,30 @@ INT8_MOST_K = 131072     # the int32 sums are exact up to here
 
 
 def _int8_rows(x: torch.Tensor):
+    """(rows, values, distance of rows) of x."""
     m, k = x.shape
     ld, one = x.stride()
+    if m == 1:
+        ld = k                                   # the stride of a dimension of one may be anything
     if x.dtype is _BF16 and one == 1 and 0 < k <= INT8_MOST_K and (k | x.data_ptr() | 2 * ld) % 16 == 0:
-        return m, k
+        return m, k, ld
     assert x.dtype == _BF16 and x.stride(1) == 1
     if k % 16 or k == 0 or k > INT8_MOST_K:
         raise ValueError(f"8-bit products take rows of a multiple of 16 values, at most {INT8_MOST_K}: got {k}")
-    if m and (x.data_ptr() % 16 or x.stride(0) % 8):
+    if m and (x.data_ptr() % 16 or ld % 8):
         raise ValueError("rows of an 8-bit product must lie on 16-byte boundaries")
-    return m, k
+    return m, k, ld
 
 
 def int8_quant_rows(x: torch.Tensor):
     """bf16 [M, K] -> (int8 [M, K], fp32 scales [M]): a row's scale is its largest magnitude / 127, values are rounded to the nearest
     multiple, ties to even. A row that holds a NaN or an infinity has such a scale."""
-    m, k = _int8_rows(x)
+    m, k, ld = _int8_rows(x)
     q = torch.empty(m, k, dtype=torch.int8, device=x.device)
     s = torch.empty(m, dtype=torch.float32, device=x.device)
     if m:
         on_this_device(x)
-        check(_lib.load().gllm_int8_quant_rows(_p(x), x.stride(0), _p(q), _p(s), m, k, stream_ptr()), "int8_quant_rows")
+        check(_lib.load().gllm_int8_quant_rows(_p(x), ld, _p(q), _p(s), m, k, stream_ptr()), "int8_quant_rows")
         _count()
     return q, s
 
@@ -558,12 +561,12 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
     """x bf16 [M, K] (rows quantised here, `int8_quant_rows`); w8 int8 [N, K], w_scale fp32 [N] -> bf16 [M, N] (+ bias). `silu`: w8 is
     [gate rows ; up rows] and the result silu(gate) * up [M, N / 2]. `plan`: a form by name (csrc/gemm/gemm_int8.cu) instead of the
     one chosen by size."""
-    m, k = _int8_rows(x)
+    m, k, ld = _int8_rows(x)
     n = w8.shape[0]
     n_out = n // 2 if silu else n
     if out is None:
         out = x.new_empty((m, n_out))
-    w_at, s_at, o_at, ldc = w8.data_ptr(), w_scale.data_ptr(), out.data_ptr(), out.stride(0)
+    w_at, s_at, o_at, ldc = w8.data_ptr(), w_scale.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else n_out
     b_at = None if bias is None else bias.data_ptr()
     if not (w8.dtype is torch.int8 and w8.shape == (n, k) and w8.is_contiguous() and w_scale.dtype is torch.float32 and
             w_scale.shape == (n,) and w_scale.stride(0) == 1 and out.dtype is _BF16 and out.shape == (m, n_out) and
@@ -588,7 +591,7 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
         scratch = w8.new_empty(m * k + 4 * m)    # k % 16: the scales lie on 16-byte boundaries
         xq_at = scratch.data_ptr()
         xs_at = xq_at + m * k
-    check(_lib.load().gllm_linear_int8(x.data_ptr(), x.stride(0), xq_at, xs_at, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,
+    check(_lib.load().gllm_linear_int8(x.data_ptr(), ld, xq_at, xs_at, w_at, s_at, o_at, ldc, m, n, k, b_at, silu, form, bt, parts,
                                        smem, stream_ptr()), "linear_int8")
     _count(1 if inside else 2)
     return out

@@ -30,7 +30,7 @@ def _pair(k_cache, v_cache):
 
 
 def _index(t: torch.Tensor, what: str, dims: int = 1):
-    assert t.dtype == torch.int32 and t.dim() == dims and t.stride(-1) == 1, f"{what}: int32, contiguous rows"
+    assert t.dtype == torch.int32 and t.dim() == dims and (t.stride(-1) == 1 or t.shape[-1] < 2), f"{what}: int32, contiguous rows"
 
 
 def _refuse_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, heads, dim, slots, mrope):
@@ -49,7 +49,7 @@ def _refuse_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, he
     _index(positions, "positions", 2 if mrope else 1)
     assert positions.shape[-1] >= t
     rows = [x for x in (q, k, v) if x.numel()]
-    if any(x.data_ptr() % 16 or x.stride(0) % 8 or (x.shape[1] > 1 and x.stride(1) % 8) for x in rows) or \
+    if any(x.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(x.shape[:2], x.stride())) for x in rows) or \
             any(w is not None and w.data_ptr() % 16 for w in (q_norm_w, k_norm_w)):
         raise ValueError("rows and norm weights written to a 4-bit cache must lie on 16-byte boundaries")
 
@@ -70,6 +70,12 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         if not mrope:
             positions = positions[0]
     (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride()
+    if t == 1:                                                # the stride of a dimension of one may be anything
+        qt = kt = vt = d
+    if hq == 1:
+        qh = d
+    if heads == 1:
+        kh = vh = d
     q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
     ends = q_at | k_at | v_at | 2 * (qt | qh | kt | kh | vt | vh)
     qw_at = kw_at = None
@@ -97,10 +103,8 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         else:
             sec0, sec1 = int(mrope_section[0]), int(mrope_section[1])
         pos_stride = positions.stride(0)
-    if heads == 1:                                            # the stride of a dimension of one may be anything
-        kh = vh = d
     check(_lib.load().gllm_rope_kv4_write(
-        q_at, qt, qh if hq > 1 else d, hq, k_at, kt, kh, heads, v_at, vt, vh, qw_at, kw_at, cos_sin.data_ptr() if rot else None, d, rot,
+        q_at, qt, qh, hq, k_at, kt, kh, heads, v_at, vt, vh, qw_at, kw_at, cos_sin.data_ptr() if rot else None, d, rot,
         neox, t, positions.data_ptr(), slots.data_ptr(), eps, k_cache.data_ptr(), v_cache.data_ptr(), pages, sec0, sec1, page_size,
         pos_stride, stream_ptr()), "rope_kv4_write")
     _count()
@@ -160,6 +164,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _index(seq_lens, "seq_lens")
     assert block_table.shape[0] >= num_seqs and seq_lens.shape[0] >= num_seqs and t >= num_decode_seqs
     q_at = q.data_ptr()
+    if t == 1:                                                # the stride of a dimension of one may be anything
+        q_ts = hq * d
     if (q_at | 2 * q_ts) % 16 and t:
         raise ValueError("queries over a 4-bit cache must lie on 16-byte boundaries")
     if out is None:

@@ -54,3 +54,11 @@ def test_refuses(over):
 def test_checks_its_arguments(over):
     with pytest.raises(AssertionError):
         _call(**over)
+
+
+@pytest.mark.parametrize("rows,form", [(9, 0), (5, 3), (1, 4), (1, 2)])
+def test_the_entry_refuses_before_it_launches(rows, form):
+    """No room for the quantised rows; more rows than the form for few takes; no such form; a cluster without rows."""
+    from gllm_b200.ops import lib
+    at = 1 << 20
+    assert lib.load().gllm_linear_int8(at, 64, None, None, at, at, at, 16, rows, 16, 64, None, False, form, 0, 0, 0, None) == 1

@@ -125,6 +125,17 @@ def test_few_rows_give_the_bits_of_the_other_forms(m, n, k, silu):
     assert torch.equal(y, sm100.linear_int8(x, w8, ws, bias, silu=silu))
 
 
+def test_one_row_of_a_buffer_of_any_width():
+    """The stride of a dimension of one does not matter."""
+    from gllm_b200.ops import sm100
+    x, w8, ws = _inputs(1, 16, 64)
+    odd, out = torch.zeros(1, 67, dtype=BF16, device=DEV)[:, :64], torch.zeros(1, 19, dtype=BF16, device=DEV)[:, :16]
+    odd.copy_(x)
+    for plan in (None, (1, 0, 0, 0), (2, 16, 1, 108 * 1024)):
+        assert torch.equal(sm100.linear_int8(odd, w8, ws, out=out, plan=plan), sm100.linear_int8(x, w8, ws))
+    assert torch.equal(sm100.int8_quant_rows(odd)[0], sm100.int8_quant_rows(x)[0])
+
+
 def test_few_rows_that_are_no_numbers():
     from gllm_b200.ops import sm100
     x, w8, ws = _inputs(4, 16, 64)

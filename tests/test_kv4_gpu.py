@@ -351,6 +351,26 @@ def test_tables_that_are_views(news):
                 assert ((got[at] - want).abs() <= tol).all()
 
 
+def test_one_row_of_a_buffer_of_any_width():
+    """The stride of a dimension of one does not matter."""
+    from gllm_b200.ops import sm100_kv4
+    hq, hkv, d = 4, 1, 64
+    x = _write_inputs(1, hq, hkv, d, d, 16, "qk")
+    odd = [torch.zeros(1, y.shape[1] * d + 5, dtype=BF16, device=DEV)[:, :y.shape[1] * d] for y in (x.q, x.k, x.v)]
+    for a, b in zip(odd, (x.q, x.k, x.v)):
+        a.copy_(b.flatten(1))
+    got = [c.clone() for c in x.caches]
+    views = [y.as_strided((1, y.shape[1] // d, d), (y.stride(0), d, 1)) for y in odd]
+    assert all(y.stride(0) % 8 for y in odd + views)
+    sm100_kv4.rope_kv_write(*views, x.pos, x.cs, d, True, *x.w, 1e-6, *got, x.slots)
+    sm100_kv4.rope_kv_write(x.q, x.k, x.v, x.pos, x.cs, d, True, *x.w, 1e-6, *x.caches, x.slots)
+    assert torch.equal(views[0], x.q) and all(torch.equal(a, b) for a, b in zip(got, x.caches))
+    caches, rows, table = _filled([50], hkv, d, 16)
+    for decodes in (1, 0):
+        a, b = (_attend(q, caches, table, [50], [1], decodes, hq, hkv, d) for q in (odd[0], x.q.flatten(1).clone()))
+        assert torch.equal(a, b)
+
+
 def test_attention_refuses():
     from gllm_b200.ops import sm100_kv4
     caches, rows, table = _filled([20], 2, 64, 16)
@@ -359,6 +379,8 @@ def test_attention_refuses():
         _attend(q[:, 4:], caches, table, [20], [1], 1, 4, 2, 64)             # rows off 16-byte boundaries
     with pytest.raises(AssertionError):
         _attend(q[:, :256].contiguous(), caches, table, [20], [1], 1, 2, 2, 128)
+    with pytest.raises(RuntimeError):
+        _attend(q[:, :256].contiguous(), caches, table[:, :0], [20], [1], 1, 4, 2, 64)                   # a table without columns
     with pytest.raises(ValueError):
         sm100_kv4.paged_attention(q[:, :256].contiguous(), caches[0], caches[1][:1], table, _i32([20]), None, 1.0, 4, 64, 1, 1, 1, 20)
 
