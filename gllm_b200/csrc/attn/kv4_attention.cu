@@ -7,10 +7,11 @@
 // so the codes go into the matrix instructions as they are and scales and low ends stay outside: four fused operations a score, two a
 // probability, instead of one or two for each of the D values of a key.
 //
-// Codes as 16-bit operands: a byte of two codes in an fp16 is the subnormal (c0 + 16 c1) 2^-24, and with its lower half cleared 16 c1 2^-24,
-// both exact, and the matrix instructions take subnormals: four ANDs or byte moves for eight codes, and what belongs to c0 alone comes
-// off the other operand (keys: q0 c0 + q1 c1 = q0 b + (q1 / 16 - q0) u, the second factor rounded to 2^-11) or off the sums
-// (values: four of fp32's bits). Queries are scaled by a power of two to the upper end of fp16. Probabilities times scales are rounded to
+// Codes as 16-bit operands: the lower half of a byte of two codes is the fp16 subnormal c0 2^-24, the upper one 16 c1 2^-24, both exact, and
+// the matrix instructions take subnormals: four ANDs and a byte move for eight codes. A query's factor of c1 is divided by 16 (exact), sums of
+// values by 16 at their end. Queries are scaled by a power of two to the upper end of fp16, so that their eight bits are exact down to 2^-28 of a
+// head's largest. (The whole byte as c0's operand saves an instruction, but q0 c0 + q1 c1 = q0 (c0 + 16 c1) + (q1 / 16 - q0) 16 c1 rounds the
+// second factor, which costs odd dims 2^-7 of their even neighbour's query.) Probabilities times scales are rounded to
 // fp16 (2^-11 of each): the exponentials' reference is the head's maximum plus the logarithm of the largest scale met so far, so that
 // they stay below 2^14, and what vanishes below 2^-25 is 2^-32 of the largest that can stand beside it.
 //
@@ -42,6 +43,7 @@ namespace {
 
 constexpr int kV4Keys = 32, kV4Stages = 2, kV4Least = 8;      // tiles of a CTA's share, at least
 constexpr int kV4Snap = 1;                               // tiles by which a cut moves to a head group's start or end (two: 256 x 75 16.5 for 18.5 us, all others longer, by up to 5 %)
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;      // the two codes of bytes 0 and 2
 constexpr float kV4Lazy = 8.f;                           // scores pass the maximum that the reference is taken from by no more than this
 constexpr float kV4Room = 6.f;                           // and exponentials times scales stay below 2^(kV4Lazy + kV4Room)
 
@@ -396,12 +398,11 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
             f[2 * e] = v.x * up;
             f[2 * e + 1] = v.y * up;
           }
-          // step 2c: bytes 0 and 2 (codes 0, 1 and 4, 5); step 2c + 1: bytes 1 and 3. With the byte b = c0 + 16 c1 and its upper part
-          // u = 16 c1: q0 c0 + q1 c1 = q0 b + (q1 / 16 - q0) u
+          // step 2c: bytes 0 and 2 (codes 0, 1 and 4, 5); step 2c + 1: bytes 1 and 3. The second code of a byte comes as 16 c1.
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             qf[nt][gr * 4 + 2 * c + i][0] = pack_f16(f[2 * i], f[2 * i + 4]);
-            qf[nt][gr * 4 + 2 * c + i][1] = pack_f16(fmaf(f[2 * i + 1], 0.0625f, -f[2 * i]), fmaf(f[2 * i + 5], 0.0625f, -f[2 * i + 4]));
+            qf[nt][gr * 4 + 2 * c + i][1] = pack_f16(f[2 * i + 1] * 0.0625f, f[2 * i + 5] * 0.0625f);
           }
         }
       }
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
       }
     }
 
-    // o: sums of bytes (even dim + 16 odd dim) and of their upper parts (16 odd dim), in units of 2^-24; o, l and lows relative to
+    // o: sums of codes of even dims and of 16 times those of odd dims, in units of 2^-24; o, l and lows relative to
     // 2^base, base = maximum (m) + log2 of the largest scale (top_scale) - kV4Room
     float o[NT][KS][4], lows[NT][GR][2], m[NT][2], l[NT][2], base[NT][2], top_scale = 8.6736174e-19f;      // 2^-60: scales below it count as that
 #pragma unroll
@@ -461,13 +462,11 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t x = w[0][c * GR + gr], y = w[1][c * GR + gr];
-            const uint32_t x0 = x & 0x00ff00ffu, y0 = y & 0x00ff00ffu, x1 = __byte_perm(x, 0u, 0x4341), y1 = __byte_perm(y, 0u, 0x4341);
+            const uint32_t x = w[0][c * GR + gr], y = w[1][c * GR + gr], x1 = x >> 8, y1 = y >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(acc[nt][gr], x0, y0, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][gr * 4 + 2 * c][0], qf[nt][gr * 4 + 2 * c][1]);
-              mma_f16(acc[nt][gr], x1, y1, x1 & 0x00f000f0u, y1 & 0x00f000f0u, qf[nt][gr * 4 + 2 * c + 1][0],
-                      qf[nt][gr * 4 + 2 * c + 1][1]);
+              mma_f16(acc[nt][gr], x & kEven, y & kEven, x & kOdd, y & kOdd, qf[nt][gr * 4 + 2 * c][0], qf[nt][gr * 4 + 2 * c][1]);
+              mma_f16(acc[nt][gr], x1 & kEven, y1 & kEven, x1 & kOdd, y1 & kOdd, qf[nt][gr * 4 + 2 * c + 1][0], qf[nt][gr * 4 + 2 * c + 1][1]);
             }
           }
         }
@@ -585,11 +584,11 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
 #pragma unroll
           for (int i = 0; i < 2; ++i) {                  // bytes 2i, 2i + 1 of the chunk: dims 4i .. 4i + 3
             const uint32_t x = __byte_perm(w[0][gr], w[1][gr], i == 0 ? 0x5410 : 0x7632), y = __byte_perm(w[2][gr], w[3][gr], i == 0 ? 0x5410 : 0x7632);
-            const uint32_t x0 = x & 0x00ff00ffu, y0 = y & 0x00ff00ffu, x1 = __byte_perm(x, 0u, 0x4341), y1 = __byte_perm(y, 0u, 0x4341);
+            const uint32_t x1 = x >> 8, y1 = y >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(o[nt][gr * 4 + 2 * i], x0, x & 0x00f000f0u, y0, y & 0x00f000f0u, pf[nt][gr][0], pf[nt][gr][1]);
-              mma_f16(o[nt][gr * 4 + 2 * i + 1], x1, x1 & 0x00f000f0u, y1, y1 & 0x00f000f0u, pf[nt][gr][0], pf[nt][gr][1]);
+              mma_f16(o[nt][gr * 4 + 2 * i], x & kEven, x & kOdd, y & kEven, y & kOdd, pf[nt][gr][0], pf[nt][gr][1]);
+              mma_f16(o[nt][gr * 4 + 2 * i + 1], x1 & kEven, x1 & kOdd, y1 & kEven, y1 & kOdd, pf[nt][gr][0], pf[nt][gr][1]);
             }
           }
         }
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(Kv4Smem<D, NT>::kV4Threads, 1) kv4_decode_kern
         }
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          o[nt][i][c] = fmaf(o[nt][i][c] - o[nt][i][2 + c], 16777216.f, lows[nt][i / 4][c]);
+          o[nt][i][c] = fmaf(o[nt][i][c], 16777216.f, lows[nt][i / 4][c]);
           o[nt][i][2 + c] = fmaf(o[nt][i][2 + c], 1048576.f, lows[nt][i / 4][c]);
         }
         if (m[nt][c] == -INFINITY) base[nt][c] = -INFINITY;          // no keys: no part in a sum
