@@ -68,6 +68,9 @@ int8_quant_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, uint8_t
   }
 }
 
+// Does nothing, launched in stream order: what comes before it is complete when it starts, whenever that let its dependents go ahead.
+__global__ void int8_rows_complete_kernel() {}
+
 int quant_rows(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, float* scales, int M, int K, cudaStream_t st) {
   auto go = [&](auto kern, int rows) {
     return launch_pdl(kern, dim3((M + rows - 1) / rows), dim3(256), 0, st, x, ldx, q, scales, M, K);
@@ -137,15 +140,22 @@ bool plan_int8(int M, int N, int K, bool gated, ClusterPlan* plan) {
 
 using namespace b200;
 
-// x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude / 127)
+// x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude / 127). These may be the weights of a product that is launched
+// next. Products fetch their first weights before they wait for the kernels ahead of them, and the quantiser lets its dependents start
+// at once, so an empty kernel without an early start stands between the two (2 us, once per weight; the product's own rows go without).
 GLLM_EXPORT int gllm_int8_quant_rows(const void* x, int64_t ldx, void* q, void* scales, int M, int K, void* stream) {
   if (M <= 0 || K <= 0) return 0;
   if (K % 16 != 0 || ldx % 8 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) {
     fprintf(stderr, "[gllm_b200] int8_quant_rows: K %% 16 and rows on 16-byte boundaries required\n");
     return 1;
   }
-  return quant_rows(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<uint8_t*>(q), reinterpret_cast<float*>(scales), M,
-                    K, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (const int rc = quant_rows(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<uint8_t*>(q), reinterpret_cast<float*>(scales),
+                                M, K, st))
+    return rc;
+  int8_rows_complete_kernel<<<1, 1, 0, st>>>();
+  CUDA_CHECK_RET(cudaGetLastError());
+  return 0;
 }
 
 // Whether the form that is taken for M rows needs no scratch.

@@ -539,14 +539,15 @@ def _int8_rows(x: torch.Tensor):
 
 def int8_quant_rows(x: torch.Tensor):
     """bf16 [M, K] -> (int8 [M, K], fp32 scales [M]): a row's scale is its largest magnitude / 127, values are rounded to the nearest
-    multiple, ties to even. A row that holds a NaN or an infinity has such a scale."""
+    multiple, ties to even. A row that holds a NaN or an infinity has such a scale. The pair may be the weight of a product that is called next
+    (`linear_int8`)."""
     m, k, ld = _int8_rows(x)
     q = torch.empty(m, k, dtype=torch.int8, device=x.device)
     s = torch.empty(m, dtype=torch.float32, device=x.device)
     if m:
         on_this_device(x)
         check(_lib.load().gllm_int8_quant_rows(_p(x), ld, _p(q), _p(s), m, k, stream_ptr()), "int8_quant_rows")
-        _count()
+        _count(2)
     return q, s
 
 
@@ -560,7 +561,8 @@ def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: 
                 out: Optional[torch.Tensor] = None, silu: bool = False, plan: Optional[tuple] = None) -> torch.Tensor:
     """x bf16 [M, K] (rows quantised here, `int8_quant_rows`); w8 int8 [N, K], w_scale fp32 [N] -> bf16 [M, N] (+ bias). `silu`: w8 is
     [gate rows ; up rows] and the result silu(gate) * up [M, N / 2]. `plan`: a form by name (csrc/gemm/gemm_int8.cu) instead of the
-    one chosen by size."""
+    one chosen by size. Weights are fetched before the library's kernels ahead of the product have ended: only `int8_quant_rows` among
+    them may have written w8 (torch's operations may)."""
     m, k, ld = _int8_rows(x)
     n = w8.shape[0]
     n_out = n // 2 if silu else n

@@ -235,3 +235,32 @@ def test_waits_that_run_out_are_reported(plan):
         _lib.watch_waits()
     want, tol = product(x, w8, ws)
     assert ((sm100.linear_int8(x, w8, ws, plan=plan).to(F64) - want).abs() <= tol).all() and not _lib.waits_gave_up()
+
+
+@pytest.mark.parametrize("m", [1, 4, 7, 200, 1200])
+@pytest.mark.parametrize("n,k", [(64, 256), (2048, 4096), (9728, 1024)])
+def test_weights_quantised_just_before_their_product(m, n, k):
+    """The quantiser's pair is a weight: both calls behind one another in one graph, where no gap of the host lies between them, with other
+    weights at every replay. The same bits as with all the time in the world between them."""
+    from gllm_b200.layers import functional as Fn
+    from gllm_b200.ops import sm100
+    torch.manual_seed(m + n)
+    x, w = torch.randn(m, k, device=DEV).to(BF16), torch.empty(n, k, dtype=BF16, device=DEV)
+    weights = [(torch.randn(n, k, device=DEV) * 0.1).to(BF16) for _ in range(3)]
+    w.copy_(weights[0])
+    Fn.linear(x, sm100.int8_quant_rows(w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, s = sm100.int8_quant_rows(w)
+        y = Fn.linear(x, (q, s))
+    for turn in range(6):
+        w.copy_(weights[turn % 3])
+        q.zero_()                                          # what a product that came too early would find
+        graph.replay()
+        got = y.clone()
+        torch.cuda.synchronize()
+        q1, s1 = sm100.int8_quant_rows(weights[turn % 3])
+        torch.cuda.synchronize()
+        assert torch.equal(q, q1) and torch.equal(s, s1)
+        assert torch.equal(got, Fn.linear(x, (q1, s1)))
