@@ -130,9 +130,8 @@ def _qw(w, s):
 
 def _linear_weight(reader, name: str, quant: Optional[str]):
     """A checkpoint's linear weight: a tensor, or, where it is held in 8 bits, (int8 [N, K], fp32 scales [N, 1])."""
-    if quant == "int8" and reader.has(name + "_scale"):
-        return reader.get_raw(name), reader.get_raw(name + "_scale").float().reshape(-1, 1)
-    return reader.get(name)
+    pair = reader.get_int8(name) if quant == "int8" else None
+    return reader.get(name) if pair is None else pair
 
 
 def _by_rows(fn, *ws):

@@ -166,8 +166,12 @@ class CheckpointReader:
     def get(self, name: str) -> torch.Tensor:
         """Tensor by name. Block-quantised fp8 weights (`<name>` e4m3 + `<name>_scale_inv` fp32 per
         128x128 block — DeepSeek-V3 / Qwen3-FP8 checkpoints, reference: gllm/layers/linear.py:68-112)
-        are de-quantised to bf16 here unless the caller asks for the raw pair via `get_fp8`."""
+        are de-quantised to bf16 here unless the caller asks for the raw pair via `get_fp8`. Weights held as int8 or fp8 codes with one
+        scale per output channel or tensor (`<name>_scale`) are de-quantised to fp32 (`get_int8`: the pair); other int8 weights are refused."""
         t = self.get_raw(name)
+        if t.dtype == torch.int8 and name.endswith("weight") or \
+                t.dtype in (torch.float8_e4m3fn, torch.float8_e5m2) and self.has(name + "_scale"):
+            return t.float() * self._channel_scale(name, t)
         if t.dtype in (torch.float8_e4m3fn, torch.float8_e5m2) and self.has(name + "_scale_inv"):
             s = self.get_raw(name + "_scale_inv").float()
             n, k = t.shape
@@ -175,6 +179,24 @@ class CheckpointReader:
             full = s.repeat_interleave(bn, 0)[:n].repeat_interleave(bk, 1)[:, :k]
             return (t.float() * full).to(torch.bfloat16)
         return t
+
+    def _channel_scale(self, name: str, t: torch.Tensor) -> torch.Tensor:
+        """fp32 scales of a coded weight, shaped to multiply it: one per output channel (a scale per tensor is repeated)."""
+        if not self.has(name + "_scale"):
+            raise ValueError(f"{name}: {t.dtype} codes without scales ({name}_scale)")
+        s = self.get_raw(name + "_scale").float()
+        if s.numel() not in (1, t.shape[0]) or s.dim() > 0 and s.shape[0] != s.numel():
+            raise ValueError(f"{name}: scales of {tuple(s.shape)} for a weight of {tuple(t.shape)}; one per output channel or tensor is taken")
+        if self.has(name + "_zero_point") and bool(self.get_raw(name + "_zero_point").any()):
+            raise ValueError(f"{name}: codes with zero points are not taken")
+        return s.reshape(-1, *[1] * (t.dim() - 1)).expand(t.shape[0], *[1] * (t.dim() - 1))
+
+    def get_int8(self, name: str):
+        """(int8 [N, K], fp32 scales [N, 1]) of a weight that is held so, else None."""
+        if not self.has(name + "_scale"):
+            return None
+        t = self.get_raw(name)
+        return (t, self._channel_scale(name, t)) if t.dtype == torch.int8 else None
 
     def is_fp8(self, name: str) -> bool:
         key = self.resolve(name)
