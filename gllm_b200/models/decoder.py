@@ -77,6 +77,7 @@ class ModelSpec:
     extra: dict = field(default_factory=dict)
     # "fp8": block-scaled e4m3 linears (HF quantization_config, 128x128 blocks); "int8": 8-bit linears, a scale per output channel
     quant: Optional[str] = None
+    quantise: bool = False       # "int8": weights that a checkpoint holds in floating point are quantised while loading, else refused
 
     def is_moe_layer(self, layer_id: int) -> bool:
         if self.moe is None:
@@ -128,9 +129,12 @@ def _qw(w, s):
     return w if s is None else (w, s)
 
 
-def _linear_weight(reader, name: str, quant: Optional[str]):
+def _linear_weight(reader, name: str, spec: ModelSpec):
     """A checkpoint's linear weight: a tensor, or, where it is held in 8 bits, (int8 [N, K], fp32 scales [N, 1])."""
-    pair = reader.get_int8(name) if quant == "int8" else None
+    pair = reader.get_int8(name) if spec.quant == "int8" else None
+    if pair is None and spec.quant == "int8" and not spec.quantise:
+        raise ValueError(f"{name} is not held in 8 bits as the checkpoint's other linears are; linears left out of its quantisation have "
+                         "no form of their own here (quantization=\"int8\" quantises them)")
     return reader.get(name) if pair is None else pair
 
 
@@ -528,10 +532,10 @@ class CausalLM(nn.Module):
         spec, tp, tr, d = self.spec, self.tp_size, self.tp_rank, self.spec.head_dim
         sizes = [spec.num_heads * d, spec.num_kv_heads * d, spec.num_kv_heads * d]
         if "qkv_fused" in nm:  # ChatGLM: one [ (hq + 2 hkv) * D, H ] tensor
-            w = _linear_weight(reader, pre + nm["qkv_fused"] + ".weight", spec.quant)
+            w = _linear_weight(reader, pre + nm["qkv_fused"] + ".weight", spec)
             q, k, v = (_by_rows(lambda x, i=i: x.split(sizes, dim=0)[i], w) for i in range(3))
         else:
-            q, k, v = (_linear_weight(reader, pre + nm[x] + ".weight", spec.quant) for x in ("q", "k", "v"))
+            q, k, v = (_linear_weight(reader, pre + nm[x] + ".weight", spec) for x in ("q", "k", "v"))
         _store_linear(at.qkv_w, at.qkv_ws,
                       _by_rows(lambda *ws: wu.shard_qkv(*ws, spec.num_heads, spec.num_kv_heads, d, tr, tp), q, k, v))
         if at.qkv_b is not None:
@@ -542,7 +546,7 @@ class CausalLM(nn.Module):
                 qb, kb, vb = (reader.get(pre + nm[x] + ".bias") for x in ("q", "k", "v"))
             at.qkv_b.data.copy_(wu.shard_qkv(qb, kb, vb, spec.num_heads, spec.num_kv_heads, d, tr, tp))
         _store_linear(at.o_w, at.o_ws, _by_cols(lambda w: wu.shard_cols(w, tr, tp),
-                                                _linear_weight(reader, pre + nm["o"] + ".weight", spec.quant)))
+                                                _linear_weight(reader, pre + nm["o"] + ".weight", spec)))
         if at.o_b is not None:
             at.o_b.data.copy_(reader.get(pre + nm["o"] + ".bias"))
         if at.q_norm_w is not None:
@@ -552,11 +556,11 @@ class CausalLM(nn.Module):
     def _load_dense_mlp(self, reader, pre, nm, mlp: DenseMLP):
         tp, tr = self.tp_size, self.tp_rank
         if "gate_up_fused" in nm:  # ChatGLM dense_h_to_4h = [gate; up]
-            w = _linear_weight(reader, pre + nm["gate_up_fused"] + ".weight", self.spec.quant)
+            w = _linear_weight(reader, pre + nm["gate_up_fused"] + ".weight", self.spec)
             gate, up = (_by_rows(lambda x, i=i: x.chunk(2, dim=0)[i], w) for i in range(2))
         else:
-            gate = _linear_weight(reader, pre + nm["gate"] + ".weight", self.spec.quant)
-            up = _linear_weight(reader, pre + nm["up"] + ".weight", self.spec.quant)
+            gate = _linear_weight(reader, pre + nm["gate"] + ".weight", self.spec)
+            up = _linear_weight(reader, pre + nm["up"] + ".weight", self.spec)
         mlp.set_gate_up(_by_rows(lambda *ws: wu.shard_gate_up(*ws, tr, tp), gate, up))
         _store_linear(mlp.down_w, mlp.down_ws, _by_cols(lambda w: wu.shard_cols(w, tr, tp),
-                                                        _linear_weight(reader, pre + nm["down"] + ".weight", self.spec.quant)))
+                                                        _linear_weight(reader, pre + nm["down"] + ".weight", self.spec)))

@@ -77,7 +77,7 @@ def _base_spec(cfg: HFConfig, arch: str, **kw) -> ModelSpec:
         max_position=cfg.get("max_position_embeddings", 8192), rope_theta=rope_theta,
         rope_scaling=dict(rope_scaling) if rope_scaling else None, dtype=_dtype(cfg),
         eos_token_id=cfg.get("eos_token_id"))
-    spec.quant = _quant(cfg)
+    spec.quant, spec.quantise = _quant(cfg), bool(cfg.get("weights_int8"))
     for k, v in kw.items():
         setattr(spec, k, v)
     return spec
@@ -147,7 +147,7 @@ def spec_chatglm(cfg):
         rms_eps=cfg.get("layernorm_epsilon", 1e-5), qkv_bias=bool(cfg.get("add_qkv_bias", False)),
         max_position=cfg.get("seq_length", 8192), rope_theta=10000.0 * cfg.get("rope_ratio", 1.0),
         rot_dim=head_dim // 2, rope_neox=False, dtype=_dtype(cfg), eos_token_id=cfg.get("eos_token_id"),
-        quant="int8" if _quant(cfg) == "int8" else None)
+        quant="int8" if _quant(cfg) == "int8" else None, quantise=bool(cfg.get("weights_int8")))
     spec.names = {
         "embed": "transformer.embedding.word_embeddings.weight",
         "final_norm": "transformer.encoder.final_layernorm.weight",

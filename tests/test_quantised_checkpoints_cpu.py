@@ -87,3 +87,46 @@ def test_zero_points_of_zero_are_none():
     name = "model.layers.1.mlp.down_proj.weight"
     sd[name + "_zero_point"] = torch.zeros(sd[name].shape[0], 1, dtype=torch.int8)
     assert torch.equal(_load(cfg, sd).layers[1].mlp.down_w, sd[name])
+
+
+@pytest.mark.parametrize("name", ["self_attn.o_proj", "mlp.down_proj"])
+def test_linears_left_out_of_the_quantisation(name):
+    """A checkpoint in 8 bits that keeps some linears in floating point is not quantised behind its back; who asks for it has them quantised."""
+    left_out = f"model.layers.0.{name}.weight"
+    sd = _state(_cfg(), True)
+    sd[left_out] = torch.randn(sd[left_out].shape, generator=torch.Generator().manual_seed(1)) * 0.1
+    del sd[left_out + "_scale"]
+    config = {**W8A8, "ignore": ["lm_head", left_out.removesuffix(".weight")]}
+    with pytest.raises(ValueError, match=name):
+        _load(_cfg(quantization_config=config), sd)
+    model = _load(_cfg(quantization_config=config, weights_int8=True), sd)
+    w, s = {"self_attn.o_proj": (model.layers[0].attn.o_w, model.layers[0].attn.o_ws),
+            "mlp.down_proj": (model.layers[0].mlp.down_w, model.layers[0].mlp.down_ws)}[name]
+    assert float((w.float() * s[:, None] - sd[left_out]).abs().max()) <= 0.51 * float(s.max())
+    assert torch.equal(model.layers[1].mlp.down_w, sd["model.layers.1.mlp.down_proj.weight"])
+
+
+def test_a_fused_projection_left_out():
+    """Models with one tensor for queries, keys and values, or for gate and up."""
+    cfg = _cfg("ChatGLMModel", kv_channels=64, multi_query_group_num=2, ffn_hidden_size=192, num_layers=2, add_qkv_bias=False,
+               layernorm_epsilon=1e-5, padded_vocab_size=256, quantization_config=W8A8)
+    model = registry.build_model(cfg, "cpu")
+    sd, pre = {}, "transformer.encoder.layers.{}."
+    h = cfg["hidden_size"]
+    sd["transformer.embedding.word_embeddings.weight"] = torch.randn(256, h)
+    sd["transformer.encoder.final_layernorm.weight"] = torch.ones(h)
+    sd["transformer.output_layer.weight"] = torch.randn(256, h)
+    for i, layer in enumerate(model.layers):
+        p = pre.format(i)
+        sd[p + "input_layernorm.weight"] = sd[p + "post_attention_layernorm.weight"] = torch.ones(h)
+        for name, w in (("self_attention.query_key_value", layer.attn.qkv_w), ("self_attention.dense", layer.attn.o_w),
+                        ("mlp.dense_h_to_4h", layer.mlp.gate_up_w), ("mlp.dense_4h_to_h", layer.mlp.down_w)):
+            sd[p + name + ".weight"] = torch.randint(-127, 128, w.shape, dtype=torch.int8)
+            sd[p + name + ".weight_scale"] = torch.rand(w.shape[0], 1) * 0.01
+    model.load_weights(CheckpointReader.from_state_dict(sd))
+    name = pre.format(1) + "mlp.dense_h_to_4h.weight"
+    assert torch.equal(model.layers[1].mlp.gate_up_w, sd[name]) and torch.equal(model.layers[1].mlp.gate_up_ws, sd[name + "_scale"][:, 0])
+    sd[name] = sd[name].float()
+    del sd[name + "_scale"]
+    with pytest.raises(ValueError, match="dense_h_to_4h"):
+        registry.build_model(cfg, "cpu").load_weights(CheckpointReader.from_state_dict(sd))
