@@ -201,7 +201,7 @@ class ModelRunner:
             free -= getattr(self.model, "step_scratch_bytes", lambda max_len: 0)(self.model_max_length)
             if self.four_bit:
                 from gllm_b200.ops import sm100_kv4
-                free -= sm100_kv4.scratch_bytes(kvh, kvd, self.model_max_length)
+                free -= sm100_kv4.scratch_bytes(kvh, kvd, self.model_max_length, max(self.max_running_seqs, 1))
             num = int((max(free, 0) // max(per_page, 1)) * cfg.gpu_memory_util)
         if ps.get_world_size() > 1 and torch.distributed.is_initialized():
             all_n = [None] * ps.get_world_size()

@@ -130,9 +130,11 @@ def _decode_scratch(d: int) -> int:
     return _lib.load().gllm_kv4_decode_scratch(d, _DECODE_CTAS)
 
 
-def scratch_bytes(kv_heads: int, d: int, max_len: int) -> int:
-    """The most that one step's `paged_attention` allocates beside its result: expanded tiles of prompts, parts of decoding sequences."""
-    return max(EXPAND_BYTES, 4 * kv_heads * d * (max_len + 63)) + _DECODE_CTAS * (2 * 16 * (d + 2) * 4 + 16) + (1 << 20)
+def scratch_bytes(kv_heads: int, d: int, max_len: int, max_seqs: int = 256) -> int:
+    """The most that one step's `paged_attention` allocates beside its result: expanded tiles of prompts and their table, parts of decoding
+    sequences."""
+    table = 4 * max_seqs * ((max_len + 63) // 64)
+    return max(EXPAND_BYTES, 4 * kv_heads * d * (max_len + 63)) + table + _DECODE_CTAS * (2 * 16 * (d + 2) * 4 + 16) + (1 << 20)
 
 
 def expand_rounds(lens, token_bytes: int, limit: int):
@@ -192,17 +194,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             lens = [max_seq_len] * prompts if host_lens is None else host_lens[num_decode_seqs:num_seqs]
             lens = lens.tolist() if hasattr(lens, "tolist") else list(lens)
         start_at = query_start_loc.data_ptr()
-        for first, end, tiles in expand_rounds(lens, 4 * hkv * d, EXPAND_BYTES):
-            if tiles == 0:
-                continue
-            a, n = num_decode_seqs + first, end - first
-            longest = max(lens[first:end])
-            # the tiles' table, keys, values. The table comes first: a sequence that is longer than its room (not what the caller said)
-            # has entries read behind it, which lie in the keys, and tiles that do not exist, which are read as zeros
-            max_tiles, tile = (longest + 63) // 64, hkv * d * 128
-            head = (4 * n * max_tiles + 255) // 256 * 256
-            room = k_cache.new_empty(head + 2 * tiles * tile)
-            t_at = room.data_ptr()
+        # (first sequence, sequences, the longest's tokens, tiles), a round each
+        rounds = [(a, b - a, max(lens[a:b]), tiles) for a, b, tiles in expand_rounds(lens, 4 * hkv * d, EXPAND_BYTES) if tiles]
+        # the tiles' table, keys, values, in one buffer for all rounds, which follow one another. The table comes first: a sequence that is
+        # longer than its room (not what the caller said) has entries read behind it, which lie in the keys, and tiles that do not exist,
+        # which are read as zeros
+        tile = hkv * d * 128
+        heads = [(4 * n * ((longest + 63) // 64) + 255) // 256 * 256 for _, n, longest, _ in rounds]
+        room = k_cache.new_empty(max((head + 2 * r[3] * tile for head, r in zip(heads, rounds)), default=0))
+        t_at = room.data_ptr()
+        for head, (first, n, longest, tiles) in zip(heads, rounds):
+            a, max_tiles = num_decode_seqs + first, (longest + 63) // 64
             kt_at = t_at + head
             vt_at = kt_at + tiles * tile
             check(L.gllm_kv4_expand(k_at, v_at, table_at + 4 * a * pitch, pitch, width, lens_at + 4 * a, n, hkv, d, page_size, pages, tiles,

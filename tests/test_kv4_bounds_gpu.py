@@ -1,4 +1,4 @@
-"""Decode attention over a 4-bit cache within the roundings that it makes (GPU)."""
+"""Decode attention over a 4-bit cache within the roundings that it makes, and what a step allocates (GPU)."""
 import pytest
 import torch
 
@@ -51,3 +51,22 @@ def test_queries_with_a_few_large_dims(lens, hq, hkv, d, loud, parity):
     off = (got.view_as(want).to(F64) - want).abs()
     assert float((off / (slack + 2.0 ** -8 * (want.abs() + slack))).max()) <= 1
     assert off.norm() <= 1.1 * 2.0 ** -8 / 3 ** 0.5 * want.norm() + slack.norm(), (off.norm() / want.norm(), slack.norm() / want.norm())
+
+
+def test_rounds_of_prompts_allocate_what_is_counted(monkeypatch):
+    """Several rounds of expanded prompts, of unequal sizes: no more is live at a time than `scratch_bytes`, by which the engine sizes its pages."""
+    from gllm_b200.ops import sm100_kv4
+    hq, hkv, d = 8, 8, 128
+    monkeypatch.setattr(sm100_kv4, "EXPAND_BYTES", 4 * hkv * d * 4096)
+    lens, news = [2000, 2096, 4000, 3000, 1000, 4096], [3, 40, 1, 7, 200, 9]
+    caches, rows, table = _filled(lens, hkv, d, 16)
+    q = torch.randn(sum(news), hq * d, device=DEV).to(BF16)
+    want = _attend(q, caches, table, lens, news, 0, hq, hkv, d)
+    del want
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = _attend(q, caches, table, lens, news, 0, hq, hkv, d)
+    most = torch.cuda.max_memory_allocated() - before - got.numel() * 2
+    counted = sm100_kv4.scratch_bytes(hkv, d, max(lens))
+    assert most <= counted, (most, counted)
