@@ -1,6 +1,6 @@
 // Products in 8-bit integers with a scale per token and per output channel:
 //
-//   a_t = max_k |x_tk|,  X_tk = rne(127 x_tk / a_t),  y_tn = (a_t / 127) s_n sum_k X_tk W_nk (+ b_n)  -> bf16
+//   a_t = max(max_k |x_tk|, 2^-100),  X_tk = rne(127 x_tk / a_t),  y_tn = (a_t / 127) s_n sum_k X_tk W_nk (+ b_n)  -> bf16
 //
 // x bf16, W int8 with fp32 scales s; gated: W = [gate rows ; up rows] and y = silu(gate) * up. The sums are int32, exact for K up to
 // 131,072 (127 x 128 x K < 2^31); scales, bias and gate are fp32, and y is rounded once.
@@ -140,9 +140,10 @@ bool plan_int8(int M, int N, int K, bool gated, ClusterPlan* plan) {
 
 using namespace b200;
 
-// x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude / 127). These may be the weights of a product that is launched
-// next. Products fetch their first weights before they wait for the kernels ahead of them, and the quantiser lets its dependents start
-// at once, so an empty kernel without an early start stands between the two (2 us, once per weight; the product's own rows go without).
+// x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude, 2^-100 at least, / 127). These may be the weights of a
+// product that is launched next. Products fetch their first weights before they wait for the kernels ahead of them, and the quantiser lets its
+// dependents start at once, so an empty kernel without an early start stands between the two (2 us, once per weight; the product's own rows
+// go without).
 GLLM_EXPORT int gllm_int8_quant_rows(const void* x, int64_t ldx, void* q, void* scales, int M, int K, void* stream) {
   if (M <= 0 || K <= 0) return 0;
   if (K % 16 != 0 || ldx % 8 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) {

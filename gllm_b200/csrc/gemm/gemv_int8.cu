@@ -1,6 +1,6 @@
 // 8-bit products of a few rows (the decode step of a sequence or two), the rows quantised on the way:
 //
-//   a_m = max_k |x_mk|,  X_mk = rne(127 x_mk / a_m),  y_mn = (a_m / 127) s_n sum_k X_mk W_nk (+ b_n);  gated: W = [gate rows ; up rows]
+//   a_m = max(max_k |x_mk|, 2^-100),  X_mk = rne(127 x_mk / a_m),  y_mn = (a_m / 127) s_n sum_k X_mk W_nk (+ b_n);  gated: W = [gate rows ; up rows]
 //
 // Bound by the weight bytes and, for the matrices of a layer, by latency: launch, one trip to HBM, the sum. As in gemv_bf16.cu a warp owns
 // one or two weight rows with the whole of K and has its first 4 KB of weights in flight before the previous kernel ends. Meanwhile

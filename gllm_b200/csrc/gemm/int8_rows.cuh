@@ -1,5 +1,5 @@
-// How a row is quantised to 8-bit integers (gemm_int8.cu, gemv_int8.cu): scale a / 127 with its largest magnitude a, values to the
-// nearest multiple, ties to even.
+// How a row is quantised to 8-bit integers (gemm_int8.cu, gemv_int8.cu): scale a / 127 with its largest magnitude a, 2^-100 at least, values
+// to the nearest multiple, ties to even.
 #pragma once
 
 #include "../common/ptx.cuh"
@@ -7,7 +7,7 @@
 
 namespace b200 {
 
-constexpr float kQuantFloor = 7.888609052210118e-31f;    // 2^-100: rows below it become zeros
+constexpr float kQuantFloor = 7.888609052210118e-31f;    // 2^-100: rows below it are quantised with its step, so that 128 / a and scales are normal numbers
 
 // the larger of two pairs of magnitudes, as bits: NaN is above infinity
 __device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }

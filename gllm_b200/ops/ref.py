@@ -459,10 +459,11 @@ def linear_fp8_block(x: torch.Tensor, w: torch.Tensor, w_scale_inv: torch.Tensor
 
 
 def int8_quant_rows(x: torch.Tensor):
-    """(int8 [M, K], fp32 scales [M]): the largest magnitude of a row / 127, values to the nearest multiple, ties to even."""
-    a = x.float().abs().amax(1, keepdim=True)
-    q = torch.where(a > 0, torch.round(x.float() * 127 / a), 0.0)
-    return torch.nan_to_num(q).to(torch.int8), (a / 127)[:, 0]
+    """(int8 [M, K], fp32 scales [M]): the largest magnitude of a row (2^-100 at least) / 127, values to the nearest multiple, ties to
+    even. Rows that are not finite: codes of 0, the scale says the rest."""
+    a = x.float().abs().amax(1, keepdim=True).clamp_min(2.0 ** -100)
+    q = torch.where(a < torch.inf, torch.round(x.float() * 127 / a), 0.0)
+    return q.to(torch.int8), (a / 127)[:, 0]
 
 
 def linear_int8(x: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, silu: bool = False):

@@ -538,8 +538,8 @@ def _int8_rows(x: torch.Tensor):
 
 
 def int8_quant_rows(x: torch.Tensor):
-    """bf16 [M, K] -> (int8 [M, K], fp32 scales [M]): a row's scale is its largest magnitude / 127, values are rounded to the nearest
-    multiple, ties to even. A row that holds a NaN or an infinity has such a scale. The pair may be the weight of a product that is called next
+    """bf16 [M, K] -> (int8 [M, K], fp32 scales [M]): a row's scale is its largest magnitude (2^-100 at least) / 127, values are rounded
+    to the nearest multiple, ties to even. A row that holds a NaN or an infinity has such a scale. The pair may be the weight of a product that is called next
     (`linear_int8`)."""
     m, k, ld = _int8_rows(x)
     q = torch.empty(m, k, dtype=torch.int8, device=x.device)

@@ -62,3 +62,26 @@ def test_the_entry_refuses_before_it_launches(rows, form):
     from gllm_b200.ops import lib
     at = 1 << 20
     assert lib.load().gllm_linear_int8(at, 64, None, None, at, at, at, 16, rows, 16, 64, None, False, form, 0, 0, 0, None) == 1
+
+
+def _definition(x):
+    """(whole numbers, scales), fp64: the step is the largest magnitude, 2^-100 at least, / 127."""
+    a = x.double().abs().amax(1, keepdim=True).clamp_min(2.0 ** -100)
+    return torch.round(127 * x.double() / a), a / 127
+
+
+def test_small_rows_have_the_least_step():
+    """Rows whose largest magnitude lies on either side of 2^-100, zeros and rows that are not finite."""
+    torch.manual_seed(1)
+    x = torch.randn(12, 64).clamp(-1, 1)
+    x[:, 0] = 1.0
+    x = (x.double() * 2.0 ** -torch.arange(98, 110).double()[:, None]).to(BF16)
+    x = torch.cat([x, torch.zeros(1, 64, dtype=BF16)])
+    q, s = ref.int8_quant_rows(x)
+    want, scale = _definition(x)
+    assert torch.equal(q.double(), want) and (q[3] != 0).any() and (q[:, 0] <= 127).all()
+    torch.testing.assert_close(s.double(), scale[:, 0], rtol=2 ** -24, atol=0)
+    bad = torch.randn(2, 64).to(BF16)
+    bad[0, 3], bad[1, 4] = float("nan"), float("-inf")
+    q, s = ref.int8_quant_rows(bad)
+    assert (q == 0).all() and not torch.isfinite(s).any()

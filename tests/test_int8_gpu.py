@@ -264,3 +264,23 @@ def test_weights_quantised_just_before_their_product(m, n, k):
         torch.cuda.synchronize()
         assert torch.equal(q, q1) and torch.equal(s, s1)
         assert torch.equal(got, Fn.linear(x, (q1, s1)))
+
+
+@pytest.mark.parametrize("m,k", [(24, 64), (24, 2048), (3, 32768)])
+def test_small_rows_are_quantised_as_the_plain_form_does(m, k):
+    """Largest magnitudes on either side of 2^-100, the least step: codes and scales of the plain form, in the product of few rows too."""
+    from gllm_b200.ops import ref, sm100
+    torch.manual_seed(k)
+    x = torch.randn(m, k, device=DEV, dtype=F64).clamp(-1, 1)
+    x[:, 0] = 1.0
+    x = (x * 2.0 ** -(96 + torch.arange(m, device=DEV) % 12).double()[:, None]).to(BF16)
+    q, s = sm100.int8_quant_rows(x)
+    want_q, want_s = ref.int8_quant_rows(x.cpu())
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s) and (want_q[5:] != 0).any() == (m > 5)
+    w8 = torch.randint(-128, 128, (32, k), device=DEV, dtype=torch.int8)
+    ws = torch.full((32,), 2.0 ** 60, device=DEV)
+    for rows in (x[:1], x[m // 4:m // 4 + 2], x):
+        y = sm100.linear_int8(rows, w8, ws)
+        want = (ref.int8_quant_rows(rows.cpu())[0].double() @ w8.cpu().double().t()) * ref.int8_quant_rows(rows.cpu())[1].double()[:, None] * 2.0 ** 60
+        # the definition's value through one rounding to bf16 (2^-8) behind three of fp32
+        assert ((y.cpu().double() - want).abs() <= (2 ** -8 + 2 ** -22) * want.abs()).all()
