@@ -5,7 +5,8 @@
 // then 16 x D / 64 pairs (scale, low) of bf16. Each 64 dims y of a token's head:
 //   low = min y,  scale = bf16((max y - low) / 15),  code = min(15, rne((y - low) / scale)),  value = code * scale + low.
 // y is rounded to bf16 before it is coded (what a bf16 cache would hold), so low needs no rounding of its own. Many quotients
-// are ties (both sides are multiples of the same power of two), which a product with the reciprocal alone would send either way.
+// are ties (both sides are multiples of the same power of two), which a product with the reciprocal alone would send either way. A scale below
+// 2^-126 counts as 0 (its reciprocal may be beyond fp32); the steps up to there keep subnormal numbers.
 //
 // What bounds it: issue slots and the latency of short blocks. 4096 tokens x (32 + 8 + 8) heads of 128 with norms take 22.6 us, 3.9 TB/s of
 // what is read and written (floor 13.5 us; 19.3 without norms); with IEEE divisions in every lane it took 80, with one fp32 operation an
@@ -74,11 +75,16 @@ __device__ __forceinline__ void kv4_ends(uint32_t& lo, uint32_t& hi) {
 __device__ __forceinline__ uint32_t min4(const uint32_t (&w)[4]) { return min_nan2(min_nan2(w[0], w[1]), min_nan2(w[2], w[3])); }
 __device__ __forceinline__ uint32_t max4(const uint32_t (&w)[4]) { return max_nan2(max_nan2(w[0], w[1]), max_nan2(w[2], w[3])); }
 
+__device__ __forceinline__ float fma_full(float a, float b, float c) {                // the build flushes subnormal numbers elsewhere
+  float d;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // A quotient to the nearest from an estimate of the reciprocal: the remainder of the first estimate is exact, and adding its share leaves
 // an error far below half a step (Markstein). So a quotient that is a tie between two codes comes out as one.
 __device__ __forceinline__ float quotient(float d, float s, float inv) {
-  const float q = __fmul_rn(d, inv);
-  return fmaf(fmaf(-q, s, d), inv, q);
+  const float q = fma_full(d, inv, 0.f);
+  return fma_full(fma_full(q, -s, d), inv, q);          // (-q would be flushed)
 }
 
 // A group's pair from its ends, and what its codes are made with. A NaN or an infinity (or a span beyond fp32) makes the scale a
@@ -89,10 +95,11 @@ struct Kv4Group {
   __device__ __forceinline__ Kv4Group(uint32_t lo, uint32_t hi) {
     low = __uint_as_float(lo << 16);
     const float high = __uint_as_float(hi << 16);
-    const __nv_bfloat16 scale16 = __float2bfloat16_rn(quotient(__fsub_rn(high, low), 15.f, 1.f / 15.f));
-    scale = __bfloat162float(scale16);
-    const bool fine = scale <= 3.3895e38f;               // false for NaN as well
-    pair = (lo & 0xffff0000u) | (fine ? __bfloat16_as_ushort(scale16) : 0x7fffu);
+    uint32_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(quotient(fma_full(-1.f, low, high), 15.f, 1.f / 15.f)));
+    bits = bits < 0x0080u ? 0u : bits < 0x7f80u ? bits : 0x7fffu;          // below 2^-126: 0; infinities and NaN
+    scale = __uint_as_float(bits << 16);
+    const bool fine = bits < 0x7f80u;
+    pair = (lo & 0xffff0000u) | bits;
     inv = fine && scale > 0.f ? __fdividef(1.f, scale) : 0.f;       // no scale: codes of 0
   }
   // Eight codes. The scale is at least (1 - 2^-8) / 15 of the span, so none is over 15.
@@ -391,7 +398,7 @@ kv4_rows_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
       const float2 p = unpack_bf16(pair[n][kv]);
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = fmaf(static_cast<float>((codes[n][kv] >> (4 * e)) & 15u), p.x, p.y);
+      for (int e = 0; e < 8; ++e) f[e] = fma_full(static_cast<float>((codes[n][kv] >> (4 * e)) & 15u), p.x, p.y);
       *reinterpret_cast<uint4*>((kv ? v_out : k_out) + (static_cast<int64_t>(t) * Hkv + h0 + n) * D + e0) =
           make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
     }

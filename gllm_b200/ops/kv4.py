@@ -4,7 +4,7 @@ One uint8 tensor each for keys and values, [pages, kv heads, page_size / 16, 9 *
 block 16 rows of D / 2 bytes and behind them 16 x D / 64 pairs (scale, low) of bf16, one pair for each 64 dims of a token's head.
 A block is one contiguous copy, codes and pairs together, whatever the page size.
 
-Each 64 dims y of a token's head are coded by themselves: low = min y, scale = bf16((max y - low) / 15), code =
+Each 64 dims y of a token's head are coded by themselves: low = min y, scale = bf16((max y - low) / 15) (below 2^-126: 0), code =
 min(15, round((y - low) / scale)), ties to even; 0 where the scale is 0. A code c stands for c * scale + low. Four bits and, for the
 pair, half a bit a value. Keys are coded as rotated and rounded to bf16, so that low is exact. A group that holds a NaN or an
 infinity (or spans more than fp32 holds) reads back as NaN.
@@ -65,7 +65,7 @@ def encode(x: torch.Tensor):
     y = x.to(torch.bfloat16).float().unflatten(-1, (d // 64, 64))
     low, high = y.amin(-1, keepdim=True), y.amax(-1, keepdim=True)
     scale = ((high - low) / 15).to(torch.bfloat16).float()
-    scale = torch.where(torch.isfinite(scale), scale, torch.nan)
+    scale = torch.where(scale < 2.0 ** -126, 0.0, torch.where(torch.isfinite(scale), scale, torch.nan))
     codes = torch.where(scale > 0, torch.round((y - low) / scale), 0.0).clamp(0, 15).to(torch.uint8).flatten(-2)
     codes = codes[..., _order(d)[0].to(x.device)].unflatten(-1, (d // 2, 2))
     pairs = torch.cat((scale, low), -1).to(torch.bfloat16).view(torch.uint8).flatten(-2)

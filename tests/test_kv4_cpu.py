@@ -148,3 +148,17 @@ def test_write_refuses(over):
 def test_write_checks_its_arguments(over):
     with pytest.raises(AssertionError):
         _call(**over)
+
+
+@pytest.mark.parametrize("power", [-110, -122, -126, -130, -133])
+def test_groups_of_tiny_values(power):
+    """A scale below 2^-126 counts as 0: its group reads back as its lowest value, within 15 2^-126 of what was written."""
+    torch.manual_seed(0)
+    x = (torch.randn(40, 1, 64).double() * 2.0 ** power).to(BF16)
+    low, scale, _ = U.coded(x)
+    got, want = kv4.decode(*kv4.encode(x)), U.values(x)
+    flat = (scale < 2.0 ** -126)[..., 0].expand(-1, -1, 64)
+    assert flat.all() == flat.any() == (power <= -126)     # spans of 64 normal numbers: some 4.7, 0.3 of a scale at 2^-126, 5 at 2^-122
+    assert torch.equal(got[flat].double(), low[..., 0].expand_as(x)[flat]) and float((got.double() - x.double()).abs().max()) <= max(
+        15 * 2.0 ** -126, float((want - x.double()).abs().max()))
+    torch.testing.assert_close(got[~flat].double(), want[~flat], rtol=2 ** -23, atol=2 ** -149)
