@@ -47,7 +47,7 @@ def _refuse_write(q, k, v, positions, cos_sin, rot, neox, q_norm_w, k_norm_w, he
     for w in (q_norm_w, k_norm_w):
         assert w is None or (w.dtype == _BF16 and w.shape == (d,) and w.is_contiguous())
     _index(positions, "positions", 2 if mrope else 1)
-    assert positions.shape[-1] >= t
+    assert positions.shape[-1] >= t and (not mrope or positions.shape[0] >= 3), positions.shape
     rows = [x for x in (q, k, v) if x.numel()]
     if any(x.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(x.shape[:2], x.stride())) for x in rows) or \
             any(w is not None and w.data_ptr() % 16 for w in (q_norm_w, k_norm_w)):
@@ -164,7 +164,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     assert q.dtype is _BF16 and width >= hq * d and one == 1 and d == head_dim and hq % hkv == 0
     _index(block_table, "block_table", 2)
     _index(seq_lens, "seq_lens")
-    assert block_table.shape[0] >= num_seqs and seq_lens.shape[0] >= num_seqs and t >= num_decode_seqs
+    assert block_table.shape[0] >= num_seqs and seq_lens.shape[0] >= num_seqs and t >= num_decode_seqs and 0 <= num_decode_seqs <= num_seqs
+    prompts = num_seqs - num_decode_seqs if max_q_len > 0 else 0
+    if prompts:
+        _index(query_start_loc, "query_start_loc")
+        assert query_start_loc.shape[0] > num_seqs and (host_lens is None or len(host_lens) >= num_seqs), (query_start_loc.shape, num_seqs)
     q_at = q.data_ptr()
     if t == 1:                                                # the stride of a dimension of one may be anything
         q_ts = hq * d
@@ -174,7 +178,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = q.new_empty((t, hq * d))
     else:
         assert out.dtype == _BF16 and out.shape == (t, hq * d) and out.is_contiguous()
-    on_this_device(q, out, k_cache, v_cache, block_table, seq_lens)
+    on_this_device(q, out, k_cache, v_cache, block_table, seq_lens, query_start_loc if prompts else None)
     L, st = _lib.load(), stream_ptr()
     pitch, width = block_table.stride(0), block_table.shape[1]
     k_at, v_at, out_at, table_at, lens_at = k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
@@ -184,10 +188,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         check(L.gllm_kv4_decode(q_at, q_ts, out_at, k_at, v_at, pages, table_at, pitch, width, lens_at, num_decode_seqs, hq, hkv, d, page_size,
                                 scale, _DECODE_CTAS, scratch.data_ptr(), size, st), "kv4_decode")
         _count(2)
-    prompts = num_seqs - num_decode_seqs
-    if prompts > 0 and max_q_len > 0:
-        _index(query_start_loc, "query_start_loc")
-        on_this_device(query_start_loc)
+    if prompts:
         if torch.cuda.is_current_stream_capturing():          # replayed at other lengths
             lens = [width * page_size] * prompts
         else:

@@ -162,3 +162,30 @@ def test_groups_of_tiny_values(power):
     assert torch.equal(got[flat].double(), low[..., 0].expand_as(x)[flat]) and float((got.double() - x.double()).abs().max()) <= max(
         15 * 2.0 ** -126, float((want - x.double()).abs().max()))
     torch.testing.assert_close(got[~flat].double(), want[~flat], rtol=2 ** -23, atol=2 ** -149)
+
+
+def _attend(**over):
+    d = 64
+    a = dict(q=torch.zeros(5, 4 * d, dtype=BF16), k_cache=torch.zeros(kv4.cache_shape(4, 2, d, 16), dtype=torch.uint8),
+             v_cache=torch.zeros(kv4.cache_shape(4, 2, d, 16), dtype=torch.uint8), block_table=torch.zeros(3, 2, dtype=torch.int32),
+             seq_lens=torch.ones(3, dtype=torch.int32), query_start_loc=torch.zeros(4, dtype=torch.int32), scale=1.0, num_q_heads=4, head_dim=d,
+             num_decode_seqs=1, num_seqs=3, max_q_len=2, max_seq_len=20)
+    a.update(over)
+    return sm100_kv4.paged_attention(**a)
+
+
+@pytest.mark.parametrize("over", [
+    dict(query_start_loc=torch.zeros(3, dtype=torch.int32)), dict(query_start_loc=torch.zeros(4, dtype=torch.int64)),
+    dict(host_lens=[5, 6]), dict(num_decode_seqs=4), dict(num_decode_seqs=-1), dict(block_table=torch.zeros(2, 2, dtype=torch.int32)),
+    dict(seq_lens=torch.ones(2, dtype=torch.int32)), dict(q=torch.zeros(0, 256, dtype=BF16)), dict(num_q_heads=3),
+])
+def test_attention_checks_its_arguments_before_it_launches(over):
+    """Indexes that end before the last sequence would be read past their end on the device."""
+    with pytest.raises(AssertionError):
+        _attend(**over)
+
+
+def test_write_takes_three_rows_of_positions():
+    positions = torch.zeros(2, 4, dtype=torch.int32)
+    with pytest.raises(AssertionError):
+        _call(positions=positions, mrope_section=[16, 24, 24])
