@@ -10,8 +10,9 @@ pair, half a bit a value. Keys are coded as rotated and rounded to bf16, so that
 infinity (or spans more than fp32 holds) reads back as NaN.
 
 What attention makes of held values on the GPU: decoding sequences take codes, scales and low ends as they are; a query's dims are exact down to
-2^-28 of its head's largest, sums are fp32, and a probability times a value's scale is rounded to fp16 (2^-11). Prompt portions see held
-values rounded to bf16 (2^-8, as `kv_cache_rows` gives them) and round probabilities to bf16, as over a bf16 cache. The plain form keeps fp32.
+2^-28 of its head's largest, sums are fp32, and a probability times a value's scale is rounded to fp16: 2^-11, or 2^-31 of the largest scale among
+the head's values (2^-60 at least) where that is more. Prompt portions see held values rounded to bf16 (2^-8, as `kv_cache_rows` gives
+them) and round probabilities to bf16, as over a bf16 cache. The plain form keeps fp32.
 
 A row's 32-bit unit u holds eight dims, the first in the lowest four bits: those from 64 (u % (D / 64)) + 8 (u // (D / 64)) on. So
 16 bytes hold as many dims of each group, which is what a lane of the attention kernel takes (csrc/attn/kv4_attention.cu).
