@@ -142,8 +142,8 @@ using namespace b200;
 
 // x [M, K] bf16 (rows ldx apart) -> q [M, K] int8, scales [M] (largest magnitude, 2^-100 at least, / 127). These may be the weights of a
 // product that is launched next. Products fetch their first weights before they wait for the kernels ahead of them, and the quantiser lets its
-// dependents start at once, so an empty kernel without an early start stands between the two (2 us, once per weight; the product's own rows
-// go without).
+// dependents start at once, so an empty kernel without an early start stands between the two (1 us: 6144 x 4096 14.9 us for 13.7; the product's
+// own rows go without).
 GLLM_EXPORT int gllm_int8_quant_rows(const void* x, int64_t ldx, void* q, void* scales, int M, int K, void* stream) {
   if (M <= 0 || K <= 0) return 0;
   if (K % 16 != 0 || ldx % 8 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15) != 0) {
