@@ -114,8 +114,8 @@ def build(force: bool = False, verbose: bool = False, groups=None) -> str:
     def compile_one(item):
         s, obj, dig, digf = item
         flags = NVCC_FLAGS
-        if os.sep + "seq" + os.sep in s:
-            # recurrences, softplus and decays there are specified in accurate fp32: no approximate intrinsics
+        if os.sep + "seq" + os.sep in s or os.sep + "draft" + os.sep in s:
+            # recurrences, softplus, decays and probabilities there are specified in accurate fp32: no approximate intrinsics
             flags = [f for f in NVCC_FLAGS if f != "--use_fast_math"]
         cmd = [nvcc_path(), *flags, "-I", CSRC, "-c", s, "-o", obj]
         if verbose:

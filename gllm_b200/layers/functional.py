@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from gllm_b200.ops import kv4, ref
+from gllm_b200.ops import draft, kv4, ref
 
 
 _modules = {}      # imported on first use: a lookup a call instead of the import statement
@@ -28,6 +28,14 @@ def _kv4():
     if m is None:
         from gllm_b200.ops import sm100_kv4 as m
         _modules["kv4"] = m
+    return m
+
+
+def _draft():
+    m = _modules.get("draft")
+    if m is None:
+        from gllm_b200.ops import sm100_draft as m
+        _modules["draft"] = m
     return m
 
 
@@ -176,6 +184,34 @@ def kv_cache_rows(k_cache, v_cache, slots):
     if k_cache.is_cuda:
         return _kv4().kv_cache_rows(k_cache, v_cache, slots)
     return tuple(kv4.read_rows(c, slots).to(torch.bfloat16) for c in (k_cache, v_cache))
+
+
+# -- decoding with drafted tokens (ops/draft.py has the definitions) -------------------------------------------
+def draft_plan(parents, inp, page_size):
+    """(seen int64 [T], positions int32 [T], slots int32 [T]) of a step's drafted nodes: whom each sees (bit j: node j of its sequence),
+    its rotary position and its place in the cache. `parents` int32 [T]: a node's parent within its sequence, -1 none; at most 64
+    nodes a sequence. `inp.seq_lens` counts the nodes."""
+    return (_draft() if parents.is_cuda else draft).plan(parents, inp, page_size)
+
+
+def draft_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out=None):
+    """Attention of the nodes' queries [T, Hq * D] over the paged cache that holds their own keys and values too: each sees the context and the
+    nodes in its word of `seen`, whatever lies in those it does not see."""
+    return (_draft() if q.is_cuda else draft).attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out)
+
+
+def draft_verify(tokens, parents, inp, target, draft_probs=None, uniform=None):
+    """(tokens int32 [T], path int32 [T], count int32 [sequences]): in each sequence's rows the tokens that it goes on with, count of
+    them (the last is new), and the nodes that were taken, node 0 first; -1 behind them. `target`: the target's tokens int32 [T] at the nodes
+    (from `sample`, say), or its probabilities fp32 [T, V] with `uniform` [T] in [0, 1) and, where drafts were drawn, their
+    distributions `draft_probs` [T, V] (row i: what node i's children were drawn from)."""
+    return (_draft() if tokens.is_cuda else draft).verify(tokens, parents, inp, target, draft_probs, uniform)
+
+
+def draft_keep(k_caches, v_caches, inp, path, count):
+    """In every layer's caches (lists of tensors, None for layers without), in place: keys and values of the nodes in `path` to
+    the places from the end of the context on."""
+    return (_draft() if path.is_cuda else draft).keep(k_caches, v_caches, inp, path, count)
 
 
 def sample(logits, inp, seen_bits=None, seed=0, step=None):

@@ -100,6 +100,10 @@ def _declare(lib):
     sig("gllm_kv4_expand", [P, P, P, L, I, P, I, I, I, I, L, L, P, P, P, I, I, P])
     sig("gllm_attn_prefill_tc_tiles", [P, L, P, P, P, L, P, I, P, P, I, I, I, I, I, I, F, P])
     sig("gllm_gemm_fp8_block", [P, P, P, P, P, L, I, I, I, P, I, P])
+    sig("gllm_draft_plan", [P, P, P, P, L, I, I, I, I, P, P, P, P])
+    sig("gllm_draft_attention", [P, L, P, P, P, L, P, L, I, P, P, P, I, I, I, I, I, I, I, F, P])
+    sig("gllm_draft_verify", [P, P, P, P, P, L, P, L, P, I, I, I, P, P, P, I, P])
+    sig("gllm_draft_keep", [P, I, L, I, I, I, P, P, P, P, P, L, I, I, I, P])
 
 
 _NEEDED = None     # csrc groups this process needs (None: all of them)
