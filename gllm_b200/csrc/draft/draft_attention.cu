@@ -1,102 +1,690 @@
 // Attention of drafted nodes over a paged bf16 cache. Definition: ops/draft.py.
-#include "../common/host_utils.h"
-#include "../common/ptx.cuh"
+//
+// A kv head's rows are node x query head, in blocks of 128: a block's scores S = Q K^T and results O += P V are tcgen05 products with all
+// of M = 128, whatever the rows; that costs the tensor core 1024 cycles per 128 keys (heads of 128), where their bytes take some 2700 of an
+// SM's share of the memory, so few rows waste nothing that is missed.
+//
+// Work: units (sequence, kv head, block of rows), each as long as its sequence's 128-key tiles. All units lie in one row that is cut into
+// equal shares for the CTAs, one an SM, on the device: lengths may differ from those at the time a graph was captured, and long contexts
+// beside short ones leave no SM idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined
+// by a second launch in a fixed order.
+//
+//   warps 0-3, 4-7     softmax, one row a thread (tcgen05.ld 32x32b): the CTA's units in turn, so that a unit's results are written while
+//                      the next one's scores are formed. Reference of the exponents follows the maximum in steps of 2^8
+//   warp 8             copies: page boxes [page][64] of K and V -> ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V
+//   warp 9 (1 thread)  products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two)
+//   warps 10, 11       queries of the units to come (two buffers)
+//
+// Masks: only tiles that reach behind the context are masked, with the bits of the row's word shifted to the tile. A value that is not seen must
+// not reach the sum even as 0 x NaN: rows behind the last key are zeroed, and so are values of nodes that are no numbers; rows that see
+// those have them added at the end.
+#include "../attn/attn_common.cuh"
+#include "../common/bounded.cuh"
 
 namespace b200 {
 
 static constexpr int kNodes = 64;
-static constexpr int kWarps = 4;
+static constexpr int kRows = 128, kKeys = 128;           // of a unit's block, of a tile
+static constexpr int kSoftmaxWarps = 8;
+static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
+// 128 x 72 + 256 x 216 registers are what 384 threads are launched with (168 each)
+static constexpr int kRegsIssue = 72, kRegsSoftmax = 216;
+static constexpr float kLazy = 8.f;                      // P stays below 2^8 between two rescales of O
 
 struct DraftAttnParams {
   const __nv_bfloat16* q;
   int64_t q_ts;
   __nv_bfloat16* out;
-  const __nv_bfloat16* k;
-  const __nv_bfloat16* v;
+  const __nv_bfloat16* v;                                // for nodes whose values are no numbers
   int64_t pages;
   const int32_t* table;
   int64_t table_ld;
   const int32_t* seq_lens;
   const int32_t* q_start;
   const int64_t* seen;
-  int table_width, num_seqs, rows, Hq, Hkv, page_size;
+  int table_width, num_seqs, rows, Hq, Hkv, G, page_size;
   float scale_log2;
+  float4* part_o;                                        // [2 CTA][D / 4][128 rows]
+  float2* part_ml;                                       // [2 CTA][128 rows]: reference of the exponents, sum
+  int4* cut;                                             // [CTA][2]: what the join of a unit that the CTA begins needs
+  WaitConfig waits;
 };
 
-// One CTA per (node, query head), its warps take every fourth key; a lane has D / 32 neighbouring dims. Grid: (heads, 64 nodes, sequences).
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) draft_attention_plain_kernel(const DraftAttnParams p) {
-  constexpr int E = D / 32;
+struct DraftSmem {
+  static constexpr int kQBytes = kRows * D * 2, kTileBytes = kKeys * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kRingOff = 2 * kQBytes, kBarOff = kRingOff + kStages * kTileBytes;
+  static constexpr int kBytes = kBarOff + 512 + 1024;
+  static_assert(kBytes <= 232448, "shared memory of a CTA");
+  static constexpr int kTmemO = 2 * kKeys, kTmemCols = 512;
+};
+
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// V as it lies in the cache, keys along the rows: MN-major, 64 dims (128 bytes) then the next slab LBO bytes on, 8 keys SBO
+__device__ __forceinline__ uint64_t mn_major_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF) | static_cast<uint64_t>((kKeys * 128) >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// What a sequence is to the units: rows [first, first + n) of the batch, ctx tokens before its nodes
+struct Seq {
+  int first, n, ctx, len, tiles, blocks;
+  __device__ __forceinline__ Seq(const DraftAttnParams& p, int s) {
+    first = p.q_start[s];
+    const int n_all = first < 0 ? 0 : min(p.q_start[s + 1], p.rows) - first;
+    n = max(min(n_all, kNodes), 0);
+    ctx = max(p.seq_lens[s] - max(n_all, 0), 0);
+    len = ctx + n;
+    blocks = (n * p.G + kRows - 1) / kRows;
+    tiles = n > 0 ? (len + kKeys - 1) / kKeys : 0;
+  }
+  __device__ __forceinline__ int64_t work(const DraftAttnParams& p) const { return static_cast<int64_t>(tiles) * blocks * p.Hkv; }
+};
+
+// The CTA's items: its share of one unit each, tiles [t0, t1)
+struct Items {
+  const DraftAttnParams& p;
+  int s;
+  int64_t off, left;                                     // in the sequence's work; tiles to come
+  int first, n, ctx, len, tiles, blocks, kvh, blk, t0, t1;
+  __device__ __forceinline__ Items(const DraftAttnParams& p_, int s_, int64_t off_, int64_t left_) : p(p_), s(s_), off(off_), left(left_) {}
+  __device__ __forceinline__ bool next() {
+    if (left <= 0) return false;
+    for (;;) {                                           // the sequence that `off` lies in: there is one, as tiles are left
+      const Seq q(p, s);
+      if (off < q.work(p)) {
+        first = q.first; n = q.n; ctx = q.ctx; len = q.len; tiles = q.tiles; blocks = q.blocks;
+        break;
+      }
+      off = 0;
+      if (++s >= p.num_seqs) {
+        left = 0;
+        return false;
+      }
+    }
+    const int unit = static_cast<int>(off / tiles);
+    t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
+    t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + left));
+    kvh = unit / blocks;
+    blk = unit - kvh * blocks;
+    off += t1 - t0;
+    left -= t1 - t0;
+    return true;
+  }
+  __device__ __forceinline__ int block_rows() const { return min(kRows, n * p.G - blk * kRows); }
+  // keys of tile t that there are
+  __device__ __forceinline__ int keys(int t) const { return min(len - t * kKeys, kKeys); }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DraftAttnParams p) {
+  using SM = DraftSmem<D>;
+  constexpr int NS = SM::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
+  uint64_t* empty = full + NS;                           // [NS] products -> copies
+  uint64_t* s_full = empty + NS;                         // [2 warpgroups][2] S of the warpgroup's k-th tile: barrier k % 2
+  uint64_t* p_full = s_full + 4;                         // [2] P of the CTA's tile g written (4 warps): barrier g % 2
+  uint64_t* o_full = p_full + 2;                         // [2 warpgroups] P V of the warpgroup's k-th tile is in O: phase k
+  uint64_t* o_free = o_full + 2;                         // [2 warpgroups] O of its item has been read (4 warps)
+  uint64_t* q_full = o_free + 2;                         // [2] queries of item i: barrier i % 2 (2 warps)
+  uint64_t* q_free = q_full + 2;                         // [2]
+  uint64_t* mma_end = q_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
+  const WaitGuard guard{tmem_slot + 1, p.waits};
+  unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [2 warpgroups][2 items in turn]
+  int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // sequence and offset that the share begins at, tiles, all tiles
+  int64_t* warp_work = begin + 4;                        // [12]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[2 * i], 1); mbar_init(&s_full[2 * i + 1], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4);
+      mbar_init(&q_full[i], 2); mbar_init(&q_free[i], 1);
+      bad_nodes[2 * i] = bad_nodes[2 * i + 1] = 0ull;
+    }
+    mbar_init(mma_end, 1);
+    *guard.dead = 0;
+    begin[0] = begin[1] = begin[2] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
+  if (warp == 8 && lane < 2) tma_prefetch_desc(lane == 0 ? &tmap_k : &tmap_v);
+  griddep_launch();
   griddep_wait();
-  const int seq = blockIdx.z, node = blockIdx.y, head = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = p.q_start[seq], n = min(p.q_start[seq + 1], p.rows) - first;
-  if (first < 0 || node >= n) return;
-  const int ctx = max(p.seq_lens[seq] - n, 0), len = ctx + min(n, kNodes), kvh = head / (p.Hq / p.Hkv);
-  const unsigned long long seen = static_cast<unsigned long long>(p.seen[first + node]);
-  const int64_t row = first + node;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
+
+  // ---- the share: prefix sums of the sequences' work, a run of sequences a thread
+  {
+    const int per = (p.num_seqs + kThreads - 1) / kThreads, s0 = threadIdx.x * per, s1 = min(s0 + per, p.num_seqs);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += Seq(p, s).work(p);
+    int64_t upto = mine;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __bfloat162float(p.q[row * p.q_ts + static_cast<int64_t>(head) * D + lane * E + e]) * p.scale_log2;
-    o[e] = 0.f;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) warp_work[warp] = upto;
+    __syncthreads();
+    int64_t before = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += warp_work[w];
+      all += warp_work[w];
+    }
+    // no more CTAs than tiles take part, so that no share between two others is empty
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), all);
+    const bool works = blockIdx.x < ctas;
+    const int64_t x0 = works ? all * blockIdx.x / ctas : 0, x1 = works ? all * (blockIdx.x + 1) / ctas : 0;
+    if (x0 < x1 && x0 >= before && x0 < before + mine) {
+      int s = s0;
+      for (;; ++s) {
+        const int64_t w = Seq(p, s).work(p);
+        if (x0 < before + w || s + 1 >= s1) break;
+        before += w;
+      }
+      begin[0] = s;
+      begin[1] = x0 - before;
+      begin[2] = x1 - x0;
+    }
+    if (threadIdx.x == 0) begin[3] = all;
   }
-  for (int key = warp; key < len; key += kWarps) {
-    if (key >= ctx && !((seen >> (key - ctx)) & 1)) continue;
-    const int block = key / p.page_size;
-    const int64_t page = block < p.table_width ? p.table[seq * p.table_ld + block] : -1;
-    if (page < 0 || page >= p.pages) continue;
-    const int64_t at = (((page * p.Hkv + kvh) * (D / 64) + lane * E / 64) * p.page_size + key % p.page_size) * 64 + lane * E % 64;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += q[e] * __bfloat162float(p.k[at + e]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float top = s > m ? s : m, alpha = m == -INFINITY ? 0.f : exp2f(m - top), w = exp2f(s - top);
-    m = top;
-    l = l * alpha + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + w * __bfloat162float(p.v[at + e]);
-  }
-  __shared__ float so[kWarps][D], sm[kWarps], sl[kWarps];
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+  tc_fence_before();
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
-  for (int w = 0; w < kWarps; ++w) sum += sm[w] == -INFINITY ? 0.f : sl[w] * exp2f(sm[w] - top);
-  for (int d = threadIdx.x; d < D; d += kWarps * 32) {
-    float x = 0.f;
-    for (int w = 0; w < kWarps; ++w) x += sm[w] == -INFINITY ? 0.f : so[w][d] * exp2f(sm[w] - top);
-    p.out[(row * p.Hq + head) * D + d] = __float2bfloat16(sum == 0.f ? 0.f : x / sum);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Items it(p, static_cast<int>(begin[0]), begin[1], begin[2]);
+  const bool idle = begin[2] == 0;
+
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 8 && !idle) {
+      // ------------------------------------------------------------------ copies
+      const int box = min(p.page_size, 64), boxes = kKeys / box, j = lane % boxes, sl = lane / boxes;
+      uint32_t pos = 0;
+      bool ok = true;
+      auto copy = [&](const CUtensorMap* map, int page, int kvh, int tile, int n) {
+        const uint32_t st = pos % NS;
+        ok = __all_sync(0xffffffffu, pos < NS || guard.wait<true>(&empty[st], ((pos / NS) & 1) ^ 1));
+        if (!ok) return;
+        if (lane == 0) mbar_expect_tx(&full[st], n * box * D * 2);
+        __syncwarp();
+        if (sl < D / 64 && j < n)
+          tma_load_3d(smem + SM::kRingOff + st * SM::kTileBytes + sl * (kKeys * 128) + j * box * 128, map, &full[st], 0,
+                      (tile * kKeys + j * box) % p.page_size, (page * p.Hkv + kvh) * (D / 64) + sl);
+        ++pos;
+      };
+      int v_page = 0, v_kvh = 0, v_tile = 0, v_n = 0;      // the tile whose V is to come (v_n: its boxes)
+      while (ok && it.next()) {
+        const int32_t* bt = p.table + it.s * p.table_ld;
+        const int last_page = min((it.len - 1) / p.page_size, p.table_width - 1);
+        auto page_of = [&](int tile) { return bt[min((tile * kKeys + j * box) / p.page_size, last_page)]; };
+        int page = page_of(it.t0);
+        for (int t = it.t0; t < it.t1 && ok; ++t) {
+          const int next = t + 1 < it.t1 ? page_of(t + 1) : 0;
+          const int n = (((it.keys(t) + 15) & ~15) + box - 1) / box;   // boxes with a key that there is, in steps of the product with V
+          copy(&tmap_k, page, it.kvh, t, n);
+          if (ok && v_n > 0) copy(&tmap_v, v_page, v_kvh, v_tile, v_n);
+          v_page = page; v_kvh = it.kvh; v_tile = t; v_n = n;
+          page = next;
+        }
+      }
+      if (ok && v_n > 0) copy(&tmap_v, v_page, v_kvh, v_tile, v_n);
+      for (uint32_t i = pos > NS ? pos - NS : 0; i < pos; ++i) guard.land(&full[i % NS], (i / NS) & 1);   // in flight
+    } else if (warp == 9 && lane == 0 && !idle) {
+      // ------------------------------------------------------------------ products
+      constexpr uint32_t idesc_s = make_idesc_bf16(kRows, kKeys);
+      constexpr uint32_t idesc_pv = make_idesc_bf16(kRows, D) | (1u << 16);
+      uint32_t pos = 0, g = 0;                             // place in the ring, tile
+      uint32_t begun0 = 0, begun1 = 0;                     // tiles of the two warpgroups whose scores have been issued
+      bool ok = true;
+      // S of the next tile of `it`, from the queries in buffer `buf` (of the item's parity, as its warpgroup is)
+      auto scores = [&](uint32_t tile_no, uint32_t buf, bool last) {
+        const uint32_t st = pos % NS;
+        ok = guard.wait<true>(&full[st], (pos / NS) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(smem + buf * SM::kQBytes), k_addr = smem_u32(smem + SM::kRingOff + st * SM::kTileBytes);
+        const uint32_t d_tmem = tmem + (tile_no & 1) * kKeys;
+#pragma unroll
+        for (int kd = 0; kd < D / 64; ++kd) {
+          const uint64_t da = make_sw128_kmajor_desc(q_addr + kd * (kRows * 128)), db = make_sw128_kmajor_desc(k_addr + kd * (kKeys * 128));
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) umma_bf16<1>(d_tmem, da + kk * 2, db + kk * 2, idesc_s, (kd | kk) != 0);
+        }
+        uint32_t& begun = buf == 0 ? begun0 : begun1;
+        umma_commit(&s_full[2 * buf + (begun & 1)]);
+        ++begun;
+        umma_commit(&empty[st]);
+        if (last) umma_commit(&q_free[buf]);
+        ++pos;
+      };
+      bool have = it.next();                               // the tile whose P V is to come: of item `now`, with `keys` keys
+      ok = have && guard.first(&q_full[0]) && guard.wait<true>(&q_full[0], 0);
+      int t = it.t0;
+      if (ok) scores(0, 0, t + 1 == it.t1);
+      uint32_t now = 0;
+      while (ok) {
+        const int keys = it.keys(t);
+        const bool first_tile = t == it.t0, last_tile = t + 1 == it.t1;
+        // scores of the next tile
+        bool more = true;
+        uint32_t next = now;
+        if (!last_tile) {
+          ++t;
+        } else {
+          more = it.next();
+          if (more) {
+            t = it.t0;
+            next = now + 1;
+            ok = guard.wait<true>(&q_full[next & 1], (next >> 1) & 1);
+            if (!ok) break;
+          }
+        }
+        if (more) scores(g + 1, next & 1, t + 1 == it.t1);
+        if (!ok) break;
+        // P V of this one
+        const uint32_t wg = now & 1, st = pos % NS;
+        ok = guard.wait<true>(&full[st], (pos / NS) & 1) && guard.wait<true>(&p_full[g & 1], (g >> 1) & 1) &&
+             (!first_tile || now < 2 || guard.wait<true>(&o_free[wg], ((now >> 1) & 1) ^ 1));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = mn_major_desc(smem_u32(smem + SM::kRingOff + st * SM::kTileBytes));
+        const uint32_t o_tmem = tmem + SM::kTmemO + wg * D, p_tmem = tmem + (g & 1) * kKeys;
+        const uint32_t acc = first_tile ? 0u : 1u;
+        if (keys == kKeys) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < (keys + 15) / 16; ++kk)
+            umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+        }
+        umma_commit(&o_full[wg]);
+        umma_commit(&empty[st]);
+        ++pos;
+        ++g;
+        if (!more) break;
+        now = next;
+      }
+      umma_commit(mma_end);                                // nothing is in flight when the columns are given back
+      guard.land(mma_end, 0);
+    } else if (warp >= 10 && !idle) {
+      // ------------------------------------------------------------------ queries
+      for (uint32_t item = 0; it.next(); ++item) {
+        const uint32_t buf = item & 1;
+        if (item >= 2 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1))) break;
+        const int rows = it.block_rows();
+        const uint32_t dst = smem_u32(smem + buf * SM::kQBytes);
+        for (int e = threadIdx.x - 320; e < rows * (D / 8); e += 64) {
+          const int r = e / (D / 8), c = e % (D / 8), at = it.blk * kRows + r, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
+          const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(head) * D + c * 8;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                       "l"(src) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[buf]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ------------------------------------------------------------------ softmax: one row a thread
+    const int wg = warp >> 2, row = threadIdx.x & 127;     // row == TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_o = tmem + SM::kTmemO + wg * D + lane_base;
+    uint32_t g = 0, done = 0;                              // tiles of the CTA; tiles of this warpgroup
+    bool cut_tail = false;
+    // A wait that gives up leaves the warps in step: they go on with what is there, and every later wait ends at once
+    auto await = [&](uint64_t* bar, uint32_t parity) {
+      guard.wait<true>(bar, parity);
+      __syncwarp();
+      tc_fence_after();
+    };
+    for (uint32_t item = 0; it.next(); ++item) {
+      const bool cut = it.t0 > 0 || it.t1 < it.tiles;
+      if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
+      if ((item & 1) != static_cast<uint32_t>(wg)) {
+        g += it.t1 - it.t0;
+        continue;
+      }
+      const int rows = it.block_rows();
+      const bool warp_ok = (warp & 3) * 32 < rows, row_ok = row < rows;
+      const int at = it.blk * kRows + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
+      const int64_t tok = it.first + (row_ok ? node : 0);
+      unsigned long long word = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;
+      if (it.n < kNodes) word &= (1ull << it.n) - 1;
+      float m_run = -INFINITY, l_run = 0.f;
+      unsigned long long* bad_here = bad_nodes + 2 * wg + ((item >> 1) & 1);
+      for (int t = it.t0; t < it.t1; ++t, ++g, ++done) {
+        const uint32_t t_s = tmem + (g & 1) * kKeys + lane_base;
+        const int key0 = t * kKeys;
+        await(&s_full[2 * wg + (done & 1)], (done >> 1) & 1);
+        bool free_o = done == 0;                           // the product of the warpgroup's tile before has ended
+        const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
+        if (warp_ok) {
+          float f[kKeys];
+          {
+            uint32_t v[kKeys / 32][32];
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(t_s + c * 32, v[c]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < kKeys; ++e) f[e] = __uint_as_float(v[e / 32][e % 32]);
+          }
+          if (behind) {
+            // bits of this tile's keys: all of the context, then the row's word from its first node on
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c) {
+              const int j0 = key0 + c * 32 - it.ctx;       // node of the first of 32 keys
+              const uint32_t bits = j0 >= 64 ? 0u
+                                    : j0 >= 0 ? static_cast<uint32_t>(word >> j0)
+                                    : j0 <= -32 ? 0xffffffffu : (static_cast<uint32_t>(word << -j0) | ((1u << -j0) - 1u));
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) f[c * 32 + e] = -INFINITY;
+            }
+          }
+          float m4[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+          for (int e = 4; e < kKeys; e += 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], e + 4 < kKeys ? fmaxf(f[e + i], f[e + 4 + i]) : f[e + i]);
+          }
+          const float m_new = fmaxf(m_run, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2);
+          float alpha = 1.f;
+          if (m_new > m_run + kLazy) {
+            alpha = ex2(m_run - m_new);
+            m_run = m_new;
+          }
+          if (t > it.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            await(&o_full[wg], (done - 1) & 1);
+            free_o = true;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t v[16];
+              tmem_ld_32x16(t_o + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_store16(t_o + c, v);
+            }
+          }
+          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t sc2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-m_use, -m_use);
+          uint64_t sum2[2] = {0, 0};
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 32) {            // 32 keys: 16 columns of P
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 x = unpair(fma_pair(pair(f[c + 2 * e], f[c + 2 * e + 1]), sc2, nm2));
+              const float2 y = make_float2(ex2(x.x), ex2(x.y));
+              sum2[e & 1] = add_pair(sum2[e & 1], pair(y.x, y.y));
+              pk[e] = pack_bf16(y.x, y.y);                 // probabilities enter the product in bf16, the sum in fp32
+            }
+            tmem_store16(t_s + c / 2, pk);
+          }
+          const float2 sa = unpair(add_pair(sum2[0], sum2[1]));
+          l_run = l_run * alpha + (sa.x + sa.y);
+          tmem_store_wait();
+        }
+        if (behind) {
+          // Values that nobody sees, or not every row, are finite before the product reads them
+          const uint32_t vp = (t + 1 < it.t1 || it.left > 0) ? 2 * g + 2 : 2 * g + 1, st = vp % NS;    // where V of tile g is in the ring
+          await(&full[st], (vp / NS) & 1);
+          uint8_t* tile = smem + SM::kRingOff + st * SM::kTileBytes;
+          const int lo = max(it.ctx - key0, 0), hi = it.keys(t), end = min((hi + 15) & ~15, kKeys);
+          for (int e = lo * (D / 8) + (threadIdx.x & 127); e < end * (D / 8); e += 128) {
+            const int r = e / (D / 8), c = e % (D / 8);
+            uint4* w = reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            if (r >= hi) {
+              *w = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 x = *w;
+            uint32_t* u = reinterpret_cast<uint32_t*>(&x);
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t b = ((u[i] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((u[i] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+              if (b != 0u) { u[i] &= ~b; bad = true; }
+            }
+            if (bad) {
+              *w = x;
+              atomicOr(bad_here, 1ull << (key0 + r - it.ctx));
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        if (!free_o) await(&o_full[wg], (done - 1) & 1);   // every phase is waited for, once: parities stay unambiguous
+        tc_fence_before();                                 // P and the rescaled O are in TMEM, S has been read
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+      }
+      // ---- results
+      await(&o_full[wg], (done - 1) & 1);
+      if (row == 0) bad_nodes[2 * wg + (((item >> 1) & 1) ^ 1)] = 0ull;   // the item before's, read by all (their P of this one is there)
+      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");         // bad_here of all four warps
+      else asm volatile("bar.sync 2, 128;" ::: "memory");
+      const unsigned long long bad = *static_cast<volatile unsigned long long*>(bad_here) & word;
+      if (warp_ok) {
+        const float inv = cut ? 1.f : l_run > 0.f ? 1.f / l_run : 0.f;
+        const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
+        __nv_bfloat16* op = p.out + (tok * p.Hq + head) * D;
+        float4* po = p.part_o + static_cast<size_t>(slot) * (D / 4) * kRows + row;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(t_o + c, v);
+          tmem_ld_wait();
+          float x[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(v[e]) * inv;
+          if (row_ok) {
+            for (unsigned long long b = bad; b != 0ull; b &= b - 1) {   // seen values that are no numbers
+              const int place = it.ctx + __ffsll(static_cast<long long>(b)) - 1;
+              const int64_t page = p.table[it.s * p.table_ld + min(place / p.page_size, p.table_width - 1)];
+              if (page < 0 || page >= p.pages) continue;
+              const __nv_bfloat16* vr = p.v + (((page * p.Hkv + it.kvh) * (D / 64) + c / 64) * p.page_size + place % p.page_size) * 64 + c % 64;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float y = __bfloat162float(vr[e]);
+                if (!(fabsf(y) < INFINITY)) x[e] += y;
+              }
+            }
+            if (cut) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) po[(c / 4 + e) * kRows] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint4 w;
+                w.x = pack_bf16(x[8 * e], x[8 * e + 1]);
+                w.y = pack_bf16(x[8 * e + 2], x[8 * e + 3]);
+                w.z = pack_bf16(x[8 * e + 4], x[8 * e + 5]);
+                w.w = pack_bf16(x[8 * e + 6], x[8 * e + 7]);
+                *reinterpret_cast<uint4*>(op + c + e * 8) = w;
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * kRows + row] = make_float2(m_run, l_run);
+        if (cut && it.t0 == 0 && row == 0) {
+          // CTAs before the one whose share ends at the unit's end or behind it
+          const int64_t all = begin[3], ctas = min(static_cast<int64_t>(gridDim.x), all);
+          const int64_t end = all * (blockIdx.x + 1) / ctas + (it.tiles - it.t1);
+          const int last = static_cast<int>((end * ctas + all - 1) / all) - 1;
+          p.cut[2 * blockIdx.x] = make_int4(last, it.first, it.kvh, it.blk);
+          p.cut[2 * blockIdx.x + 1] = make_int4(rows, 0, 0, 0);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[wg]);
+    }
+    if (threadIdx.x == 0 && !cut_tail) p.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);   // no unit begins here that ends elsewhere
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, SM::kTmemCols);
+  }
+}
+
+// Joins the parts of the unit that CTA blockIdx.x begins and CTA `last` ends: 32 rows a block, a lane each, a warp every eighth four dims
+static constexpr int kJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) draft_join_kernel(const DraftAttnParams p) {
+  griddep_wait();
+  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
+  const int4 c0 = p.cut[2 * cta], c1 = p.cut[2 * cta + 1];
+  const int last = c0.x;
+  if (last <= cta || last >= static_cast<int>(gridDim.x) || row >= c1.x) return;
+  auto slot = [&](int c) { return static_cast<size_t>(2 * c + (c == cta ? 1 : 0)); };
+  float m = -INFINITY;
+  for (int c = cta; c <= last; ++c) m = fmaxf(m, p.part_ml[slot(c) * kRows + row].x);
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o[D / 4 / kJoinWarps];
+#pragma unroll
+  for (int i = 0; i < D / 4 / kJoinWarps; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = cta; c <= last; ++c) {
+    const float2 ml = p.part_ml[slot(c) * kRows + row];
+    const float w = ex2(ml.x - m_use);
+    l += w * ml.y;
+#pragma unroll
+    for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
+      const float4 x = p.part_o[(slot(c) * (D / 4) + warp + i * kJoinWarps) * kRows + row];
+      o[i].x += w * x.x; o[i].y += w * x.y; o[i].z += w * x.z; o[i].w += w * x.w;
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int at = c0.w * kRows + row, node = at / p.G, head = c0.z * p.G + at - node * p.G;
+  __nv_bfloat16* op = p.out + (static_cast<int64_t>(c0.y + node) * p.Hq + head) * D;
+#pragma unroll
+  for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
+    uint2 w;
+    w.x = pack_bf16(o[i].x * inv, o[i].y * inv);
+    w.y = pack_bf16(o[i].z * inv, o[i].w * inv);
+    *reinterpret_cast<uint2*>(op + (warp + i * kJoinWarps) * 4) = w;
+  }
+}
+
+// boxes of one 64-wide slab of a page ([page][64], at most 64 rows)
+static int page_tmap(const void* base, int64_t pages, int Hkv, int D, int page_size, CUtensorMap* out) {
+  const cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(pages * Hkv * (D / 64))};
+  const cuuint64_t strides[2] = {128, static_cast<cuuint64_t>(page_size) * 128};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(page_size < 64 ? page_size : 64), 1}, estr[3] = {1, 1, 1};
+  const CUresult r = get_encode_fn()(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "[gllm_b200] cache tensor-map encode failed (%d)\n", static_cast<int>(r));
+    return 1;
+  }
+  return 0;
+}
+
+template <int D>
+static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, const DraftAttnParams& p, int ctas, int max_nodes, cudaStream_t st) {
+  using SM = DraftSmem<D>;
+  static PerDeviceOnce configured;
+  if (configured.need()) {
+    CUDA_CHECK_RET(cudaFuncSetAttribute(draft_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
+    configured.done();
+  }
+  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, p));
+  const int rows = max_nodes * p.G < kRows ? max_nodes * p.G : kRows;
+  CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
+  return 0;
 }
 
 }  // namespace b200
 
 using namespace b200;
 
+// bytes of scratch for a launch of `ctas` CTAs
+GLLM_EXPORT int64_t gllm_draft_attention_scratch(int D, int ctas) { return static_cast<int64_t>(ctas) * (2 * kRows * (D * 4 + 8) + 32); }
+
 GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, const void* k_cache, const void* v_cache, int64_t pages,
                                      const void* table, int64_t table_ld, int table_width, const void* seq_lens, const void* q_start,
                                      const void* seen, int num_seqs, int rows, int max_nodes, int Hq, int Hkv, int D, int page_size,
-                                     float scale, void* stream) {
+                                     float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (num_seqs <= 0 || rows <= 0 || max_nodes <= 0) return 0;
-  if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || num_seqs > 65535) return 1;
+  if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || page_size < 8 || kKeys % page_size || pages <= 0 || table_width <= 0 || ctas <= 0 ||
+      q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
+      scratch_bytes < gllm_draft_attention_scratch(D, ctas))
+    return 1;
+  CUtensorMap tk, tv;
+  if (page_tmap(k_cache, pages, Hkv, D, page_size, &tk) || page_tmap(v_cache, pages, Hkv, D, page_size, &tv)) return 1;
   DraftAttnParams p;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.q_ts = q_ts;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  p.k = reinterpret_cast<const __nv_bfloat16*>(k_cache);
   p.v = reinterpret_cast<const __nv_bfloat16*>(v_cache);
   p.pages = pages;
   p.table = reinterpret_cast<const int32_t*>(table); p.table_ld = table_ld; p.table_width = table_width;
   p.seq_lens = reinterpret_cast<const int32_t*>(seq_lens);
   p.q_start = reinterpret_cast<const int32_t*>(q_start);
   p.seen = reinterpret_cast<const int64_t*>(seen);
-  p.num_seqs = num_seqs; p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.page_size = page_size;
+  p.num_seqs = num_seqs; p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.page_size = page_size;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(Hq, max_nodes < kNodes ? max_nodes : kNodes, num_seqs);
+  p.part_o = reinterpret_cast<float4*>(scratch);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(2) * ctas * (D / 4) * kRows);
+  p.cut = reinterpret_cast<int4*>(p.part_ml + static_cast<size_t>(2) * ctas * kRows);
+  p.waits = g_wait_config;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (D == 128) CUDA_CHECK_RET(launch_pdl(draft_attention_plain_kernel<128>, grid, dim3(kWarps * 32), 0, st, p));
-  else CUDA_CHECK_RET(launch_pdl(draft_attention_plain_kernel<64>, grid, dim3(kWarps * 32), 0, st, p));
-  return 0;
+  return D == 128 ? launch_draft_attention<128>(tk, tv, p, ctas, max_nodes, st) : launch_draft_attention<64>(tk, tv, p, ctas, max_nodes, st);
 }

@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -32,6 +33,11 @@ def plan(parents: torch.Tensor, inp, page_size: int):
     return seen, positions, slots
 
 
+@functools.lru_cache(maxsize=None)
+def _attention_scratch(head_dim: int) -> int:
+    return _lib.load().gllm_draft_attention_scratch(head_dim, NUM_SMS)
+
+
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp, seen: torch.Tensor, scale: float, num_q_heads: int,
               head_dim: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, Hq * D] bf16 (any row stride) -> [T, Hq * D]; rows behind the last sequence are left as they are."""
@@ -50,11 +56,13 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
         return out
     table = inp.block_table
     on_this_device(q, k_cache, v_cache, table, inp.seq_lens, inp.query_start_loc, seen, out)
+    size = _attention_scratch(head_dim)
+    scratch = k_cache.new_empty(size, dtype=torch.uint8)       # of this call: captured graphs and streams share none
     check(_lib.load().gllm_draft_attention(q.data_ptr(), q_ts, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages,
                                            table.data_ptr(), table.stride(0), table.shape[1], inp.seq_lens.data_ptr(),
                                            inp.query_start_loc.data_ptr(), seen.data_ptr(), b, t, inp.max_q_len, num_q_heads, hkv,
-                                           head_dim, page_size, scale, stream_ptr()), "draft_attention")
-    _count()
+                                           head_dim, page_size, scale, NUM_SMS, scratch.data_ptr(), size, stream_ptr()), "draft_attention")
+    _count(2)
     return out
 
 
