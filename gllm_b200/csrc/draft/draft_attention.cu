@@ -9,8 +9,9 @@
 // beside short ones leave no SM idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined
 // by a second launch in a fixed order.
 //
-//   warps 0-3, 4-7     softmax, one row a thread (tcgen05.ld 32x32b): the CTA's units in turn, so that a unit's results are written while
-//                      the next one's scores are formed. Reference of the exponents follows the maximum in steps of 2^8
+//   warps 0-3, 4-7     softmax, one row a thread (tcgen05.ld 32x32b): the CTA's tiles in turn. A tile takes a warpgroup some 2 us, most of it
+//                      latency of its steps one after the other, where its bytes take 1.5. Both have one reference of the exponents, which
+//                      follows the maximum in steps of 2^8 and is handed on from tile to tile, so that their products add up in one O
 //   warp 8             copies: page boxes [page][64] of K and V -> ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V
 //   warp 9 (1 thread)  products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two)
 //   warps 10, 11       queries of the units to come (two buffers)
@@ -27,8 +28,6 @@ static constexpr int kNodes = 64;
 static constexpr int kRows = 128, kKeys = 128;           // of a unit's block, of a tile
 static constexpr int kSoftmaxWarps = 8;
 static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
-// 128 x 72 + 256 x 216 registers are what 384 threads are launched with (168 each)
-static constexpr int kRegsIssue = 72, kRegsSoftmax = 216;
 static constexpr float kLazy = 8.f;                      // P stays below 2^8 between two rescales of O
 
 struct DraftAttnParams {
@@ -42,7 +41,7 @@ struct DraftAttnParams {
   const int32_t* seq_lens;
   const int32_t* q_start;
   const int64_t* seen;
-  int table_width, num_seqs, rows, Hq, Hkv, G, page_size;
+  int table_width, num_seqs, rows, Hq, Hkv, G, page_shift;   // a page has 2^page_shift tokens
   float scale_log2;
   float4* part_o;                                        // [2 CTA][D / 4][128 rows]
   float2* part_ml;                                       // [2 CTA][128 rows]: reference of the exponents, sum
@@ -55,7 +54,9 @@ struct DraftSmem {
   static constexpr int kQBytes = kRows * D * 2, kTileBytes = kKeys * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kRingOff = 2 * kQBytes, kBarOff = kRingOff + kStages * kTileBytes;
-  static constexpr int kBytes = kBarOff + 512 + 1024;
+  // barriers, words and per-row floats (see the kernel), and up to 1 KB before the first 1024-byte boundary
+  static constexpr int kBarBytes = (2 * kStages + 25) * 8 + 8 + 4 * 8 + 4 * 8 + 12 * 8 + 3 * kRows * 4 + kStages * 4;
+  static constexpr int kBytes = kBarOff + (kBarBytes + 15) / 16 * 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr int kTmemO = 2 * kKeys, kTmemCols = 512;
 };
@@ -114,42 +115,50 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 // What a sequence is to the units: rows [first, first + n) of the batch, ctx tokens before its nodes
 struct Seq {
   int first, n, ctx, len, tiles, blocks;
-  __device__ __forceinline__ Seq(const DraftAttnParams& p, int s) {
-    first = p.q_start[s];
-    const int n_all = first < 0 ? 0 : min(p.q_start[s + 1], p.rows) - first;
+  __device__ __forceinline__ void set(const DraftAttnParams& p, int start, int end, int seq_len) {
+    first = start;
+    const int n_all = first < 0 ? 0 : min(end, p.rows) - first;
     n = max(min(n_all, kNodes), 0);
-    ctx = max(p.seq_lens[s] - max(n_all, 0), 0);
-    len = ctx + n;
+    ctx = min(max(seq_len - max(n_all, 0), 0), p.table_width << p.page_shift);
+    len = min(ctx + n, p.table_width << p.page_shift);   // what the table holds
     blocks = (n * p.G + kRows - 1) / kRows;
     tiles = n > 0 ? (len + kKeys - 1) / kKeys : 0;
   }
-  __device__ __forceinline__ int64_t work(const DraftAttnParams& p) const { return static_cast<int64_t>(tiles) * blocks * p.Hkv; }
+  __device__ __forceinline__ int work(const DraftAttnParams& p) const { return tiles * blocks * p.Hkv; }
 };
 
-// The CTA's items: its share of one unit each, tiles [t0, t1)
-struct Items {
+// The CTA's items: its share of one unit each, tiles [t0, t1). What the next sequence is to be made of is on its way while this one's items run.
+struct Items : Seq {
   const DraftAttnParams& p;
   int s;
-  int64_t off, left;                                     // in the sequence's work; tiles to come
-  int first, n, ctx, len, tiles, blocks, kvh, blk, t0, t1;
-  __device__ __forceinline__ Items(const DraftAttnParams& p_, int s_, int64_t off_, int64_t left_) : p(p_), s(s_), off(off_), left(left_) {}
+  int off, left;                                         // in the sequence's work; tiles to come
+  int kvh, blk, t0, t1;
+  int end, next_end, next_len;                           // q_start[s + 1], q_start[s + 2], seq_lens[s + 1]
+  __device__ __forceinline__ Items(const DraftAttnParams& p_, int s_, int off_, int left_) : p(p_), s(s_), off(off_), left(left_) {
+    end = p.q_start[s + 1];
+    set(p, p.q_start[s], end, p.seq_lens[s]);
+    ahead();
+  }
+  __device__ __forceinline__ void ahead() {
+    const int t = min(s + 1, p.num_seqs - 1);
+    next_end = p.q_start[t + 1];
+    next_len = p.seq_lens[t];
+  }
   __device__ __forceinline__ bool next() {
     if (left <= 0) return false;
-    for (;;) {                                           // the sequence that `off` lies in: there is one, as tiles are left
-      const Seq q(p, s);
-      if (off < q.work(p)) {
-        first = q.first; n = q.n; ctx = q.ctx; len = q.len; tiles = q.tiles; blocks = q.blocks;
-        break;
-      }
+    while (off >= work(p)) {                             // the sequence that `off` lies in: there is one, as tiles are left
       off = 0;
       if (++s >= p.num_seqs) {
         left = 0;
         return false;
       }
+      set(p, end, next_end, next_len);
+      end = next_end;
+      ahead();
     }
-    const int unit = static_cast<int>(off / tiles);
-    t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-    t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + left));
+    const int unit = off / tiles;
+    t0 = off - unit * tiles;
+    t1 = min(tiles, t0 + left);
     kvh = unit / blocks;
     blk = unit - kvh * blocks;
     off += t1 - t0;
@@ -170,26 +179,33 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
   uint64_t* empty = full + NS;                           // [NS] products -> copies
-  uint64_t* s_full = empty + NS;                         // [2 warpgroups][2] S of the warpgroup's k-th tile: barrier k % 2
-  uint64_t* p_full = s_full + 4;                         // [2] P of the CTA's tile g written (4 warps): barrier g % 2
-  uint64_t* o_full = p_full + 2;                         // [2 warpgroups] P V of the warpgroup's k-th tile is in O: phase k
-  uint64_t* o_free = o_full + 2;                         // [2 warpgroups] O of its item has been read (4 warps)
-  uint64_t* q_full = o_free + 2;                         // [2] queries of item i: barrier i % 2 (2 warps)
+  uint64_t* s_full = empty + NS;                         // [2] S of the CTA's tile g: barrier g % 2
+  uint64_t* p_full = s_full + 2;                         // [2] P of tile g written (4 warps)
+  uint64_t* pv_full = p_full + 2;                        // [2] P V of tile g is in O
+  uint64_t* o_free = pv_full + 2;                        // [2] O of item i has been read (4 warps): barrier i % 2
+  uint64_t* q_full = o_free + 2;                         // [2] queries of item i
   uint64_t* q_free = q_full + 2;                         // [2]
-  uint64_t* mma_end = q_free + 2;
+  uint64_t* m_set = q_free + 2;                          // [2 warpgroups][4 warps] references of tile g, by its warpgroup
+  uint64_t* l_set = m_set + 8;                           // [2 warpgroups][item % 2] its part of an item's sums, for the one with the last tile (4 warps)
+  uint64_t* mma_end = l_set + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   const WaitGuard guard{tmem_slot + 1, p.waits};
-  unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [2 warpgroups][2 items in turn]
+  unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [item % 4]
   int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // sequence and offset that the share begins at, tiles, all tiles
   int64_t* warp_work = begin + 4;                        // [12]
+  float* m_ref = reinterpret_cast<float*>(warp_work + 12);            // [128 rows] reference of the exponents
+  float* l_part = m_ref + kRows;                         // [item % 2][128 rows] sums of the warpgroup without an item's last tile
+  volatile uint32_t* filled = reinterpret_cast<uint32_t*>(l_part + 2 * kRows);   // [NS] copies into a stage
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); filled[i] = 0; }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[2 * i], 1); mbar_init(&s_full[2 * i + 1], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4);
-      mbar_init(&q_full[i], 2); mbar_init(&q_free[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_full[i], 1); mbar_init(&o_free[i], 4);
+      mbar_init(&l_set[2 * i], 4); mbar_init(&l_set[2 * i + 1], 4);
+      mbar_init(&q_full[i], 1); mbar_init(&q_free[i], 1);
       bad_nodes[2 * i] = bad_nodes[2 * i + 1] = 0ull;
+      for (int w = 0; w < 4; ++w) mbar_init(&m_set[4 * i + w], 1);
     }
     mbar_init(mma_end, 1);
     *guard.dead = 0;
@@ -205,7 +221,11 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   {
     const int per = (p.num_seqs + kThreads - 1) / kThreads, s0 = threadIdx.x * per, s1 = min(s0 + per, p.num_seqs);
     int64_t mine = 0;
-    for (int s = s0; s < s1; ++s) mine += Seq(p, s).work(p);
+    Seq q;
+    for (int s = s0; s < s1; ++s) {
+      q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
+      mine += q.work(p);
+    }
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -227,7 +247,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (x0 < x1 && x0 >= before && x0 < before + mine) {
       int s = s0;
       for (;; ++s) {
-        const int64_t w = Seq(p, s).work(p);
+        q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
+        const int w = q.work(p);
         if (x0 < before + w || s + 1 >= s1) break;
         before += w;
       }
@@ -241,52 +262,49 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Items it(p, static_cast<int>(begin[0]), begin[1], begin[2]);
+  Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
   const bool idle = begin[2] == 0;
 
   if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-    if (warp == 8 && !idle) {
-      // ------------------------------------------------------------------ copies
-      const int box = min(p.page_size, 64), boxes = kKeys / box, j = lane % boxes, sl = lane / boxes;
-      uint32_t pos = 0;
+    if ((warp == 8 || warp == 10) && !idle) {
+      // ------------------------------------------------------------------ copies: K by warp 8, V by warp 10
+      const bool is_v = warp == 10;
+      const CUtensorMap* map = is_v ? &tmap_v : &tmap_k;
+      const int box = 1 << min(p.page_shift, 6), boxes = kKeys / box, j = lane % boxes, sl = lane / boxes;
+      const int in_page = (1 << p.page_shift) - 1;
+      uint32_t g = 0;
       bool ok = true;
-      auto copy = [&](const CUtensorMap* map, int page, int kvh, int tile, int n) {
-        const uint32_t st = pos % NS;
-        ok = __all_sync(0xffffffffu, pos < NS || guard.wait<true>(&empty[st], ((pos / NS) & 1) ^ 1));
-        if (!ok) return;
-        if (lane == 0) mbar_expect_tx(&full[st], n * box * D * 2);
-        __syncwarp();
-        if (sl < D / 64 && j < n)
-          tma_load_3d(smem + SM::kRingOff + st * SM::kTileBytes + sl * (kKeys * 128) + j * box * 128, map, &full[st], 0,
-                      (tile * kKeys + j * box) % p.page_size, (page * p.Hkv + kvh) * (D / 64) + sl);
-        ++pos;
-      };
-      int v_page = 0, v_kvh = 0, v_tile = 0, v_n = 0;      // the tile whose V is to come (v_n: its boxes)
       while (ok && it.next()) {
         const int32_t* bt = p.table + it.s * p.table_ld;
-        const int last_page = min((it.len - 1) / p.page_size, p.table_width - 1);
-        auto page_of = [&](int tile) { return bt[min((tile * kKeys + j * box) / p.page_size, last_page)]; };
+        const int last_page = min((it.len - 1) >> p.page_shift, p.table_width - 1);
+        auto page_of = [&](int tile) { return bt[min((tile * kKeys + j * box) >> p.page_shift, last_page)]; };
         int page = page_of(it.t0);
-        for (int t = it.t0; t < it.t1 && ok; ++t) {
+        for (int t = it.t0; t < it.t1; ++t, ++g) {
           const int next = t + 1 < it.t1 ? page_of(t + 1) : 0;
           const int n = (((it.keys(t) + 15) & ~15) + box - 1) / box;   // boxes with a key that there is, in steps of the product with V
-          copy(&tmap_k, page, it.kvh, t, n);
-          if (ok && v_n > 0) copy(&tmap_v, v_page, v_kvh, v_tile, v_n);
-          v_page = page; v_kvh = it.kvh; v_tile = t; v_n = n;
+          // places in the ring: K0, K1, V0, K2, V1, ..., V of the last
+          const uint32_t pos = is_v ? (t + 1 < it.t1 || it.left > 0 ? 2 * g + 2 : 2 * g + 1) : g == 0 ? 0 : 2 * g - 1;
+          const uint32_t st = pos % NS;
+          ok = __all_sync(0xffffffffu, pos < NS || guard.wait<true>(&empty[st], ((pos / NS) & 1) ^ 1));
+          if (!ok) break;
+          if (lane == 0) {
+            filled[st] = pos / NS + 1;
+            mbar_expect_tx(&full[st], n * box * D * 2);
+          }
+          __syncwarp();
+          if (sl < D / 64 && j < n)
+            tma_load_3d(smem + SM::kRingOff + st * SM::kTileBytes + sl * (kKeys * 128) + j * box * 128, map, &full[st], 0,
+                        (t * kKeys + j * box) & in_page, (page * p.Hkv + it.kvh) * (D / 64) + sl);
           page = next;
         }
       }
-      if (ok && v_n > 0) copy(&tmap_v, v_page, v_kvh, v_tile, v_n);
-      for (uint32_t i = pos > NS ? pos - NS : 0; i < pos; ++i) guard.land(&full[i % NS], (i / NS) & 1);   // in flight
     } else if (warp == 9 && lane == 0 && !idle) {
       // ------------------------------------------------------------------ products
       constexpr uint32_t idesc_s = make_idesc_bf16(kRows, kKeys);
       constexpr uint32_t idesc_pv = make_idesc_bf16(kRows, D) | (1u << 16);
       uint32_t pos = 0, g = 0;                             // place in the ring, tile
-      uint32_t begun0 = 0, begun1 = 0;                     // tiles of the two warpgroups whose scores have been issued
       bool ok = true;
-      // S of the next tile of `it`, from the queries in buffer `buf` (of the item's parity, as its warpgroup is)
+      // S of tile `tile_no`, from the queries in buffer `buf`
       auto scores = [&](uint32_t tile_no, uint32_t buf, bool last) {
         const uint32_t st = pos % NS;
         ok = guard.wait<true>(&full[st], (pos / NS) & 1);
@@ -300,9 +318,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_bf16<1>(d_tmem, da + kk * 2, db + kk * 2, idesc_s, (kd | kk) != 0);
         }
-        uint32_t& begun = buf == 0 ? begun0 : begun1;
-        umma_commit(&s_full[2 * buf + (begun & 1)]);
-        ++begun;
+        umma_commit(&s_full[tile_no & 1]);
         umma_commit(&empty[st]);
         if (last) umma_commit(&q_free[buf]);
         ++pos;
@@ -332,13 +348,13 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (more) scores(g + 1, next & 1, t + 1 == it.t1);
         if (!ok) break;
         // P V of this one
-        const uint32_t wg = now & 1, st = pos % NS;
+        const uint32_t buf = now & 1, st = pos % NS;
         ok = guard.wait<true>(&full[st], (pos / NS) & 1) && guard.wait<true>(&p_full[g & 1], (g >> 1) & 1) &&
-             (!first_tile || now < 2 || guard.wait<true>(&o_free[wg], ((now >> 1) & 1) ^ 1));
+             (!first_tile || now < 2 || guard.wait<true>(&o_free[buf], ((now >> 1) & 1) ^ 1));
         if (!ok) break;
         tc_fence_after();
         const uint64_t dv = mn_major_desc(smem_u32(smem + SM::kRingOff + st * SM::kTileBytes));
-        const uint32_t o_tmem = tmem + SM::kTmemO + wg * D, p_tmem = tmem + (g & 1) * kKeys;
+        const uint32_t o_tmem = tmem + SM::kTmemO + buf * D, p_tmem = tmem + (g & 1) * kKeys;
         const uint32_t acc = first_tile ? 0u : 1u;
         if (keys == kKeys) {
 #pragma unroll
@@ -348,7 +364,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           for (int kk = 0; kk < (keys + 15) / 16; ++kk)
             umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
         }
-        umma_commit(&o_full[wg]);
+        umma_commit(&pv_full[g & 1]);
         umma_commit(&empty[st]);
         ++pos;
         ++g;
@@ -357,16 +373,19 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
       umma_commit(mma_end);                                // nothing is in flight when the columns are given back
       guard.land(mma_end, 0);
-    } else if (warp >= 10 && !idle) {
+    } else if (warp == 11 && !idle) {
       // ------------------------------------------------------------------ queries
       for (uint32_t item = 0; it.next(); ++item) {
         const uint32_t buf = item & 1;
         if (item >= 2 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1))) break;
         const int rows = it.block_rows();
         const uint32_t dst = smem_u32(smem + buf * SM::kQBytes);
-        for (int e = threadIdx.x - 320; e < rows * (D / 8); e += 64) {
-          const int r = e / (D / 8), c = e % (D / 8), at = it.blk * kRows + r, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
-          const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(head) * D + c * 8;
+        constexpr int kStep = 32 / (D / 8);                // rows of a round
+        const int c = lane % (D / 8);
+        int at = it.blk * kRows + lane / (D / 8), node = at / p.G, h = at - node * p.G;
+        for (int r = lane / (D / 8); r < rows; r += kStep) {
+          const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(it.kvh * p.G + h) * D + c * 8;
+          for (h += kStep; h >= p.G; h -= p.G) ++node;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
                        "l"(src) : "memory");
         }
@@ -377,12 +396,11 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    // ------------------------------------------------------------------ softmax: one row a thread
+    // ------------------------------------------------------------------ softmax: one row a thread, the CTA's tiles in turn
     const int wg = warp >> 2, row = threadIdx.x & 127;     // row == TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_o = tmem + SM::kTmemO + wg * D + lane_base;
-    uint32_t g = 0, done = 0;                              // tiles of the CTA; tiles of this warpgroup
+    const uint32_t t_s = tmem + wg * kKeys + lane_base;
+    uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
     bool cut_tail = false;
     // A wait that gives up leaves the warps in step: they go on with what is there, and every later wait ends at once
     auto await = [&](uint64_t* bar, uint32_t parity) {
@@ -393,62 +411,72 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     for (uint32_t item = 0; it.next(); ++item) {
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
       if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
-      if ((item & 1) != static_cast<uint32_t>(wg)) {
-        g += it.t1 - it.t0;
-        continue;
-      }
       const int rows = it.block_rows();
       const bool warp_ok = (warp & 3) * 32 < rows, row_ok = row < rows;
       const int at = it.blk * kRows + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
       const int64_t tok = it.first + (row_ok ? node : 0);
-      unsigned long long word = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;
-      if (it.n < kNodes) word &= (1ull << it.n) - 1;
-      float m_run = -INFINITY, l_run = 0.f;
-      unsigned long long* bad_here = bad_nodes + 2 * wg + ((item >> 1) & 1);
-      for (int t = it.t0; t < it.t1; ++t, ++g, ++done) {
-        const uint32_t t_s = tmem + (g & 1) * kKeys + lane_base;
+      const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
+      const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
+      unsigned long long* bad_here = bad_nodes + (item & 3);
+      const uint32_t t_o = tmem + SM::kTmemO + (item & 1) * D + lane_base;
+      float m_run = -INFINITY, l_run = 0.f;                // reference of this warpgroup's sum, the sum
+      float m_old = -INFINITY;                             // reference of the tile before this warpgroup's last
+      for (int t = it.t0; t < it.t1; ++t, ++g) {
+        if ((g & 1) != static_cast<uint32_t>(wg)) continue;
         const int key0 = t * kKeys;
-        await(&s_full[2 * wg + (done & 1)], (done >> 1) & 1);
-        bool free_o = done == 0;                           // the product of the warpgroup's tile before has ended
+        await(&s_full[wg], (g >> 1) & 1);
         const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
+        float mx = -INFINITY;
+        // 32 scores at a time, the next 32 on their way: a row of 128 in registers spills
+        float f[2][32];
+        auto load = [&](int c) { tmem_ld_32x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(f[c & 1])); };
+        auto mask = [&](int c) {
+          // bits of these keys: all of the context, then the row's word from its first node on
+          const unsigned long long word = word_all & nodes;
+          const int j0 = key0 + c * 32 - it.ctx;           // node of the first of 32 keys
+          const uint32_t bits = j0 >= 64 ? 0u
+                                : j0 >= 0 ? static_cast<uint32_t>(word >> j0)
+                                : j0 <= -32 ? 0xffffffffu : (static_cast<uint32_t>(word << -j0) | ((1u << -j0) - 1u));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((bits >> e) & 1u)) f[c & 1][e] = -INFINITY;
+        };
         if (warp_ok) {
-          float f[kKeys];
-          {
-            uint32_t v[kKeys / 32][32];
+          load(0);
+          tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(t_s + c * 32, v[c]);
-            tmem_ld_wait();
+          for (int c = 0; c < kKeys / 32; ++c) {
+            if (c + 1 < kKeys / 32) load(c + 1);
+            if (behind) mask(c);
+            float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e) f[e] = __uint_as_float(v[e / 32][e % 32]);
-          }
-          if (behind) {
-            // bits of this tile's keys: all of the context, then the row's word from its first node on
+            for (int e = 0; e < 32; e += 8) {
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) {
-              const int j0 = key0 + c * 32 - it.ctx;       // node of the first of 32 keys
-              const uint32_t bits = j0 >= 64 ? 0u
-                                    : j0 >= 0 ? static_cast<uint32_t>(word >> j0)
-                                    : j0 <= -32 ? 0xffffffffu : (static_cast<uint32_t>(word << -j0) | ((1u << -j0) - 1u));
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((bits >> e) & 1u)) f[c * 32 + e] = -INFINITY;
+              for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], fmaxf(f[c & 1][e + i], f[c & 1][e + 4 + i]));
             }
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            if (c + 1 < kKeys / 32) tmem_ld_wait();
           }
-          float m4[4] = {f[0], f[1], f[2], f[3]};
-#pragma unroll
-          for (int e = 4; e < kKeys; e += 8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], e + 4 < kKeys ? fmaxf(f[e + i], f[e + 4 + i]) : f[e + i]);
-          }
-          const float m_new = fmaxf(m_run, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2);
-          float alpha = 1.f;
-          if (m_new > m_run + kLazy) {
-            alpha = ex2(m_run - m_new);
-            m_run = m_new;
+          load(0);
+          mx *= p.scale_log2;
+        }
+        // The reference of both warpgroups: the other's of the tile before, raised where this tile's maximum is 2^8 over it
+        if (g > 0) await(&m_set[4 * (wg ^ 1) + (warp & 3)], ((g - 1) >> 1) & 1);
+        m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + row) : -INFINITY;
+        const float m_now = mx > m_old + kLazy ? mx : m_old;
+        *static_cast<volatile float*>(m_ref + row) = m_now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_set[4 * wg + (warp & 3)]);
+        if (warp_ok) {
+          const float alpha = m_now != m_old ? ex2(m_old - m_now) : 1.f;
+          if (m_now != m_run) {                            // this warpgroup's sum, from the reference of two tiles ago
+            l_run *= ex2(m_run - m_now);
+            m_run = m_now;
           }
           if (t > it.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            await(&o_full[wg], (done - 1) & 1);
-            free_o = true;
+            // O is free when the product before this tile's has ended. (S of this tile was formed behind the one before that: the phase
+            // before the awaited one has passed, the one behind it needs this tile's P.)
+            await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t v[16];
@@ -462,20 +490,24 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           const float m_use = m_run == -INFINITY ? 0.f : m_run;
           const uint64_t sc2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-m_use, -m_use);
           uint64_t sum2[2] = {0, 0};
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < kKeys; c += 32) {            // 32 keys: 16 columns of P
+          for (int c = 0; c < kKeys / 32; ++c) {           // 32 keys: 16 columns of P
+            if (c + 1 < kKeys / 32) load(c + 1);
+            if (behind) mask(c);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float2 x = unpair(fma_pair(pair(f[c + 2 * e], f[c + 2 * e + 1]), sc2, nm2));
+              const float2 x = unpair(fma_pair(pair(f[c & 1][2 * e], f[c & 1][2 * e + 1]), sc2, nm2));
               const float2 y = make_float2(ex2(x.x), ex2(x.y));
               sum2[e & 1] = add_pair(sum2[e & 1], pair(y.x, y.y));
               pk[e] = pack_bf16(y.x, y.y);                 // probabilities enter the product in bf16, the sum in fp32
             }
-            tmem_store16(t_s + c / 2, pk);
+            if (c + 1 < kKeys / 32) tmem_ld_wait();        // before P takes columns that are still to be read
+            tmem_store16(t_s + c * 16, pk);
           }
           const float2 sa = unpair(add_pair(sum2[0], sum2[1]));
-          l_run = l_run * alpha + (sa.x + sa.y);
+          l_run += sa.x + sa.y;
           tmem_store_wait();
         }
         if (behind) {
@@ -506,58 +538,77 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           fence_proxy_async_smem();
         }
-        if (!free_o) await(&o_full[wg], (done - 1) & 1);   // every phase is waited for, once: parities stay unambiguous
         tc_fence_before();                                 // P and the rescaled O are in TMEM, S has been read
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+        if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (t + 2 == it.t1) {                              // the item's last tile is the other warpgroup's
+          *static_cast<volatile float*>(l_part + (item & 1) * kRows + row) = l_run;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&l_set[2 * wg + (item & 1)]);
+        }
       }
-      // ---- results
-      await(&o_full[wg], (done - 1) & 1);
-      if (row == 0) bad_nodes[2 * wg + (((item >> 1) & 1) ^ 1)] = 0ull;   // the item before's, read by all (their P of this one is there)
-      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");         // bad_here of all four warps
+      if (((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
+      // ---- results, by the warpgroup that had the last tile; the other one goes on
+      await(&pv_full[wg], ((g - 1) >> 1) & 1);
+      if (it.t1 - it.t0 > 1) {
+        // Of an item of this parity: the other one may have set that of the next item already, should that have two tiles
+        await(&l_set[2 * (wg ^ 1) + (item & 1)], (sums >> (item & 1)) & 1);
+        sums ^= 1u << (item & 1);
+        // the other's reference is that of the tile before the last
+        l_run += *static_cast<volatile float*>(l_part + (item & 1) * kRows + row) * (m_old == m_run ? 1.f : ex2(m_old - m_run));
+      }
+      // The words are two items old when they are used again: the other warpgroup is at the next item's first tile at most
+      if (row == 0) bad_nodes[(item + 2) & 3] = 0ull;
+      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");         // bad_here of all four warps (the other warpgroup's: l_set)
       else asm volatile("bar.sync 2, 128;" ::: "memory");
-      const unsigned long long bad = *static_cast<volatile unsigned long long*>(bad_here) & word;
+      const unsigned long long bad = *static_cast<volatile unsigned long long*>(bad_here) & word_all & nodes;
       if (warp_ok) {
-        const float inv = cut ? 1.f : l_run > 0.f ? 1.f / l_run : 0.f;
+        const float inv = cut ? 1.f : l_run > 0.f ? __frcp_rn(l_run) : 0.f;
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         __nv_bfloat16* op = p.out + (tok * p.Hq + head) * D;
-        float4* po = p.part_o + static_cast<size_t>(slot) * (D / 4) * kRows + row;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32(t_o + c, v);
-          tmem_ld_wait();
-          float x[32];
+        uint4* po = reinterpret_cast<uint4*>(p.part_o) + static_cast<size_t>(slot) * (D / 4) * kRows + row;
+        uint32_t v[2][32];
+        tmem_ld_32x32(t_o, v[0]);
+        tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(v[e]) * inv;
-          if (row_ok) {
-            for (unsigned long long b = bad; b != 0ull; b &= b - 1) {   // seen values that are no numbers
-              const int place = it.ctx + __ffsll(static_cast<long long>(b)) - 1;
-              const int64_t page = p.table[it.s * p.table_ld + min(place / p.page_size, p.table_width - 1)];
-              if (page < 0 || page >= p.pages) continue;
-              const __nv_bfloat16* vr = p.v + (((page * p.Hkv + it.kvh) * (D / 64) + c / 64) * p.page_size + place % p.page_size) * 64 + c % 64;
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t(&x)[32] = v[c & 1];
+          if (c + 1 < D / 32) tmem_ld_32x32(t_o + (c + 1) * 32, v[(c + 1) & 1]);
+          for (unsigned long long b = bad; b != 0ull; b &= b - 1) {   // seen values that are no numbers
+            const int place = it.ctx + __ffsll(static_cast<long long>(b)) - 1;
+            const int64_t page = p.table[it.s * p.table_ld + min(place >> p.page_shift, p.table_width - 1)];
+            if (page < 0 || page >= p.pages) continue;
+            const __nv_bfloat16* vr =
+                p.v + ((((page * p.Hkv + it.kvh) * (D / 64) + c / 2) << p.page_shift) + (place & ((1 << p.page_shift) - 1))) * 64 + (c & 1) * 32;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float y = __bfloat162float(vr[e]);
-                if (!(fabsf(y) < INFINITY)) x[e] += y;
-              }
+            for (int e = 0; e < 32; ++e) {
+              const float y = __bfloat162float(vr[e]);
+              if (!(fabsf(y) < INFINITY)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
             }
+          }
+          if (row_ok) {
             if (cut) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) po[(c / 4 + e) * kRows] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+              for (int e = 0; e < 8; ++e) po[(c * 8 + e) * kRows] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 uint4 w;
-                w.x = pack_bf16(x[8 * e], x[8 * e + 1]);
-                w.y = pack_bf16(x[8 * e + 2], x[8 * e + 3]);
-                w.z = pack_bf16(x[8 * e + 4], x[8 * e + 5]);
-                w.w = pack_bf16(x[8 * e + 6], x[8 * e + 7]);
-                *reinterpret_cast<uint4*>(op + c + e * 8) = w;
+                w.x = pack_bf16(__uint_as_float(x[8 * e]) * inv, __uint_as_float(x[8 * e + 1]) * inv);
+                w.y = pack_bf16(__uint_as_float(x[8 * e + 2]) * inv, __uint_as_float(x[8 * e + 3]) * inv);
+                w.z = pack_bf16(__uint_as_float(x[8 * e + 4]) * inv, __uint_as_float(x[8 * e + 5]) * inv);
+                w.w = pack_bf16(__uint_as_float(x[8 * e + 6]) * inv, __uint_as_float(x[8 * e + 7]) * inv);
+                *reinterpret_cast<uint4*>(op + c * 32 + e * 8) = w;
               }
             }
           }
           __syncwarp();
+          if (c + 1 < D / 32) tmem_ld_wait();
+          if (c + 2 == D / 32) {                           // O has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[item & 1]);
+          }
         }
         if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * kRows + row] = make_float2(m_run, l_run);
         if (cut && it.t0 == 0 && row == 0) {
@@ -568,15 +619,16 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           p.cut[2 * blockIdx.x] = make_int4(last, it.first, it.kvh, it.blk);
           p.cut[2 * blockIdx.x + 1] = make_int4(rows, 0, 0, 0);
         }
+      } else if (lane == 0) {
+        mbar_arrive(&o_free[item & 1]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[wg]);
     }
     if (threadIdx.x == 0 && !cut_tail) p.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);   // no unit begins here that ends elsewhere
   }
   tc_fence_before();
   __syncthreads();
+  // copies that nobody waited for, because a wait gave up, land before the CTA ends
+  if (threadIdx.x < NS && guard.gave_up() && filled[threadIdx.x] != 0) guard.land(&full[threadIdx.x], (filled[threadIdx.x] - 1) & 1);
   if (warp == 9) {
     __syncwarp();
     tc_fence_after();
@@ -664,7 +716,7 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
                                      const void* seen, int num_seqs, int rows, int max_nodes, int Hq, int Hkv, int D, int page_size,
                                      float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (num_seqs <= 0 || rows <= 0 || max_nodes <= 0) return 0;
-  if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || page_size < 8 || kKeys % page_size || pages <= 0 || table_width <= 0 || ctas <= 0 ||
+  if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || page_size < 8 || kKeys % page_size || (page_size & (page_size - 1)) || pages <= 0 || table_width <= 0 || ctas <= 0 ||
       q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
       scratch_bytes < gllm_draft_attention_scratch(D, ctas))
     return 1;
@@ -679,7 +731,8 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
   p.seq_lens = reinterpret_cast<const int32_t*>(seq_lens);
   p.q_start = reinterpret_cast<const int32_t*>(q_start);
   p.seen = reinterpret_cast<const int64_t*>(seen);
-  p.num_seqs = num_seqs; p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.page_size = page_size;
+  p.num_seqs = num_seqs; p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
+  p.page_shift = 31 - __builtin_clz(static_cast<unsigned>(page_size));
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part_o = reinterpret_cast<float4*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(2) * ctas * (D / 4) * kRows);

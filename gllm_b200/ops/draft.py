@@ -29,7 +29,8 @@ that are not over 0 (NaN among them) have no mass, and a token outside of the vo
 """
 from __future__ import annotations
 
-from typing import Optional
+import functools
+import operator
 
 import torch
 
@@ -40,101 +41,122 @@ PAGE_SIZES = (8, 16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 
 
-# -- checks, the same on either device -------------------------------------------------------------------------------------
+# -- checks, the same on either device. What a common call passes comes first: a step makes one call a layer ---------------------
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+
+
 def num_seqs(inp) -> int:
     return getattr(inp, "padded_tokens", 0) or inp.num_seqs
 
 
 def _index(t, what: str, n: int, dims: int = 1):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    if isinstance(t, torch.Tensor) and t.dtype is _I32 and t.dim() == dims and t.shape[0] >= n and (t.is_contiguous() or t.stride(-1) == 1):
+        return t
+    if not isinstance(t, torch.Tensor) or t.dtype != _I32 or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what}: int32 with contiguous rows, {dims}-dimensional")
     if t.shape[0] < n:
         raise ValueError(f"{what}: {t.shape[0]} entries for {n}")
+    return t
 
 
-def check_batch(inp, lens: bool = True) -> int:
-    """The number of sequences."""
+def _starts(inp):
     b = num_seqs(inp)
     if inp.max_q_len > MOST_NODES:
         raise ValueError(f"a sequence has at most {MOST_NODES} drafted nodes: got {inp.max_q_len}")
-    _index(inp.query_start_loc, "query_start_loc", b + 1)
-    if lens:
-        _index(inp.seq_lens, "seq_lens", b)
-        _index(inp.block_table, "block_table", b, 2)
-    return b
+    return b, _index(inp.query_start_loc, "query_start_loc", b + 1)
 
 
-def check_plan(parents, inp, page_size) -> int:
-    b = check_batch(inp)
+def check_batch(inp):
+    """(sequences, query_start_loc, seq_lens, block_table): each looked up once, since an engine's batch makes a view of it."""
+    b, start = _starts(inp)
+    return b, start, _index(inp.seq_lens, "seq_lens", b), _index(inp.block_table, "block_table", b, 2)
+
+
+def check_plan(parents, inp, page_size):
     _index(parents, "parents", 0)
     if page_size < 1:
         raise ValueError(f"pages of {page_size} tokens")
-    return b
+    return check_batch(inp)
 
 
-def check_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out) -> int:
-    b = check_batch(inp)
-    for c in (k_cache, v_cache):
-        if kv4.held(c):
-            raise ValueError("drafted tokens are attended over bf16 caches, not over one held in 4 bits")
-    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.dtype != q.dtype:
-        raise ValueError(f"caches [pages, heads, slabs, page, slab] of the queries' type: got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}, "
+def check_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out):
+    batch = check_batch(inp)
+    if kv4.held(k_cache) or kv4.held(v_cache):
+        raise ValueError("drafted tokens are attended over bf16 caches, not over one held in 4 bits")
+    shape = k_cache.shape
+    if len(shape) != 5 or v_cache.shape != shape or not k_cache.dtype is v_cache.dtype is q.dtype:
+        raise ValueError(f"caches [pages, heads, slabs, page, slab] of the queries' type: got {tuple(shape)}, {tuple(v_cache.shape)}, "
                          f"{k_cache.dtype}, {v_cache.dtype}, {q.dtype}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches are contiguous")
-    _, hkv, slabs, _, w = k_cache.shape
-    if slabs * w != head_dim or num_q_heads % hkv or q.dim() != 2 or q.shape[1] < num_q_heads * head_dim or q.stride(1) != 1:
+    _, hkv, slabs, _, w = shape
+    rows, width = q.shape if q.dim() == 2 else (0, -1)
+    if slabs * w != head_dim or num_q_heads % hkv or width < num_q_heads * head_dim or q.stride(1) != 1:
         raise ValueError(f"queries {tuple(q.shape)} of {num_q_heads} heads of {head_dim} over {hkv} heads of {slabs * w}")
-    if seen.dtype != torch.int64 or seen.dim() != 1 or seen.shape[0] < q.shape[0] or (seen.shape[0] > 1 and seen.stride(0) != 1):
+    if seen.dtype is not _I64 or seen.dim() != 1 or seen.shape[0] < rows or not seen.is_contiguous():
         raise ValueError("seen: int64, contiguous, a word for each row of q")
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"a scale over 0: got {scale}")
-    if out is not None and (out.dtype != q.dtype or out.shape != (q.shape[0], num_q_heads * head_dim) or not out.is_contiguous()):
+    if out is not None and (out.dtype != q.dtype or out.shape != (rows, num_q_heads * head_dim) or not out.is_contiguous()):
         raise ValueError("out: contiguous, [rows of q, heads * dim], of its type")
-    return b
+    return batch
 
 
-def check_verify(tokens, parents, inp, target, draft, uniform) -> int:
-    b = check_batch(inp, lens=False)
-    t = tokens.shape[0]
-    _index(tokens, "tokens", 0)
+def check_verify(tokens, parents, inp, target, draft, uniform):
+    """(sequences, query_start_loc, whether the target's tokens are given)"""
+    b, start = _starts(inp)
+    t = _index(tokens, "tokens", 0).shape[0]
     _index(parents, "parents", t)
-    if not target.is_floating_point():
+    if target.dtype is not _F32 and not target.is_floating_point():
         _index(target, "target tokens", t)
         if draft is not None or uniform is not None:
             raise ValueError("target tokens are compared: no draft probabilities and no random numbers go with them")
-        return b
+        return b, start, True
     for x, what in ((target, "target"), (draft, "draft")):
-        if x is not None and (x.dtype != torch.float32 or x.dim() != 2 or x.shape[0] < t or (x.stride(1) != 1 and x.shape[1] > 1)):
+        if x is not None and (x.dtype is not _F32 or x.dim() != 2 or x.shape[0] < t or (x.stride(1) != 1 and x.shape[1] > 1)):
             raise ValueError(f"{what}: fp32 probabilities [rows, vocabulary], rows contiguous")
     if target.shape[1] < 1 or (draft is not None and draft.shape[1] != target.shape[1]):
         raise ValueError("target and draft are over one vocabulary")
-    if uniform is None or uniform.dtype != torch.float32 or uniform.dim() != 1 or uniform.shape[0] < t or (t > 1 and uniform.stride(0) != 1):
+    if uniform is None or uniform.dtype is not _F32 or uniform.dim() != 1 or uniform.shape[0] < t or not uniform.is_contiguous():
         raise ValueError("uniform: fp32 in [0, 1), one for each row")
-    return b
+    return b, start, False
 
 
-def cache_list(k_caches, v_caches):
-    """The tensors of all layers, each once (layers may share one; None: a layer without)."""
-    seen, out = set(), []
-    for c in (*([k_caches] if isinstance(k_caches, torch.Tensor) else k_caches), *([v_caches] if isinstance(v_caches, torch.Tensor) else v_caches or ())):
-        if c is None:
-            continue
+_shape_of, _dtype_of = operator.attrgetter("shape"), operator.attrgetter("dtype")
+
+
+def cache_groups(k_caches, v_caches):
+    """[(shape, bytes of an element, addresses, tensors)]: the tensors of all layers by shape, each once (layers may share one; None: a
+    layer without)."""
+    caches = [c for c in (*k_caches, *(v_caches or ())) if c is not None]
+    if not caches:
+        return []
+    shape, dtype, n = caches[0].shape, caches[0].dtype, len(caches)
+    at = list(map(torch.Tensor.data_ptr, caches))
+    size = caches[0].element_size()
+    if len(shape) == 5 and dtype is not torch.uint8 and shape[4] * size % 16 == 0 and all(map(torch.Tensor.is_contiguous, caches)) and \
+            list(map(_shape_of, caches)).count(shape) == n and list(map(_dtype_of, caches)).count(dtype) == n and len(set(at)) == n and \
+            functools.reduce(operator.or_, at) % 16 == 0:
+        return [(shape, size, at, caches)]
+    groups, seen = {}, set()
+    for c, a in zip(caches, at):
         if kv4.held(c):
             raise ValueError("rows of a cache held in 4 bits are not moved")
-        if c.dim() != 5 or not c.is_contiguous() or c.shape[4] * c.element_size() % 16 or c.data_ptr() % 16:
+        if c.dim() != 5 or not c.is_contiguous() or c.shape[4] * c.element_size() % 16 or a % 16:
             raise ValueError(f"caches [pages, heads, slabs, page, slab], contiguous, slabs of whole 16-byte words: got {tuple(c.shape)} {c.dtype}")
-        if c.data_ptr() not in seen or c.numel() == 0:
-            seen.add(c.data_ptr())
-            out.append(c)
-    return out
+        if a not in seen and c.numel():
+            seen.add(a)
+            _, _, some, tensors = groups.setdefault((c.shape, c.element_size()), (c.shape, c.element_size(), [], []))
+            some.append(a)
+            tensors.append(c)
+    return list(groups.values())
 
 
-def check_keep(inp, path, count) -> int:
-    b = check_batch(inp)
+def check_keep(inp, path, count):
+    batch = check_batch(inp)
     _index(path, "path", 0)
-    _index(count, "count", b)
-    return b
+    _index(count, "count", batch[0])
+    return batch
 
 
 # -- plain form ------------------------------------------------------------------------------------------------------------
@@ -244,13 +266,13 @@ def _draw(rest, u: float) -> int:
 
 
 def keep(k_caches, v_caches, inp, path, count):
-    b = check_keep(inp, path, count)
+    check_keep(inp, path, count)
     table, lens, way, taken = inp.block_table, inp.seq_lens.tolist(), path.tolist(), count.tolist()
     moves = []
     for s, a, n in _sequences(inp, path.shape[0]):
         ctx = max(lens[s] - n, 0)
         moves += [(s, ctx + way[a + j], ctx + j) for j in range(1, min(taken[s], n, MOST_NODES)) if j < way[a + j] < min(n, MOST_NODES)]
-    for c in cache_list(k_caches, v_caches):
+    for c in (c for group in cache_groups(k_caches, v_caches) for c in group[3]):
         pages, page = c.shape[0], c.shape[3]
         places = []
         for s, old, new in moves:
