@@ -42,6 +42,7 @@ struct DraftAttnParams {
   const int32_t* q_start;
   const int64_t* seen;
   int table_width, num_seqs, rows, Hq, Hkv, G, page_shift;   // a page has 2^page_shift tokens
+  int block_rows;
   float scale_log2;
   float4* part_o;                                        // [2 CTA][D / 4][128 rows]
   float2* part_ml;                                       // [2 CTA][128 rows]: reference of the exponents, sum
@@ -113,6 +114,7 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 }
 
 // What a sequence is to the units: rows [first, first + n) of the batch, ctx tokens before its nodes
+template <int BR>
 struct Seq {
   int first, n, ctx, len, tiles, blocks;
   __device__ __forceinline__ void set(const DraftAttnParams& p, int start, int end, int seq_len) {
@@ -121,14 +123,21 @@ struct Seq {
     n = max(min(n_all, kNodes), 0);
     ctx = min(max(seq_len - max(n_all, 0), 0), p.table_width << p.page_shift);
     len = min(ctx + n, p.table_width << p.page_shift);   // what the table holds
-    blocks = (n * p.G + kRows - 1) / kRows;
+    blocks = (n * p.G + BR - 1) / BR;
     tiles = n > 0 ? (len + kKeys - 1) / kKeys : 0;
   }
   __device__ __forceinline__ int work(const DraftAttnParams& p) const { return tiles * blocks * p.Hkv; }
 };
 
 // The CTA's items: its share of one unit each, tiles [t0, t1). What the next sequence is to be made of is on its way while this one's items run.
-struct Items : Seq {
+template <int BR>
+struct Items : Seq<BR> {
+  using Seq<BR>::first;
+  using Seq<BR>::n;
+  using Seq<BR>::ctx;
+  using Seq<BR>::len;
+  using Seq<BR>::tiles;
+  using Seq<BR>::blocks;
   const DraftAttnParams& p;
   int s;
   int off, left;                                         // in the sequence's work; tiles to come
@@ -136,7 +145,7 @@ struct Items : Seq {
   int end, next_end, next_len;                           // q_start[s + 1], q_start[s + 2], seq_lens[s + 1]
   __device__ __forceinline__ Items(const DraftAttnParams& p_, int s_, int off_, int left_) : p(p_), s(s_), off(off_), left(left_) {
     end = p.q_start[s + 1];
-    set(p, p.q_start[s], end, p.seq_lens[s]);
+    this->set(p, p.q_start[s], end, p.seq_lens[s]);
     ahead();
   }
   __device__ __forceinline__ void ahead() {
@@ -146,13 +155,13 @@ struct Items : Seq {
   }
   __device__ __forceinline__ bool next() {
     if (left <= 0) return false;
-    while (off >= work(p)) {                             // the sequence that `off` lies in: there is one, as tiles are left
+    while (off >= this->work(p)) {                             // the sequence that `off` lies in: there is one, as tiles are left
       off = 0;
       if (++s >= p.num_seqs) {
         left = 0;
         return false;
       }
-      set(p, end, next_end, next_len);
+      this->set(p, end, next_end, next_len);
       end = next_end;
       ahead();
     }
@@ -165,16 +174,18 @@ struct Items : Seq {
     left -= t1 - t0;
     return true;
   }
-  __device__ __forceinline__ int block_rows() const { return min(kRows, n * p.G - blk * kRows); }
+  __device__ __forceinline__ int block_rows() const { return min(BR, n * p.G - blk * BR); }
   // keys of tile t that there are
   __device__ __forceinline__ int keys(int t) const { return min(len - t * kKeys, kKeys); }
 };
 
-template <int D>
+template <int D, int REP>
 __global__ void __launch_bounds__(kThreads, 1)
 draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DraftAttnParams p) {
   using SM = DraftSmem<D>;
   constexpr int NS = SM::kStages;
+  constexpr int BR = kRows / REP;                        // rows of a block: TMEM lane = part of the keys x BR + row
+  constexpr int kChunks = kKeys / 32 / REP;              // of 32 keys that a lane has of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
@@ -203,7 +214,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_full[i], 1); mbar_init(&o_free[i], 4);
       mbar_init(&l_set[2 * i], 4); mbar_init(&l_set[2 * i + 1], 4);
-      mbar_init(&q_full[i], 1); mbar_init(&q_free[i], 1);
+      mbar_init(&q_full[i], 1); mbar_init(&q_free[i], REP > 1 ? 2 : 1);
       bad_nodes[2 * i] = bad_nodes[2 * i + 1] = 0ull;
       for (int w = 0; w < 4; ++w) mbar_init(&m_set[4 * i + w], 1);
     }
@@ -221,7 +232,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   {
     const int per = (p.num_seqs + kThreads - 1) / kThreads, s0 = threadIdx.x * per, s1 = min(s0 + per, p.num_seqs);
     int64_t mine = 0;
-    Seq q;
+    Seq<BR> q;
     for (int s = s0; s < s1; ++s) {
       q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
       mine += q.work(p);
@@ -262,7 +273,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
+  Items<BR> it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
   const bool idle = begin[2] == 0;
 
   if (warp >= kSoftmaxWarps) {
@@ -382,12 +393,16 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const uint32_t dst = smem_u32(smem + buf * SM::kQBytes);
         constexpr int kStep = 32 / (D / 8);                // rows of a round
         const int c = lane % (D / 8);
-        int at = it.blk * kRows + lane / (D / 8), node = at / p.G, h = at - node * p.G;
+        int at = it.blk * BR + lane / (D / 8), node = at / p.G, h = at - node * p.G;
         for (int r = lane / (D / 8); r < rows; r += kStep) {
           const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(it.kvh * p.G + h) * D + c * 8;
           for (h += kStep; h >= p.G; h -= p.G) ++node;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                       "l"(src) : "memory");
+#pragma unroll
+          for (int part = 0; part < REP; ++part) {
+            const int l = part * BR + r;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (c >> 3) * (kRows * 128) + l * 128 + (((c & 7) ^ (l & 7)) << 4)),
+                         "l"(src) : "memory");
+          }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -397,7 +412,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
   } else {
     // ------------------------------------------------------------------ softmax: one row a thread, the CTA's tiles in turn
-    const int wg = warp >> 2, row = threadIdx.x & 127;     // row == TMEM lane
+    const int wg = warp >> 2, tl = threadIdx.x & 127;      // TMEM lane
+    const int row = tl % BR, part = REP == 1 ? 0 : (warp & 3) / (4 / REP);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + wg * kKeys + lane_base;
     uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
@@ -408,12 +424,16 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       __syncwarp();
       tc_fence_after();
     };
+    auto sync_group = [&] {
+      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+      else asm volatile("bar.sync 2, 128;" ::: "memory");
+    };
     for (uint32_t item = 0; it.next(); ++item) {
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
       if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
       const int rows = it.block_rows();
-      const bool warp_ok = (warp & 3) * 32 < rows, row_ok = row < rows;
-      const int at = it.blk * kRows + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
+      const bool warp_ok = (warp & 3) % (4 / REP) * 32 < rows, row_ok = row < rows;
+      const int at = it.blk * BR + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
       const int64_t tok = it.first + (row_ok ? node : 0);
       const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
       const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
@@ -427,44 +447,48 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         await(&s_full[wg], (g >> 1) & 1);
         const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
         float mx = -INFINITY;
-        // 32 scores at a time, the next 32 on their way: a row of 128 in registers spills
-        float f[2][32];
-        auto load = [&](int c) { tmem_ld_32x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(f[c & 1])); };
-        auto mask = [&](int c) {
-          // bits of these keys: all of the context, then the row's word from its first node on
-          const unsigned long long word = word_all & nodes;
-          const int j0 = key0 + c * 32 - it.ctx;           // node of the first of 32 keys
-          const uint32_t bits = j0 >= 64 ? 0u
-                                : j0 >= 0 ? static_cast<uint32_t>(word >> j0)
-                                : j0 <= -32 ? 0xffffffffu : (static_cast<uint32_t>(word << -j0) | ((1u << -j0) - 1u));
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1u)) f[c & 1][e] = -INFINITY;
+        // 32 scores at a time in loops that are not unrolled: the warps are at different places of the code, and what is not in the instruction
+        // caches costs some five cycles an instruction (and a row of 128 in registers spills)
+        float f[32];
+        auto load = [&](int c) {
+          tmem_ld_32x32(t_s + (part * kChunks + c) * 32, reinterpret_cast<uint32_t(&)[32]>(f));
+          tmem_ld_wait();
         };
         if (warp_ok) {
-          load(0);
-          tmem_ld_wait();
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {
+            load(c);
+            if (behind) {
+              // bits of these keys: all of the context, then the row's word from its first node on
+              const unsigned long long word = word_all & nodes;
+              const int j0 = key0 + (part * kChunks + c) * 32 - it.ctx;   // node of the first of 32 keys
+              const uint32_t bits = j0 >= 64 ? 0u
+                                    : j0 >= 0 ? static_cast<uint32_t>(word >> j0)
+                                    : j0 <= -32 ? 0xffffffffu : (static_cast<uint32_t>(word << -j0) | ((1u << -j0) - 1u));
 #pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) {
-            if (c + 1 < kKeys / 32) load(c + 1);
-            if (behind) mask(c);
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) f[e] = -INFINITY;
+              if (kChunks > 1) {                           // read once more below
+                tmem_store16(t_s + (part * kChunks + c) * 32, *reinterpret_cast<uint32_t(*)[16]>(f));
+                tmem_store16(t_s + (part * kChunks + c) * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(f + 16));
+              }
+            }
             float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], fmaxf(f[c & 1][e + i], f[c & 1][e + 4 + i]));
+              for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], fmaxf(f[e + i], f[e + 4 + i]));
             }
             mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            if (c + 1 < kKeys / 32) tmem_ld_wait();
           }
-          load(0);
+          if (kChunks > 1 && behind) tmem_store_wait();
           mx *= p.scale_log2;
         }
         // The reference of both warpgroups: the other's of the tile before, raised where this tile's maximum is 2^8 over it
         if (g > 0) await(&m_set[4 * (wg ^ 1) + (warp & 3)], ((g - 1) >> 1) & 1);
-        m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + row) : -INFINITY;
+        m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + tl) : -INFINITY;
         const float m_now = mx > m_old + kLazy ? mx : m_old;
-        *static_cast<volatile float*>(m_ref + row) = m_now;
+        *static_cast<volatile float*>(m_ref + tl) = m_now;
         __syncwarp();
         if (lane == 0) mbar_arrive(&m_set[4 * wg + (warp & 3)]);
         if (warp_ok) {
@@ -490,21 +514,26 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           const float m_use = m_run == -INFINITY ? 0.f : m_run;
           const uint64_t sc2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-m_use, -m_use);
           uint64_t sum2[2] = {0, 0};
-          tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) {           // 32 keys: 16 columns of P
-            if (c + 1 < kKeys / 32) load(c + 1);
-            if (behind) mask(c);
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {              // 32 keys: 16 columns of P, which never reach scores that are still to be read
+            if (kChunks > 1) load(c);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float2 x = unpair(fma_pair(pair(f[c & 1][2 * e], f[c & 1][2 * e + 1]), sc2, nm2));
+              const float2 x = unpair(fma_pair(pair(f[2 * e], f[2 * e + 1]), sc2, nm2));
               const float2 y = make_float2(ex2(x.x), ex2(x.y));
               sum2[e & 1] = add_pair(sum2[e & 1], pair(y.x, y.y));
               pk[e] = pack_bf16(y.x, y.y);                 // probabilities enter the product in bf16, the sum in fp32
             }
-            if (c + 1 < kKeys / 32) tmem_ld_wait();        // before P takes columns that are still to be read
-            tmem_store16(t_s + c * 16, pk);
+            tmem_store16(t_s + (part * kChunks + c) * 16, pk);
+          }
+          if (REP > 1) {                                   // the keys that other lanes have of this row
+            uint32_t none[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) none[e] = 0u;
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c)
+              if (c / kChunks != part) tmem_store16(t_s + c * 16, none);
           }
           const float2 sa = unpair(add_pair(sum2[0], sum2[1]));
           l_run += sa.x + sa.y;
@@ -542,7 +571,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
         if (t + 2 == it.t1) {                              // the item's last tile is the other warpgroup's
-          *static_cast<volatile float*>(l_part + (item & 1) * kRows + row) = l_run;
+          *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) = l_run;
           __syncwarp();
           if (lane == 0) mbar_arrive(&l_set[2 * wg + (item & 1)]);
         }
@@ -555,25 +584,39 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         await(&l_set[2 * (wg ^ 1) + (item & 1)], (sums >> (item & 1)) & 1);
         sums ^= 1u << (item & 1);
         // the other's reference is that of the tile before the last
-        l_run += *static_cast<volatile float*>(l_part + (item & 1) * kRows + row) * (m_old == m_run ? 1.f : ex2(m_old - m_run));
+        l_run += *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) * (m_old == m_run ? 1.f : ex2(m_old - m_run));
       }
       // The words are two items old when they are used again: the other warpgroup is at the next item's first tile at most
-      if (row == 0) bad_nodes[(item + 2) & 3] = 0ull;
-      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");         // bad_here of all four warps (the other warpgroup's: l_set)
-      else asm volatile("bar.sync 2, 128;" ::: "memory");
+      if (tl == 0) bad_nodes[(item + 2) & 3] = 0ull;
+      // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
+      float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
+      if (REP > 1) lanes[tl] = make_float2(m_run, l_run);
+      sync_group();                                        // and bad_here of all four warps (the other warpgroup's: l_set)
+      float weight = 1.f;
+      if (REP > 1) {
+        float2 o[REP];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < REP; ++i) {
+          o[i] = lanes[i * BR + row];
+          top = fmaxf(top, o[i].x);
+        }
+        if (top != -INFINITY) {
+#pragma unroll
+          for (int i = 0; i < REP; ++i) sum += o[i].y * ex2(o[i].x - top);
+          weight = ex2(m_run - top);
+        }
+        m_run = top;
+        l_run = sum;
+      }
       const unsigned long long bad = *static_cast<volatile unsigned long long*>(bad_here) & word_all & nodes;
-      if (warp_ok) {
-        const float inv = cut ? 1.f : l_run > 0.f ? __frcp_rn(l_run) : 0.f;
+      {
+        const float inv = weight * (cut ? 1.f : l_run > 0.f ? __frcp_rn(l_run) : 0.f);
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         __nv_bfloat16* op = p.out + (tok * p.Hq + head) * D;
         uint4* po = reinterpret_cast<uint4*>(p.part_o) + static_cast<size_t>(slot) * (D / 4) * kRows + row;
-        uint32_t v[2][32];
-        tmem_ld_32x32(t_o, v[0]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t(&x)[32] = v[c & 1];
-          if (c + 1 < D / 32) tmem_ld_32x32(t_o + (c + 1) * 32, v[(c + 1) & 1]);
+        // 32 finished columns from column 32 c on
+        auto put = [&](int c, uint32_t(&x)[32]) {
           for (unsigned long long b = bad; b != 0ull; b &= b - 1) {   // seen values that are no numbers
             const int place = it.ctx + __ffsll(static_cast<long long>(b)) - 1;
             const int64_t page = p.table[it.s * p.table_ld + min(place >> p.page_shift, p.table_width - 1)];
@@ -586,32 +629,87 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
               if (!(fabsf(y) < INFINITY)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
             }
           }
-          if (row_ok) {
-            if (cut) {
+          if (!row_ok) return;
+          if (cut) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) po[(c * 8 + e) * kRows] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-            } else {
+            for (int e = 0; e < 8; ++e) po[(c * 8 + e) * kRows] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+          } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint4 w;
-                w.x = pack_bf16(__uint_as_float(x[8 * e]) * inv, __uint_as_float(x[8 * e + 1]) * inv);
-                w.y = pack_bf16(__uint_as_float(x[8 * e + 2]) * inv, __uint_as_float(x[8 * e + 3]) * inv);
-                w.z = pack_bf16(__uint_as_float(x[8 * e + 4]) * inv, __uint_as_float(x[8 * e + 5]) * inv);
-                w.w = pack_bf16(__uint_as_float(x[8 * e + 6]) * inv, __uint_as_float(x[8 * e + 7]) * inv);
-                *reinterpret_cast<uint4*>(op + c * 32 + e * 8) = w;
-              }
+            for (int e = 0; e < 4; ++e) {
+              uint4 w;
+              w.x = pack_bf16(__uint_as_float(x[8 * e]), __uint_as_float(x[8 * e + 1]));
+              w.y = pack_bf16(__uint_as_float(x[8 * e + 2]), __uint_as_float(x[8 * e + 3]));
+              w.z = pack_bf16(__uint_as_float(x[8 * e + 4]), __uint_as_float(x[8 * e + 5]));
+              w.w = pack_bf16(__uint_as_float(x[8 * e + 6]), __uint_as_float(x[8 * e + 7]));
+              *reinterpret_cast<uint4*>(op + c * 32 + e * 8) = w;
             }
           }
-          __syncwarp();
-          if (c + 1 < D / 32) tmem_ld_wait();
-          if (c + 2 == D / 32) {                           // O has been read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[item & 1]);
+        };
+        // O of a row's lanes adds up by way of the item's query buffer, half of the columns at a time: the first lane's stay in registers
+        constexpr int kHalf = REP > 1 ? D / 64 : D / 32;   // chunks of 32 columns between two barriers
+        float4* stage = reinterpret_cast<float4*>(smem + (item & 1) * SM::kQBytes + kRows * 8);
+        static_assert(REP == 1 || (kRows - BR) * (D / 2) * 4 + kRows * 8 <= SM::kQBytes, "lanes' results fit in a query buffer");
+        uint32_t x[32];
+        auto take = [&](int c) {
+          tmem_ld_32x32(t_o + c * 32, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * inv);
+        };
+        if (REP == 1) {
+          if (warp_ok) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              take(c);
+              put(c, x);
+              __syncwarp();
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D / 32; c0 += kHalf) {
+            if (part > 0 && warp_ok) {
+#pragma unroll 1
+              for (int c = 0; c < kHalf; ++c) {
+                take(c0 + c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  stage[(c * 8 + e) * (kRows - BR) + tl - BR] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
+                                                                            __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+              }
+            }
+            sync_group();
+            if (part == 0 && warp_ok) {
+#pragma unroll 1
+              for (int c = 0; c < kHalf; ++c) {
+                take(c0 + c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                  for (int i = 1; i < REP; ++i) {
+                    const float4 y = stage[(c * 8 + e) * (kRows - BR) + (i - 1) * BR + row];
+                    x[4 * e] = __float_as_uint(__uint_as_float(x[4 * e]) + y.x);
+                    x[4 * e + 1] = __float_as_uint(__uint_as_float(x[4 * e + 1]) + y.y);
+                    x[4 * e + 2] = __float_as_uint(__uint_as_float(x[4 * e + 2]) + y.z);
+                    x[4 * e + 3] = __float_as_uint(__uint_as_float(x[4 * e + 3]) + y.w);
+                  }
+                }
+                put(c0 + c, x);
+                __syncwarp();
+              }
+            }
+            sync_group();
           }
         }
+        tc_fence_before();                                 // O has been read
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[item & 1]);
+        if (REP > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
+      }
+      if (warp_ok && part == 0) {
+        const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * kRows + row] = make_float2(m_run, l_run);
-        if (cut && it.t0 == 0 && row == 0) {
+        if (cut && it.t0 == 0 && tl == 0) {
           // CTAs before the one whose share ends at the unit's end or behind it
           const int64_t all = begin[3], ctas = min(static_cast<int64_t>(gridDim.x), all);
           const int64_t end = all * (blockIdx.x + 1) / ctas + (it.tiles - it.t1);
@@ -619,8 +717,6 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           p.cut[2 * blockIdx.x] = make_int4(last, it.first, it.kvh, it.blk);
           p.cut[2 * blockIdx.x + 1] = make_int4(rows, 0, 0, 0);
         }
-      } else if (lane == 0) {
-        mbar_arrive(&o_free[item & 1]);
       }
     }
     if (threadIdx.x == 0 && !cut_tail) p.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);   // no unit begins here that ends elsewhere
@@ -664,7 +760,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) draft_join_kernel(const Draft
     }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int at = c0.w * kRows + row, node = at / p.G, head = c0.z * p.G + at - node * p.G;
+  const int at = c0.w * p.block_rows + row, node = at / p.G, head = c0.z * p.G + at - node * p.G;
   __nv_bfloat16* op = p.out + (static_cast<int64_t>(c0.y + node) * p.Hq + head) * D;
 #pragma unroll
   for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
@@ -690,16 +786,17 @@ static int page_tmap(const void* base, int64_t pages, int Hkv, int D, int page_s
   return 0;
 }
 
-template <int D>
-static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, const DraftAttnParams& p, int ctas, int max_nodes, cudaStream_t st) {
+template <int D, int REP>
+static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, DraftAttnParams p, int ctas, int max_rows, cudaStream_t st) {
   using SM = DraftSmem<D>;
   static PerDeviceOnce configured;
   if (configured.need()) {
-    CUDA_CHECK_RET(cudaFuncSetAttribute(draft_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
+    CUDA_CHECK_RET(cudaFuncSetAttribute(draft_attention_kernel<D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
     configured.done();
   }
-  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, p));
-  const int rows = max_nodes * p.G < kRows ? max_nodes * p.G : kRows;
+  p.block_rows = kRows / REP;
+  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, p));
+  const int rows = max_rows < p.block_rows ? max_rows : p.block_rows;
   CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
   return 0;
 }
@@ -739,5 +836,10 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
   p.cut = reinterpret_cast<int4*>(p.part_ml + static_cast<size_t>(2) * ctas * kRows);
   p.waits = g_wait_config;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return D == 128 ? launch_draft_attention<128>(tk, tv, p, ctas, max_nodes, st) : launch_draft_attention<64>(tk, tv, p, ctas, max_nodes, st);
+  // Rows that a sequence may have decide how many lanes share a row (a sequence with more has more blocks)
+  const int max_rows = (max_nodes < kNodes ? max_nodes : kNodes) * p.G;
+#define GLLM_DRAFT(REP) \
+  (D == 128 ? launch_draft_attention<128, REP>(tk, tv, p, ctas, max_rows, st) : launch_draft_attention<64, REP>(tk, tv, p, ctas, max_rows, st))
+  return max_rows <= 32 ? GLLM_DRAFT(4) : max_rows <= 64 ? GLLM_DRAFT(2) : GLLM_DRAFT(1);
+#undef GLLM_DRAFT
 }
