@@ -614,89 +614,94 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const float inv = weight * (cut ? 1.f : l_run > 0.f ? __frcp_rn(l_run) : 0.f);
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         __nv_bfloat16* op = p.out + (tok * p.Hq + head) * D;
-        uint4* po = reinterpret_cast<uint4*>(p.part_o) + static_cast<size_t>(slot) * (D / 4) * kRows + row;
-        // 32 finished columns from column 32 c on
-        auto put = [&](int c, uint32_t(&x)[32]) {
+        float4* po = p.part_o + static_cast<size_t>(slot) * (D / 4) * kRows + row;
+        // F finished columns from column c on
+        auto put = [&](int c, auto& x) {
+          constexpr int F = sizeof(x) / sizeof(float);
           for (unsigned long long b = bad; b != 0ull; b &= b - 1) {   // seen values that are no numbers
             const int place = it.ctx + __ffsll(static_cast<long long>(b)) - 1;
             const int64_t page = p.table[it.s * p.table_ld + min(place >> p.page_shift, p.table_width - 1)];
             if (page < 0 || page >= p.pages) continue;
             const __nv_bfloat16* vr =
-                p.v + ((((page * p.Hkv + it.kvh) * (D / 64) + c / 2) << p.page_shift) + (place & ((1 << p.page_shift) - 1))) * 64 + (c & 1) * 32;
+                p.v + ((((page * p.Hkv + it.kvh) * (D / 64) + c / 64) << p.page_shift) + (place & ((1 << p.page_shift) - 1))) * 64 + c % 64;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < F; ++e) {
               const float y = __bfloat162float(vr[e]);
-              if (!(fabsf(y) < INFINITY)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
+              if (!(fabsf(y) < INFINITY)) x[e] += y;
             }
           }
           if (!row_ok) return;
           if (cut) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) po[(c * 8 + e) * kRows] = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            for (int e = 0; e < F / 4; ++e) po[(c / 4 + e) * kRows] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < F / 8; ++e) {
               uint4 w;
-              w.x = pack_bf16(__uint_as_float(x[8 * e]), __uint_as_float(x[8 * e + 1]));
-              w.y = pack_bf16(__uint_as_float(x[8 * e + 2]), __uint_as_float(x[8 * e + 3]));
-              w.z = pack_bf16(__uint_as_float(x[8 * e + 4]), __uint_as_float(x[8 * e + 5]));
-              w.w = pack_bf16(__uint_as_float(x[8 * e + 6]), __uint_as_float(x[8 * e + 7]));
-              *reinterpret_cast<uint4*>(op + c * 32 + e * 8) = w;
+              w.x = pack_bf16(x[8 * e], x[8 * e + 1]);
+              w.y = pack_bf16(x[8 * e + 2], x[8 * e + 3]);
+              w.z = pack_bf16(x[8 * e + 4], x[8 * e + 5]);
+              w.w = pack_bf16(x[8 * e + 6], x[8 * e + 7]);
+              *reinterpret_cast<uint4*>(op + c + e * 8) = w;
             }
           }
         };
-        // O of a row's lanes adds up by way of the item's query buffer, half of the columns at a time: the first lane's stay in registers
-        constexpr int kHalf = REP > 1 ? D / 64 : D / 32;   // chunks of 32 columns between two barriers
-        float4* stage = reinterpret_cast<float4*>(smem + (item & 1) * SM::kQBytes + kRows * 8);
-        static_assert(REP == 1 || (kRows - BR) * (D / 2) * 4 + kRows * 8 <= SM::kQBytes, "lanes' results fit in a query buffer");
-        uint32_t x[32];
-        auto take = [&](int c) {
-          tmem_ld_32x32(t_o + c * 32, x);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * inv);
-        };
-        if (REP == 1) {
+        if constexpr (REP == 1) {
           if (warp_ok) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              take(c);
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              float x[32];
+              tmem_ld_32x32(t_o + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(v[e]) * inv;
               put(c, x);
               __syncwarp();
             }
           }
         } else {
+          // A row's lanes hand each other, by way of the item's query buffer, what they have of the columns that the other one finishes: F columns
+          // a lane, half of all columns at a time
+          constexpr int F = D / 2 / REP;
+          float4* stage = reinterpret_cast<float4*>(smem + (item & 1) * SM::kQBytes + kRows * 8);   // [part][its sources][F / 4][row]
+          static_assert(REP * (REP - 1) * F * 4 * BR + kRows * 8 <= SM::kQBytes, "lanes' results fit in a query buffer");
 #pragma unroll 1
-          for (int c0 = 0; c0 < D / 32; c0 += kHalf) {
-            if (part > 0 && warp_ok) {
-#pragma unroll 1
-              for (int c = 0; c < kHalf; ++c) {
-                take(c0 + c);
+          for (int c0 = 0; c0 < D; c0 += D / 2) {
+            float own[F];
+            if (warp_ok) {
+              uint32_t v[D / 64][32];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  stage[(c * 8 + e) * (kRows - BR) + tl - BR] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
-                                                                            __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+              for (int c = 0; c < D / 64; ++c) tmem_ld_32x32(t_o + c0 + c * 32, v[c]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int to = 0; to < REP; ++to) {
+                float x[F];
+#pragma unroll
+                for (int e = 0; e < F; ++e) x[e] = __uint_as_float(v[(to * F + e) / 32][(to * F + e) % 32]) * inv;
+                if (to == part) {
+#pragma unroll
+                  for (int e = 0; e < F; ++e) own[e] = x[e];
+                } else {
+                  float4* at = stage + (to * (REP - 1) + (part < to ? part : part - 1)) * (F / 4) * BR + row;
+#pragma unroll
+                  for (int e = 0; e < F / 4; ++e) at[e * BR] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                }
               }
             }
             sync_group();
-            if (part == 0 && warp_ok) {
-#pragma unroll 1
-              for (int c = 0; c < kHalf; ++c) {
-                take(c0 + c);
+            if (warp_ok) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+              for (int i = 0; i < REP - 1; ++i) {
+                const float4* at = stage + (part * (REP - 1) + i) * (F / 4) * BR + row;
 #pragma unroll
-                  for (int i = 1; i < REP; ++i) {
-                    const float4 y = stage[(c * 8 + e) * (kRows - BR) + (i - 1) * BR + row];
-                    x[4 * e] = __float_as_uint(__uint_as_float(x[4 * e]) + y.x);
-                    x[4 * e + 1] = __float_as_uint(__uint_as_float(x[4 * e + 1]) + y.y);
-                    x[4 * e + 2] = __float_as_uint(__uint_as_float(x[4 * e + 2]) + y.z);
-                    x[4 * e + 3] = __float_as_uint(__uint_as_float(x[4 * e + 3]) + y.w);
-                  }
+                for (int e = 0; e < F / 4; ++e) {
+                  const float4 y = at[e * BR];
+                  own[4 * e] += y.x; own[4 * e + 1] += y.y; own[4 * e + 2] += y.z; own[4 * e + 3] += y.w;
                 }
-                put(c0 + c, x);
-                __syncwarp();
               }
+              put(c0 + part * F, own);
+              __syncwarp();
             }
             sync_group();
           }
