@@ -12,7 +12,7 @@
 namespace b200 {
 
 static constexpr int kNodes = 64;
-static constexpr int kVerifyThreads = 1024, kVerifyWarps = kVerifyThreads / 32;
+static constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
 static constexpr int kVerifyParts = 8;                 // CTAs of a cluster at most
 
 enum VerifyForm : int { kMatch = 0, kGiven = 1, kDraws = 2 };
@@ -39,47 +39,36 @@ struct VerifyShared {
   int taken[kNodes], chosen[kNodes];
   double warp_sum[kVerifyWarps];
   double part_sum[2][kVerifyParts];             // of the cluster's CTAs
-  int after;
+  int after, first_over, last_with;
 };
 
-// Four tokens at once where both rows allow it: the row's first 16-byte boundary is `lead` tokens before its first token, group g has
-// the tokens 4 g - lead and on.
+// Four tokens at once: the row's first 16-byte boundary is `lead` tokens before its first token, group g has the tokens 4 g - lead and on
 struct Rows {
   const float* p;
   const float* q;            // null: none
   int vocab, lead, groups;
-  bool together;
+  bool together;             // both rows have their boundaries at the same tokens
   double past;
   const int* word;           // tokens of the nodes
-  unsigned long long gone;   // kGiven: nodes whose tokens are out of the row (those in this warp's range: `near`)
+  unsigned long long gone;   // kGiven: nodes whose tokens are out of the row
 
   __device__ __forceinline__ Rows(const float* p_, const float* q_, int v) : p(p_), q(q_), vocab(v), past(0.0), word(nullptr), gone(0) {
     lead = static_cast<int>((reinterpret_cast<uintptr_t>(p) >> 2) & 3);
     groups = (lead + v + 3) / 4;
     together = q == nullptr || ((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p)) & 15) == 0;
   }
-  __device__ __forceinline__ void raw(int g, float (&a)[4], float (&b)[4]) const {
+  // any group
+  __device__ __forceinline__ void raw(int g, float4& a, float4& b) const {
     const int i = 4 * g - lead;
-    if (i >= 0 && i + 4 <= vocab) {
-      const float4 x = *reinterpret_cast<const float4*>(p + i);
-      a[0] = x.x; a[1] = x.y; a[2] = x.z; a[3] = x.w;
-      if (q != nullptr) {
-        if (together) {
-          const float4 y = *reinterpret_cast<const float4*>(q + i);
-          b[0] = y.x; b[1] = y.y; b[2] = y.z; b[3] = y.w;
-        } else {
+    float x[4], y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = q[i + e];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = i + e >= 0 && i + e < vocab;
-        a[e] = in ? p[i + e] : 0.f;
-        if (q != nullptr) b[e] = in ? q[i + e] : 0.f;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const bool in = i + e >= 0 && i + e < vocab;
+      x[e] = in ? p[i + e] : 0.f;
+      y[e] = in && q != nullptr ? q[i + e] : 0.f;
     }
+    a = make_float4(x[0], x[1], x[2], x[3]);
+    b = make_float4(y[0], y[1], y[2], y[3]);
   }
   // of the nodes in `gone`, those whose tokens lie in groups [g0, g1): none for most warps
   __device__ __forceinline__ unsigned long long near(int g0, int g1) const {
@@ -90,12 +79,15 @@ struct Rows {
     }
     return m;
   }
-  __device__ __forceinline__ void mass(int g, unsigned long long out, const float (&a)[4], const float (&b)[4], double (&r)[4]) const {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      double x = static_cast<double>(a[e]);
-      if (q != nullptr) x = __dadd_rn(x, -__dmul_rn(past, static_cast<double>(b[e])));
-      r[e] = x > 0.0 ? x : 0.0;
+  __device__ __forceinline__ double left_of(float a, float b) const {
+    const double x = __dadd_rn(static_cast<double>(a), -__dmul_rn(past, static_cast<double>(b)));
+    return x > 0.0 ? x : 0.0;
+  }
+  __device__ __forceinline__ void mass(int g, unsigned long long out, const float4& a, const float4& b, double (&r)[4]) const {
+    if (q != nullptr) {
+      r[0] = left_of(a.x, b.x); r[1] = left_of(a.y, b.y); r[2] = left_of(a.z, b.z); r[3] = left_of(a.w, b.w);
+    } else {
+      r[0] = fmaxf(a.x, 0.f); r[1] = fmaxf(a.y, 0.f); r[2] = fmaxf(a.z, 0.f); r[3] = fmaxf(a.w, 0.f);   // not a number: 0
     }
     for (; out != 0ull; out &= out - 1) {
       const int at = word[__ffsll(static_cast<long long>(out)) - 1] + lead - 4 * g;
@@ -112,11 +104,48 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
-// groups of this warp: [first, end)
+// groups of a warp: [first, end)
 __device__ __forceinline__ void share(int groups, int part, int parts, int warp, int& first, int& end) {
   const int64_t all = static_cast<int64_t>(parts) * kVerifyWarps, w = static_cast<int64_t>(part) * kVerifyWarps + warp;
   first = static_cast<int>(groups * w / all);
   end = static_cast<int>(groups * (w + 1) / all);
+}
+
+// This lane's part of the mass of groups [g0, g1). Whole groups have their loads four at a time ahead of their arithmetic: one at a time the
+// latency of each is waited for.
+__device__ __forceinline__ double range_mass(const Rows& r, int g0, int g1, int lane) {
+  constexpr int kAhead = 4;
+  const unsigned long long out = r.near(g0, g1);
+  const int w0 = max(g0, r.lead != 0 ? 1 : 0), w1 = min(g1, (r.lead + r.vocab) / 4);
+  double sum = 0.0, m[4];
+  float4 a[kAhead], b[kAhead];
+  for (int g = w0 + lane; g < w1; g += 32 * kAhead) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int h = g + 32 * u;
+      a[u] = b[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (h < w1) {
+        a[u] = *reinterpret_cast<const float4*>(r.p + 4 * h - r.lead);
+        if (r.q != nullptr) {
+          const float* at = r.q + 4 * h - r.lead;
+          b[u] = r.together ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      r.mass(g + 32 * u, out, a[u], b[u], m);
+      sum += (m[0] + m[1]) + (m[2] + m[3]);
+    }
+  }
+  // the groups at the row's ends
+  const int edge = lane == 0 && g0 < min(w0, g1) ? g0 : lane == 1 && w1 < g1 && w1 >= w0 ? w1 : -1;
+  if (edge >= 0) {
+    r.raw(edge, a[0], b[0]);
+    r.mass(edge, out, a[0], b[0], m);
+    sum += (m[0] + m[1]) + (m[2] + m[3]);
+  }
+  return sum;
 }
 
 // sum of the row's mass, the same in every thread of the cluster
@@ -124,16 +153,7 @@ __device__ __forceinline__ double row_sum(const Rows& r, VerifyShared& s, int pa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int g0, g1;
   share(r.groups, part, parts, warp, g0, g1);
-  double sum = 0.0;
-  const unsigned long long out = r.near(g0, g1);
-  for (int g = g0 + lane; g < g1; g += 32) {
-    float a[4], b[4];
-    double m[4];
-    r.raw(g, a, b);
-    r.mass(g, out, a, b, m);
-    sum += (m[0] + m[1]) + (m[2] + m[3]);
-  }
-  sum = warp_sum(sum);
+  const double sum = warp_sum(range_mass(r, g0, g1, lane));
   __syncthreads();                                       // the sums of the pass before have been read
   if (lane == 0) s.warp_sum[warp] = sum;
   __syncthreads();
@@ -151,7 +171,7 @@ __device__ __forceinline__ double row_sum(const Rows& r, VerifyShared& s, int pa
   return all;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads)
+__global__ void __launch_bounds__(kVerifyThreads, 2)
 draft_verify_kernel(const VerifyParams v) {
   __shared__ VerifyShared s;
   if (v.parts > 1) cluster_sync();                       // every CTA's shared memory is there
@@ -281,47 +301,58 @@ draft_verify_kernel(const VerifyParams v) {
         if (m > 0.0 && run > border) break;
       }
     }
-    if (warp == max(mine, 0)) {
-      int found = -1, last = 0;
-      if (mine >= 0) {
-        int g0, g1;
-        share(rows.groups, part, parts, warp, g0, g1);
-        double run = start;
-        const unsigned long long out = rows.near(g0, g1);
-        for (int g = g0; g < g1 && found < 0; g += 32) {
-          float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-          double m[4] = {0.0, 0.0, 0.0, 0.0};
-          if (g + lane < g1) {
-            rows.raw(g + lane, a, b);
-            rows.mass(g + lane, out, a, b, m);
-          }
-          const double own = (m[0] + m[1]) + (m[2] + m[3]);
-          double upto = own;
+    // Its range, by the whole CTA: consecutive groups a thread, their running sums, the first thread whose sum is over the border (or the last
+    // with mass) looks at its tokens
+    int g0 = 0, g1 = 0;
+    if (mine >= 0) share(rows.groups, part, parts, mine, g0, g1);
+    const unsigned long long out = rows.near(g0, g1);
+    const int each = (g1 - g0 + kVerifyThreads - 1) / kVerifyThreads;
+    const int h0 = min(g0 + static_cast<int>(threadIdx.x) * each, g1), h1 = min(h0 + each, g1);
+    float4 a, b;
+    double m[4], own = 0.0;
+    for (int g = h0; g < h1; ++g) {
+      rows.raw(g, a, b);
+      rows.mass(g, out, a, b, m);
+      own += (m[0] + m[1]) + (m[2] + m[3]);
+    }
+    double upto = own;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-          }
-          const unsigned with = __ballot_sync(0xffffffffu, own > 0.0), over = __ballot_sync(0xffffffffu, own > 0.0 && run + upto > border);
-          const int lane_hit = over != 0u ? __ffs(over) - 1 : -1, lane_last = with != 0u ? 31 - __clz(with) : -1;
-          double at = run + (upto - own);
-          int hit = -1, end = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();                                     // s.warp_sum has been read
+    if (lane == 31) s.warp_sum[warp] = upto;
+    if (threadIdx.x == 0) {
+      s.first_over = kVerifyThreads;
+      s.last_with = -1;
+      s.after = 0;
+    }
+    __syncthreads();
+    double before_me = start;
+    for (int w = 0; w < warp; ++w) before_me += s.warp_sum[w];
+    before_me += upto - own;
+    if (own > 0.0) {
+      atomicMax(&s.last_with, static_cast<int>(threadIdx.x));
+      if (before_me + own > border) atomicMin(&s.first_over, static_cast<int>(threadIdx.x));
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) == (s.first_over < kVerifyThreads ? s.first_over : s.last_with)) {
+      int hit = -1, last = 0;
+      double at = before_me;
+      for (int g = h0; g < h1; ++g) {
+        rows.raw(g, a, b);
+        rows.mass(g, out, a, b, m);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            at += m[e];
-            if (m[e] > 0.0) {
-              end = 4 * (g + lane) - rows.lead + e;
-              if (hit < 0 && at > border) hit = end;
-            }
+        for (int e = 0; e < 4; ++e) {
+          at += m[e];
+          if (m[e] > 0.0) {
+            last = 4 * g - rows.lead + e;
+            if (hit < 0 && at > border) hit = last;
           }
-          if (hit < 0) hit = end;                        // the group's sum is over the border, rounding left no token of it there
-          if (lane_last >= 0) last = __shfl_sync(0xffffffffu, end, lane_last);
-          if (lane_hit >= 0) found = __shfl_sync(0xffffffffu, hit, lane_hit);
-          run += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (found < 0) found = last;
       }
-      if (lane == 0) s.after = max(found, 0);
+      s.after = hit >= 0 ? hit : last;                   // rounding left no token of it over the border: the last one
     }
     __syncthreads();
     after = s.after;
