@@ -42,13 +42,16 @@ struct DraftAttnParams {
   const int32_t* q_start;
   const int64_t* seen;
   int table_width, num_seqs, rows, Hq, Hkv, G, page_shift;   // a page has 2^page_shift tokens
-  int block_rows;
+  int block_rows, part_rows;                             // of a block; rows that parts have room for
   float scale_log2;
   float4* part_o;                                        // [2 CTA][D / 4][128 rows]
   float2* part_ml;                                       // [2 CTA][128 rows]: reference of the exponents, sum
   int4* cut;                                             // [CTA][2]: what the join of a unit that the CTA begins needs
   WaitConfig waits;
 };
+
+inline int part_rows_of(int max_rows) { return max_rows > kRows ? 2 * kRows : kRows; }
+constexpr int block_rows_of(int rep) { return rep == 0 ? 2 * kRows : kRows / rep; }
 
 template <int D>
 struct DraftSmem {
@@ -184,8 +187,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DraftAttnParams p) {
   using SM = DraftSmem<D>;
   constexpr int NS = SM::kStages;
-  constexpr int BR = kRows / REP;                        // rows of a block: TMEM lane = part of the keys x BR + row
-  constexpr int kChunks = kKeys / 32 / REP;              // of 32 keys that a lane has of a tile
+  // REP 1, 2, 4: a block of 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups take the tiles in turn.
+  // REP 0 (WIDE): a block of 256 rows, each warpgroup has 128 of them and every tile.
+  constexpr bool WIDE = REP == 0;
+  constexpr int BR = block_rows_of(REP);
+  constexpr int kChunks = kKeys / 32 / (WIDE ? 1 : REP);              // of 32 keys that a lane has of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
@@ -315,21 +321,78 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       constexpr uint32_t idesc_pv = make_idesc_bf16(kRows, D) | (1u << 16);
       uint32_t pos = 0, g = 0;                             // place in the ring, tile
       bool ok = true;
-      // S of tile `tile_no`, from the queries in buffer `buf`
-      auto scores = [&](uint32_t tile_no, uint32_t buf, bool last) {
-        const uint32_t st = pos % NS;
-        ok = guard.wait<true>(&full[st], (pos / NS) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t q_addr = smem_u32(smem + buf * SM::kQBytes), k_addr = smem_u32(smem + SM::kRingOff + st * SM::kTileBytes);
-        const uint32_t d_tmem = tmem + (tile_no & 1) * kKeys;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return guard.wait<true>(bar, parity); };
+      // S in buffer s_buf from the queries in buffer q_buf and the tile in stage st
+      auto issue_s = [&](uint32_t s_buf, uint32_t q_buf, uint32_t st) {
+        const uint32_t q_addr = smem_u32(smem + q_buf * SM::kQBytes), k_addr = smem_u32(smem + SM::kRingOff + st * SM::kTileBytes);
+        const uint32_t d_tmem = tmem + s_buf * kKeys;
 #pragma unroll
         for (int kd = 0; kd < D / 64; ++kd) {
           const uint64_t da = make_sw128_kmajor_desc(q_addr + kd * (kRows * 128)), db = make_sw128_kmajor_desc(k_addr + kd * (kKeys * 128));
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_bf16<1>(d_tmem, da + kk * 2, db + kk * 2, idesc_s, (kd | kk) != 0);
         }
-        umma_commit(&s_full[tile_no & 1]);
+        umma_commit(&s_full[s_buf]);
+      };
+      // P in buffer s_buf times the tile in stage st, added to O in o_buf: the steps of 16 keys that there are
+      auto issue_pv = [&](uint32_t s_buf, uint32_t o_buf, uint32_t st, int keys, uint32_t acc) {
+        const uint64_t dv = mn_major_desc(smem_u32(smem + SM::kRingOff + st * SM::kTileBytes));
+        const uint32_t o_tmem = tmem + SM::kTmemO + o_buf * D, p_tmem = tmem + s_buf * kKeys;
+        if (keys == kKeys) {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < (keys + 15) / 16; ++kk)
+            umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+        }
+        umma_commit(&pv_full[s_buf]);
+      };
+      if constexpr (WIDE) {
+        uint32_t seen0 = 0, seen1 = 0, items1 = 0;           // tiles of each half so far; items that had a second half
+        for (uint32_t item = 0; ok && it.next(); ++item) {
+          const int halves = it.block_rows() > kRows ? 2 : 1;
+          if (item == 0) ok = guard.first(&q_full[0]);
+          ok = ok && wait(&q_full[0], item & 1);
+          uint32_t k_pos = g == 0 ? 0 : 2 * g - 1;
+          ok = ok && wait(&full[k_pos % NS], (k_pos / NS) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          for (int h = 0; h < halves; ++h) issue_s(h, h, k_pos % NS);
+          umma_commit(&empty[k_pos % NS]);
+          if (it.t0 + 1 == it.t1) umma_commit(&q_free[0]);
+          for (int t = it.t0; ok && t < it.t1; ++t, ++g) {
+            const bool more = t + 1 < it.t1;
+            const uint32_t v_pos = more || it.left > 0 ? 2 * g + 2 : 2 * g + 1;
+            k_pos = 2 * g + 1;
+            if (more) ok = wait(&full[k_pos % NS], (k_pos / NS) & 1);
+            ok = ok && wait(&full[v_pos % NS], (v_pos / NS) & 1);
+            for (int h = 0; h < halves && ok; ++h) {
+              uint32_t& seen = h == 0 ? seen0 : seen1;
+              // O of this half's item before has been read
+              if (t == it.t0) ok = h == 0 ? item == 0 || wait(&o_free[0], (item & 1) ^ 1) : items1 == 0 || wait(&o_free[1], (items1 & 1) ^ 1);
+              ok = ok && wait(&p_full[h], seen & 1);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(h, h, v_pos % NS, it.keys(t), t == it.t0 ? 0u : 1u);
+              if (more) issue_s(h, h, k_pos % NS);
+              ++seen;
+            }
+            if (!ok) break;
+            umma_commit(&empty[v_pos % NS]);
+            if (more) umma_commit(&empty[k_pos % NS]);
+            if (t + 2 == it.t1) umma_commit(&q_free[0]);
+          }
+          items1 += halves == 2;
+        }
+      } else {
+      // S of tile `tile_no`, from the queries in buffer `buf`
+      auto scores = [&](uint32_t tile_no, uint32_t buf, bool last) {
+        const uint32_t st = pos % NS;
+        ok = wait(&full[st], (pos / NS) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        issue_s(tile_no & 1, buf, st);
         umma_commit(&empty[st]);
         if (last) umma_commit(&q_free[buf]);
         ++pos;
@@ -364,31 +427,25 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
              (!first_tile || now < 2 || guard.wait<true>(&o_free[buf], ((now >> 1) & 1) ^ 1));
         if (!ok) break;
         tc_fence_after();
-        const uint64_t dv = mn_major_desc(smem_u32(smem + SM::kRingOff + st * SM::kTileBytes));
-        const uint32_t o_tmem = tmem + SM::kTmemO + buf * D, p_tmem = tmem + (g & 1) * kKeys;
-        const uint32_t acc = first_tile ? 0u : 1u;
-        if (keys == kKeys) {
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
-        } else {
-#pragma unroll 1
-          for (int kk = 0; kk < (keys + 15) / 16; ++kk)
-            umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
-        }
-        umma_commit(&pv_full[g & 1]);
+        issue_pv(g & 1, buf, st, keys, first_tile ? 0u : 1u);
         umma_commit(&empty[st]);
         ++pos;
         ++g;
         if (!more) break;
         now = next;
       }
+      }
       umma_commit(mma_end);                                // nothing is in flight when the columns are given back
       guard.land(mma_end, 0);
     } else if (warp == 11 && !idle) {
       // ------------------------------------------------------------------ queries
       for (uint32_t item = 0; it.next(); ++item) {
-        const uint32_t buf = item & 1;
-        if (item >= 2 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1))) break;
+        const uint32_t buf = WIDE ? 0 : item & 1;
+        if (WIDE) {                                        // both buffers have this item's rows
+          if (item >= 1 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[0], (item & 1) ^ 1))) break;
+        } else if (item >= 2 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1))) {
+          break;
+        }
         const int rows = it.block_rows();
         const uint32_t dst = smem_u32(smem + buf * SM::kQBytes);
         constexpr int kStep = 32 / (D / 8);                // rows of a round
@@ -398,10 +455,10 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(it.kvh * p.G + h) * D + c * 8;
           for (h += kStep; h >= p.G; h -= p.G) ++node;
 #pragma unroll
-          for (int part = 0; part < REP; ++part) {
+          for (int part = 0; part < (WIDE ? 1 : REP); ++part) {
             const int l = part * BR + r;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (c >> 3) * (kRows * 128) + l * 128 + (((c & 7) ^ (l & 7)) << 4)),
-                         "l"(src) : "memory");
+            const uint32_t to = dst + (WIDE && r >= kRows ? SM::kQBytes : 0) + (c >> 3) * (kRows * 128) + l % kRows * 128 + (((c & 7) ^ (l & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -413,10 +470,12 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   } else {
     // ------------------------------------------------------------------ softmax: one row a thread, the CTA's tiles in turn
     const int wg = warp >> 2, tl = threadIdx.x & 127;      // TMEM lane
-    const int row = tl % BR, part = REP == 1 ? 0 : (warp & 3) / (4 / REP);
+    constexpr int kParts = WIDE ? 1 : REP;                 // lanes of a row
+    const int row = WIDE ? wg * kRows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + wg * kKeys + lane_base;
     uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
+    uint32_t mine = 0;                                     // WIDE: tiles of this half
     bool cut_tail = false;
     // A wait that gives up leaves the warps in step: they go on with what is there, and every later wait ends at once
     auto await = [&](uint64_t* bar, uint32_t parity) {
@@ -432,19 +491,23 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
       if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
       const int rows = it.block_rows();
-      const bool warp_ok = (warp & 3) % (4 / REP) * 32 < rows, row_ok = row < rows;
+      const bool warp_ok = row - lane < rows, row_ok = row < rows;
       const int at = it.blk * BR + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
       const int64_t tok = it.first + (row_ok ? node : 0);
       const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
       const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
       unsigned long long* bad_here = bad_nodes + (item & 3);
-      const uint32_t t_o = tmem + SM::kTmemO + (item & 1) * D + lane_base;
+      const uint32_t t_o = tmem + SM::kTmemO + (WIDE ? wg : item & 1) * D + lane_base;
+      if (WIDE && wg * kRows >= rows) {                    // no second half
+        g += it.t1 - it.t0;
+        continue;
+      }
       float m_run = -INFINITY, l_run = 0.f;                // reference of this warpgroup's sum, the sum
       float m_old = -INFINITY;                             // reference of the tile before this warpgroup's last
       for (int t = it.t0; t < it.t1; ++t, ++g) {
-        if ((g & 1) != static_cast<uint32_t>(wg)) continue;
+        if (!WIDE && (g & 1) != static_cast<uint32_t>(wg)) continue;
         const int key0 = t * kKeys;
-        await(&s_full[wg], (g >> 1) & 1);
+        await(&s_full[wg], (WIDE ? mine : g >> 1) & 1);
         const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
         float mx = -INFINITY;
         // 32 scores at a time in loops that are not unrolled: the warps are at different places of the code, and what is not in the instruction
@@ -484,13 +547,19 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           if (kChunks > 1 && behind) tmem_store_wait();
           mx *= p.scale_log2;
         }
-        // The reference of both warpgroups: the other's of the tile before, raised where this tile's maximum is 2^8 over it
-        if (g > 0) await(&m_set[4 * (wg ^ 1) + (warp & 3)], ((g - 1) >> 1) & 1);
-        m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + tl) : -INFINITY;
-        const float m_now = mx > m_old + kLazy ? mx : m_old;
-        *static_cast<volatile float*>(m_ref + tl) = m_now;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m_set[4 * wg + (warp & 3)]);
+        float m_now;
+        if (WIDE) {
+          m_old = m_run;
+          m_now = mx > m_old + kLazy ? mx : m_old;
+        } else {
+          // The reference of both warpgroups: the other's of the tile before, raised where this tile's maximum is 2^8 over it
+          if (g > 0) await(&m_set[4 * (wg ^ 1) + (warp & 3)], ((g - 1) >> 1) & 1);
+          m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + tl) : -INFINITY;
+          m_now = mx > m_old + kLazy ? mx : m_old;
+          *static_cast<volatile float*>(m_ref + tl) = m_now;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_set[4 * wg + (warp & 3)]);
+        }
         if (warp_ok) {
           const float alpha = m_now != m_old ? ex2(m_old - m_now) : 1.f;
           if (m_now != m_run) {                            // this warpgroup's sum, from the reference of two tiles ago
@@ -499,8 +568,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           if (t > it.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             // O is free when the product before this tile's has ended. (S of this tile was formed behind the one before that: the phase
-            // before the awaited one has passed, the one behind it needs this tile's P.)
-            await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
+            // before the awaited one has passed, the one behind it needs this tile's P. WIDE: S was formed behind that product.)
+            if (!WIDE) await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t v[16];
@@ -527,7 +596,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
             tmem_store16(t_s + (part * kChunks + c) * 16, pk);
           }
-          if (REP > 1) {                                   // the keys that other lanes have of this row
+          if (kParts > 1) {                                // the keys that other lanes have of this row
             uint32_t none[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) none[e] = 0u;
@@ -539,7 +608,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           l_run += sa.x + sa.y;
           tmem_store_wait();
         }
-        if (behind) {
+        if (behind && (!WIDE || wg == 0)) {                // (WIDE: the first half's product comes first)
           // Values that nobody sees, or not every row, are finite before the product reads them
           const uint32_t vp = (t + 1 < it.t1 || it.left > 0) ? 2 * g + 2 : 2 * g + 1, st = vp % NS;    // where V of tile g is in the ring
           await(&full[st], (vp / NS) & 1);
@@ -570,40 +639,42 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         tc_fence_before();                                 // P and the rescaled O are in TMEM, S has been read
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
-        if (t + 2 == it.t1) {                              // the item's last tile is the other warpgroup's
+        ++mine;
+        if (!WIDE && t + 2 == it.t1) {                     // the item's last tile is the other warpgroup's
           *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) = l_run;
           __syncwarp();
           if (lane == 0) mbar_arrive(&l_set[2 * wg + (item & 1)]);
         }
       }
-      if (((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
+      if (!WIDE && ((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
       // ---- results, by the warpgroup that had the last tile; the other one goes on
-      await(&pv_full[wg], ((g - 1) >> 1) & 1);
-      if (it.t1 - it.t0 > 1) {
+      await(&pv_full[wg], (WIDE ? mine - 1 : (g - 1) >> 1) & 1);
+      if (!WIDE && it.t1 - it.t0 > 1) {
         // Of an item of this parity: the other one may have set that of the next item already, should that have two tiles
         await(&l_set[2 * (wg ^ 1) + (item & 1)], (sums >> (item & 1)) & 1);
         sums ^= 1u << (item & 1);
         // the other's reference is that of the tile before the last
         l_run += *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) * (m_old == m_run ? 1.f : ex2(m_old - m_run));
       }
-      // The words are two items old when they are used again: the other warpgroup is at the next item's first tile at most
-      if (tl == 0) bad_nodes[(item + 2) & 3] = 0ull;
+      // The words are two items old when they are used again: the other warpgroup is at the next item's first tile at most (WIDE: has
+      // its results of the item before, or none)
+      if (tl == 0 && (!WIDE || wg == 0)) bad_nodes[(item + 2) & 3] = 0ull;
       // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
       float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
-      if (REP > 1) lanes[tl] = make_float2(m_run, l_run);
+      if (kParts > 1) lanes[tl] = make_float2(m_run, l_run);
       sync_group();                                        // and bad_here of all four warps (the other warpgroup's: l_set)
       float weight = 1.f;
-      if (REP > 1) {
-        float2 o[REP];
+      if (kParts > 1) {
+        float2 o[kParts];
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < REP; ++i) {
+        for (int i = 0; i < kParts; ++i) {
           o[i] = lanes[i * BR + row];
           top = fmaxf(top, o[i].x);
         }
         if (top != -INFINITY) {
 #pragma unroll
-          for (int i = 0; i < REP; ++i) sum += o[i].y * ex2(o[i].x - top);
+          for (int i = 0; i < kParts; ++i) sum += o[i].y * ex2(o[i].x - top);
           weight = ex2(m_run - top);
         }
         m_run = top;
@@ -614,7 +685,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const float inv = weight * (cut ? 1.f : l_run > 0.f ? __frcp_rn(l_run) : 0.f);
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         __nv_bfloat16* op = p.out + (tok * p.Hq + head) * D;
-        float4* po = p.part_o + static_cast<size_t>(slot) * (D / 4) * kRows + row;
+        constexpr int kPartRows = WIDE ? 2 * kRows : kRows;
+        float4* po = p.part_o + static_cast<size_t>(slot) * (D / 4) * kPartRows + row;
         // F finished columns from column c on
         auto put = [&](int c, auto& x) {
           constexpr int F = sizeof(x) / sizeof(float);
@@ -633,7 +705,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           if (!row_ok) return;
           if (cut) {
 #pragma unroll
-            for (int e = 0; e < F / 4; ++e) po[(c / 4 + e) * kRows] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            for (int e = 0; e < F / 4; ++e) po[(c / 4 + e) * kPartRows] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
           } else {
 #pragma unroll
             for (int e = 0; e < F / 8; ++e) {
@@ -646,7 +718,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
           }
         };
-        if constexpr (REP == 1) {
+        if constexpr (kParts == 1) {
           if (warp_ok) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -708,13 +780,13 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
         tc_fence_before();                                 // O has been read
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[item & 1]);
-        if (REP > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
+        if (lane == 0) mbar_arrive(&o_free[WIDE ? wg : item & 1]);
+        if (kParts > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
       }
       if (warp_ok && part == 0) {
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
-        if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * kRows + row] = make_float2(m_run, l_run);
-        if (cut && it.t0 == 0 && tl == 0) {
+        if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * (WIDE ? 2 * kRows : kRows) + row] = make_float2(m_run, l_run);
+        if (cut && it.t0 == 0 && row == 0) {
           // CTAs before the one whose share ends at the unit's end or behind it
           const int64_t all = begin[3], ctas = min(static_cast<int64_t>(gridDim.x), all);
           const int64_t end = all * (blockIdx.x + 1) / ctas + (it.tiles - it.t1);
@@ -748,19 +820,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) draft_join_kernel(const Draft
   if (last <= cta || last >= static_cast<int>(gridDim.x) || row >= c1.x) return;
   auto slot = [&](int c) { return static_cast<size_t>(2 * c + (c == cta ? 1 : 0)); };
   float m = -INFINITY;
-  for (int c = cta; c <= last; ++c) m = fmaxf(m, p.part_ml[slot(c) * kRows + row].x);
+  for (int c = cta; c <= last; ++c) m = fmaxf(m, p.part_ml[slot(c) * p.part_rows + row].x);
   const float m_use = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 o[D / 4 / kJoinWarps];
 #pragma unroll
   for (int i = 0; i < D / 4 / kJoinWarps; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = cta; c <= last; ++c) {
-    const float2 ml = p.part_ml[slot(c) * kRows + row];
+    const float2 ml = p.part_ml[slot(c) * p.part_rows + row];
     const float w = ex2(ml.x - m_use);
     l += w * ml.y;
 #pragma unroll
     for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
-      const float4 x = p.part_o[(slot(c) * (D / 4) + warp + i * kJoinWarps) * kRows + row];
+      const float4 x = p.part_o[(slot(c) * (D / 4) + warp + i * kJoinWarps) * p.part_rows + row];
       o[i].x += w * x.x; o[i].y += w * x.y; o[i].z += w * x.z; o[i].w += w * x.w;
     }
   }
@@ -799,7 +871,10 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
     CUDA_CHECK_RET(cudaFuncSetAttribute(draft_attention_kernel<D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
     configured.done();
   }
-  p.block_rows = kRows / REP;
+  p.block_rows = block_rows_of(REP);
+  p.part_rows = part_rows_of(p.block_rows);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(2) * ctas * (D / 4) * p.part_rows);
+  p.cut = reinterpret_cast<int4*>(p.part_ml + static_cast<size_t>(2) * ctas * p.part_rows);
   CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, p));
   const int rows = max_rows < p.block_rows ? max_rows : p.block_rows;
   CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
@@ -810,8 +885,10 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
 
 using namespace b200;
 
-// bytes of scratch for a launch of `ctas` CTAs
-GLLM_EXPORT int64_t gllm_draft_attention_scratch(int D, int ctas) { return static_cast<int64_t>(ctas) * (2 * kRows * (D * 4 + 8) + 32); }
+// bytes of scratch for a launch of `ctas` CTAs over sequences of at most max_rows rows (nodes x query heads a kv head)
+GLLM_EXPORT int64_t gllm_draft_attention_scratch(int D, int max_rows, int ctas) {
+  return static_cast<int64_t>(ctas) * (2 * part_rows_of(max_rows) * (D * 4 + 8) + 32);
+}
 
 GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, const void* k_cache, const void* v_cache, int64_t pages,
                                      const void* table, int64_t table_ld, int table_width, const void* seq_lens, const void* q_start,
@@ -820,7 +897,7 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
   if (num_seqs <= 0 || rows <= 0 || max_nodes <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || page_size < 8 || kKeys % page_size || (page_size & (page_size - 1)) || pages <= 0 || table_width <= 0 || ctas <= 0 ||
       q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
-      scratch_bytes < gllm_draft_attention_scratch(D, ctas))
+      scratch_bytes < gllm_draft_attention_scratch(D, (max_nodes < kNodes ? max_nodes : kNodes) * (Hq / Hkv), ctas))
     return 1;
   CUtensorMap tk, tv;
   if (page_tmap(k_cache, pages, Hkv, D, page_size, &tk) || page_tmap(v_cache, pages, Hkv, D, page_size, &tv)) return 1;
@@ -837,14 +914,14 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
   p.page_shift = 31 - __builtin_clz(static_cast<unsigned>(page_size));
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part_o = reinterpret_cast<float4*>(scratch);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(2) * ctas * (D / 4) * kRows);
-  p.cut = reinterpret_cast<int4*>(p.part_ml + static_cast<size_t>(2) * ctas * kRows);
+  p.part_ml = nullptr;
+  p.cut = nullptr;
   p.waits = g_wait_config;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows that a sequence may have decide how many lanes share a row (a sequence with more has more blocks)
   const int max_rows = (max_nodes < kNodes ? max_nodes : kNodes) * p.G;
 #define GLLM_DRAFT(REP) \
   (D == 128 ? launch_draft_attention<128, REP>(tk, tv, p, ctas, max_rows, st) : launch_draft_attention<64, REP>(tk, tv, p, ctas, max_rows, st))
-  return max_rows <= 32 ? GLLM_DRAFT(4) : max_rows <= 64 ? GLLM_DRAFT(2) : GLLM_DRAFT(1);
+  return max_rows <= 32 ? GLLM_DRAFT(4) : max_rows <= 64 ? GLLM_DRAFT(2) : max_rows <= kRows ? GLLM_DRAFT(1) : GLLM_DRAFT(0);
 #undef GLLM_DRAFT
 }

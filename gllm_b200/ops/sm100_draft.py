@@ -33,8 +33,8 @@ def plan(parents: torch.Tensor, inp, page_size: int):
 
 
 @functools.lru_cache(maxsize=None)
-def _attention_scratch(head_dim: int) -> int:
-    return _lib.load().gllm_draft_attention_scratch(head_dim, NUM_SMS)
+def _attention_scratch(head_dim: int, max_rows: int) -> int:
+    return _lib.load().gllm_draft_attention_scratch(head_dim, max_rows, NUM_SMS)
 
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp, seen: torch.Tensor, scale: float, num_q_heads: int,
@@ -57,7 +57,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
     if t == 0 or b == 0:
         return out
     on_this_device(q, k_cache, v_cache, table, lens, start, seen, out)
-    size = _attention_scratch(head_dim)
+    size = _attention_scratch(head_dim, min(inp.max_q_len, draft.MOST_NODES) * (num_q_heads // hkv))
     scratch = k_cache.new_empty(size, dtype=torch.uint8)       # of this call: captured graphs and streams share none
     check(_lib.load().gllm_draft_attention(q_at, q_ts, out_at, k_at, v_at, pages, table.data_ptr(), table.stride(0), table.shape[1],
                                            lens.data_ptr(), start.data_ptr(), seen.data_ptr(), b, t, inp.max_q_len, num_q_heads, hkv,
