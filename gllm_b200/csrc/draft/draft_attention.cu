@@ -14,7 +14,7 @@
 //                      follows the maximum in steps of 2^8 and is handed on from tile to tile, so that their products add up in one O
 //   warp 8             copies: page boxes [page][64] of K and V -> ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V
 //   warp 9 (1 thread)  products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two)
-//   warps 10, 11       queries of the units to come (two buffers)
+//   warp 11 (1 thread) queries of the units to come (two buffers)
 //
 // Masks: only tiles that reach behind the context are masked, with the bits of the row's word shifted to the tile. A value that is not seen must
 // not reach the sum even as 0 x NaN: rows behind the last key are zeroed, and so are values of nodes that are no numbers; rows that see
@@ -42,7 +42,7 @@ struct DraftAttnParams {
   const int32_t* q_start;
   const int64_t* seen;
   int table_width, num_seqs, rows, Hq, Hkv, G, page_shift;   // a page has 2^page_shift tokens
-  int block_rows, part_rows;                             // of a block; rows that parts have room for
+  int block_rows, half_rows, part_rows;                  // of a block, of a box of queries; rows that parts have room for
   float scale_log2;
   float4* part_o;                                        // [2 CTA][D / 4][128 rows]
   float2* part_ml;                                       // [2 CTA][128 rows]: reference of the exponents, sum
@@ -51,7 +51,6 @@ struct DraftAttnParams {
 };
 
 inline int part_rows_of(int max_rows) { return max_rows > kRows ? 2 * kRows : kRows; }
-constexpr int block_rows_of(int rep) { return rep == 0 ? 2 * kRows : kRows / rep; }
 
 template <int D>
 struct DraftSmem {
@@ -117,7 +116,6 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
 }
 
 // What a sequence is to the units: rows [first, first + n) of the batch, ctx tokens before its nodes
-template <int BR>
 struct Seq {
   int first, n, ctx, len, tiles, blocks;
   __device__ __forceinline__ void set(const DraftAttnParams& p, int start, int end, int seq_len) {
@@ -126,21 +124,14 @@ struct Seq {
     n = max(min(n_all, kNodes), 0);
     ctx = min(max(seq_len - max(n_all, 0), 0), p.table_width << p.page_shift);
     len = min(ctx + n, p.table_width << p.page_shift);   // what the table holds
-    blocks = (n * p.G + BR - 1) / BR;
+    blocks = (n * p.G + p.block_rows - 1) / p.block_rows;
     tiles = n > 0 ? (len + kKeys - 1) / kKeys : 0;
   }
   __device__ __forceinline__ int work(const DraftAttnParams& p) const { return tiles * blocks * p.Hkv; }
 };
 
 // The CTA's items: its share of one unit each, tiles [t0, t1). What the next sequence is to be made of is on its way while this one's items run.
-template <int BR>
-struct Items : Seq<BR> {
-  using Seq<BR>::first;
-  using Seq<BR>::n;
-  using Seq<BR>::ctx;
-  using Seq<BR>::len;
-  using Seq<BR>::tiles;
-  using Seq<BR>::blocks;
+struct Items : Seq {
   const DraftAttnParams& p;
   int s;
   int off, left;                                         // in the sequence's work; tiles to come
@@ -148,7 +139,7 @@ struct Items : Seq<BR> {
   int end, next_end, next_len;                           // q_start[s + 1], q_start[s + 2], seq_lens[s + 1]
   __device__ __forceinline__ Items(const DraftAttnParams& p_, int s_, int off_, int left_) : p(p_), s(s_), off(off_), left(left_) {
     end = p.q_start[s + 1];
-    this->set(p, p.q_start[s], end, p.seq_lens[s]);
+    set(p, p.q_start[s], end, p.seq_lens[s]);
     ahead();
   }
   __device__ __forceinline__ void ahead() {
@@ -158,13 +149,13 @@ struct Items : Seq<BR> {
   }
   __device__ __forceinline__ bool next() {
     if (left <= 0) return false;
-    while (off >= this->work(p)) {                             // the sequence that `off` lies in: there is one, as tiles are left
+    while (off >= work(p)) {                             // the sequence that `off` lies in: there is one, as tiles are left
       off = 0;
       if (++s >= p.num_seqs) {
         left = 0;
         return false;
       }
-      this->set(p, end, next_end, next_len);
+      set(p, end, next_end, next_len);
       end = next_end;
       ahead();
     }
@@ -177,20 +168,21 @@ struct Items : Seq<BR> {
     left -= t1 - t0;
     return true;
   }
-  __device__ __forceinline__ int block_rows() const { return min(BR, n * p.G - blk * BR); }
+  __device__ __forceinline__ int block_rows() const { return min(p.block_rows, n * p.G - blk * p.block_rows); }
   // keys of tile t that there are
   __device__ __forceinline__ int keys(int t) const { return min(len - t * kKeys, kKeys); }
 };
 
 template <int D, int REP>
 __global__ void __launch_bounds__(kThreads, 1)
-draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const DraftAttnParams p) {
+draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q,
+                       const DraftAttnParams p) {
   using SM = DraftSmem<D>;
   constexpr int NS = SM::kStages;
-  // REP 1, 2, 4: a block of 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups take the tiles in turn.
-  // REP 0 (WIDE): a block of 256 rows, each warpgroup has 128 of them and every tile.
+  // A block's rows are whole nodes. REP 1, 2, 4: at most BR = 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups
+  // take the tiles in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them and every tile.
   constexpr bool WIDE = REP == 0;
-  constexpr int BR = block_rows_of(REP);
+  constexpr int BR = kRows / (WIDE ? 1 : REP);
   constexpr int kChunks = kKeys / 32 / (WIDE ? 1 : REP);              // of 32 keys that a lane has of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -230,7 +222,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
-  if (warp == 8 && lane < 2) tma_prefetch_desc(lane == 0 ? &tmap_k : &tmap_v);
+  if (warp == 8 && lane < 3) tma_prefetch_desc(lane == 0 ? &tmap_k : lane == 1 ? &tmap_v : &tmap_q);
   griddep_launch();
   griddep_wait();
 
@@ -238,7 +230,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   {
     const int per = (p.num_seqs + kThreads - 1) / kThreads, s0 = threadIdx.x * per, s1 = min(s0 + per, p.num_seqs);
     int64_t mine = 0;
-    Seq<BR> q;
+    Seq q;
     for (int s = s0; s < s1; ++s) {
       q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
       mine += q.work(p);
@@ -279,7 +271,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Items<BR> it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
+  Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
   const bool idle = begin[2] == 0;
 
   if (warp >= kSoftmaxWarps) {
@@ -351,7 +343,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if constexpr (WIDE) {
         uint32_t seen0 = 0, seen1 = 0, items1 = 0;           // tiles of each half so far; items that had a second half
         for (uint32_t item = 0; ok && it.next(); ++item) {
-          const int halves = it.block_rows() > kRows ? 2 : 1;
+          const int halves = it.block_rows() > p.half_rows ? 2 : 1;
           if (item == 0) ok = guard.first(&q_full[0]);
           ok = ok && wait(&q_full[0], item & 1);
           uint32_t k_pos = g == 0 ? 0 : 2 * g - 1;
@@ -437,41 +429,33 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
       umma_commit(mma_end);                                // nothing is in flight when the columns are given back
       guard.land(mma_end, 0);
-    } else if (warp == 11 && !idle) {
-      // ------------------------------------------------------------------ queries
-      for (uint32_t item = 0; it.next(); ++item) {
+    } else if (warp == 11 && lane == 0 && !idle) {
+      // ------------------------------------------------------------------ queries: a box is a block's (a half's) nodes x heads, 64 columns
+      uint32_t item = 0;
+      for (; it.next(); ++item) {
         const uint32_t buf = WIDE ? 0 : item & 1;
         if (WIDE) {                                        // both buffers have this item's rows
-          if (item >= 1 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[0], (item & 1) ^ 1))) break;
-        } else if (item >= 2 && !__all_sync(0xffffffffu, guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1))) {
+          if (item >= 1 && !guard.wait<true>(&q_free[0], (item & 1) ^ 1)) break;
+        } else if (item >= 2 && !guard.wait<true>(&q_free[buf], ((item >> 1) & 1) ^ 1)) {
           break;
         }
-        const int rows = it.block_rows();
-        const uint32_t dst = smem_u32(smem + buf * SM::kQBytes);
-        constexpr int kStep = 32 / (D / 8);                // rows of a round
-        const int c = lane % (D / 8);
-        int at = it.blk * BR + lane / (D / 8), node = at / p.G, h = at - node * p.G;
-        for (int r = lane / (D / 8); r < rows; r += kStep) {
-          const __nv_bfloat16* src = p.q + static_cast<int64_t>(it.first + node) * p.q_ts + static_cast<int64_t>(it.kvh * p.G + h) * D + c * 8;
-          for (h += kStep; h >= p.G; h -= p.G) ++node;
-#pragma unroll
-          for (int part = 0; part < (WIDE ? 1 : REP); ++part) {
-            const int l = part * BR + r;
-            const uint32_t to = dst + (WIDE && r >= kRows ? SM::kQBytes : 0) + (c >> 3) * (kRows * 128) + l % kRows * 128 + (((c & 7) ^ (l & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[buf]);
+        const int copies = WIDE ? (it.block_rows() > p.half_rows ? 2 : 1) : REP, nodes = p.half_rows / p.G;
+        const int node = it.first + it.blk * (p.block_rows / p.G);
+        mbar_expect_tx(&q_full[buf], copies * p.half_rows * D * 2);
+        for (int i = 0; i < copies; ++i)
+          for (int sl = 0; sl < D / 64; ++sl)
+            tma_load_3d(smem + (WIDE ? i : buf) * SM::kQBytes + sl * (kRows * 128) + (WIDE ? 0 : i * BR * 128), &tmap_q, &q_full[buf], sl * 64,
+                        it.kvh * p.G, node + (WIDE ? i * nodes : 0));
       }
+      // the last copies land, whichever role gave up (after a wait that did not, they have)
+      for (uint32_t i = WIDE ? (item >= 1 ? item - 1 : 0) : (item >= 2 ? item - 2 : 0); i < item; ++i)
+        guard.land(&q_full[WIDE ? 0 : i & 1], (WIDE ? i : i >> 1) & 1);
     }
   } else {
     // ------------------------------------------------------------------ softmax: one row a thread, the CTA's tiles in turn
     const int wg = warp >> 2, tl = threadIdx.x & 127;      // TMEM lane
     constexpr int kParts = WIDE ? 1 : REP;                 // lanes of a row
-    const int row = WIDE ? wg * kRows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
+    const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + wg * kKeys + lane_base;
     uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
@@ -491,14 +475,14 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
       if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
       const int rows = it.block_rows();
-      const bool warp_ok = row - lane < rows, row_ok = row < rows;
-      const int at = it.blk * BR + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
+      const bool row_ok = row < rows && (!WIDE || tl < p.half_rows), warp_ok = row - lane < rows && (!WIDE || tl - lane < p.half_rows);
+      const int at = it.blk * p.block_rows + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
       const int64_t tok = it.first + (row_ok ? node : 0);
       const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
       const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
       unsigned long long* bad_here = bad_nodes + (item & 3);
       const uint32_t t_o = tmem + SM::kTmemO + (WIDE ? wg : item & 1) * D + lane_base;
-      if (WIDE && wg * kRows >= rows) {                    // no second half
+      if (WIDE && wg * p.half_rows >= rows) {                    // no second half
         g += it.t1 - it.t0;
         continue;
       }
@@ -871,11 +855,25 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
     CUDA_CHECK_RET(cudaFuncSetAttribute(draft_attention_kernel<D, REP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes));
     configured.done();
   }
-  p.block_rows = block_rows_of(REP);
-  p.part_rows = part_rows_of(p.block_rows);
+  constexpr int most = kRows / (REP == 0 ? 1 : REP);
+  const int nodes = most / p.G;                            // of a box
+  p.half_rows = nodes * p.G;
+  p.block_rows = REP == 0 ? 2 * p.half_rows : p.half_rows;
+  p.part_rows = part_rows_of(max_rows);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(2) * ctas * (D / 4) * p.part_rows);
   p.cut = reinterpret_cast<int4*>(p.part_ml + static_cast<size_t>(2) * ctas * p.part_rows);
-  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, p));
+  CUtensorMap tq;                                          // queries [row][head][D]
+  const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(p.Hq), static_cast<cuuint64_t>(p.rows)};
+  const cuuint64_t strides[2] = {D * 2, static_cast<cuuint64_t>(p.q_ts) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(nodes)}, estr[3] = {1, 1, 1};
+  const CUresult r = get_encode_fn()(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(p.q), dims, strides, box, estr,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "[gllm_b200] query tensor-map encode failed (%d)\n", static_cast<int>(r));
+    return 1;
+  }
+  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, tq, p));
   const int rows = max_rows < p.block_rows ? max_rows : p.block_rows;
   CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
   return 0;
@@ -895,7 +893,7 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
                                      const void* seen, int num_seqs, int rows, int max_nodes, int Hq, int Hkv, int D, int page_size,
                                      float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (num_seqs <= 0 || rows <= 0 || max_nodes <= 0) return 0;
-  if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || page_size < 8 || kKeys % page_size || (page_size & (page_size - 1)) || pages <= 0 || table_width <= 0 || ctas <= 0 ||
+  if ((D != 64 && D != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > kRows || page_size < 8 || kKeys % page_size || (page_size & (page_size - 1)) || pages <= 0 || table_width <= 0 || ctas <= 0 ||
       q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
       scratch_bytes < gllm_draft_attention_scratch(D, (max_nodes < kNodes ? max_nodes : kNodes) * (Hq / Hkv), ctas))
     return 1;

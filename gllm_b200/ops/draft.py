@@ -39,6 +39,7 @@ from gllm_b200.ops import kv4
 MOST_NODES = 64
 PAGE_SIZES = (8, 16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
+MOST_GROUP = 128          # query heads a kv head
 
 
 # -- checks, the same on either device. What a common call passes comes first: a step makes one call a layer ---------------------

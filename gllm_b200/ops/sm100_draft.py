@@ -43,9 +43,10 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
     b, start, lens, table = draft.check_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out)
     pages, hkv, _, page_size, w = k_cache.shape
     t, q_ts = q.shape[0], q.stride(0)
-    if q.dtype is not _BF16 or w != 64 or head_dim not in draft.HEAD_DIMS or page_size not in draft.PAGE_SIZES:
-        raise ValueError(f"drafted tokens are attended in bf16, heads of 64 or 128, pages of 8 to 128 tokens (a power of two): got {q.dtype}, "
-                         f"heads of {head_dim}, pages of {page_size}")
+    if q.dtype is not _BF16 or w != 64 or head_dim not in draft.HEAD_DIMS or page_size not in draft.PAGE_SIZES or \
+            num_q_heads // hkv > draft.MOST_GROUP:
+        raise ValueError(f"drafted tokens are attended in bf16, heads of 64 or 128, at most {draft.MOST_GROUP} query heads a kv head, pages of 8 "
+                         f"to 128 tokens (a power of two): got {q.dtype}, {num_q_heads} / {hkv} heads of {head_dim}, pages of {page_size}")
     if t <= 1:
         q_ts = num_q_heads * head_dim                          # the stride of a dimension of one may be anything
     q_at, k_at, v_at = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()

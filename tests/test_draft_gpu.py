@@ -76,7 +76,8 @@ def _check_attention(x, scale=None, masks=None):
     ([100], [64], 8, 1, 64, 8, 0), ([120, 64, 0], [16, 64, 5], 7, 1, 128, 16, 8), ([700], [8], 32, 8, 128, 16, 0),
     ([5, 0, 31, 2, 300], [8, 0, 3, 1, 64], 6, 2, 64, 32, 0), ([1000, 3, 517], [13, 64, 2], 14, 2, 64, 64, 0), ([255, 256, 257], [7, 7, 7], 5, 5, 128, 128, 0),
     ([2000], [64], 64, 8, 128, 16, 0), ([1500] * 3, [40, 17, 64], 16, 1, 128, 16, 0), ([33] * 70, [3] * 70, 8, 2, 128, 16, 0),
-    ([5000, 1], [26, 26], 32, 4, 128, 16, 0), ([9000], [5], 8, 8, 64, 16, 0), ([4000], [1], 4, 1, 128, 16, 0),
+    ([5000, 1], [26, 26], 32, 4, 128, 16, 0), ([300, 90], [5, 2], 128, 1, 64, 16, 0), ([200, 700], [3, 64], 71, 1, 64, 16, 8), ([260], [40], 100, 2, 128, 32, 0),
+    ([500, 2, 1300], [43, 44, 9], 9, 3, 128, 16, 0), ([1000, 200], [22, 64], 12, 2, 128, 16, 8), ([130] * 30, [11] * 30, 6, 1, 64, 16, 0), ([9000], [5], 8, 8, 64, 16, 0), ([4000], [1], 4, 1, 128, 16, 0),
     ([17 * i % 900 for i in range(40)], [1 + i % 20 for i in range(40)], 10, 2, 64, 16, 0)])
 def test_attention(ctx, nodes, hq, hkv, d, page, extra):
     _check_attention(_attention_case(ctx, nodes, hq, hkv, d, page, extra=extra))
@@ -166,7 +167,8 @@ def test_attention_refuses_on_the_gpu():
     args = dict(q=x.q, k_cache=x.k, v_cache=x.v, inp=x.b, seen=x.seen, scale=0.1, num_q_heads=4, head_dim=64)
     wide = torch.zeros(kv_cache_shape(4, 1, 256, 16), dtype=BF16, device=DEV)
     odd = torch.zeros(kv_cache_shape(4, 2, 64, 24), dtype=BF16, device=DEV)
-    for over in [dict(q=torch.zeros(6, 264, dtype=BF16, device=DEV)[:, 1:257]), dict(q=torch.zeros(6, 257, dtype=BF16, device=DEV)[:, :256]),
+    many = torch.zeros(6, 129 * 64, dtype=BF16, device=DEV)
+    for over in [dict(q=many, k_cache=x.k[:, :1].contiguous(), v_cache=x.v[:, :1].contiguous(), num_q_heads=129), dict(q=torch.zeros(6, 264, dtype=BF16, device=DEV)[:, 1:257]), dict(q=torch.zeros(6, 257, dtype=BF16, device=DEV)[:, :256]),
                  dict(k_cache=odd, v_cache=odd), dict(k_cache=wide, v_cache=wide, num_q_heads=1, head_dim=256), dict(seen=x.seen.cpu()),
                  dict(k_cache=x.k.float(), v_cache=x.v.float(), q=x.q.float())]:
         with pytest.raises(ValueError):
