@@ -42,6 +42,7 @@ struct DraftAttnParams {
   const int32_t* q_start;
   const int64_t* seen;
   int table_width, num_seqs, rows, Hq, Hkv, G, page_shift;   // a page has 2^page_shift tokens
+  int whole;                                             // no unit is cut: nothing to join
   int block_rows, half_rows, part_rows;                  // of a block, of a box of queries; rows that parts have room for
   float scale_log2;
   float4* part_o;                                        // [2 CTA][D / 4][128 rows]
@@ -58,7 +59,7 @@ struct DraftSmem {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kRingOff = 2 * kQBytes, kBarOff = kRingOff + kStages * kTileBytes;
   // barriers, words and per-row floats (see the kernel), and up to 1 KB before the first 1024-byte boundary
-  static constexpr int kBarBytes = (2 * kStages + 25) * 8 + 8 + 4 * 8 + 4 * 8 + 12 * 8 + 3 * kRows * 4 + kStages * 4;
+  static constexpr int kBarBytes = (2 * kStages + 25) * 8 + 8 + 4 * 8 + 5 * 8 + 12 * 8 + 3 * kRows * 4 + kStages * 4;
   static constexpr int kBytes = kBarOff + (kBarBytes + 15) / 16 * 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr int kTmemO = 2 * kKeys, kTmemCols = 512;
@@ -200,8 +201,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   const WaitGuard guard{tmem_slot + 1, p.waits};
   unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [item % 4]
-  int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // sequence and offset that the share begins at, tiles, all tiles
-  int64_t* warp_work = begin + 4;                        // [12]
+  int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // share: first sequence, offset in it, end; all tiles; begin
+  int64_t* warp_work = begin + 5;                        // [12]
   float* m_ref = reinterpret_cast<float*>(warp_work + 12);            // [128 rows] reference of the exponents
   float* l_part = m_ref + kRows;                         // [item % 2][128 rows] sums of the warpgroup without an item's last tile
   volatile uint32_t* filled = reinterpret_cast<uint32_t*>(l_part + 2 * kRows);   // [NS] copies into a stage
@@ -218,7 +219,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     mbar_init(mma_end, 1);
     *guard.dead = 0;
-    begin[0] = begin[1] = begin[2] = 0;
+    begin[0] = begin[1] = begin[2] = begin[4] = 0;
     fence_mbar_init();
   }
   if (warp == 9) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
@@ -251,19 +252,30 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     // no more CTAs than tiles take part, so that no share between two others is empty
     const int64_t ctas = min(static_cast<int64_t>(gridDim.x), all);
-    const bool works = blockIdx.x < ctas;
-    const int64_t x0 = works ? all * blockIdx.x / ctas : 0, x1 = works ? all * (blockIdx.x + 1) / ctas : 0;
-    if (x0 < x1 && x0 >= before && x0 < before + mine) {
-      int s = s0;
-      for (;; ++s) {
-        q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
-        const int w = q.work(p);
-        if (x0 < before + w || s + 1 >= s1) break;
-        before += w;
+    if (blockIdx.x < ctas) {
+      const int64_t x[2] = {all * blockIdx.x / ctas, all * (blockIdx.x + 1) / ctas};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {                        // where the share begins and ends; WHOLE: at the next unit's first tile
+        if (x[i] < before || x[i] >= before + mine) continue;
+        int64_t at = before;
+        int s = s0;
+        for (;; ++s) {
+          q.set(p, p.q_start[s], p.q_start[s + 1], p.seq_lens[s]);
+          const int w = q.work(p);
+          if (x[i] < at + w || s + 1 >= s1) break;
+          at += w;
+        }
+        int off = static_cast<int>(x[i] - at);
+        if (p.whole) off = (off + q.tiles - 1) / q.tiles * q.tiles;
+        if (i == 0) {
+          begin[0] = s;
+          begin[1] = off;
+          begin[4] = at + off;
+        } else {
+          begin[2] = at + off;
+        }
       }
-      begin[0] = s;
-      begin[1] = x0 - before;
-      begin[2] = x1 - x0;
+      if (threadIdx.x == 0 && x[1] == all) begin[2] = all;
     }
     if (threadIdx.x == 0) begin[3] = all;
   }
@@ -271,8 +283,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2]));
-  const bool idle = begin[2] == 0;
+  Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2] - begin[4]));
+  const bool idle = begin[2] <= begin[4];
 
   if (warp >= kSoftmaxWarps) {
     if ((warp == 8 || warp == 10) && !idle) {
@@ -780,7 +792,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
       }
     }
-    if (threadIdx.x == 0 && !cut_tail) p.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);   // no unit begins here that ends elsewhere
+    if (threadIdx.x == 0 && !cut_tail && !p.whole) p.cut[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);   // no unit begins here that ends elsewhere
   }
   tc_fence_before();
   __syncthreads();
@@ -874,6 +886,7 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
     return 1;
   }
   CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, tq, p));
+  if (p.whole) return 0;
   const int rows = max_rows < p.block_rows ? max_rows : p.block_rows;
   CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
   return 0;
@@ -890,12 +903,13 @@ GLLM_EXPORT int64_t gllm_draft_attention_scratch(int D, int max_rows, int ctas) 
 
 GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, const void* k_cache, const void* v_cache, int64_t pages,
                                      const void* table, int64_t table_ld, int table_width, const void* seq_lens, const void* q_start,
-                                     const void* seen, int num_seqs, int rows, int max_nodes, int Hq, int Hkv, int D, int page_size,
-                                     float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
+                                     const void* seen, int num_seqs, int rows, int max_nodes, int whole, int Hq, int Hkv, int D,
+                                     int page_size, float scale, int ctas, void* scratch, int64_t scratch_bytes, void* stream) {
   if (num_seqs <= 0 || rows <= 0 || max_nodes <= 0) return 0;
   if ((D != 64 && D != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > kRows || page_size < 8 || kKeys % page_size || (page_size & (page_size - 1)) || pages <= 0 || table_width <= 0 || ctas <= 0 ||
-      q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) ||
-      scratch_bytes < gllm_draft_attention_scratch(D, (max_nodes < kNodes ? max_nodes : kNodes) * (Hq / Hkv), ctas))
+      q_ts % 8 || (reinterpret_cast<uintptr_t>(q) & 15))
+    return 1;
+  if (!whole && ((reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < gllm_draft_attention_scratch(D, (max_nodes < kNodes ? max_nodes : kNodes) * (Hq / Hkv), ctas)))
     return 1;
   CUtensorMap tk, tv;
   if (page_tmap(k_cache, pages, Hkv, D, page_size, &tk) || page_tmap(v_cache, pages, Hkv, D, page_size, &tv)) return 1;
@@ -911,6 +925,7 @@ GLLM_EXPORT int gllm_draft_attention(const void* q, int64_t q_ts, void* out, con
   p.num_seqs = num_seqs; p.rows = rows; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   p.page_shift = 31 - __builtin_clz(static_cast<unsigned>(page_size));
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.whole = whole;
   p.part_o = reinterpret_cast<float4*>(scratch);
   p.part_ml = nullptr;
   p.cut = nullptr;

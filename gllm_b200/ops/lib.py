@@ -102,7 +102,7 @@ def _declare(lib):
     sig("gllm_gemm_fp8_block", [P, P, P, P, P, L, I, I, I, P, I, P])
     sig("gllm_draft_plan", [P, P, P, P, L, I, I, I, I, P, P, P, P])
     sig("gllm_draft_attention_scratch", [I, I, I], L)
-    sig("gllm_draft_attention", [P, L, P, P, P, L, P, L, I, P, P, P, I, I, I, I, I, I, I, F, I, P, L, P])
+    sig("gllm_draft_attention", [P, L, P, P, P, L, P, L, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P])
     sig("gllm_draft_verify", [P, P, P, P, P, L, P, L, P, I, I, I, P, P, P, I, P])
     sig("gllm_draft_keep", [P, I, L, I, I, I, P, P, P, P, P, L, I, I, I, P])
 
