@@ -887,8 +887,7 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
   }
   CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, tq, p));
   if (p.whole) return 0;
-  const int rows = max_rows < p.block_rows ? max_rows : p.block_rows;
-  CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
+  CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (p.block_rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
   return 0;
 }
 

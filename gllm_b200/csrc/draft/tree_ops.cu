@@ -99,7 +99,7 @@ draft_keep_kernel(const __grid_constant__ CachePtrs caches, const KeepParams p) 
   __shared__ int64_t from[kMostNodes], to[kMostNodes];   // rows, counted in slab rows of a page: (page * slabs * page_size + row)
   __shared__ int moves;
   griddep_wait();
-  const int seq = blockIdx.y;
+  const int seq = blockIdx.x;
   const int first = p.q_start[seq], n_all = min(p.q_start[seq + 1], p.rows) - first;
   if (first < 0 || n_all <= 0) return;
   const int n = min(n_all, kMostNodes), ctx = max(p.seq_lens[seq] - n_all, 0), taken = min(p.count[seq], n);
@@ -134,7 +134,7 @@ draft_keep_kernel(const __grid_constant__ CachePtrs caches, const KeepParams p) 
   }
   __syncthreads();
   const int total = moves, columns = p.slabs * p.words;
-  uint4* cache = caches.at[blockIdx.x];
+  uint4* cache = caches.at[blockIdx.y];
   for (int c = threadIdx.x; c < columns; c += kKeepThreads) {
     const int slab = c / p.words, w = c - slab * p.words;
     uint4* base = cache + static_cast<int64_t>(slab) * p.page_size * p.words + w;
@@ -173,7 +173,7 @@ GLLM_EXPORT int gllm_draft_keep(const void* const* caches, int n, int64_t pages,
                                 const void* count, const void* q_start, const void* seq_lens, const void* table, int64_t table_ld,
                                 int table_width, int num_seqs, int rows, void* stream) {
   if (n <= 0 || num_seqs <= 0 || rows <= 0 || slabs <= 0 || words <= 0) return 0;
-  if (n > kMostCaches || num_seqs > 65535 || page_size < 1) return 1;
+  if (n > kMostCaches || page_size < 1) return 1;
   CachePtrs ptrs;
   for (int i = 0; i < n; ++i) ptrs.at[i] = reinterpret_cast<uint4*>(const_cast<void*>(caches[i]));
   KeepParams p;
@@ -184,6 +184,6 @@ GLLM_EXPORT int gllm_draft_keep(const void* const* caches, int n, int64_t pages,
   p.table = reinterpret_cast<const int32_t*>(table);
   p.table_ld = table_ld; p.pages = pages;
   p.table_width = table_width; p.rows = rows; p.page_size = page_size; p.slabs = slabs; p.words = words;
-  CUDA_CHECK_RET(launch_pdl(draft_keep_kernel, dim3(n, num_seqs), dim3(kKeepThreads), 0, reinterpret_cast<cudaStream_t>(stream), ptrs, p));
+  CUDA_CHECK_RET(launch_pdl(draft_keep_kernel, dim3(num_seqs, n), dim3(kKeepThreads), 0, reinterpret_cast<cudaStream_t>(stream), ptrs, p));
   return 0;
 }

@@ -88,8 +88,8 @@ def check_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim
     if len(shape) != 5 or v_cache.shape != shape or not k_cache.dtype is v_cache.dtype is q.dtype:
         raise ValueError(f"caches [pages, heads, slabs, page, slab] of the queries' type: got {tuple(shape)}, {tuple(v_cache.shape)}, "
                          f"{k_cache.dtype}, {v_cache.dtype}, {q.dtype}")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError("caches are contiguous")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or shape[0] < 1 or batch[3].shape[1] < 1:
+        raise ValueError("caches are contiguous and have pages, block_table has columns")
     _, hkv, slabs, _, w = shape
     rows, width = q.shape if q.dim() == 2 else (0, -1)
     if slabs * w != head_dim or num_q_heads % hkv or width < num_q_heads * head_dim or q.stride(1) != 1:

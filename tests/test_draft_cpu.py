@@ -135,7 +135,7 @@ def test_attention_refuses():
     Fn.draft_attention(**ok)
     four = torch.zeros(kv4.cache_shape(4, 2, 64, 16), dtype=torch.uint8)
     bad = [dict(k_cache=four, v_cache=four), dict(k_cache=ok["k_cache"].float()), dict(q=ok["q"].float()), dict(v_cache=ok["v_cache"][:1]),
-           dict(k_cache=ok["k_cache"][..., ::2]), dict(num_q_heads=3), dict(head_dim=128), dict(q=ok["q"][:, :128]), dict(seen=ok["seen"].to(I32)),
+           dict(k_cache=ok["k_cache"][..., ::2]), dict(k_cache=ok["k_cache"][:0], v_cache=ok["v_cache"][:0]), dict(num_q_heads=3), dict(head_dim=128), dict(q=ok["q"][:, :128]), dict(seen=ok["seen"].to(I32)),
            dict(seen=ok["seen"][:2]), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
            dict(out=torch.zeros(3, 256)), dict(out=torch.zeros(2, 256, dtype=BF16)), dict(out=torch.zeros(3, 512, dtype=BF16)[:, ::2])]
     for over in bad:
