@@ -53,6 +53,8 @@ struct DraftAttnParams {
 
 inline int part_rows_of(int max_rows) { return max_rows > kRows ? 2 * kRows : kRows; }
 
+constexpr bool solo_of(int d, int rep) { return d == 128 && rep >= 2; }
+
 template <int D>
 struct DraftSmem {
   static constexpr int kQBytes = kRows * D * 2, kTileBytes = kKeys * D * 2;
@@ -183,6 +185,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   // A block's rows are whole nodes. REP 1, 2, 4: at most BR = 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups
   // take the tiles in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them and every tile.
   constexpr bool WIDE = REP == 0;
+  // The warpgroups take items in turn, not tiles
+  constexpr bool SOLO = solo_of(D, REP);
   constexpr int BR = kRows / (WIDE ? 1 : REP);
   constexpr int kChunks = kKeys / 32 / (WIDE ? 1 : REP);              // of 32 keys that a lane has of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -198,6 +202,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint64_t* m_set = q_free + 2;                          // [2 warpgroups][4 warps] references of tile g, by its warpgroup
   uint64_t* l_set = m_set + 8;                           // [2 warpgroups][item % 2] its part of an item's sums, for the one with the last tile (4 warps)
   uint64_t* mma_end = l_set + 4;
+  uint64_t* s_solo = m_set;                              // SOLO: [2 warpgroups][2] S of the warpgroup's k-th tile: barrier k % 2; pv_full by warpgroup
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   const WaitGuard guard{tmem_slot + 1, p.waits};
   unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [item % 4]
@@ -327,6 +332,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return guard.wait<true>(bar, parity); };
       // S in buffer s_buf from the queries in buffer q_buf and the tile in stage st
+      uint32_t own0 = 0, own1 = 0;                         // SOLO: tiles of either warpgroup
       auto issue_s = [&](uint32_t s_buf, uint32_t q_buf, uint32_t st) {
         const uint32_t q_addr = smem_u32(smem + q_buf * SM::kQBytes), k_addr = smem_u32(smem + SM::kRingOff + st * SM::kTileBytes);
         const uint32_t d_tmem = tmem + s_buf * kKeys;
@@ -336,7 +342,13 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_bf16<1>(d_tmem, da + kk * 2, db + kk * 2, idesc_s, (kd | kk) != 0);
         }
-        umma_commit(&s_full[s_buf]);
+        if (SOLO) {
+          uint32_t& own = q_buf == 0 ? own0 : own1;
+          umma_commit(&s_solo[2 * q_buf + (own & 1)]);
+          ++own;
+        } else {
+          umma_commit(&s_full[s_buf]);
+        }
       };
       // P in buffer s_buf times the tile in stage st, added to O in o_buf: the steps of 16 keys that there are
       auto issue_pv = [&](uint32_t s_buf, uint32_t o_buf, uint32_t st, int keys, uint32_t acc) {
@@ -350,7 +362,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           for (int kk = 0; kk < (keys + 15) / 16; ++kk)
             umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
         }
-        umma_commit(&pv_full[s_buf]);
+        umma_commit(&pv_full[SOLO ? o_buf : s_buf]);
       };
       if constexpr (WIDE) {
         uint32_t seen0 = 0, seen1 = 0, items1 = 0;           // tiles of each half so far; items that had a second half
@@ -469,9 +481,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     constexpr int kParts = WIDE ? 1 : REP;                 // lanes of a row
     const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + wg * kKeys + lane_base;
     uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
-    uint32_t mine = 0;                                     // WIDE: tiles of this half
+    uint32_t mine = 0;                                     // WIDE, SOLO: tiles of this warpgroup
     bool cut_tail = false;
     // A wait that gives up leaves the warps in step: they go on with what is there, and every later wait ends at once
     auto await = [&](uint64_t* bar, uint32_t parity) {
@@ -498,12 +509,18 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         g += it.t1 - it.t0;
         continue;
       }
+      if (SOLO && (item & 1) != static_cast<uint32_t>(wg)) {
+        g += it.t1 - it.t0;
+        continue;
+      }
       float m_run = -INFINITY, l_run = 0.f;                // reference of this warpgroup's sum, the sum
       float m_old = -INFINITY;                             // reference of the tile before this warpgroup's last
       for (int t = it.t0; t < it.t1; ++t, ++g) {
-        if (!WIDE && (g & 1) != static_cast<uint32_t>(wg)) continue;
+        if (!WIDE && !SOLO && (g & 1) != static_cast<uint32_t>(wg)) continue;
         const int key0 = t * kKeys;
-        await(&s_full[wg], (WIDE ? mine : g >> 1) & 1);
+        const uint32_t s_buf = SOLO ? g & 1 : wg, t_s = tmem + s_buf * kKeys + lane_base;
+        if (SOLO) await(&s_solo[2 * wg + (mine & 1)], (mine >> 1) & 1);
+        else await(&s_full[wg], (WIDE ? mine : g >> 1) & 1);
         const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
         float mx = -INFINITY;
         // 32 scores at a time in loops that are not unrolled: the warps are at different places of the code, and what is not in the instruction
@@ -544,7 +561,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           mx *= p.scale_log2;
         }
         float m_now;
-        if (WIDE) {
+        if (WIDE || SOLO) {
           m_old = m_run;
           m_now = mx > m_old + kLazy ? mx : m_old;
         } else {
@@ -565,7 +582,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           if (t > it.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             // O is free when the product before this tile's has ended. (S of this tile was formed behind the one before that: the phase
             // before the awaited one has passed, the one behind it needs this tile's P. WIDE: S was formed behind that product.)
-            if (!WIDE) await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
+            if (SOLO) await(&pv_full[wg], (mine - 1) & 1);
+            else if (!WIDE) await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t v[16];
@@ -634,18 +652,18 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
         tc_fence_before();                                 // P and the rescaled O are in TMEM, S has been read
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (lane == 0) mbar_arrive(&p_full[s_buf]);
         ++mine;
-        if (!WIDE && t + 2 == it.t1) {                     // the item's last tile is the other warpgroup's
+        if (!WIDE && !SOLO && t + 2 == it.t1) {                     // the item's last tile is the other warpgroup's
           *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) = l_run;
           __syncwarp();
           if (lane == 0) mbar_arrive(&l_set[2 * wg + (item & 1)]);
         }
       }
-      if (!WIDE && ((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
+      if (!WIDE && !SOLO && ((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
       // ---- results, by the warpgroup that had the last tile; the other one goes on
-      await(&pv_full[wg], (WIDE ? mine - 1 : (g - 1) >> 1) & 1);
-      if (!WIDE && it.t1 - it.t0 > 1) {
+      await(&pv_full[wg], (WIDE || SOLO ? mine - 1 : (g - 1) >> 1) & 1);
+      if (!WIDE && !SOLO && it.t1 - it.t0 > 1) {
         // Of an item of this parity: the other one may have set that of the next item already, should that have two tiles
         await(&l_set[2 * (wg ^ 1) + (item & 1)], (sums >> (item & 1)) & 1);
         sums ^= 1u << (item & 1);
