@@ -1,24 +1,33 @@
 // Attention of drafted nodes over a paged bf16 cache. Definition: ops/draft.py.
 //
-// A kv head's rows are node x query head, in blocks of 128: a block's scores S = Q K^T and results O += P V are tcgen05 products with all
-// of M = 128, whatever the rows; that costs the tensor core 1024 cycles per 128 keys (heads of 128), where their bytes take some 2700 of an
-// SM's share of the memory, so few rows waste nothing that is missed.
+// Work: a unit is a sequence, a kv head and a block of its rows (node x query head), as long as the sequence's 128-key tiles. A block's scores
+// S = Q K^T and results O += P V are tcgen05 products of M = 128, whatever the rows: 1024 cycles of tensor core per 128 keys (heads of 128),
+// where their 64 KB take some 2700 of an SM's share of the memory. All units lie in one row that is cut into equal shares for the CTAs, one an
+// SM, on the device, so that lengths may differ from those at the time a graph was captured and long contexts beside short ones leave no SM
+// idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined by a second launch in a
+// fixed order. Or no unit is cut, where that costs less (ops/sm100_draft.py).
 //
-// Work: units (sequence, kv head, block of rows), each as long as its sequence's 128-key tiles. All units lie in one row that is cut into
-// equal shares for the CTAs, one an SM, on the device: lengths may differ from those at the time a graph was captured, and long contexts
-// beside short ones leave no SM idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined
-// by a second launch in a fixed order.
+// Rows, by what a sequence may have (host):  up to 32, 64, 128  one block; with few rows 4 or 2 TMEM lanes share a row, each has a part of
+// every tile's keys, so that all four schedulers form exponentials (a lane's 128 take a warp 1700 cycles and more, 32 take 650).
+// More: blocks of two halves of 128, a warpgroup each, so that keys and values are read once for 256 rows.
 //
-//   warps 0-3, 4-7     softmax, one row a thread (tcgen05.ld 32x32b): the CTA's tiles in turn. A tile takes a warpgroup some 2 us, most of it
-//                      latency of its steps one after the other, where its bytes take 1.5. Both have one reference of the exponents, which
-//                      follows the maximum in steps of 2^8 and is handed on from tile to tile, so that their products add up in one O
-//   warp 8             copies: page boxes [page][64] of K and V -> ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V
+//   warps 0-3, 4-7     softmax, a row a lane (tcgen05.ld 32x32b), the CTA's items in turn: one's results, some 3000 cycles of which most is
+//                      instruction fetch, are written while the other has the next one. (Tiles in turn, with one reference of the
+//                      exponents handed on: 128 x 600 tokens, 24 nodes, 32 / 8 heads 79 us, items 69; one long item an SM no faster.) The
+//                      reference follows the maximum in steps of 2^8; P goes over S, as the A operand of the product with V
+//   warps 8, 10        copies of K and V: page boxes [page][64] -> one ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V. (One
+//                      warp for both issues 32 boxes of 2 KB in 3300 cycles, more than their bytes take)
 //   warp 9 (1 thread)  products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two)
-//   warp 11 (1 thread) queries of the units to come (two buffers)
+//   warp 11 (1 thread) queries, a box a block, of the items to come (two buffers)
 //
 // Masks: only tiles that reach behind the context are masked, with the bits of the row's word shifted to the tile. A value that is not seen must
 // not reach the sum even as 0 x NaN: rows behind the last key are zeroed, and so are values of nodes that are no numbers; rows that see
 // those have them added at the end.
+//
+// What bounds it: HBM where histories are long (two of 60,000, 64 / 8 heads, 16 nodes: 84 us for 61 of bytes; 64 of 2500, 8 nodes 91 for 74;
+// some 10 us are the first data and the last results). Blocks of 256 rows: the chain softmax (2300 cycles) -> P V -> S of a half, 4050 cycles
+// per 128 keys for 2048 of tensor core and of the 2^x unit each (4 of 30,000, 64 nodes, 64 / 8 heads: 173 us, 740 TFLOP/s). Steps of 64 keys
+// with two buffers of S a half were slower (278): twice the products and commits of the one issuing thread.
 #include "../attn/attn_common.cuh"
 #include "../common/bounded.cuh"
 
@@ -53,15 +62,13 @@ struct DraftAttnParams {
 
 inline int part_rows_of(int max_rows) { return max_rows > kRows ? 2 * kRows : kRows; }
 
-constexpr bool solo_of(int d, int rep) { return d == 128 && rep >= 2; }
-
 template <int D>
 struct DraftSmem {
   static constexpr int kQBytes = kRows * D * 2, kTileBytes = kKeys * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kRingOff = 2 * kQBytes, kBarOff = kRingOff + kStages * kTileBytes;
-  // barriers, words and per-row floats (see the kernel), and up to 1 KB before the first 1024-byte boundary
-  static constexpr int kBarBytes = (2 * kStages + 25) * 8 + 8 + 4 * 8 + 5 * 8 + 12 * 8 + 3 * kRows * 4 + kStages * 4;
+  // barriers and words (see the kernel), and up to 1 KB before the first 1024-byte boundary
+  static constexpr int kBarBytes = (2 * kStages + 17) * 8 + 8 + 4 * 8 + 5 * 8 + 12 * 8 + kStages * 4;
   static constexpr int kBytes = kBarOff + (kBarBytes + 15) / 16 * 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr int kTmemO = 2 * kKeys, kTmemCols = 512;
@@ -183,44 +190,35 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   using SM = DraftSmem<D>;
   constexpr int NS = SM::kStages;
   // A block's rows are whole nodes. REP 1, 2, 4: at most BR = 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups
-  // take the tiles in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them and every tile.
+  // take the items in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them of every item.
   constexpr bool WIDE = REP == 0;
-  // The warpgroups take items in turn, not tiles
-  constexpr bool SOLO = solo_of(D, REP);
   constexpr int BR = kRows / (WIDE ? 1 : REP);
   constexpr int kChunks = kKeys / 32 / (WIDE ? 1 : REP);              // of 32 keys that a lane has of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
   uint64_t* empty = full + NS;                           // [NS] products -> copies
-  uint64_t* s_full = empty + NS;                         // [2] S of the CTA's tile g: barrier g % 2
-  uint64_t* p_full = s_full + 2;                         // [2] P of tile g written (4 warps)
-  uint64_t* pv_full = p_full + 2;                        // [2] P V of tile g is in O
-  uint64_t* o_free = pv_full + 2;                        // [2] O of item i has been read (4 warps): barrier i % 2
-  uint64_t* q_full = o_free + 2;                         // [2] queries of item i
+  uint64_t* s_full = empty + NS;                         // [2 warpgroups][2] S of the warpgroup's k-th tile: barrier k % 2 (WIDE: the first)
+  uint64_t* p_full = s_full + 4;                         // [2] P of the CTA's tile g written (4 warps): barrier g % 2 (WIDE: of a half)
+  uint64_t* pv_full = p_full + 2;                        // [2 warpgroups][2] P V of its k-th tile is in O: barrier k % 2 (WIDE: the first)
+  uint64_t* o_free = pv_full + 4;                        // [2 warpgroups] O of its item has been read (4 warps)
+  uint64_t* q_full = o_free + 2;                         // [2] queries of item i: barrier i % 2 (WIDE: the first)
   uint64_t* q_free = q_full + 2;                         // [2]
-  uint64_t* m_set = q_free + 2;                          // [2 warpgroups][4 warps] references of tile g, by its warpgroup
-  uint64_t* l_set = m_set + 8;                           // [2 warpgroups][item % 2] its part of an item's sums, for the one with the last tile (4 warps)
-  uint64_t* mma_end = l_set + 4;
-  uint64_t* s_solo = m_set;                              // SOLO: [2 warpgroups][2] S of the warpgroup's k-th tile: barrier k % 2; pv_full by warpgroup
+  uint64_t* mma_end = q_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   const WaitGuard guard{tmem_slot + 1, p.waits};
   unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [item % 4]
   int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // share: first sequence, offset in it, end; all tiles; begin
   int64_t* warp_work = begin + 5;                        // [12]
-  float* m_ref = reinterpret_cast<float*>(warp_work + 12);            // [128 rows] reference of the exponents
-  float* l_part = m_ref + kRows;                         // [item % 2][128 rows] sums of the warpgroup without an item's last tile
-  volatile uint32_t* filled = reinterpret_cast<uint32_t*>(l_part + 2 * kRows);   // [NS] copies into a stage
+  volatile uint32_t* filled = reinterpret_cast<uint32_t*>(warp_work + 12);   // [NS] copies into a stage
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); filled[i] = 0; }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_full[i], 1); mbar_init(&o_free[i], 4);
-      mbar_init(&l_set[2 * i], 4); mbar_init(&l_set[2 * i + 1], 4);
-      mbar_init(&q_full[i], 1); mbar_init(&q_free[i], REP > 1 ? 2 : 1);
+      mbar_init(&s_full[2 * i], 1); mbar_init(&s_full[2 * i + 1], 1); mbar_init(&p_full[i], 4);
+      mbar_init(&pv_full[2 * i], 1); mbar_init(&pv_full[2 * i + 1], 1); mbar_init(&o_free[i], 4); mbar_init(&q_full[i], 1); mbar_init(&q_free[i], REP > 1 ? 2 : 1);
       bad_nodes[2 * i] = bad_nodes[2 * i + 1] = 0ull;
-      for (int w = 0; w < 4; ++w) mbar_init(&m_set[4 * i + w], 1);
     }
     mbar_init(mma_end, 1);
     *guard.dead = 0;
@@ -332,7 +330,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return guard.wait<true>(bar, parity); };
       // S in buffer s_buf from the queries in buffer q_buf and the tile in stage st
-      uint32_t own0 = 0, own1 = 0;                         // SOLO: tiles of either warpgroup
+      uint32_t own0 = 0, own1 = 0, own_pv0 = 0, own_pv1 = 0;   // tiles of either warpgroup whose S, whose P V has been issued
       auto issue_s = [&](uint32_t s_buf, uint32_t q_buf, uint32_t st) {
         const uint32_t q_addr = smem_u32(smem + q_buf * SM::kQBytes), k_addr = smem_u32(smem + SM::kRingOff + st * SM::kTileBytes);
         const uint32_t d_tmem = tmem + s_buf * kKeys;
@@ -342,13 +340,9 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_bf16<1>(d_tmem, da + kk * 2, db + kk * 2, idesc_s, (kd | kk) != 0);
         }
-        if (SOLO) {
-          uint32_t& own = q_buf == 0 ? own0 : own1;
-          umma_commit(&s_solo[2 * q_buf + (own & 1)]);
-          ++own;
-        } else {
-          umma_commit(&s_full[s_buf]);
-        }
+        uint32_t& own = q_buf == 0 ? own0 : own1;          // the queries' buffer goes with the warpgroup
+        umma_commit(&s_full[2 * q_buf + (WIDE ? 0 : own & 1)]);
+        ++own;
       };
       // P in buffer s_buf times the tile in stage st, added to O in o_buf: the steps of 16 keys that there are
       auto issue_pv = [&](uint32_t s_buf, uint32_t o_buf, uint32_t st, int keys, uint32_t acc) {
@@ -362,7 +356,9 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           for (int kk = 0; kk < (keys + 15) / 16; ++kk)
             umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
         }
-        umma_commit(&pv_full[SOLO ? o_buf : s_buf]);
+        uint32_t& own = o_buf == 0 ? own_pv0 : own_pv1;
+        umma_commit(&pv_full[2 * o_buf + (WIDE ? 0 : own & 1)]);
+        ++own;
       };
       if constexpr (WIDE) {
         uint32_t seen0 = 0, seen1 = 0, items1 = 0;           // tiles of each half so far; items that had a second half
@@ -476,19 +472,24 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         guard.land(&q_full[WIDE ? 0 : i & 1], (WIDE ? i : i >> 1) & 1);
     }
   } else {
-    // ------------------------------------------------------------------ softmax: one row a thread, the CTA's tiles in turn
+    // ------------------------------------------------------------------ softmax
     const int wg = warp >> 2, tl = threadIdx.x & 127;      // TMEM lane
     constexpr int kParts = WIDE ? 1 : REP;                 // lanes of a row
     const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint32_t g = 0, sums = 0;                              // tile; parities of the other warpgroup's l_set
-    uint32_t mine = 0;                                     // WIDE, SOLO: tiles of this warpgroup
+    uint32_t g = 0, mine = 0;                              // tile of the CTA, of this warpgroup
     bool cut_tail = false;
     // A wait that gives up leaves the warps in step: they go on with what is there, and every later wait ends at once
     auto await = [&](uint64_t* bar, uint32_t parity) {
       guard.wait<true>(bar, parity);
       __syncwarp();
       tc_fence_after();
+    };
+    // P V of the warpgroup's tile k. A wait tells a phase from the next one only: tile k + 2 needs this warpgroup's P, and S of tile k + 1, or of
+    // tile k itself, which it has, was formed behind P V of tile k - 2 (WIDE: k - 1), the phase before.
+    auto await_pv = [&](uint32_t k) {
+      if (WIDE) await(&pv_full[2 * wg], k & 1);
+      else await(&pv_full[2 * wg + (k & 1)], (k >> 1) & 1);
     };
     auto sync_group = [&] {
       if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -504,23 +505,17 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
       const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
       unsigned long long* bad_here = bad_nodes + (item & 3);
-      const uint32_t t_o = tmem + SM::kTmemO + (WIDE ? wg : item & 1) * D + lane_base;
-      if (WIDE && wg * p.half_rows >= rows) {                    // no second half
+      const uint32_t t_o = tmem + SM::kTmemO + wg * D + lane_base;
+      if (WIDE ? wg * p.half_rows >= rows : (item & 1) != static_cast<uint32_t>(wg)) {   // no second half; the other's
         g += it.t1 - it.t0;
         continue;
       }
-      if (SOLO && (item & 1) != static_cast<uint32_t>(wg)) {
-        g += it.t1 - it.t0;
-        continue;
-      }
-      float m_run = -INFINITY, l_run = 0.f;                // reference of this warpgroup's sum, the sum
-      float m_old = -INFINITY;                             // reference of the tile before this warpgroup's last
+      float m_run = -INFINITY, l_run = 0.f;                // reference of the exponents, their sum
       for (int t = it.t0; t < it.t1; ++t, ++g) {
-        if (!WIDE && !SOLO && (g & 1) != static_cast<uint32_t>(wg)) continue;
         const int key0 = t * kKeys;
-        const uint32_t s_buf = SOLO ? g & 1 : wg, t_s = tmem + s_buf * kKeys + lane_base;
-        if (SOLO) await(&s_solo[2 * wg + (mine & 1)], (mine >> 1) & 1);
-        else await(&s_full[wg], (WIDE ? mine : g >> 1) & 1);
+        const uint32_t s_buf = WIDE ? wg : g & 1, t_s = tmem + s_buf * kKeys + lane_base;
+        if (WIDE) await(&s_full[2 * wg], mine & 1);
+        else await(&s_full[2 * wg + (mine & 1)], (mine >> 1) & 1);
         const bool behind = key0 + kKeys > it.ctx;         // the tile has nodes, or ends behind the last key
         float mx = -INFINITY;
         // 32 scores at a time in loops that are not unrolled: the warps are at different places of the code, and what is not in the instruction
@@ -559,31 +554,15 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           if (kChunks > 1 && behind) tmem_store_wait();
           mx *= p.scale_log2;
-        }
-        float m_now;
-        if (WIDE || SOLO) {
-          m_old = m_run;
-          m_now = mx > m_old + kLazy ? mx : m_old;
-        } else {
-          // The reference of both warpgroups: the other's of the tile before, raised where this tile's maximum is 2^8 over it
-          if (g > 0) await(&m_set[4 * (wg ^ 1) + (warp & 3)], ((g - 1) >> 1) & 1);
-          m_old = t > it.t0 ? *static_cast<volatile float*>(m_ref + tl) : -INFINITY;
-          m_now = mx > m_old + kLazy ? mx : m_old;
-          *static_cast<volatile float*>(m_ref + tl) = m_now;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&m_set[4 * wg + (warp & 3)]);
-        }
-        if (warp_ok) {
-          const float alpha = m_now != m_old ? ex2(m_old - m_now) : 1.f;
-          if (m_now != m_run) {                            // this warpgroup's sum, from the reference of two tiles ago
-            l_run *= ex2(m_run - m_now);
-            m_run = m_now;
+          float alpha = 1.f;
+          if (mx > m_run + kLazy) {
+            alpha = ex2(m_run - mx);
+            m_run = mx;
+            l_run *= alpha;
           }
           if (t > it.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // O is free when the product before this tile's has ended. (S of this tile was formed behind the one before that: the phase
-            // before the awaited one has passed, the one behind it needs this tile's P. WIDE: S was formed behind that product.)
-            if (SOLO) await(&pv_full[wg], (mine - 1) & 1);
-            else if (!WIDE) await(&pv_full[wg ^ 1], ((g - 1) >> 1) & 1);
+            // O is free when the product of the warpgroup's tile before has ended (WIDE: S of this tile was formed behind it)
+            if (!WIDE) await_pv(mine - 1);
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t v[16];
@@ -654,29 +633,15 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[s_buf]);
         ++mine;
-        if (!WIDE && !SOLO && t + 2 == it.t1) {                     // the item's last tile is the other warpgroup's
-          *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) = l_run;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&l_set[2 * wg + (item & 1)]);
-        }
       }
-      if (!WIDE && !SOLO && ((g - 1) & 1) != static_cast<uint32_t>(wg)) continue;
-      // ---- results, by the warpgroup that had the last tile; the other one goes on
-      await(&pv_full[wg], (WIDE || SOLO ? mine - 1 : (g - 1) >> 1) & 1);
-      if (!WIDE && !SOLO && it.t1 - it.t0 > 1) {
-        // Of an item of this parity: the other one may have set that of the next item already, should that have two tiles
-        await(&l_set[2 * (wg ^ 1) + (item & 1)], (sums >> (item & 1)) & 1);
-        sums ^= 1u << (item & 1);
-        // the other's reference is that of the tile before the last
-        l_run += *static_cast<volatile float*>(l_part + (item & 1) * kRows + tl) * (m_old == m_run ? 1.f : ex2(m_old - m_run));
-      }
-      // The words are two items old when they are used again: the other warpgroup is at the next item's first tile at most (WIDE: has
-      // its results of the item before, or none)
+      // ---- results; the other warpgroup has the next item meanwhile
+      await_pv(mine - 1);
+      // The word of the item after the next is free: it was that of an item whose results both warpgroups have, or had no part in
       if (tl == 0 && (!WIDE || wg == 0)) bad_nodes[(item + 2) & 3] = 0ull;
       // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
       float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
       if (kParts > 1) lanes[tl] = make_float2(m_run, l_run);
-      sync_group();                                        // and bad_here of all four warps (the other warpgroup's: l_set)
+      sync_group();                                        // and bad_here of all four warps
       float weight = 1.f;
       if (kParts > 1) {
         float2 o[kParts];
@@ -794,7 +759,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
         tc_fence_before();                                 // O has been read
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[WIDE ? wg : item & 1]);
+        if (lane == 0) mbar_arrive(&o_free[wg]);
         if (kParts > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
       }
       if (warp_ok && part == 0) {

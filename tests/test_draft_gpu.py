@@ -162,6 +162,19 @@ def test_attention_is_the_same_twice_and_on_another_stream():
     assert torch.equal(a[:t], b[:t])
 
 
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("ctx,nodes,hq,hkv,d", [
+    ([9000], [5], 8, 8, 64), ([9000], [5], 8, 8, 128), ([30000], [4], 2, 1, 128), ([3000] * 9, [8] * 9, 32, 8, 128), ([2500, 9000, 40], [12, 3, 7], 8, 2, 64),
+    ([9000], [40], 8, 8, 128), ([5000, 700], [50, 64], 2, 2, 64), ([3000] * 9, [15] * 9, 32, 8, 128), ([9000], [32], 16, 4, 128), ([4000] * 5, [24] * 5, 10, 2, 64),
+    ([4000] * 5, [18] * 5, 49, 7, 128), ([6000, 300], [64, 40], 16, 4, 128), ([2000] * 8, [33] * 8, 16, 2, 64), ([7000] * 2, [20, 64], 24, 3, 128)])
+def test_attention_with_units_cut_and_whole(ctx, nodes, hq, hkv, d, whole, monkeypatch):
+    """Shares of several tiles and several units, for every number of lanes a row and for blocks of two halves."""
+    from gllm_b200.ops import sm100_draft
+    monkeypatch.setattr(sm100_draft, "_whole_units", lambda *a: whole)
+    for seed in range(2):
+        _check_attention(_attention_case(ctx, nodes, hq, hkv, d, 16, seed=seed))
+
+
 def test_attention_refuses_on_the_gpu():
     x = _attention_case([50], [3], 4, 2, 64, 16)
     args = dict(q=x.q, k_cache=x.k, v_cache=x.v, inp=x.b, seen=x.seen, scale=0.1, num_q_heads=4, head_dim=64)
