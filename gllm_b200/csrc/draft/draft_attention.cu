@@ -788,42 +788,76 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   }
 }
 
-// Joins the parts of the unit that CTA blockIdx.x begins and CTA `last` ends: 32 rows a block, a lane each, a warp every eighth four dims
+// Joins the parts of the unit that CTA blockIdx.x begins and CTA `last` ends: 32 rows a block, a lane each. A warp has 32 columns and every
+// second part (fourth, with heads of 64), two of them on their way at a time, in order; the warps' results are joined in order. Latency bounds
+// it: few parts and many units (256 rows, two parts) want few blocks, many parts (16 units of ten) few waits one after the other.
 static constexpr int kJoinWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) draft_join_kernel(const DraftAttnParams p) {
+  constexpr int kColumns = D / 32, kSub = kJoinWarps / kColumns;      // warps beside and behind one another
+  __shared__ float sm[kSub][kColumns][32], sl[kSub][kColumns][32];
+  __shared__ float4 so[kSub - 1][kColumns][8][32];
   griddep_wait();
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
+  const int column = warp % kColumns, sub = warp / kColumns;
   const int4 c0 = p.cut[2 * cta], c1 = p.cut[2 * cta + 1];
-  const int last = c0.x;
-  if (last <= cta || last >= static_cast<int>(gridDim.x) || row >= c1.x) return;
+  const int last = c0.x, rows = c1.x;
+  if (last <= cta || last >= static_cast<int>(gridDim.x) || static_cast<int>(blockIdx.y) * 32 >= rows) return;
+  const bool ok = row < rows;
+  float m = -INFINITY, l = 0.f;
+  float4 o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   auto slot = [&](int c) { return static_cast<size_t>(2 * c + (c == cta ? 1 : 0)); };
-  float m = -INFINITY;
-  for (int c = cta; c <= last; ++c) m = fmaxf(m, p.part_ml[slot(c) * p.part_rows + row].x);
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 o[D / 4 / kJoinWarps];
+  auto load = [&](int c, float2& ml, float4 (&x)[8]) {
+    ml = p.part_ml[slot(c) * p.part_rows + row];
 #pragma unroll
-  for (int i = 0; i < D / 4 / kJoinWarps; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = cta; c <= last; ++c) {
-    const float2 ml = p.part_ml[slot(c) * p.part_rows + row];
-    const float w = ex2(ml.x - m_use);
-    l += w * ml.y;
+    for (int i = 0; i < 8; ++i) x[i] = p.part_o[(slot(c) * (D / 4) + column * 8 + i) * p.part_rows + row];
+  };
+  auto add = [&](const float2& ml, const float4 (&x)[8]) {
+    const float top = fmaxf(m, ml.x), use = top == -INFINITY ? 0.f : top, a = ex2(m - use), w = ex2(ml.x - use);
+    m = top;
+    l = l * a + ml.y * w;
 #pragma unroll
-    for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
-      const float4 x = p.part_o[(slot(c) * (D / 4) + warp + i * kJoinWarps) * p.part_rows + row];
-      o[i].x += w * x.x; o[i].y += w * x.y; o[i].z += w * x.z; o[i].w += w * x.w;
+    for (int i = 0; i < 8; ++i) {
+      o[i].x = o[i].x * a + x[i].x * w; o[i].y = o[i].y * a + x[i].y * w;
+      o[i].z = o[i].z * a + x[i].z * w; o[i].w = o[i].w * a + x[i].w * w;
     }
+  };
+  for (int c = cta + sub; c <= last && ok; c += 2 * kSub) {
+    float2 ml[2];
+    float4 x[2][8];
+    const bool more = c + kSub <= last;
+    load(c, ml[0], x[0]);
+    if (more) load(c + kSub, ml[1], x[1]);
+    add(ml[0], x[0]);
+    if (more) add(ml[1], x[1]);
+  }
+  if (sub > 0) {
+    sm[sub][column][lane] = m;
+    sl[sub][column][lane] = l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) so[sub - 1][column][i][lane] = o[i];
+  }
+  __syncthreads();
+  if (!ok || sub > 0) return;
+  for (int w = 1; w < kSub && cta + w <= last; ++w) {
+    float4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = so[w - 1][column][i][lane];
+    add(make_float2(sm[w][column][lane], sl[w][column][lane]), x);
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int at = c0.w * p.block_rows + row, node = at / p.G, head = c0.z * p.G + at - node * p.G;
-  __nv_bfloat16* op = p.out + (static_cast<int64_t>(c0.y + node) * p.Hq + head) * D;
+  __nv_bfloat16* op = p.out + (static_cast<int64_t>(c0.y + node) * p.Hq + head) * D + column * 32;
 #pragma unroll
-  for (int i = 0; i < D / 4 / kJoinWarps; ++i) {
-    uint2 w;
-    w.x = pack_bf16(o[i].x * inv, o[i].y * inv);
-    w.y = pack_bf16(o[i].z * inv, o[i].w * inv);
-    *reinterpret_cast<uint2*>(op + (warp + i * kJoinWarps) * 4) = w;
+  for (int i = 0; i < 4; ++i) {
+    uint4 w;
+    w.x = pack_bf16(o[2 * i].x * inv, o[2 * i].y * inv);
+    w.y = pack_bf16(o[2 * i].z * inv, o[2 * i].w * inv);
+    w.z = pack_bf16(o[2 * i + 1].x * inv, o[2 * i + 1].y * inv);
+    w.w = pack_bf16(o[2 * i + 1].z * inv, o[2 * i + 1].w * inv);
+    *reinterpret_cast<uint4*>(op + i * 8) = w;
   }
 }
 
