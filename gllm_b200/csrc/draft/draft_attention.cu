@@ -35,8 +35,8 @@ namespace b200 {
 
 static constexpr int kNodes = 64;
 static constexpr int kRows = 128, kKeys = 128;           // of a unit's block, of a tile
-static constexpr int kSoftmaxWarps = 8;
-static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
+constexpr int softmax_warps(int rep) { return rep == 0 ? 16 : 8; }
+constexpr int cta_threads(int rep) { return (softmax_warps(rep) + 4) * 32; }
 static constexpr float kLazy = 8.f;                      // P stays below 2^8 between two rescales of O
 
 struct DraftAttnParams {
@@ -68,7 +68,7 @@ struct DraftSmem {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kRingOff = 2 * kQBytes, kBarOff = kRingOff + kStages * kTileBytes;
   // barriers and words (see the kernel), and up to 1 KB before the first 1024-byte boundary
-  static constexpr int kBarBytes = (2 * kStages + 17) * 8 + 8 + 4 * 8 + 5 * 8 + 12 * 8 + kStages * 4;
+  static constexpr int kBarBytes = (2 * kStages + 17) * 8 + 8 + 4 * 8 + 5 * 8 + 20 * 8 + 2 * kRows * 4 + kStages * 4;
   static constexpr int kBytes = kBarOff + (kBarBytes + 15) / 16 * 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
   static constexpr int kTmemO = 2 * kKeys, kTmemCols = 512;
@@ -93,12 +93,17 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// P of 16 keys, the kk-th of a tile: in the first columns of its 32 keys' scores
+__device__ __forceinline__ uint32_t p_column(uint32_t kk) { return (kk >> 1) * 32 + (kk & 1) * 8; }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // V as it lies in the cache, keys along the rows: MN-major, 64 dims (128 bytes) then the next slab LBO bytes on, 8 keys SBO
 __device__ __forceinline__ uint64_t mn_major_desc(uint32_t smem_addr) {
   return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF) | static_cast<uint64_t>((kKeys * 128) >> 4) << 16 |
          static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
+// an order of fp32 that integers have too (and back: the same)
+__device__ __forceinline__ int ordered(int bits) { return bits ^ ((bits >> 31) & 0x7fffffff); }
+static constexpr int kNoScore = static_cast<int>(0x807fffffu);       // -infinity
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -184,16 +189,19 @@ struct Items : Seq {
 };
 
 template <int D, int REP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(cta_threads(REP), 1)
 draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q,
                        const DraftAttnParams p) {
   using SM = DraftSmem<D>;
   constexpr int NS = SM::kStages;
   // A block's rows are whole nodes. REP 1, 2, 4: at most BR = 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups
   // take the items in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them of every item.
+  // and two threads a row (a TMEM lane), with 64 keys of a tile each.
   constexpr bool WIDE = REP == 0;
-  constexpr int BR = kRows / (WIDE ? 1 : REP);
-  constexpr int kChunks = kKeys / 32 / (WIDE ? 1 : REP);              // of 32 keys that a lane has of a tile
+  constexpr int kLanes = WIDE ? 1 : REP, kParts = WIDE ? 2 : REP;    // TMEM lanes, threads of a row
+  constexpr int BR = kRows / kLanes;
+  constexpr int kChunks = kKeys / 32 / kParts;           // of 32 keys that a thread has of a tile
+  constexpr int kThreads = cta_threads(REP), W0 = softmax_warps(REP), kGroup = W0 * 16;   // a warpgroup's (a half's) threads
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);   // [NS] copies -> products (and softmax: V)
@@ -209,15 +217,16 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   const WaitGuard guard{tmem_slot + 1, p.waits};
   unsigned long long* bad_nodes = reinterpret_cast<unsigned long long*>(tmem_slot + 2);   // [item % 4]
   int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // share: first sequence, offset in it, end; all tiles; begin
-  int64_t* warp_work = begin + 5;                        // [12]
-  volatile uint32_t* filled = reinterpret_cast<uint32_t*>(warp_work + 12);   // [NS] copies into a stage
+  int64_t* warp_work = begin + 5;                        // [20]
+  volatile uint32_t* filled = reinterpret_cast<uint32_t*>(warp_work + 20);   // [NS] copies into a stage
+  int* row_max = reinterpret_cast<int*>(warp_work + 20) + NS;        // WIDE: [2 halves][128] maximum of a row's scores, as an integer of the same order
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); filled[i] = 0; }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[2 * i], 1); mbar_init(&s_full[2 * i + 1], 1); mbar_init(&p_full[i], 4);
-      mbar_init(&pv_full[2 * i], 1); mbar_init(&pv_full[2 * i + 1], 1); mbar_init(&o_free[i], 4); mbar_init(&q_full[i], 1); mbar_init(&q_free[i], REP > 1 ? 2 : 1);
+      mbar_init(&s_full[2 * i], 1); mbar_init(&s_full[2 * i + 1], 1); mbar_init(&p_full[i], W0 / 2);
+      mbar_init(&pv_full[2 * i], 1); mbar_init(&pv_full[2 * i + 1], 1); mbar_init(&o_free[i], W0 / 2); mbar_init(&q_full[i], 1); mbar_init(&q_free[i], REP > 1 ? 2 : 1);
       bad_nodes[2 * i] = bad_nodes[2 * i + 1] = 0ull;
     }
     mbar_init(mma_end, 1);
@@ -225,8 +234,9 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     begin[0] = begin[1] = begin[2] = begin[4] = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
-  if (warp == 8 && lane < 3) tma_prefetch_desc(lane == 0 ? &tmap_k : lane == 1 ? &tmap_v : &tmap_q);
+  if (warp == W0 + 1) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
+  if (WIDE && threadIdx.x < 2 * kRows) row_max[threadIdx.x] = kNoScore;
+  if (warp == W0 && lane < 3) tma_prefetch_desc(lane == 0 ? &tmap_k : lane == 1 ? &tmap_v : &tmap_q);
   griddep_launch();
   griddep_wait();
 
@@ -289,10 +299,10 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   Items it(p, static_cast<int>(begin[0]), static_cast<int>(begin[1]), static_cast<int>(begin[2] - begin[4]));
   const bool idle = begin[2] <= begin[4];
 
-  if (warp >= kSoftmaxWarps) {
-    if ((warp == 8 || warp == 10) && !idle) {
-      // ------------------------------------------------------------------ copies: K by warp 8, V by warp 10
-      const bool is_v = warp == 10;
+  if (warp >= W0) {
+    if ((warp == W0 || warp == W0 + 2) && !idle) {
+      // ------------------------------------------------------------------ copies: K, V
+      const bool is_v = warp == W0 + 2;
       const CUtensorMap* map = is_v ? &tmap_v : &tmap_k;
       const int box = 1 << min(p.page_shift, 6), boxes = kKeys / box, j = lane % boxes, sl = lane / boxes;
       const int in_page = (1 << p.page_shift) - 1;
@@ -322,7 +332,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           page = next;
         }
       }
-    } else if (warp == 9 && lane == 0 && !idle) {
+    } else if (warp == W0 + 1 && !idle && elect_one()) {
       // ------------------------------------------------------------------ products
       constexpr uint32_t idesc_s = make_idesc_bf16(kRows, kKeys);
       constexpr uint32_t idesc_pv = make_idesc_bf16(kRows, D) | (1u << 16);
@@ -350,11 +360,11 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const uint32_t o_tmem = tmem + SM::kTmemO + o_buf * D, p_tmem = tmem + s_buf * kKeys;
         if (keys == kKeys) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+          for (int kk = 0; kk < kKeys / 16; ++kk) umma_ts(o_tmem, p_tmem + p_column(kk), dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
         } else {
 #pragma unroll 1
           for (int kk = 0; kk < (keys + 15) / 16; ++kk)
-            umma_ts(o_tmem, p_tmem + kk * 8, dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
+            umma_ts(o_tmem, p_tmem + p_column(kk), dv + static_cast<uint64_t>(kk) * (2048 >> 4), idesc_pv, kk != 0 ? 1u : acc);
         }
         uint32_t& own = o_buf == 0 ? own_pv0 : own_pv1;
         umma_commit(&pv_full[2 * o_buf + (WIDE ? 0 : own & 1)]);
@@ -449,7 +459,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
       umma_commit(mma_end);                                // nothing is in flight when the columns are given back
       guard.land(mma_end, 0);
-    } else if (warp == 11 && lane == 0 && !idle) {
+    } else if (warp == W0 + 3 && lane == 0 && !idle) {
       // ------------------------------------------------------------------ queries: a box is a block's (a half's) nodes x heads, 64 columns
       uint32_t item = 0;
       for (; it.next(); ++item) {
@@ -473,9 +483,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
   } else {
     // ------------------------------------------------------------------ softmax
-    const int wg = warp >> 2, tl = threadIdx.x & 127;      // TMEM lane
-    constexpr int kParts = WIDE ? 1 : REP;                 // lanes of a row
-    const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = kParts == 1 ? 0 : (warp & 3) / (4 / kParts);
+    const int wg = threadIdx.x / kGroup, tl = threadIdx.x & 127;   // TMEM lane
+    const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = WIDE ? (warp >> 2) & 1 : kLanes == 1 ? 0 : (warp & 3) / (4 / kLanes);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t g = 0, mine = 0;                              // tile of the CTA, of this warpgroup
     bool cut_tail = false;
@@ -492,9 +501,11 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       else await(&pv_full[2 * wg + (k & 1)], (k >> 1) & 1);
     };
     auto sync_group = [&] {
-      if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-      else asm volatile("bar.sync 2, 128;" ::: "memory");
+      if (wg == 0) asm volatile("bar.sync 1, %0;" ::"n"(kGroup) : "memory");
+      else asm volatile("bar.sync 2, %0;" ::"n"(kGroup) : "memory");
     };
+    // WIDE: the two warps that have a row between them
+    auto sync_pair = [&] { asm volatile("bar.sync %0, 64;" ::"r"(3 + wg * 4 + (warp & 3)) : "memory"); };
     for (uint32_t item = 0; it.next(); ++item) {
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
       if (it.t0 == 0 && it.t1 < it.tiles) cut_tail = true; // the last item, if any
@@ -539,7 +550,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!((bits >> e) & 1u)) f[e] = -INFINITY;
-              if (kChunks > 1) {                           // read once more below
+              if (c + 1 < kChunks) {                       // read once more below
                 tmem_store16(t_s + (part * kChunks + c) * 32, *reinterpret_cast<uint32_t(*)[16]>(f));
                 tmem_store16(t_s + (part * kChunks + c) * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(f + 16));
               }
@@ -553,6 +564,12 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           }
           if (kChunks > 1 && behind) tmem_store_wait();
+          if constexpr (WIDE) {
+            // the item's maximum so far, of both warps: neither comes to the next tile before the other has read it, as that needs both's P
+            atomicMax(&row_max[wg * kRows + tl], ordered(__float_as_int(mx)));
+            sync_pair();
+            mx = __int_as_float(ordered(*static_cast<volatile int*>(&row_max[wg * kRows + tl])));
+          }
           mx *= p.scale_log2;
           float alpha = 1.f;
           if (mx > m_run + kLazy) {
@@ -564,7 +581,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             // O is free when the product of the warpgroup's tile before has ended (WIDE: S of this tile was formed behind it)
             if (!WIDE) await_pv(mine - 1);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = WIDE ? part * (D / 2) : 0; c < (WIDE ? (part + 1) * (D / 2) : D); c += 16) {
               uint32_t v[16];
               tmem_ld_32x16(t_o + c, v);
               tmem_ld_wait();
@@ -577,8 +594,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           const uint64_t sc2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-m_use, -m_use);
           uint64_t sum2[2] = {0, 0};
 #pragma unroll 1
-          for (int c = 0; c < kChunks; ++c) {              // 32 keys: 16 columns of P, which never reach scores that are still to be read
-            if (kChunks > 1) load(c);
+          for (int c = kChunks - 1; c >= 0; --c) {         // 32 keys: 16 columns of P over their scores; the last ones are still there
+            if (c + 1 < kChunks) load(c);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -587,15 +604,15 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
               sum2[e & 1] = add_pair(sum2[e & 1], pair(y.x, y.y));
               pk[e] = pack_bf16(y.x, y.y);                 // probabilities enter the product in bf16, the sum in fp32
             }
-            tmem_store16(t_s + (part * kChunks + c) * 16, pk);
+            tmem_store16(t_s + (part * kChunks + c) * 32, pk);
           }
-          if (kParts > 1) {                                // the keys that other lanes have of this row
+          if (kLanes > 1) {                                // the keys that other lanes have of this row
             uint32_t none[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) none[e] = 0u;
 #pragma unroll
             for (int c = 0; c < kKeys / 32; ++c)
-              if (c / kChunks != part) tmem_store16(t_s + c * 16, none);
+              if (c / kChunks != part) tmem_store16(t_s + c * 32, none);
           }
           const float2 sa = unpair(add_pair(sum2[0], sum2[1]));
           l_run += sa.x + sa.y;
@@ -607,7 +624,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           await(&full[st], (vp / NS) & 1);
           uint8_t* tile = smem + SM::kRingOff + st * SM::kTileBytes;
           const int lo = max(it.ctx - key0, 0), hi = it.keys(t), end = min((hi + 15) & ~15, kKeys);
-          for (int e = lo * (D / 8) + (threadIdx.x & 127); e < end * (D / 8); e += 128) {
+          for (int e = lo * (D / 8) + (threadIdx.x & (kGroup - 1)); e < end * (D / 8); e += kGroup) {
             const int r = e / (D / 8), c = e % (D / 8);
             uint4* w = reinterpret_cast<uint4*>(tile + (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
             if (r >= hi) {
@@ -637,23 +654,35 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       // ---- results; the other warpgroup has the next item meanwhile
       await_pv(mine - 1);
       // The word of the item after the next is free: it was that of an item whose results both warpgroups have, or had no part in
-      if (tl == 0 && (!WIDE || wg == 0)) bad_nodes[(item + 2) & 3] = 0ull;
+      if (tl == 0 && (!WIDE || (wg == 0 && part == 0))) bad_nodes[(item + 2) & 3] = 0ull;
       // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
       float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
-      if (kParts > 1) lanes[tl] = make_float2(m_run, l_run);
+      if (kLanes > 1) lanes[tl] = make_float2(m_run, l_run);
       sync_group();                                        // and bad_here of all four warps
+      if constexpr (WIDE) {                                // the row's sum, by way of its maximum's place
+        volatile float* place = reinterpret_cast<volatile float*>(&row_max[wg * kRows + tl]);
+        if (part == 0) *place = l_run;
+        sync_pair();
+        if (part == 1) *place = l_run += *place;
+        sync_pair();
+        if (part == 0) {
+          l_run = *place;
+          *reinterpret_cast<volatile int*>(place) = kNoScore;
+        }
+        sync_pair();
+      }
       float weight = 1.f;
-      if (kParts > 1) {
-        float2 o[kParts];
+      if (kLanes > 1) {
+        float2 o[kLanes];
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
+        for (int i = 0; i < kLanes; ++i) {
           o[i] = lanes[i * BR + row];
           top = fmaxf(top, o[i].x);
         }
         if (top != -INFINITY) {
 #pragma unroll
-          for (int i = 0; i < kParts; ++i) sum += o[i].y * ex2(o[i].x - top);
+          for (int i = 0; i < kLanes; ++i) sum += o[i].y * ex2(o[i].x - top);
           weight = ex2(m_run - top);
         }
         m_run = top;
@@ -697,16 +726,15 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
           }
         };
-        if constexpr (kParts == 1) {
+        if constexpr (kLanes == 1) {
           if (warp_ok) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t v[32];
+            for (int c = WIDE ? part * (D / 2) : 0; c < (WIDE ? (part + 1) * (D / 2) : D); c += 32) {
               float x[32];
-              tmem_ld_32x32(t_o + c, v);
+              tmem_ld_32x32(t_o + c, reinterpret_cast<uint32_t(&)[32]>(x));
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(v[e]) * inv;
+              for (int e = 0; e < 32; ++e) x[e] *= inv;
               put(c, x);
               __syncwarp();
             }
@@ -760,7 +788,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         tc_fence_before();                                 // O has been read
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free[wg]);
-        if (kParts > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
+        if (kLanes > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
       }
       if (warp_ok && part == 0) {
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
@@ -781,7 +809,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   // copies that nobody waited for, because a wait gave up, land before the CTA ends
   if (threadIdx.x < NS && guard.gave_up() && filled[threadIdx.x] != 0) guard.land(&full[threadIdx.x], (filled[threadIdx.x] - 1) & 1);
-  if (warp == 9) {
+  if (warp == W0 + 1) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc<1>(tmem, SM::kTmemCols);
@@ -902,7 +930,7 @@ static int launch_draft_attention(const CUtensorMap& tk, const CUtensorMap& tv, 
     fprintf(stderr, "[gllm_b200] query tensor-map encode failed (%d)\n", static_cast<int>(r));
     return 1;
   }
-  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(kThreads), SM::kBytes, st, tk, tv, tq, p));
+  CUDA_CHECK_RET(launch_pdl(draft_attention_kernel<D, REP>, dim3(ctas), dim3(cta_threads(REP)), SM::kBytes, st, tk, tv, tq, p));
   if (p.whole) return 0;
   CUDA_CHECK_RET(launch_pdl(draft_join_kernel<D>, dim3(ctas, (p.block_rows + 31) / 32), dim3(kJoinWarps * 32), 0, st, p));
   return 0;
