@@ -35,7 +35,7 @@ namespace b200 {
 
 static constexpr int kNodes = 64;
 static constexpr int kRows = 128, kKeys = 128;           // of a unit's block, of a tile
-constexpr int softmax_warps(int rep) { return rep == 0 ? 16 : 8; }
+constexpr int softmax_warps(int rep) { return rep <= 1 ? 16 : 8; }
 constexpr int cta_threads(int rep) { return (softmax_warps(rep) + 4) * 32; }
 static constexpr float kLazy = 8.f;                      // P stays below 2^8 between two rescales of O
 
@@ -196,9 +196,9 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   constexpr int NS = SM::kStages;
   // A block's rows are whole nodes. REP 1, 2, 4: at most BR = 128 / REP rows, TMEM lane = part of the keys x BR + row, the warpgroups
   // take the items in turn. REP 0 (WIDE): two halves of at most 128 rows, each warpgroup has one of them of every item.
-  // and two threads a row (a TMEM lane), with 64 keys of a tile each.
-  constexpr bool WIDE = REP == 0;
-  constexpr int kLanes = WIDE ? 1 : REP, kParts = WIDE ? 2 : REP;    // TMEM lanes, threads of a row
+  // PAIR: two threads have a TMEM lane, 64 keys of a tile each.
+  constexpr bool WIDE = REP == 0, PAIR = REP <= 1;
+  constexpr int kLanes = WIDE ? 1 : REP, kParts = PAIR ? 2 : REP;    // TMEM lanes, threads of a row
   constexpr int BR = kRows / kLanes;
   constexpr int kChunks = kKeys / 32 / kParts;           // of 32 keys that a thread has of a tile
   constexpr int kThreads = cta_threads(REP), W0 = softmax_warps(REP), kGroup = W0 * 16;   // a warpgroup's (a half's) threads
@@ -219,7 +219,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   int64_t* begin = reinterpret_cast<int64_t*>(bad_nodes + 4);         // share: first sequence, offset in it, end; all tiles; begin
   int64_t* warp_work = begin + 5;                        // [20]
   volatile uint32_t* filled = reinterpret_cast<uint32_t*>(warp_work + 20);   // [NS] copies into a stage
-  int* row_max = reinterpret_cast<int*>(warp_work + 20) + NS;        // WIDE: [2 halves][128] maximum of a row's scores, as an integer of the same order
+  int* row_max = reinterpret_cast<int*>(warp_work + 20) + NS;        // PAIR: [2 warpgroups][128] maximum of a row's scores, as an integer of the same order
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -235,7 +235,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     fence_mbar_init();
   }
   if (warp == W0 + 1) tmem_alloc<1>(tmem_slot, SM::kTmemCols);
-  if (WIDE && threadIdx.x < 2 * kRows) row_max[threadIdx.x] = kNoScore;
+  if (PAIR && threadIdx.x < 2 * kRows) row_max[threadIdx.x] = kNoScore;
   if (warp == W0 && lane < 3) tma_prefetch_desc(lane == 0 ? &tmap_k : lane == 1 ? &tmap_v : &tmap_q);
   griddep_launch();
   griddep_wait();
@@ -484,7 +484,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   } else {
     // ------------------------------------------------------------------ softmax
     const int wg = threadIdx.x / kGroup, tl = threadIdx.x & 127;   // TMEM lane
-    const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = WIDE ? (warp >> 2) & 1 : kLanes == 1 ? 0 : (warp & 3) / (4 / kLanes);
+    const int row = WIDE ? wg * p.half_rows + tl : tl % BR, part = PAIR ? (warp >> 2) & 1 : kLanes == 1 ? 0 : (warp & 3) / (4 / kLanes);
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t g = 0, mine = 0;                              // tile of the CTA, of this warpgroup
     bool cut_tail = false;
@@ -504,7 +504,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if (wg == 0) asm volatile("bar.sync 1, %0;" ::"n"(kGroup) : "memory");
       else asm volatile("bar.sync 2, %0;" ::"n"(kGroup) : "memory");
     };
-    // WIDE: the two warps that have a row between them
+    // PAIR: the two warps that have a row between them
     auto sync_pair = [&] { asm volatile("bar.sync %0, 64;" ::"r"(3 + wg * 4 + (warp & 3)) : "memory"); };
     for (uint32_t item = 0; it.next(); ++item) {
       const bool cut = it.t0 > 0 || it.t1 < it.tiles;
@@ -564,7 +564,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           }
           if (kChunks > 1 && behind) tmem_store_wait();
-          if constexpr (WIDE) {
+          if constexpr (PAIR) {
             // the item's maximum so far, of both warps: neither comes to the next tile before the other has read it, as that needs both's P
             atomicMax(&row_max[wg * kRows + tl], ordered(__float_as_int(mx)));
             sync_pair();
@@ -581,7 +581,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             // O is free when the product of the warpgroup's tile before has ended (WIDE: S of this tile was formed behind it)
             if (!WIDE) await_pv(mine - 1);
 #pragma unroll 1
-            for (int c = WIDE ? part * (D / 2) : 0; c < (WIDE ? (part + 1) * (D / 2) : D); c += 16) {
+            for (int c = PAIR ? part * (D / 2) : 0; c < (PAIR ? (part + 1) * (D / 2) : D); c += 16) {
               uint32_t v[16];
               tmem_ld_32x16(t_o + c, v);
               tmem_ld_wait();
@@ -654,12 +654,12 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       // ---- results; the other warpgroup has the next item meanwhile
       await_pv(mine - 1);
       // The word of the item after the next is free: it was that of an item whose results both warpgroups have, or had no part in
-      if (tl == 0 && (!WIDE || (wg == 0 && part == 0))) bad_nodes[(item + 2) & 3] = 0ull;
+      if (tl == 0 && (!PAIR || part == 0) && (!WIDE || wg == 0)) bad_nodes[(item + 2) & 3] = 0ull;
       // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
       float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
       if (kLanes > 1) lanes[tl] = make_float2(m_run, l_run);
       sync_group();                                        // and bad_here of all four warps
-      if constexpr (WIDE) {                                // the row's sum, by way of its maximum's place
+      if constexpr (PAIR) {                                // the row's sum, by way of its maximum's place
         volatile float* place = reinterpret_cast<volatile float*>(&row_max[wg * kRows + tl]);
         if (part == 0) *place = l_run;
         sync_pair();
@@ -729,7 +729,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if constexpr (kLanes == 1) {
           if (warp_ok) {
 #pragma unroll 1
-            for (int c = WIDE ? part * (D / 2) : 0; c < (WIDE ? (part + 1) * (D / 2) : D); c += 32) {
+            for (int c = part * (D / 2); c < (part + 1) * (D / 2); c += 32) {
               float x[32];
               tmem_ld_32x32(t_o + c, reinterpret_cast<uint32_t(&)[32]>(x));
               tmem_ld_wait();
