@@ -13,7 +13,7 @@ namespace b200 {
 
 static constexpr int kNodes = 64;
 static constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
-static constexpr int kVerifyParts = 8;                 // CTAs of a cluster at most
+static constexpr int kVerifyParts = 16;                // CTAs of a cluster at most
 
 enum VerifyForm : int { kMatch = 0, kGiven = 1, kDraws = 2 };
 
@@ -391,6 +391,13 @@ GLLM_EXPORT int gllm_draft_verify(const void* tokens, const void* parents, const
   v.count = reinterpret_cast<int32_t*>(count);
   const dim3 grid(static_cast<unsigned>(num_seqs + 1) * parts);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (parts > 8) {                                       // more than every device has to take
+    static PerDeviceOnce configured;
+    if (configured.need()) {
+      CUDA_CHECK_RET(cudaFuncSetAttribute(draft_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      configured.done();
+    }
+  }
   if (parts > 1) CUDA_CHECK_RET(launch_pdl_cluster(draft_verify_kernel, grid, parts, dim3(kVerifyThreads), 0, st, v));
   else CUDA_CHECK_RET(launch_pdl(draft_verify_kernel, grid, dim3(kVerifyThreads), 0, st, v));
   return 0;

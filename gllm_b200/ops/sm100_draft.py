@@ -86,9 +86,13 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
     return out
 
 
-def _verify_parts(b: int) -> int:
-    """CTAs of a cluster that share a sequence: as many as leave all clusters resident, two CTAs an SM. One sequence, 151,936 tokens, 1 to 8
-    CTAs: 36, 25, 18, 13 us; 64 of 128,257: 41, 27, 25, 33; 256 of 151,936: 68, 81, 90, 119."""
+def _verify_parts(b: int, vocab: int) -> int:
+    """CTAs of a cluster that share a sequence: as many as leave all clusters resident, two CTAs an SM. One sequence, 151,936 tokens, 1 to 16
+    CTAs: 37, 25, 18, 14, 12 us; 64 of 128,257: 36, 25, 23, 31; 256 of 151,936: 68, 81, 90, 119. Sixteen are for few sequences and long rows
+    (8 and 16 CTAs: 4 chains of 32,000 10.4 / 12.3, of 100,352 12.3 / 10.3, of 151,936 14.3 / 12.3; 8 chains 14.3 / 14.4, 8 trees of 32
+    nodes 24.6 / 20.5; 8 chains of 100,352 12.3 / 14.4; 12 of 151,936 14.4 / 16.4)."""
+    if vocab > 1 << 16 and b <= (8 if vocab > 1 << 17 else 4):
+        return 16
     return 8 if b <= 37 else 4 if b <= 74 else 2 if b <= 148 else 1
 
 
@@ -111,7 +115,7 @@ def verify(tokens: torch.Tensor, parents: torch.Tensor, inp, target: torch.Tenso
             draft_at, ld_draft = draft_probs.data_ptr(), draft_probs.stride(0)
     check(_lib.load().gllm_draft_verify(tokens.data_ptr(), parents.data_ptr(), start.data_ptr(), chosen_at, target_at, ld_target, draft_at,
                                         ld_draft, uniform_at, vocab, b, t, said.data_ptr(), path.data_ptr(), count.data_ptr(),
-                                        1 if by_token else _verify_parts(b), stream_ptr()), "draft_verify")
+                                        1 if by_token else _verify_parts(b, vocab), stream_ptr()), "draft_verify")
     _count()
     return said, path, count
 

@@ -217,6 +217,17 @@ def test_verify_of_more_and_fewer_sequences(form, seqs):
     _same(Fn.draft_verify(args[0], up, b, *args[1:]), U.verify(args[0], up, b, *args[1:]))
 
 
+@pytest.mark.parametrize("form", ["given", "draws"])
+@pytest.mark.parametrize("seqs,vocab", [(1, 65537), (4, 65536), (4, 99991), (5, 99991), (8, 131073), (9, 131073)])
+def test_verify_of_long_rows(form, seqs, vocab):
+    """Few sequences have larger clusters; the rows' starts lie off the 16-byte boundaries."""
+    nodes = [1 + (3 + s) % 5 for s in range(seqs)]
+    b, up = U.batch([3] * seqs, nodes, 16, DEV), U.trees(nodes, 2)
+    for seed in range(2):
+        args = U.drafts(nodes, up, vocab, form, DEV, seed)
+        _same(Fn.draft_verify(args[0], _i32(up), b, *args[1:]), U.verify(args[0], _i32(up), b, *args[1:]))
+
+
 @pytest.mark.parametrize("shift_p,shift_q", [(0, 0), (1, 1), (1, 3), (2, 0), (3, 2)])
 @pytest.mark.parametrize("vocab", [3, 1001])
 def test_verify_of_views(vocab, shift_p, shift_q):
