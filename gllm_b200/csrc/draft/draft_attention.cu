@@ -5,29 +5,33 @@
 // where their 64 KB take some 2700 of an SM's share of the memory. All units lie in one row that is cut into equal shares for the CTAs, one an
 // SM, on the device, so that lengths may differ from those at the time a graph was captured and long contexts beside short ones leave no SM
 // idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined by a second launch in a
-// fixed order. Or no unit is cut, where that costs less (ops/sm100_draft.py).
+// fixed order, which costs 5 to 9 us. Or no unit is cut, where that costs less (ops/sm100_draft.py).
 //
 // Rows, by what a sequence may have (host):  up to 32, 64, 128  one block; with few rows 4 or 2 TMEM lanes share a row, each has a part of
 // every tile's keys, so that all four schedulers form exponentials (a lane's 128 take a warp 1700 cycles and more, 32 take 650).
-// More: blocks of two halves of 128, a warpgroup each, so that keys and values are read once for 256 rows.
+// More: blocks of two halves of 128, so that keys and values are read once for 256 rows. Where a row has one lane two warps share it, with 64
+// keys of a tile each (128 x 600 tokens, 24 nodes, 32 / 8 heads: 67.2 us with one warp, 65.5 with two; 16 of 8000, 64 nodes: 123.5 / 121).
 //
-//   warps 0-3, 4-7     softmax, a row a lane (tcgen05.ld 32x32b), the CTA's items in turn: one's results, some 3000 cycles of which most is
-//                      instruction fetch, are written while the other has the next one. (Tiles in turn, with one reference of the
-//                      exponents handed on: 128 x 600 tokens, 24 nodes, 32 / 8 heads 79 us, items 69; one long item an SM no faster.) The
+//   softmax            two groups of four warps, or of eight (two a row); a row a lane (tcgen05.ld 32x32b). The groups have the CTA's items
+//                      in turn: one's results, some 3000 cycles of which most is instruction fetch, are written while the other has the
+//                      next one. (Tiles in turn, with one reference of the exponents handed on: the case above 79 us, items 69.) The
 //                      reference follows the maximum in steps of 2^8; P goes over S, as the A operand of the product with V
-//   warps 8, 10        copies of K and V: page boxes [page][64] -> one ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V. (One
+//   two warps          copies of K and V: page boxes [page][64] -> one ring of tiles [D / 64][128][64] (SW128), K a tile ahead of V. (One
 //                      warp for both issues 32 boxes of 2 KB in 3300 cycles, more than their bytes take)
-//   warp 9 (1 thread)  products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two)
-//   warp 11 (1 thread) queries, a box a block, of the items to come (two buffers)
+//   one thread         products: S of the tile to come before P V of this one (S and P in two buffers of TMEM, O in two). It is found by
+//                      elect.sync: eight products are issued in 300 to 420 cycles then, behind `lane == 0` in some 600
+//   one thread         queries, a box a block, of the items to come (two buffers)
 //
 // Masks: only tiles that reach behind the context are masked, with the bits of the row's word shifted to the tile. A value that is not seen must
 // not reach the sum even as 0 x NaN: rows behind the last key are zeroed, and so are values of nodes that are no numbers; rows that see
 // those have them added at the end.
 //
-// What bounds it: HBM where histories are long (two of 60,000, 64 / 8 heads, 16 nodes: 84 us for 61 of bytes; 64 of 2500, 8 nodes 91 for 74;
-// some 10 us are the first data and the last results). Blocks of 256 rows: the chain softmax (2300 cycles) -> P V -> S of a half, 4050 cycles
-// per 128 keys for 2048 of tensor core and of the 2^x unit each (4 of 30,000, 64 nodes, 64 / 8 heads: 173 us, 740 TFLOP/s). Steps of 64 keys
-// with two buffers of S a half were slower (278): twice the products and commits of the one issuing thread.
+// What bounds it: HBM where histories are long (two of 60,000, 64 / 8 heads, 16 nodes: 82 us for 61 of bytes, the copies alone 69; 64 of 2500, 8
+// nodes 89 for 74; some 10 us are the first data and the last results). Blocks of 256 rows: the chain softmax -> P V -> S of a half, 3960 cycles
+// per 128 keys for 2048 of tensor core and of the 2^x unit each (4 of 30,000, 64 nodes, 64 / 8 heads: 165 us, 775 TFLOP/s): maximum 600,
+// exponentials 1300 to 1600, the two hand-overs 530, the products 1250. A product with the first half of P while the other half is formed gains 1 %
+// (the issuing thread's waits take the rest), exponentials by polynomial lose 6 %; steps of 64 keys with two buffers of S a half were slower
+// (278 for 173): twice the products and commits of that thread.
 #include "../attn/attn_common.cuh"
 #include "../common/bounded.cuh"
 

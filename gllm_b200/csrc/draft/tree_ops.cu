@@ -10,7 +10,8 @@ static constexpr int kMostNodes = 64;
 // ---------------------------------------------------------------------------------------------------------------------
 // plan: a warp per sequence, two nodes a lane. With up_i the parent and seen_i = {i}, six rounds of
 //   seen_i |= seen[up_i],  up_i = up[up_i]
-// reach ancestors 64 levels above. Latency bounds it: lengths, parents, then the table's entries, one trip to memory each.
+// reach ancestors 64 levels above. Latency bounds it: lengths, parents, then the table's entries, one trip to memory each (1 and 256 sequences of
+// 8 and 5 nodes: 4.2 us).
 // ---------------------------------------------------------------------------------------------------------------------
 static constexpr int kPlanWarps = 4;
 
@@ -77,7 +78,9 @@ draft_plan_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict
 // ---------------------------------------------------------------------------------------------------------------------
 // keep: rows of 16-byte words; a thread has one word of a token's row in one cache and walks the sequence's path. Node indexes
 // ascend along a path (path_j >= j), so a row is written only behind the one that it is read from and what is loaded later
-// is never overwritten before: all words of a batch of rows are on their way at once, no buffer between.
+// is never overwritten before: all words of a batch of rows are on their way at once, no buffer between. A CTA has a sequence in one cache, all
+// layers' caches are in one launch. Bytes bound it where many rows move: 64 sequences, 36 layers
+// of 8 heads of 128: 29 us back to back, of which 22 the kernel, for 18 of bytes; one sequence 4.2. An eager call of 72 caches is the host's, 41.
 // ---------------------------------------------------------------------------------------------------------------------
 static constexpr int kMostCaches = 256;
 struct CachePtrs { uint4* at[kMostCaches]; };

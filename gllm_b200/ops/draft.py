@@ -26,6 +26,9 @@ token is the first whose running sum of r = max(p - S q, 0) is over u_0 sum r. D
 have q(x) = 1 at their token: M falls by p(x) (0 at least), r is p without the tokens that were not taken. Where r has no mass it is p; where p has
 none the token is 0. Probabilities are fp32, what is computed from them fp64: a token changes only where u lies within some 2^-50 of a border. Values
 that are not over 0 (NaN among them) have no mass, and a token outside of the vocabulary none either.
+
+On the GPU attention takes bf16 queries and caches, heads of 64 or 128, at most 128 query heads a kv head, pages of 8 to 128 tokens; its
+probabilities are rounded to bf16 (half a step, 2^-9 of the value) before their product with V, sums are fp32. `keep` moves rows of any type.
 """
 from __future__ import annotations
 

@@ -39,9 +39,9 @@ def _attention_scratch(head_dim: int, max_rows: int) -> int:
 
 def _whole_units(seqs: int, kv_heads: int, group: int, nodes: int, max_len: int) -> bool:
     """Whether no unit of the attention kernel (a sequence's kv head and block of rows) is cut: nothing is joined then, in a second launch of some
-    2 us and what comes before it, but the SM with the most has up to a unit more than its share. Cut and whole, us: 8 units of 1, 4, 12 and 47
-    tiles (32 / 8 heads of 128, 8 nodes) 12.4 / 10.4, 16.2 / 12.5, 17.8 / 18.5, 24.9 / 49.2; 128 of 4 and 47 22.2 / 17.1, 62.6 / 75.9; 1024 of
-    4 and 12 69.8 / 61.6, 120 / 114. Results are right either way, whatever the lengths are when a captured call is replayed."""
+    5 us, but the SM with the most has up to a unit more than its share. Cut and whole, us: 8 units of 1, 4, 12 and 47
+    tiles (32 / 8 heads of 128, 8 nodes) 11.5 / 10.3, 14.1 / 12.4, 15.7 / 16.5, 19.0 / 39.4; 128 of 4 and 47 17.3 / 14.4, 57.4 / 66.3; 1024 of
+    4 and 12 53.4 / 47.5, 111 / 108. Results are right either way, whatever the lengths are when a captured call is replayed."""
     tiles = (max_len + 127) // 128
     if tiles <= 8:
         return True
