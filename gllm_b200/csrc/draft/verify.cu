@@ -8,8 +8,8 @@
 // that of consecutive tokens. All CTAs of a cluster walk alike: they exchange their sums of a row and add them in one order.
 //
 // What bounds it: latency. A row is read behind the decisions that lead to it (lengths, tokens, their probabilities: three trips to memory, then the
-// cluster's barrier), and its warp's range once more for the border: one chain of 151,936 tokens 12.4 us, 64 chains of 128,257 24.8 for 10 of bytes
-// (66 MB, all sequences in the same phase at the same time), 256 of 151,936 68 for 47. fp64 units 12 %, issue slots 31 %.
+// cluster's barrier), and its warp's range once more for the border: one chain of 151,936 tokens 10.5 us, 64 chains of 128,257 20.9 for 10 of bytes
+// (66 MB, all sequences in the same phase at the same time), 256 of 151,936 65 for 47. fp64 units 12 %, issue slots 31 %.
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
 
@@ -115,10 +115,10 @@ __device__ __forceinline__ void share(int groups, int part, int parts, int warp,
   end = static_cast<int>(groups * (w + 1) / all);
 }
 
-// This lane's part of the mass of groups [g0, g1). Whole groups have their loads four at a time ahead of their arithmetic: one at a time the
-// latency of each is waited for.
+// This lane's part of the mass of groups [g0, g1). Whole groups have their loads two at a time ahead of their arithmetic: one at a time the
+// latency of each is waited for; four at a time need more than 64 registers (64 chains of 128,257 tokens 20.9 us, four 21.6, six 27).
 __device__ __forceinline__ double range_mass(const Rows& r, int g0, int g1, int lane) {
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 2;
   const unsigned long long out = r.near(g0, g1);
   const int w0 = max(g0, r.lead != 0 ? 1 : 0), w1 = min(g1, (r.lead + r.vocab) / 4);
   double sum = 0.0, m[4];

@@ -88,9 +88,9 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
 
 def _verify_parts(b: int, vocab: int) -> int:
     """CTAs of a cluster that share a sequence: as many as leave all clusters resident, two CTAs an SM. One sequence, 151,936 tokens, 1 to 16
-    CTAs: 37, 25, 18, 14, 12 us; 64 of 128,257: 36, 25, 23, 31; 256 of 151,936: 68, 81, 90, 119. Sixteen are for few sequences and long rows
-    (8 and 16 CTAs: 4 chains of 32,000 10.4 / 12.3, of 100,352 12.3 / 10.3, of 151,936 14.3 / 12.3; 8 chains 14.3 / 14.4, 8 trees of 32
-    nodes 24.6 / 20.5; 8 chains of 100,352 12.3 / 14.4; 12 of 151,936 14.4 / 16.4)."""
+    CTAs: 36, 22, 15.7, 12.0, 10.5 us; 64 of 128,257: 38, 23, 20.5, 27, 43; 256 of 151,936: 65, 74, 85, 109. Sixteen are for few sequences and
+    long rows (8 and 16 CTAs: 4 chains of 32,000 8.7 / 8.9, of 100,352 10.0 / 9.0, of 151,936 11.8 / 10.4; 8 chains 11.6 / 11.1, 8 trees of 32
+    nodes 21.7 / 17.0; 8 chains of 100,352 10.3 / 10.9; 12 of 151,936 12.1 / 12.9)."""
     if vocab > 1 << 16 and b <= (8 if vocab > 1 << 17 else 4):
         return 16
     return 8 if b <= 37 else 4 if b <= 74 else 2 if b <= 148 else 1
