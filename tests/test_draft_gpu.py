@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from gllm_b200.layers import functional as Fn
-from gllm_b200.ops import ref
+from gllm_b200.ops import ref, sm100_draft
 from gllm_b200.ops.ref import kv_cache_shape
 from tests import draft_util as U
 
@@ -215,6 +215,38 @@ def test_verify_of_more_and_fewer_sequences(form, seqs):
     args = U.drafts(nodes, up, 20011, form, DEV)
     up = _i32(up)
     _same(Fn.draft_verify(args[0], up, b, *args[1:]), U.verify(args[0], up, b, *args[1:]))
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("most", [8, 16, 30, 64])
+def test_attention_of_nodes_that_are_no_numbers_in_every_form(most, d, whole, monkeypatch):
+    """Rows of four heads: four, two and one lane a row, blocks of 256. Two calls at once give the same bits."""
+    monkeypatch.setattr(sm100_draft, "_whole_units", lambda *a: whole)
+    ctx, nodes = [0, 120, 127, 900, 250, 3], [most, 1, most, most // 2 + 1, 0, most]
+    x = _attention_case(ctx, nodes, 8, 2, d, 16)
+    seen, bad, first = x.seen.tolist(), {}, [sum(nodes[:s]) for s in range(len(nodes))]
+    gen = torch.Generator().manual_seed(most)
+    for s, n in enumerate(nodes):
+        for i in (torch.rand(n, generator=gen) < 0.2).nonzero()[:, 0].tolist():
+            what = (float("nan"), float("inf"), float("-inf"))[i % 3]
+            x.v[int(x.b.block_table[s, (ctx[s] + i) // 16]), :, :, (ctx[s] + i) % 16, i % 7::7] = what
+            bad[s, i] = torch.arange(d, device=DEV) % 64 % 7 == i % 7
+    got = []
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            got.append(Fn.draft_attention(x.q, x.k, x.v, x.b, x.seen, d ** -0.5, 8, d)[:x.b.num_tokens])
+    torch.cuda.synchronize()
+    assert torch.equal(got[0].view(torch.int16), got[1].view(torch.int16))
+    want, tol = U.attention(x.q[:x.b.num_tokens], x.k, torch.where(x.v.isfinite(), x.v, 0), x.b, U.sees(seen, x.b), d ** -0.5, 8)
+    out = got[0].double().view(-1, 8, d)
+    fits = (out - want).abs() <= tol
+    for (s, i), cols in bad.items():
+        for row in range(first[s], first[s] + nodes[s]):
+            if seen[row] >> i & 1:
+                fits[row][:, cols] = ~out[row][:, cols].isfinite()
+    assert bad and fits.all()
 
 
 @pytest.mark.parametrize("form", ["given", "draws"])
