@@ -1,11 +1,12 @@
 """Kernels for drafted tokens against the definitions in 64 bits (GPU)."""
+import time
 import types
 
 import pytest
 import torch
 
 from gllm_b200.layers import functional as Fn
-from gllm_b200.ops import ref, sm100_draft
+from gllm_b200.ops import lib, ref, sm100, sm100_draft
 from gllm_b200.ops.ref import kv_cache_shape
 from tests import draft_util as U
 
@@ -247,6 +248,31 @@ def test_attention_of_nodes_that_are_no_numbers_in_every_form(most, d, whole, mo
             if seen[row] >> i & 1:
                 fits[row][:, cols] = ~out[row][:, cols].isfinite()
     assert bad and fits.all()
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("most", [8, 16, 30, 64])
+def test_attention_whose_waits_run_out(most, d, whole, monkeypatch):
+    """Limits of nothing, 1 ns and 2 us: the roles give up at different places, nothing is waited for that was never issued (two seconds), the
+    host learns of it, and the next call is right again."""
+    monkeypatch.setattr(sm100_draft, "_whole_units", lambda *a: whole)
+    x = _attention_case([700, 90, 5, 3000], [most, 3, most, most], 8, 2, d, 16)
+    want = _check_attention(x)
+    assert sm100.waits_given_up() == 0
+    try:
+        for limit in (0, 1, 2000):
+            lib.watch_waits(limit_ns=limit)
+            for _ in range(3):
+                t0 = time.monotonic()
+                Fn.draft_attention(x.q, x.k, x.v, x.b, x.seen, d ** -0.5, 8, d)
+                torch.cuda.synchronize()
+                assert time.monotonic() - t0 < 0.5, limit
+            assert lib.waits_gave_up(clear=True) or limit > 0
+    finally:
+        lib.watch_waits()
+        lib.waits_gave_up(clear=True)
+    assert torch.equal(_check_attention(x), want) and sm100.waits_given_up() == 0
 
 
 @pytest.mark.parametrize("form", ["given", "draws"])
