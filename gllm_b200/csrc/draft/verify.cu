@@ -8,8 +8,9 @@
 // that of consecutive tokens. All CTAs of a cluster walk alike: they exchange their sums of a row and add them in one order.
 //
 // What bounds it: latency. A row is read behind the decisions that lead to it (lengths, tokens, their probabilities: three trips to memory, then the
-// cluster's barrier), and its warp's range once more for the border: one chain of 151,936 tokens 10.5 us, 64 chains of 128,257 20.9 for 10 of bytes
-// (66 MB, all sequences in the same phase at the same time), 256 of 151,936 65 for 47. fp64 units 12 %, issue slots 31 %.
+// cluster's barrier), and its warp's range once more for the border: one chain of 151,936 tokens 9.0 us, 64 chains of 128,257 18.0 for 10 of bytes
+// (66 MB, all sequences in the same phase at the same time), 256 of 151,936 60 for 47. The draft's row is read where a child was refused: where all
+// are taken these are 8.5, 15.2 and 43.
 #include "../common/host_utils.h"
 #include "../common/ptx.cuh"
 
@@ -49,7 +50,7 @@ struct VerifyShared {
 // Four tokens at once: the row's first 16-byte boundary is `lead` tokens before its first token, group g has the tokens 4 g - lead and on
 struct Rows {
   const float* p;
-  const float* q;            // null: none
+  const float* q;            // null: none, the mass is p's
   int vocab, lead, groups;
   bool together;             // both rows have their boundaries at the same tokens
   double past;
@@ -116,7 +117,8 @@ __device__ __forceinline__ void share(int groups, int part, int parts, int warp,
 }
 
 // This lane's part of the mass of groups [g0, g1). Whole groups have their loads two at a time ahead of their arithmetic: one at a time the
-// latency of each is waited for; four at a time need more than 64 registers (64 chains of 128,257 tokens 20.9 us, four 21.6, six 27).
+// latency of each is waited for; four at a time need more than 64 registers (64 chains of 128,257 tokens, both rows read for each: 20.9 us, four
+// 21.6, six 27).
 __device__ __forceinline__ double range_mass(const Rows& r, int g0, int g1, int lane) {
   constexpr int kAhead = 2;
   const unsigned long long out = r.near(g0, g1);
@@ -262,14 +264,15 @@ draft_verify_kernel(const VerifyParams v) {
     after = s.chosen[node];
   } else {
     __syncthreads();                                     // s.taken
-    Rows rows(v.target + (first + node) * v.ld_target, form == kDraws ? v.draft + (first + node) * v.ld_draft : nullptr, v.vocab);
+    // The draft's row counts where a child was refused only (past is 1 or more then): others may hold anything, NaN among it
+    Rows rows(v.target + (first + node) * v.ld_target, form == kDraws && past > 0.0 ? v.draft + (first + node) * v.ld_draft : nullptr, v.vocab);
     rows.past = past;
     rows.word = s.word;
     rows.gone = form == kGiven ? s.children[node] : 0ull;
     if (!summed) total = row_sum(rows, s, part, parts, pass++);
     if (!(total > 0.0)) {                                // nothing is left of p: p itself
       rows.gone = 0ull;
-      rows.past = 0.0;
+      rows.q = nullptr;
       total = row_sum(rows, s, part, parts, pass++);
     }
     // the warp that the border lies in: its range's running sum is the first over u x total, or the last with mass

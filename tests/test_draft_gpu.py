@@ -540,3 +540,29 @@ def test_a_captured_step(form):
             assert (s.said[0][n:] == -1).all() and (s.plan[0][n:] == 0).all()
             for x, y in zip(s.caches, U.kept(s.before, s.b, said[1], said[2])):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("parts", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("vocab", [5, 3001, 70001])
+def test_verify_whatever_draft_rows_hold_that_no_child_was_drawn_from(parts, vocab, monkeypatch):
+    """The draft's row of a node without children, or whose child is taken, is not part of the answer; nor is one that leaves nothing of p."""
+    monkeypatch.setattr(sm100_draft, "_verify_parts", lambda *a: parts)
+    nodes = [1, 4, 3, 2, 1, 5, 2]
+    b, up = U.batch([3] * len(nodes), nodes, 16, DEV), U.trees(nodes, 1)
+    for seed in range(3):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        tok, p, _, u = U.drafts(nodes, up, vocab, "given", DEV, seed)
+        q = 1.5 * p                                             # nothing of p is over it: a refused child's rest is p itself
+        tok[:] = torch.arange(len(up), device=DEV) % 2          # tokens 0 and 1 keep their numbers
+        first, what = 0, (float("nan"), float("inf"), float("-inf"))
+        for s, n in enumerate(nodes):
+            u[first + 1:first + n] = 0.0                        # taken
+            q[first + n - 1] = what[(s + seed) % 3]             # without children
+            if s % 2 == 0 and n > 1:                            # the last child is refused
+                u[first + n - 1] = 1 - 2.0 ** -24
+                hit = torch.rand(vocab - 2, generator=gen, device=DEV) < 0.5
+                q[first + n - 2, 2:] = torch.where(hit, torch.where(hit.roll(1), float("nan"), float("inf")), q[first + n - 2, 2:])
+            first += n
+        want = U.verify(tok, _i32(up), b, p, q, u)
+        assert want[2].tolist() == [n - (s % 2 == 0 and n > 1) for s, n in enumerate(nodes)]
+        _same(Fn.draft_verify(tok, _i32(up), b, p, q, u), want)
