@@ -570,7 +570,9 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           if (kChunks > 1 && behind) tmem_store_wait();
           if constexpr (PAIR) {
-            // the item's maximum so far, of both warps: neither comes to the next tile before the other has read it, as that needs both's P
+            // The item's maximum so far, of both warps. Neither may add the next tile's before the other has read it. WIDE: S of the next tile is
+            // formed behind both's P. Else it may be there already, and they meet once more.
+            if (!WIDE && t > it.t0) sync_pair();
             atomicMax(&row_max[wg * kRows + tl], ordered(__float_as_int(mx)));
             sync_pair();
             mx = __int_as_float(ordered(*static_cast<volatile int*>(&row_max[wg * kRows + tl])));
