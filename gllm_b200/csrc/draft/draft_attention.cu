@@ -509,6 +509,12 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if (wg == 0) asm volatile("bar.sync 1, %0;" ::"n"(kGroup) : "memory");
       else asm volatile("bar.sync 2, %0;" ::"n"(kGroup) : "memory");
     };
+    // WIDE, the first half: the second one has done with the items before this one. Its barrier is in the phase of the last of them that it had a
+    // part in, or in the next: for more it needs this half's P.
+    uint32_t halves2 = 0;                                  // items before this one that have a second half
+    auto wait_second = [&] {
+      if (halves2 > 0) guard.wait<true>(&o_free[1], (halves2 & 1) ^ 1);
+    };
     // PAIR: the two warps that have a row between them
     auto sync_pair = [&] { asm volatile("bar.sync %0, 64;" ::"r"(3 + wg * 4 + (warp & 3)) : "memory"); };
     for (uint32_t item = 0; it.next(); ++item) {
@@ -625,6 +631,10 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           l_run += sa.x + sa.y;
           tmem_store_wait();
         }
+        if (WIDE && threadIdx.x == 0 && t == it.t0 && *static_cast<volatile unsigned long long*>(bad_nodes + ((item + 1) & 3)) != 0ull) {
+          wait_second();                                   // the next item's word was that of the item three before
+          bad_nodes[(item + 1) & 3] = 0ull;
+        }
         if (behind && (!WIDE || wg == 0)) {                // (WIDE: the first half's product comes first)
           // Values that nobody sees, or not every row, are finite before the product reads them
           const uint32_t vp = (t + 1 < it.t1 || it.left > 0) ? 2 * g + 2 : 2 * g + 1, st = vp % NS;    // where V of tile g is in the ring
@@ -648,6 +658,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
             if (bad) {
               *w = x;
+              if (WIDE) wait_second();                     // the word was that of the item four before
               atomicOr(bad_here, 1ull << (key0 + r - it.ctx));
             }
           }
@@ -660,8 +671,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
       // ---- results; the other warpgroup has the next item meanwhile
       await_pv(mine - 1);
-      // The word of the item after the next is free: it was that of an item whose results both warpgroups have, or had no part in
-      if (tl == 0 && (!PAIR || part == 0) && (!WIDE || wg == 0)) bad_nodes[(item + 2) & 3] = 0ull;
+      // The word of the item after the next is free: it was that of the group's item before, whose results all of it has
+      if (!WIDE && tl == 0 && (!PAIR || part == 0)) bad_nodes[(item + 2) & 3] = 0ull;
       // Lanes that have a row's keys between them: maximum and sum of all, this lane's weight
       float2* lanes = reinterpret_cast<float2*>(smem + (item & 1) * SM::kQBytes);    // the item's queries have been read
       if (kLanes > 1) lanes[tl] = make_float2(m_run, l_run);
@@ -797,6 +808,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (lane == 0) mbar_arrive(&o_free[wg]);
         if (kLanes > 1 && tl == 0) mbar_arrive(&q_free[item & 1]);
       }
+      if (WIDE) halves2 += rows > p.half_rows;
       if (warp_ok && part == 0) {
         const int slot = 2 * blockIdx.x + (it.t0 == 0 ? 1 : 0);
         if (cut && row_ok) p.part_ml[static_cast<size_t>(slot) * (WIDE ? 2 * kRows : kRows) + row] = make_float2(m_run, l_run);

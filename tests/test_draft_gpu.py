@@ -566,3 +566,26 @@ def test_verify_whatever_draft_rows_hold_that_no_child_was_drawn_from(parts, voc
         want = U.verify(tok, _i32(up), b, p, q, u)
         assert want[2].tolist() == [n - (s % 2 == 0 and n > 1) for s, n in enumerate(nodes)]
         _same(Fn.draft_verify(tok, _i32(up), b, p, q, u), want)
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_many_items_with_and_without_a_second_half(d, whole, monkeypatch):
+    """Some seven items an SM in blocks of 256 rows, few of them with more than 128; values of nodes that are no numbers in one sequence of two."""
+    monkeypatch.setattr(sm100_draft, "_whole_units", lambda *a: whole)
+    nodes = [(64, 2, 5, 1, 40, 3, 33, 7, 1, 2)[s % 10] for s in range(500)]
+    ctx = [(7 * s) % 140 for s in range(500)]
+    x = _attention_case(ctx, nodes, 8, 2, d, 16)
+    t, seen = x.b.num_tokens, x.seen.tolist()
+    hit = torch.zeros(t, d, dtype=torch.bool, device=DEV)         # columns of a row with a value that is no number
+    first = 0
+    for s, n in enumerate(nodes):
+        if s % 2 == 0:
+            i = s // 2 % n
+            x.v[int(x.b.block_table[s, (ctx[s] + i) // 16]), :, :, (ctx[s] + i) % 16, s % 7::7] = (float("nan"), float("inf"), float("-inf"))[s % 3]
+            rows = [r for r in range(first, first + n) if seen[r] >> i & 1]
+            hit[rows] = torch.arange(d, device=DEV) % 64 % 7 == s % 7
+        first += n
+    out = Fn.draft_attention(x.q, x.k, x.v, x.b, x.seen, d ** -0.5, 8, d)[:t].double().view(-1, 8, d)
+    want, tol = U.attention(x.q[:t], x.k, torch.where(x.v.isfinite(), x.v, 0), x.b, U.sees(seen, x.b), d ** -0.5, 8)
+    assert hit.any() and torch.where(hit[:, None], ~out.isfinite(), (out - want).abs() <= tol).all()

@@ -94,3 +94,71 @@ def test_both_warps_of_a_row_see_one_maximum(wide):
     narrow = SOURCE[SOURCE.index("// S of tile `tile_no`"):SOURCE.index("umma_commit(mma_end)")]
     assert narrow.index("scores(g + 1") < narrow.index("wait<true>(&p_full[")
     assert pair(wide) > 10
+
+
+# -- blocks of 256 rows: the words of nodes whose values are no numbers --------------------------------------------------------
+def halves(two, bad):
+    """The halves' groups and the issuing thread over items of one tile: two[i]: it has a second half, bad[i]: the first half finds such nodes in
+    it. Either half has to see the item's own, no others'. A wait for o_free[1] tells a phase from the next one only, as the barrier does."""
+    n = len(two)
+    kinds = dict(clear=r"bad_nodes\[\(item \+ (\d)\) & 3\] = 0ull", set=r"atomicOr\(bad_here", free=r"wait_second\(\)")
+    order = [[(k, int(m[1]) if k == "clear" else 0) for k, m, line in steps(t, **kinds) if "!WIDE &&" not in line]
+             for t in (SOFTMAX[SOFTMAX.index("for (uint32_t item"):], RESULTS)]
+    assert [k for k, _ in order[0] + order[1]].count("set") == 1 and any(k == "clear" for k, _ in order[0] + order[1])
+
+    def first():
+        program = []
+        for i in range(n):
+            had = sum(two[:i])
+
+            def wait(v, had=had):
+                return None if had == 0 or (v["o_free1"] - 1) % 2 == (had - 1) % 2 else False
+
+            def part(order, i=i, wait=wait):
+                out, behind_wait = [], False
+                for kind, at in order:
+                    if kind == "free":
+                        behind_wait = True
+                        continue
+                    name = f"word{(i + at) % 4 if kind == 'clear' else i % 4}"
+
+                    def step(v, kind=kind, name=name, i=i, behind_wait=behind_wait):
+                        if (kind == "set" and not bad[i]) or (kind == "clear" and v[name] == ()):
+                            return None
+                        if behind_wait and wait(v) is False:
+                            return False
+                        v[name] = () if kind == "clear" else v[name] + (i,)
+                    out.append(step)
+                    behind_wait = False
+                return out
+            program += [until("s0", i + 1), *part(order[0]), add("p0"), until("pv0", i + 1), look(i), add("o_free0"), *part(order[1])]
+        return program
+
+    def look(i):
+        def step(v):
+            assert v[f"word{i % 4}"] == ((i,) if bad[i] else ()), "a word of another item"
+        return step
+
+    def second():
+        program, k = [], 0
+        for i in range(n):
+            if two[i]:
+                k += 1
+                program += [until("s1", k), add("p1"), until("pv1", k), look(i), add("o_free1")]
+        return program
+
+    issue, k = [], 0
+    for i in range(n):
+        issue += [add("s0"), *([add("s1")] if two[i] else []), until("o_free0", i), until("p0", i + 1), add("pv0")]
+        if two[i]:
+            issue += [until("o_free1", k), until("p1", k + 1), add("pv1")]
+            k += 1
+    names = [f"{x}{h}" for x in ("s", "p", "pv", "o_free") for h in range(2)]
+    return explore([first(), second(), issue], {**dict.fromkeys(names, 0), **{f"word{w}": () for w in range(4)}})
+
+
+@pytest.mark.parametrize("two", ["2111111", "2211121", "1211112", "2222222", "2121211", "1111111", "2112112"])
+def test_halves_see_the_nodes_of_their_own_item(two):
+    items = [x == "2" for x in two]
+    for word in range(1 << len(items)):
+        halves(items, [bool(word >> i & 1) for i in range(len(items))])
