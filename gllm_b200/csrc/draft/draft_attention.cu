@@ -786,6 +786,7 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 }
               }
             }
+            fence_proxy_async_smem();                      // the next queries are copied into this buffer
             sync_group();
             if (warp_ok) {
 #pragma unroll

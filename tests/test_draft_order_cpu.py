@@ -162,3 +162,14 @@ def test_halves_see_the_nodes_of_their_own_item(two):
     items = [x == "2" for x in two]
     for word in range(1 << len(items)):
         halves(items, [bool(word >> i & 1) for i in range(len(items))])
+
+
+def test_results_in_a_query_buffer_are_fenced_before_the_next_queries_are_copied_into_it():
+    """Rows that lanes share: sums and results lie in the item's query buffer for a while. Copies write by another proxy than threads: every thread's
+    writes, then its fence, a barrier of the group, then the arrival that lets the copy begin."""
+    order = [k for k, _, _ in steps(RESULTS, write=r"\blanes\[tl\] = |\bat\[e \* BR\] = ", fence=r"fence_proxy_async_smem\(\)", group=r"sync_group\(\)",
+                                    free=r"mbar_arrive\(&q_free")]
+    last = max(i for i, k in enumerate(order) if k == "write")
+    assert order.count("write") == 2 and order.count("free") == 1 and order[-1] == "free"
+    fence = order.index("fence", last)
+    assert "group" in order[fence:order.index("free")]
