@@ -5,7 +5,8 @@
 // where their 64 KB take some 2700 of an SM's share of the memory. All units lie in one row that is cut into equal shares for the CTAs, one an
 // SM, on the device, so that lengths may differ from those at the time a graph was captured and long contexts beside short ones leave no SM
 // idle. A share's units are whole but for the first and the last; those parts (O in fp32, maximum, sum) are joined by a second launch in a
-// fixed order, which costs 5 to 9 us. Or no unit is cut, where that costs less (ops/sm100_draft.py).
+// fixed order, which costs 5 to 9 us. Or no unit is cut, where none has more than 16 tiles and that costs less (ops/sm100_draft.py): the SM with the
+// longest ends last then.
 //
 // Rows, by what a sequence may have (host):  up to 32, 64, 128  one block; with few rows 4 or 2 TMEM lanes share a row, each has a part of
 // every tile's keys, so that all four schedulers form exponentials (a lane's 128 take a warp 1700 cycles and more, 32 take 650).

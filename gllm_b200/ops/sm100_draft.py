@@ -41,10 +41,13 @@ def _whole_units(seqs: int, kv_heads: int, group: int, nodes: int, max_len: int)
     """Whether no unit of the attention kernel (a sequence's kv head and block of rows) is cut: nothing is joined then, in a second launch of some
     5 us, but the SM with the most has up to a unit more than its share. Cut and whole, us: 8 units of 1, 4, 12 and 47
     tiles (32 / 8 heads of 128, 8 nodes) 11.5 / 10.3, 14.1 / 12.4, 15.7 / 16.5, 19.0 / 39.4; 128 of 4 and 47 17.3 / 14.4, 57.4 / 66.3; 1024 of
-    4 and 12 53.4 / 47.5, 111 / 108. Results are right either way, whatever the lengths are when a captured call is replayed."""
+    4 and 12 53.4 / 47.5, 111 / 108. The longest length is all that is known of them, and the others may be short, so longer units are cut
+    however many there are: 18 sequences, all of 16 tiles 39.0 / 32.9, one of 16 beside 17 of one 18.3 / 22.6; all of 32 60.6 / 54.4, one 22.1 /
+    34.9; 37 sequences, all of 32 101.6 / 100.4, one of 32 24.7 / 35.9, one of 470 116 / 394. Results are right either way, whatever the lengths are
+    when a captured call is replayed."""
     tiles = (max_len + 127) // 128
-    if tiles <= 8:
-        return True
+    if tiles <= 8 or tiles > 16:
+        return tiles <= 8
     rows = nodes * group
     block = (32 if rows <= 32 else 64 if rows <= 64 else 128 if rows <= 128 else 256) // group
     units = seqs * kv_heads * -(-nodes // max(block, 1))

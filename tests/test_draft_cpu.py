@@ -193,3 +193,13 @@ def test_64_nodes_at_most_and_names_of_limits():
     b = U.batch([20], [64], 16, "cpu")
     seen = Fn.draft_plan(_i32(list(range(-1, 63))), b, 16)[0]
     assert seen[-1] == -1 and seen[0] == 1                       # the last of a chain sees every node: all 64 bits
+
+
+@pytest.mark.parametrize("seqs", [1, 18, 37, 74, 111, 148, 300])
+@pytest.mark.parametrize("nodes,group", [(1, 1), (8, 4), (24, 4), (64, 8)])
+def test_long_units_of_attention_are_cut_however_many_there_are(seqs, nodes, group):
+    """One long context beside short ones: what counts is how long it may be, not whether the units go evenly into the SMs."""
+    from gllm_b200.ops import sm100_draft
+    for length in (32 * 128, 60000, 1 << 20):
+        assert not sm100_draft._whole_units(seqs, 8, group, nodes, length)
+    assert sm100_draft._whole_units(seqs, 8, group, nodes, 600)
