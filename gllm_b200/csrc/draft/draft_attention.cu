@@ -526,7 +526,8 @@ draft_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const int at = it.blk * p.block_rows + row, node = at / p.G, head = it.kvh * p.G + at - node * p.G;
       const int64_t tok = it.first + (row_ok ? node : 0);
       const unsigned long long word_all = row_ok ? static_cast<unsigned long long>(p.seen[tok]) : 0ull;   // first used where nodes are
-      const unsigned long long nodes = it.n < kNodes ? (1ull << it.n) - 1 : ~0ull;
+      const int placed = it.len - it.ctx;                  // nodes behind the table's end have no place: nobody sees them
+      const unsigned long long nodes = placed < kNodes ? (1ull << placed) - 1 : ~0ull;
       unsigned long long* bad_here = bad_nodes + (item & 3);
       const uint32_t t_o = tmem + SM::kTmemO + wg * D + lane_base;
       if (WIDE ? wg * p.half_rows >= rows : (item & 1) != static_cast<uint32_t>(wg)) {   // no second half; the other's

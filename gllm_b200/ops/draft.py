@@ -4,7 +4,8 @@ A step drafts a tree of tokens for every sequence and lets the model look at all
 [query_start_loc[s], query_start_loc[s + 1]) of the batch, at most 64. Node 0 is the token that stands already, as in a step without
 drafts; a parent is a node's index within its sequence and comes before it, anything else counts as none (such a node sees the context and
 itself, and is never taken). `seq_lens` counts the nodes: ctx = seq_len - nodes tokens are in the cache, node i lies at cache position
-ctx + i while the step runs. A sequence without rows takes no part; rows behind the last sequence belong to none.
+ctx + i while the step runs; what would lie behind the last entry of `block_table` has no place (slot -1) and is seen by nobody. A
+sequence without rows takes no part; rows behind the last sequence belong to none.
 
   plan     who sees whom, one 64-bit word a node (bit j: node j), the nodes' rotary positions (ctx + depth) and cache slots
   attend   softmax over the context and over the nodes whose bits are set; a row that sees nothing is zero
@@ -200,11 +201,13 @@ def attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out=
     g, lens = num_q_heads // k_cache.shape[1], inp.seq_lens.tolist()
     for s, a, n in _sequences(inp, q.shape[0]):
         ctx = max(lens[s] - n, 0)
-        k, v = (gather_kv(c, inp.block_table[s], ctx + n).float().repeat_interleave(g, 1) for c in (k_cache, v_cache))
+        length = min(ctx + n, inp.block_table.shape[1] * k_cache.shape[3])
+        k, v = (gather_kv(c, inp.block_table[s], length).float().repeat_interleave(g, 1) for c in (k_cache, v_cache))
         qq = q[a:a + n, : num_q_heads * head_dim].reshape(n, num_q_heads, head_dim).float()
         z = torch.einsum("qhd,khd->hqk", qq, k) * scale
         sees = torch.ones(n, ctx + n, dtype=torch.bool)
         sees[:, ctx:] = (seen[a:a + n, None] >> torch.arange(n)) & 1 > 0
+        sees = sees[:, :length]
         z = z.masked_fill(~sees, float("-inf"))
         p = torch.where(sees.any(-1)[:, None], z.softmax(-1), 0.0)
         hidden = torch.where(sees[None, :, :, None], p[..., None] * v.permute(1, 0, 2)[:, None], 0.0)    # 0 times what is no number: 0

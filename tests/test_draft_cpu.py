@@ -203,3 +203,15 @@ def test_long_units_of_attention_are_cut_however_many_there_are(seqs, nodes, gro
     for length in (32 * 128, 60000, 1 << 20):
         assert not sm100_draft._whole_units(seqs, 8, group, nodes, length)
     assert sm100_draft._whole_units(seqs, 8, group, nodes, 600)
+
+
+def test_attention_of_tables_that_end():
+    torch.manual_seed(4)
+    b = U.batch([14, 0, 24, 5], [8, 20, 3, 7], 16, "cpu")
+    b.block_table = b.block_table[:, :1]
+    seen = Fn.draft_plan(_i32(U.trees(b.nodes, 3)), b, 16)[0]
+    k, v = (torch.randn(kv_cache_shape(b.pages, 2, 64, 16)).to(BF16) for _ in range(2))
+    q = torch.randn(38, 256).to(BF16)
+    got = Fn.draft_attention(q, k, v, b, seen, 0.125, 4, 64).double().view(38, 4, 64)
+    want, tol = U.attention(q, k, v, b, [m[:, :16] for m in U.sees(seen.tolist(), b)], 0.125, 4)
+    assert ((got - want).abs() <= tol).all()

@@ -589,3 +589,14 @@ def test_attention_of_many_items_with_and_without_a_second_half(d, whole, monkey
     out = Fn.draft_attention(x.q, x.k, x.v, x.b, x.seen, d ** -0.5, 8, d)[:t].double().view(-1, 8, d)
     want, tol = U.attention(x.q[:t], x.k, torch.where(x.v.isfinite(), x.v, 0), x.b, U.sees(seen, x.b), d ** -0.5, 8)
     assert hit.any() and torch.where(hit[:, None], ~out.isfinite(), (out - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("most", [8, 16, 30, 64])
+@pytest.mark.parametrize("pages", [1, 2, 9])
+def test_attention_of_tables_that_end(pages, most, d):
+    """Tokens behind a table's last page have no place: nobody sees them, context or nodes."""
+    x = _attention_case([16 * pages - 2, 0, 16 * pages + 8, 5, 16 * pages], [most, most, 3, 7, 2], 8, 2, d, 16)
+    x.b.block_table = x.b.block_table[:, :pages]
+    masks = [m[:, :16 * pages] for m in U.sees(x.seen.tolist(), x.b)]
+    _check_attention(x, masks=masks)
