@@ -600,3 +600,46 @@ def test_attention_of_tables_that_end(pages, most, d):
     x.b.block_table = x.b.block_table[:, :pages]
     masks = [m[:, :16 * pages] for m in U.sees(x.seen.tolist(), x.b)]
     _check_attention(x, masks=masks)
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("most", [8, 16, 30, 64])
+def test_captured_attention_with_units_cut_and_whole(most, d, whole, monkeypatch):
+    """Two graphs in turn, replayed with lengths that change which shares begin, end and join units: many parts, then none, then others."""
+    monkeypatch.setattr(sm100_draft, "_whole_units", lambda *a: whole)
+    seqs, made = 4, []
+    for g in range(2):
+        torch.manual_seed(g)
+        inp = types.SimpleNamespace(block_table=torch.zeros(seqs, 640, dtype=I32, device=DEV), seq_lens=_i32([1] * seqs), query_start_loc=_i32(range(seqs + 1)),
+                                    num_seqs=seqs, num_tokens=seqs * most, max_q_len=most, max_seq_len=10000, padded_tokens=0)
+        s = types.SimpleNamespace(inp=inp, q=torch.randn(seqs * most, 8 * d, device=DEV).to(BF16), seen=torch.ones(seqs * most, dtype=torch.int64, device=DEV),
+                                  caches=[torch.randn(kv_cache_shape(1800, 2, d, 16), device=DEV).to(BF16) for _ in range(2)],
+                                  out=torch.zeros(seqs * most, 8 * d, dtype=BF16, device=DEV))
+
+        def step(s=s):
+            Fn.draft_attention(s.q, *s.caches, s.inp, s.seen, d ** -0.5, 8, d, out=s.out)
+        step()
+        torch.cuda.synchronize()
+        s.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(s.graph):
+            step()
+        made.append(s)
+    for ctx, nodes in [([9000, 40, 9000, 8000], [most] * 4), ([0, 0, 0, 0], [1, 0, 0, 0]), ([9900, 0, 0, 0], [most, 0, 1, 0]), ([60, 700, 5, 9000], [1, most, most, 3]),
+                       ([0] * 4, [0] * 4), ([2000] * 4, [most] * 4), ([127, 9000, 128, 1], [most, 1, most, 2])]:
+        for g, s in enumerate(made):
+            b, n = U.batch(ctx, nodes, 16, DEV, seed=g), sum(nodes)
+            s.inp.block_table.fill_(-7)
+            s.inp.block_table[:, : b.block_table.shape[1]] = b.block_table
+            s.inp.seq_lens.copy_(b.seq_lens)
+            s.inp.query_start_loc.copy_(b.query_start_loc)
+            s.seen[:n] = Fn.draft_plan(_i32(U.trees(nodes, 3, g)), b, 16)[0]
+            s.out.fill_(5)
+            s.b, s.n = b, n
+            s.graph.replay()
+        torch.cuda.synchronize()
+        for s in made:
+            assert (s.out[s.n:] == 5).all()
+            if s.n:
+                want, tol = U.attention(s.q[:s.n], *s.caches, s.b, U.sees(s.seen.tolist(), s.b), d ** -0.5, 8)
+                assert ((s.out[:s.n].double().view(-1, 8, d) - want).abs() <= tol).all(), ctx
