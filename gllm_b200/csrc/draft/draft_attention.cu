@@ -11,7 +11,8 @@
 // Rows, by what a sequence may have (host):  up to 32, 64, 128  one block; with few rows 4 or 2 TMEM lanes share a row, each has a part of
 // every tile's keys, so that all four schedulers form exponentials (a lane's 128 take a warp 1700 cycles and more, 32 take 650).
 // More: blocks of two halves of 128, so that keys and values are read once for 256 rows. Where a row has one lane two warps share it, with 64
-// keys of a tile each (128 x 600 tokens, 24 nodes, 32 / 8 heads: 67.2 us with one warp, 65.5 with two; 16 of 8000, 64 nodes: 123.5 / 121).
+// keys of a tile each (16 of 8000 tokens, 64 nodes, 32 / 8 heads: 123.5 us with one warp, 121 with two; 128 x 600, 24 nodes: 67.2 and 65.5, or
+// 66.6 to 67.1 since blocks of up to 128 rows meet once more a tile).
 //
 //   softmax            two groups of four warps, or of eight (two a row); a row a lane (tcgen05.ld 32x32b). The groups have the CTA's items
 //                      in turn: one's results, some 3000 cycles of which most is instruction fetch, are written while the other has the
@@ -30,7 +31,8 @@
 // What bounds it: HBM where histories are long (two of 60,000, 64 / 8 heads, 16 nodes: 82 us for 61 of bytes, the copies alone 69; 64 of 2500, 8
 // nodes 89 for 74; some 10 us are the first data and the last results). Blocks of 256 rows: the chain softmax -> P V -> S of a half, 3960 cycles
 // per 128 keys for 2048 of tensor core and of the 2^x unit each (4 of 30,000, 64 nodes, 64 / 8 heads: 165 us, 775 TFLOP/s): maximum 600,
-// exponentials 1300 to 1600, the two hand-overs 530, the products 1250. A product with the first half of P while the other half is formed gains 1 %
+// exponentials 1300 to 1600, the two hand-overs 530, the products 1250. The prefill kernel has the same chain at 1221 TFLOP/s, with a row of scores in
+// the registers of one thread (setmaxnreg) instead of two readings of TMEM by two; that form was not tried here. A product with the first half of P while the other half is formed gains 1 %
 // (the issuing thread's waits take the rest), exponentials by polynomial lose 6 %, a thread for either half's products loses 20 % (one thread's
 // order keeps one half at its exponentials while the other is at its products); steps of 64 keys with two buffers of S a half were slower
 // (278 for 173): twice the products and commits of that thread.

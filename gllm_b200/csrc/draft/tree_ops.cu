@@ -10,8 +10,8 @@ static constexpr int kMostNodes = 64;
 // ---------------------------------------------------------------------------------------------------------------------
 // plan: a warp per sequence, two nodes a lane. With up_i the parent and seen_i = {i}, six rounds of
 //   seen_i |= seen[up_i],  up_i = up[up_i]
-// reach ancestors 64 levels above. Latency bounds it: lengths, parents, then the table's entries, one trip to memory each (1 and 256 sequences of
-// 8 and 5 nodes: 4.2 us).
+// reach ancestors 64 levels above. Latency bounds it: lengths, parents, then the table's entries, one trip to memory each (1 sequence of
+// 8 nodes 4.1 us, 256 of 5 and 256 of up to 64 4.2).
 // ---------------------------------------------------------------------------------------------------------------------
 static constexpr int kPlanWarps = 4;
 

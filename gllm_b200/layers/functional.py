@@ -196,7 +196,8 @@ def draft_plan(parents, inp, page_size):
 
 def draft_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out=None):
     """Attention of the nodes' queries [T, Hq * D] over the paged cache that holds their own keys and values too: each sees the context and the
-    nodes in its word of `seen`, whatever lies in those it does not see."""
+    nodes in its word of `seen`, whatever lies in those it does not see. Rows behind the last sequence are left as they are in `out`, and are
+    of no meaning where it is not given."""
     return (_draft() if q.is_cuda else draft).attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out)
 
 
@@ -204,7 +205,7 @@ def draft_verify(tokens, parents, inp, target, draft_probs=None, uniform=None):
     """(tokens int32 [T], path int32 [T], count int32 [sequences]): in each sequence's rows the tokens that it goes on with, count of
     them (the last is new), and the nodes that were taken, node 0 first; -1 behind them. `target`: the target's tokens int32 [T] at the nodes
     (from `sample`, say), or its probabilities fp32 [T, V] with `uniform` [T] in [0, 1) and, where drafts were drawn, their
-    distributions `draft_probs` [T, V] (row i: what node i's children were drawn from)."""
+    distributions `draft_probs` [T, V] (row i: what node i's children were drawn from; rows of nodes without children may hold anything)."""
     return (_draft() if tokens.is_cuda else draft).verify(tokens, parents, inp, target, draft_probs, uniform)
 
 

@@ -56,7 +56,8 @@ def _whole_units(seqs: int, kv_heads: int, group: int, nodes: int, max_len: int)
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp, seen: torch.Tensor, scale: float, num_q_heads: int,
               head_dim: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """q [T, Hq * D] bf16 (any row stride) -> [T, Hq * D]; rows behind the last sequence are left as they are."""
+    """q [T, Hq * D] bf16 (any row stride) -> [T, Hq * D]; rows behind the last sequence are not written: in a result that is made here they hold
+    whatever the memory held."""
     b, start, lens, table = draft.check_attention(q, k_cache, v_cache, inp, seen, scale, num_q_heads, head_dim, out)
     pages, hkv, _, page_size, w = k_cache.shape
     t, q_ts = q.shape[0], q.stride(0)
@@ -91,9 +92,9 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, inp
 
 def _verify_parts(b: int, vocab: int) -> int:
     """CTAs of a cluster that share a sequence: as many as leave all clusters resident, two CTAs an SM. One sequence, 151,936 tokens, 1 to 16
-    CTAs: 36, 22, 15.7, 12.0, 10.5 us; 64 of 128,257: 38, 23, 20.5, 27, 43; 256 of 151,936: 65, 74, 85, 109. Sixteen are for few sequences and
-    long rows (8 and 16 CTAs: 4 chains of 32,000 8.7 / 8.9, of 100,352 10.0 / 9.0, of 151,936 11.8 / 10.4; 8 chains 11.6 / 11.1, 8 trees of 32
-    nodes 21.7 / 17.0; 8 chains of 100,352 10.3 / 10.9; 12 of 151,936 12.1 / 12.9)."""
+    CTAs: 24, 16.5, 12.3, 10.0, 9.2 us; 64 of 128,257: 36, 20.5, 18.0, 24, 40; 256 of 151,936: 60, 67, 78, 104. Sixteen are for few sequences and
+    long rows (8 and 16 CTAs: 4 chains of 32,000 8.0 / 8.5, of 100,352 9.8 / 9.0, of 151,936 10.8 / 9.5; 8 chains 11.0 / 11.0, 8 trees of 32
+    nodes 19.7 / 15.8; 8 chains of 100,352 10.0 / 10.3; 12 of 151,936 11.5 / 11.6)."""
     if vocab > 1 << 16 and b <= (8 if vocab > 1 << 17 else 4):
         return 16
     return 8 if b <= 37 else 4 if b <= 74 else 2 if b <= 148 else 1
