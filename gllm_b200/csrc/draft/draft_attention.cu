@@ -31,11 +31,11 @@
 // What bounds it: HBM where histories are long (two of 60,000, 64 / 8 heads, 16 nodes: 82 us for 61 of bytes, the copies alone 69; 64 of 2500, 8
 // nodes 89 for 74; some 10 us are the first data and the last results). Blocks of 256 rows: the chain softmax -> P V -> S of a half, 3960 cycles
 // per 128 keys for 2048 of tensor core and of the 2^x unit each (4 of 30,000, 64 nodes, 64 / 8 heads: 165 us, 775 TFLOP/s): maximum 600,
-// exponentials 1300 to 1600, the two hand-overs 530, the products 1250. The prefill kernel has the same chain at 1221 TFLOP/s, with a row of scores in
-// the registers of one thread (setmaxnreg) instead of two readings of TMEM by two; that form was not tried here. A product with the first half of P while the other half is formed gains 1 %
-// (the issuing thread's waits take the rest), exponentials by polynomial lose 6 %, a thread for either half's products loses 20 % (one thread's
-// order keeps one half at its exponentials while the other is at its products); steps of 64 keys with two buffers of S a half were slower
-// (278 for 173): twice the products and commits of that thread.
+// exponentials 1300 to 1600, the two hand-overs 530, the products 1250. The prefill kernel has the same chain at 1221 TFLOP/s, with a row of scores
+// in the registers of one thread (setmaxnreg) instead of two readings of TMEM by two; that form was not tried here. A product with the first half
+// of P while the other half is formed gains 1 % (the issuing thread's waits take the rest), exponentials by polynomial lose 6 %, a thread for
+// either half's products loses 20 % (one thread's order keeps one half at its exponentials while the other is at its products); steps of 64 keys
+// with two buffers of S a half were slower (278 for 173): twice the products and commits of that thread.
 #include "../attn/attn_common.cuh"
 #include "../common/bounded.cuh"
 

@@ -29,7 +29,7 @@ none the token is 0. Probabilities are fp32, what is computed from them fp64: a 
 that are not over 0 (NaN among them) have no mass, and a token outside of the vocabulary none either.
 
 On the GPU attention takes bf16 queries and caches, heads of 64 or 128, at most 128 query heads a kv head, pages of 8 to 128 tokens; its
-probabilities are rounded to bf16 (half a step, 2^-9 of the value) before their product with V, sums are fp32. `keep` moves rows of any type.
+probabilities are rounded to bf16 (half a step, at most 2^-8 of the value) before their product with V, sums are fp32. `keep` moves rows of any type.
 """
 from __future__ import annotations
 
